@@ -30,7 +30,7 @@ typedef enum nb_status {
     NB_ERR_TOO_LARGE = 5    /* size beyond the limit of a fixed-capacity entry point */
 } nb_status;
 
-enum { NB_DTYPE_BF16 = 0, NB_DTYPE_FP16 = 1 };
+enum { NB_DTYPE_BF16 = 0, NB_DTYPE_FP16 = 1, NB_DTYPE_FP32 = 2 /* rotary and layer norm only */ };
 
 /* epilogue selector of nb_gemm_w4a4 */
 enum {
@@ -230,6 +230,74 @@ int nb_layernorm_modulate(const void* x, const void* scale, const void* shift, v
 int nb_gated_residual(const void* x, const void* gate, const void* y, const void* y2, void* out, int32_t rows,
                       int32_t rows_per_batch, int32_t dim, int64_t stride_xr, int64_t stride_yr, int64_t stride_y2r,
                       int64_t stride_or, int64_t stride_gb, int64_t stride_gd, int32_t dtype, void* stream);
+
+/*
+ * Layer norm with a weight and a bias and its backward pass.  NO COUNTERPART IN THE REFERENCE as an operator (it runs
+ * torch's layer norm and modulates its output); the weight may be one row for all rows (`groups` 1) or one per group of
+ * `rows` rows (`groups` samples: the scale and shift of an adaptive norm, with weight_add = 1).
+ *   y  = xh * (w + weight_add) + b,   xh = (x - mean) * rstd,   rstd = 1 / sqrt(var + eps)
+ *   dx = rstd * (v - mean(v) - xh * mean(v * xh)),   v = dy * (w + weight_add)
+ *   dw = sum over the group's rows of dy * xh,   db = sum of dy
+ * Everything is computed in fp32 and rounded once.  x / dy: rows strided by stride_x / stride_dy elements; y / dx are
+ * contiguous.  w, b (either may be null: 1 and 0), dw, db: dtype when w_fp32 is 0, else fp32; the rows of w and b are
+ * stride_w apart, those of dw and db `dim`.
+ * Forward: y may be null (statistics only), mean / rstd (groups * rows fp32) may be null.
+ * Backward: mean / rstd as the forward pass wrote them; dx may be null, dw and db may be null.  Where dw or db is
+ * wanted, `workspace` holds nb_layer_norm_workspace_bytes() bytes (16-byte aligned).  The sums over the rows are taken in
+ * a fixed order: two calls give the same bits.
+ * 1 <= dim <= NB_LAYER_NORM_MAX_DIM (else NB_ERR_UNSUPPORTED).
+ */
+#define NB_LAYER_NORM_MAX_DIM 16384
+typedef struct nb_layer_norm_args {
+    const void* x; const void* w; const void* b;
+    void* y;
+    float* mean; float* rstd;
+    const void* dy;
+    void* dx; void* dw; void* db;
+    void* workspace; int64_t workspace_bytes;
+    int64_t stride_x, stride_dy, stride_w;
+    int32_t groups, rows, dim;
+    int32_t dtype, w_fp32;
+    float eps, weight_add;
+} nb_layer_norm_args;
+int nb_layer_norm(const nb_layer_norm_args* args, void* stream);
+int nb_layer_norm_backward(const nb_layer_norm_args* args, void* stream);
+int64_t nb_layer_norm_workspace_bytes(int32_t groups, int32_t rows, int32_t dim, int32_t dtype);
+
+/*
+ * Rotary positions with several axes (time, height, width).  Takes the place of `rope` / `NunchakuFluxPosEmbed` followed by
+ * the rotation (nunchaku/models/embeddings.py:11-50, 74-97) where Q and K do not come out of the fused QKV projection.
+ * Axis a owns axes_dim[a] of a head's channels; pair j of it turns by id[a] * theta^(-2 j / axes_dim[a]).  The angles are
+ * taken in fp64.  Channels behind the axes' pass through.
+ *   nb_rotary_ladder_init  fills the ladder of rates on the host (turns per unit of position); a caller keeps it
+ *   nb_rotary_axes         q_out / k_out (B, S, H or Hk, D), contiguous; pairs are neighbours, or with `half` the channels
+ *                          j and j + R / 2 of the R rotary ones; `inverse` rotates back (the backward pass); Hk = 0: no k
+ *   nb_rotary_table        (B, S, pairs) of (sin, cos) fp32, contiguous: the table that nb_qk_args.rot reads
+ * The ids (B, S, n_axes) have any strides, 0 among them.
+ */
+#define NB_ROTARY_MAX_AXES 4
+#define NB_ROTARY_MAX_PAIRS 128
+enum { NB_IDS_F32 = 0, NB_IDS_I32 = 1, NB_IDS_I64 = 2, NB_IDS_F64 = 3 };
+typedef struct nb_rotary_ladder {
+    double turns[NB_ROTARY_MAX_PAIRS];
+    int32_t pair_end[NB_ROTARY_MAX_AXES]; /* pairs of the axes 0..a together */
+    int32_t n_axes;
+    int32_t reserved;
+} nb_rotary_ladder;
+typedef struct nb_rotary_args {
+    const void* q; const void* k;
+    void* q_out; void* k_out;
+    const void* ids;
+    int64_t stride_qb, stride_qs, stride_qh;
+    int64_t stride_kb, stride_ks, stride_kh;
+    int64_t stride_ib, stride_is, stride_ia;
+    int32_t B, S, H, Hk, D;
+    int32_t dtype, ids_type, half, inverse;
+} nb_rotary_args;
+int nb_rotary_ladder_init(nb_rotary_ladder* ladder, const int32_t* axes_dim, int32_t n_axes, double theta);
+int nb_rotary_axes(const nb_rotary_args* args, const nb_rotary_ladder* ladder, void* stream);
+int nb_rotary_table(const void* ids, int32_t ids_type, int32_t B, int32_t S, int64_t stride_ib, int64_t stride_is,
+                    int64_t stride_ia, float* out, const nb_rotary_ladder* ladder, void* stream);
 
 /*
  * Checkpoint layout converter for the 4-bit weight: the stored fragment order of a SVDQuant checkpoint

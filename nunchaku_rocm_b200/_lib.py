@@ -9,6 +9,7 @@ There is no fallback: a missing library or a non-zero status raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -20,6 +21,8 @@ LIB_PATH = os.environ.get("NUNCHAKU_B200_LIB") or os.path.join(_HERE, "libnuncha
 
 NB_OK, NB_ERR_INVALID, NB_ERR_UNSUPPORTED, NB_ERR_LAUNCH, NB_ERR_DEVICE, NB_ERR_TOO_LARGE = range(6)
 DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
+DTYPE_CODE_32 = {**DTYPE_CODE, torch.float32: 2}  # the operators that take fp32 as well
+IDS_CODE = {torch.float32: 0, torch.int32: 1, torch.int64: 2, torch.float64: 3}
 EPI_STORE, EPI_QK, EPI_GELU_QUANT, EPI_SWIGLU_QUANT = range(4)
 IMPL_AUTO, IMPL_TCGEN05, IMPL_GENERIC, IMPL_TCGEN05_PAIR, IMPL_TCGEN05_SINGLE = range(5)
 NOALLOC_SCRATCH_BYTES = 16 << 20  # NB_NOALLOC_SCRATCH_BYTES
@@ -88,6 +91,43 @@ class AttnArgs(C.Structure):
     )
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("x", "w", "b", "y", "mean", "rstd", "dy", "dx", "dw", "db", "workspace")]
+        + [("workspace_bytes", C.c_int64)]
+        + [(n, C.c_int64) for n in ("stride_x", "stride_dy", "stride_w")]
+        + [(n, C.c_int32) for n in ("groups", "rows", "dim", "dtype", "w_fp32")]
+        + [("eps", C.c_float), ("weight_add", C.c_float)]
+    )
+
+
+ROTARY_MAX_AXES, ROTARY_MAX_PAIRS = 4, 128  # NB_ROTARY_MAX_AXES, NB_ROTARY_MAX_PAIRS
+
+
+class RotaryLadder(C.Structure):
+    _fields_ = [
+        ("turns", C.c_double * ROTARY_MAX_PAIRS),
+        ("pair_end", C.c_int32 * ROTARY_MAX_AXES),
+        ("n_axes", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "ids")]
+        + [
+            (n, C.c_int64)
+            for n in (
+                "stride_qb", "stride_qs", "stride_qh",
+                "stride_kb", "stride_ks", "stride_kh",
+                "stride_ib", "stride_is", "stride_ia",
+            )
+        ]
+        + [(n, C.c_int32) for n in ("B", "S", "H", "Hk", "D", "dtype", "ids_type", "half", "inverse")]
+    )
+
+
 _lock = threading.RLock()
 _lib = None
 
@@ -130,6 +170,15 @@ def lib() -> C.CDLL:
                 l.nb_qk_norm_rope.argtypes = [
                     C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.POINTER(QKArgs), C.c_void_p,
                 ]
+                l.nb_layer_norm.argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
+                l.nb_layer_norm_backward.argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
+                l.nb_layer_norm_workspace_bytes.argtypes = [C.c_int32] * 4
+                l.nb_layer_norm_workspace_bytes.restype = C.c_int64
+                l.nb_rotary_ladder_init.argtypes = [C.POINTER(RotaryLadder), C.POINTER(C.c_int32), C.c_int32, C.c_double]
+                l.nb_rotary_axes.argtypes = [C.POINTER(RotaryArgs), C.POINTER(RotaryLadder), C.c_void_p]
+                l.nb_rotary_table.argtypes = (
+                    [C.c_void_p] + [C.c_int32] * 3 + [C.c_int64] * 3 + [C.c_void_p, C.POINTER(RotaryLadder), C.c_void_p]
+                )
                 _lib = l
     return _lib
 
@@ -159,6 +208,15 @@ def ptr(t: torch.Tensor | None):
 
 def stream_of(t: torch.Tensor) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """``torch.cuda.device(dev)``, or nothing to enter where it is the current device already (the common case, and
+    entering costs more than a small launch)."""
+    return _here if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 _selftested: set[int] = set()

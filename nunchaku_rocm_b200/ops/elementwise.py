@@ -3,6 +3,9 @@ The element-wise steps around the quantised linears of a DiT block, fused to one
 (``csrc/elementwise.cu``).  The reference runs them as torch operators: ``NunchakuAdaLayerNormZero``
 (nunchaku/models/normalization.py:60-159) and the gated residuals of the transformer blocks
 (nunchaku/models/transformers/transformer_flux_v2.py:174-343).
+
+:func:`layer_norm` is a layer norm with its backward pass (``csrc/norm.cu``), for norms with a weight and a bias and for
+training the adaptive ones; :func:`layernorm_modulate` uses the same backward pass where gradients are asked for.
 """
 
 from __future__ import annotations
@@ -13,7 +16,7 @@ import torch
 
 from .. import _lib as L
 
-__all__ = ["layernorm_modulate", "gated_residual"]
+__all__ = ["layernorm_modulate", "gated_residual", "layer_norm"]
 
 
 def _bind():
@@ -36,10 +39,18 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def layernorm_modulate(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor, scale_add: float = 0.0,
                        eps: float = 1e-6) -> torch.Tensor:
     """``LayerNorm(x) * (scale[:, None] + scale_add) + shift[:, None]`` for ``x (B, T, dim)``, ``scale / shift (B, dim)``
-    (any strides), no affine; rounded to the dtype where ``layer_norm``, ``+``, ``*``, ``+`` of the reference round."""
+    (any strides), no affine; rounded to the dtype where ``layer_norm``, ``+``, ``*``, ``+`` of the reference round.
+    Differentiable in ``x``, ``scale`` and ``shift``."""
     B, T, D = x.shape
     if D % 1024 or D > 4096:
         return torch.nn.functional.layer_norm(x, (D,), eps=eps) * (scale + scale_add)[:, None] + shift[:, None]
+    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or shift.requires_grad):
+        return _LayerNormModulate.apply(x, scale, shift, scale_add, eps)
+    return _layernorm_modulate(x, scale, shift, scale_add, eps)
+
+
+def _layernorm_modulate(x, scale, shift, scale_add, eps):
+    B, T, D = x.shape
     dev = L.require_cuda(x, scale, shift)
     x = _rows(x)
     assert scale.shape == (B, D) and shift.shape == (B, D) and scale.stride() == shift.stride() and scale.dtype == x.dtype == shift.dtype
@@ -72,3 +83,171 @@ def gated_residual(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, y2: tor
             "gated_residual",
         )
     return out
+
+
+def _strided_rows(x: torch.Tensor):
+    """``x (..., D)`` and the stride between its rows: a copy only where the rows are not evenly strided."""
+    D = x.shape[-1]
+    if not x.is_contiguous():
+        try:
+            if x.stride(-1) == 1:
+                return x, x.detach().view(-1, D).stride(0)
+        except RuntimeError:
+            pass
+        x = x.contiguous()
+    return x, D
+
+
+def _ln_weight(name, w, x, groups):
+    """``w`` as the kernel reads it, with the stride between its groups' rows."""
+    D = x.shape[-1]
+    if w.dtype != x.dtype and w.dtype != torch.float32:
+        raise ValueError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
+    if w.shape != ((D,) if w.dim() == 1 else (groups, D)) or (w.dim() == 2 and x.dim() != 3):
+        raise ValueError(f"{name} must be ({D},), or (B, {D}) for x (B, T, {D}); got {tuple(w.shape)} for {tuple(x.shape)}")
+    return w if w.stride(-1) == 1 else w.contiguous()
+
+
+def _ln_args(x, stride_x, weight, bias, eps, weight_add):
+    D, a = x.shape[-1], L.LayerNormArgs()
+    first = weight if weight is not None else bias
+    grouped = first is not None and first.dim() == 2
+    rows = x.numel() // D
+    a.groups = x.shape[0] if grouped else 1
+    a.rows = rows // a.groups if a.groups else 0
+    a.dim, a.dtype = D, L.DTYPE_CODE_32[x.dtype]
+    a.x, a.stride_x = x.data_ptr(), stride_x
+    if weight is not None:
+        a.w = weight.data_ptr()
+    if bias is not None:
+        a.b = bias.data_ptr()
+    if first is not None:
+        a.w_fp32 = first.dtype == torch.float32
+        a.stride_w = first.stride(0) if grouped else 0
+    a.eps, a.weight_add = eps, weight_add
+    return a
+
+
+def _ln_prepare(x, weight, bias, weight_add):
+    """The checks of the arguments; weight and bias with one stride and unit inner stride."""
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"layer_norm needs at least one channel, got x {tuple(x.shape)}")
+    if x.shape[-1] > 16384:
+        raise NotImplementedError(f"layer_norm takes up to 16384 channels, got {x.shape[-1]}")
+    if x.dtype not in L.DTYPE_CODE_32:
+        raise ValueError(f"layer_norm takes bfloat16, float16 and float32, got {x.dtype}")
+    if weight is None and weight_add:
+        raise ValueError("weight_add without a weight")
+    groups = x.shape[0] if x.dim() == 3 else 1
+    if weight is not None:
+        weight = _ln_weight("weight", weight, x, groups)
+    if bias is not None:
+        bias = _ln_weight("bias", bias, x, groups)
+        if weight is not None:
+            if bias.dtype != weight.dtype or bias.dim() != weight.dim():
+                raise ValueError("weight and bias must have one shape and one dtype")
+            if bias.dim() == 2 and bias.stride(0) != weight.stride(0):
+                weight, bias = weight.contiguous(), bias.contiguous()
+    return weight, bias
+
+
+def _ln_forward(x, weight, bias, eps, weight_add, y, stats):
+    """``y`` and / or the rows' (mean, rstd) into the given tensors; the arguments are prepared already."""
+    if x.numel() == 0:
+        return
+    x, stride_x = _strided_rows(x)
+    a = _ln_args(x, stride_x, weight, bias, eps, weight_add)
+    if y is not None:
+        a.y = y.data_ptr()
+    if stats is not None:
+        a.mean = stats.data_ptr()
+        a.rstd = a.mean + 4 * (stats.numel() // 2)
+    with L.on_device(x.device):
+        L.check(L.lib().nb_layer_norm(a, L.stream_of(x)), "layer_norm")
+
+
+def _ln_backward(x, weight, bias, stats, dy, eps, weight_add, need):
+    """(dx, dweight, dbias), ``None`` where ``need`` says so."""
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if need[1] else None
+    db = torch.empty(bias.shape, dtype=bias.dtype, device=x.device) if need[2] else None
+    if x.numel() == 0:
+        return dx, (dw.zero_() if need[1] else None), (db.zero_() if need[2] else None)
+    x, stride_x = _strided_rows(x)
+    dy, stride_dy = _strided_rows(dy)
+    a = _ln_args(x, stride_x, weight, bias, eps, weight_add)
+    a.mean = stats.data_ptr()
+    a.rstd = a.mean + 4 * (stats.numel() // 2)
+    a.dy, a.stride_dy = dy.data_ptr(), stride_dy
+    if need[0]:
+        a.dx = dx.data_ptr()
+    lib = L.lib()
+    with L.on_device(x.device):
+        if need[1] or need[2]:
+            n = lib.nb_layer_norm_workspace_bytes(a.groups, a.rows, a.dim, a.dtype)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+            if need[1]:
+                a.dw = dw.data_ptr()
+            if need[2]:
+                a.db = db.data_ptr()
+        L.check(lib.nb_layer_norm_backward(a, L.stream_of(x)), "layer_norm backward")
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, weight_add):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty(2, x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        _ln_forward(x, weight, bias, eps, weight_add, y, stats)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.consts = eps, weight_add
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        return (*_ln_backward(x, weight, bias, stats, dy, *ctx.consts, ctx.needs_input_grad), None, None)
+
+
+class _LayerNormModulate(torch.autograd.Function):
+    """:func:`layernorm_modulate` as it is without gradients, and the backward pass of the function that it rounds."""
+
+    @staticmethod
+    def forward(ctx, x, scale, shift, scale_add, eps):
+        ctx.save_for_backward(x, scale, shift)
+        ctx.consts = eps, scale_add
+        return _layernorm_modulate(x, scale, shift, scale_add, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        eps, scale_add = ctx.consts
+        x, scale, shift = ctx.saved_tensors
+        scale, shift = _ln_prepare(x, scale, shift, scale_add)
+        stats = torch.empty(2, x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        _ln_forward(x, None, None, eps, 0.0, None, stats)
+        return (*_ln_backward(x, scale, shift, stats, dy, eps, scale_add, ctx.needs_input_grad), None, None)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-6,
+               weight_add: float = 0.0) -> torch.Tensor:
+    """
+    ``(x - mean) / sqrt(var + eps) * (weight + weight_add) + bias`` over the last dimension of ``x (..., D)``, computed in
+    fp32 and rounded once to ``x``'s dtype (bfloat16, float16 or float32).  Differentiable in ``x``, ``weight`` and ``bias``.
+
+    ``weight`` and ``bias`` are ``(D,)``, or ``(B, D)`` for ``x (B, T, D)`` (one row per sample, as an adaptive norm's scale
+    and shift, then with ``weight_add=1``), both of ``x``'s dtype or both float32; either may be ``None``.  Their gradients
+    are summed over the rows in fp32, in a fixed order.  ``D`` is at most 16384.
+    """
+    weight, bias = _ln_prepare(x, weight, bias, weight_add)
+    dev = L.require_cuda(x, weight, bias)
+    grad = torch.is_grad_enabled() and (
+        x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
+    if grad:
+        return _LayerNorm.apply(x, weight, bias, eps, weight_add)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    _ln_forward(x, weight, bias, eps, weight_add, y, None)
+    return y

@@ -1,0 +1,142 @@
+"""
+Rotary positions with several axes (time, height, width), straight from position ids (``csrc/rotary.cu``).
+
+The fused QKV projection takes its rotation from a table (:func:`nunchaku_rocm_b200.models.embeddings.flux_pos_embed`);
+:func:`rotary_table` makes that table in one launch, and :func:`rotary_axes` rotates Q and K that come from elsewhere (a
+projection with per-request adapters, a 16-bit attention layer, a training step) without one.  The reference builds tables
+with torch operators (``rope`` / ``NunchakuFluxPosEmbed``, nunchaku/models/embeddings.py:11-50, 74-97).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import functools
+
+import torch
+
+from .. import _lib as L
+
+__all__ = ["rotary_axes", "rotary_table"]
+
+
+@functools.lru_cache(maxsize=64)
+def _ladder(axes_dim: tuple, theta: float) -> L.RotaryLadder:
+    if not 1 <= len(axes_dim) <= L.ROTARY_MAX_AXES:
+        raise ValueError(f"1 to {L.ROTARY_MAX_AXES} axes, got {len(axes_dim)}")
+    if any(d <= 0 or d % 2 for d in axes_dim) or sum(axes_dim) > 2 * L.ROTARY_MAX_PAIRS:
+        raise ValueError(f"the axes' channels must be even, positive and at most {2 * L.ROTARY_MAX_PAIRS} together: {axes_dim}")
+    ladder = L.RotaryLadder()
+    L.check(L.lib().nb_rotary_ladder_init(ladder, (C.c_int32 * len(axes_dim))(*axes_dim), len(axes_dim), theta), "rotary ladder")
+    return ladder
+
+
+def _ids_strides(ids: torch.Tensor, n_axes: int, batch: int, rows: int):
+    if ids.dtype not in L.IDS_CODE:
+        raise ValueError(f"ids must be float32, float64, int32 or int64, got {ids.dtype}")
+    if ids.shape not in ((rows, n_axes), (batch, rows, n_axes)):
+        raise ValueError(f"ids must be ({rows}, {n_axes}) or ({batch}, {rows}, {n_axes}), got {tuple(ids.shape)}")
+    st = ids.stride()
+    return st if len(st) == 3 else (0, *st)
+
+
+def _rotate(q, k, ids, ladder, half, inverse):
+    """(rotated q, rotated k): one launch over the heads of both; ``k`` may be ``None``."""
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1:
+        k = k.contiguous()
+    B, S, H, D = q.shape
+    qo = torch.empty((B, S, H, D), dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    a = L.RotaryArgs()
+    a.q, a.q_out, a.ids = q.data_ptr(), qo.data_ptr(), ids.data_ptr()
+    a.stride_qb, a.stride_qs, a.stride_qh, _ = q.stride()
+    a.B, a.S, a.H, a.D = B, S, H, D
+    if k is not None:
+        a.k, a.k_out, a.Hk = k.data_ptr(), ko.data_ptr(), k.shape[2]
+        a.stride_kb, a.stride_ks, a.stride_kh, _ = k.stride()
+    a.stride_ib, a.stride_is, a.stride_ia = _ids_strides(ids, ladder.n_axes, B, S)
+    a.dtype, a.ids_type = L.DTYPE_CODE_32[q.dtype], L.IDS_CODE[ids.dtype]
+    a.half, a.inverse = half, inverse
+    with L.on_device(q.device):
+        L.check(L.lib().nb_rotary_axes(a, ladder, L.stream_of(q)), "rotary_axes")
+    return qo, ko
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, ids, ladder, half, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(ids)
+        ctx.consts = ladder, half, inverse
+        return _rotate(q, k, ids, ladder, half, inverse)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        (ids,) = ctx.saved_tensors
+        ladder, half, inverse = ctx.consts
+        if not ctx.needs_input_grad[0]:
+            dq = None
+        if not ctx.needs_input_grad[1]:
+            dk = None
+        if dq is not None:
+            dq, dk = _rotate(dq, dk, ids, ladder, half, not inverse)
+        elif dk is not None:
+            dk, _ = _rotate(dk, None, ids, ladder, half, not inverse)
+        return dq, dk, None, None, None, None
+
+
+def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes_dim, theta: float = 10000.0,
+                interleaved: bool = True, inverse: bool = False):
+    """
+    Rotate ``q (B, S, H, D)`` and ``k (B, S, Hk, D)`` by the positions ``ids (S, axes)`` or ``(B, S, axes)``; returns new
+    contiguous tensors ``(q', k')``, or ``q'`` alone when ``k`` is ``None``.  Differentiable in ``q`` and ``k``.
+
+    Axis ``a`` owns ``axes_dim[a]`` channels of every head, in order; its pair ``j`` turns by
+    ``ids[..., a] * theta ** (-2 j / axes_dim[a])`` radians (angles in fp64, the rotation in fp32, one rounding).  A pair is
+    two neighbouring channels, or with ``interleaved=False`` channels ``j`` and ``j + R / 2`` of the ``R = sum(axes_dim)``
+    rotary ones.  Channels behind those pass through.  ``inverse`` rotates back.
+
+    bfloat16, float16 or float32; any strides; ``ids`` float32, float64, int32 or int64.
+    """
+    if q.dtype not in L.DTYPE_CODE_32:
+        raise ValueError(f"rotary_axes takes bfloat16, float16 and float32, got {q.dtype}")
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, S, H, D), got {tuple(q.shape)}")
+    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]):
+        raise ValueError(f"k must be (B, S, Hk, D) beside q, got {tuple(k.shape)} {k.dtype} for {tuple(q.shape)} {q.dtype}")
+    ladder = _ladder(tuple(axes_dim), float(theta))
+    B, S, H, D = q.shape
+    _ids_strides(ids, ladder.n_axes, B, S)
+    if 2 * ladder.pair_end[ladder.n_axes - 1] > D:
+        raise ValueError(f"axes {tuple(axes_dim)} have more channels than a head ({D})")
+    if H == 0 or (k is not None and k.shape[2] == 0):
+        raise ValueError("no heads")
+    L.require_cuda(q, k, ids)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _RotaryAxes.apply(q, k, ids, ladder, not interleaved, inverse)
+    else:
+        out = _rotate(q, k, ids, ladder, not interleaved, inverse)
+    return out[0] if k is None else out
+
+
+def rotary_table(ids: torch.Tensor, axes_dim, theta: float = 10000.0) -> torch.Tensor:
+    """
+    The ``(sin, cos)`` table of ``ids (S, axes)`` -> ``(S, sum(axes_dim) / 2, 1, 2)`` fp32 (or with a leading ``B``): what
+    the fused QKV epilogue reads as ``rotary_emb``, with the angles of :func:`rotary_axes`.
+    """
+    if ids.dim() not in (2, 3):
+        raise ValueError(f"ids must be (S, axes) or (B, S, axes), got {tuple(ids.shape)}")
+    ladder = _ladder(tuple(axes_dim), float(theta))
+    B, S = (1, ids.shape[0]) if ids.dim() == 2 else ids.shape[:2]
+    st = _ids_strides(ids, ladder.n_axes, B, S)
+    pairs = ladder.pair_end[ladder.n_axes - 1]
+    L.require_cuda(ids)
+    out = torch.empty((*ids.shape[:-1], pairs, 1, 2), dtype=torch.float32, device=ids.device)
+    with L.on_device(ids.device):
+        L.check(
+            L.lib().nb_rotary_table(ids.data_ptr(), L.IDS_CODE[ids.dtype], B, S, *st, out.data_ptr(), ladder, L.stream_of(out)),
+            "rotary_table",
+        )
+    return out
