@@ -232,6 +232,35 @@ int nb_gated_residual(const void* x, const void* gate, const void* y, const void
                       int64_t stride_or, int64_t stride_gb, int64_t stride_gd, int32_t dtype, void* stream);
 
 /*
+ * Low-rank adapters of many requests at once beside a shared projection.  The reference appends one LoRA set to a layer's
+ * low-rank branch (nunchaku/lora/runtime.py:475-535); here rows [offsets[i], offsets[i + 1]) use adapter adapters[i]:
+ *   out[t] = base[t] + scale[a] * (x[t] down[a]^T) up[a]^T,   down (A, R, K), up (A, N, R), contiguous
+ * Rows of a request whose adapter is outside 0 .. A - 1, rows before offsets[0] and rows from offsets[requests] on have
+ * none: out is base there (zero when base is null).  `offsets` (requests + 1) and `adapters` (requests) are DEVICE arrays,
+ * read by the kernels only; offsets must not go down (no access is out of bounds if they do, but the result is undefined).
+ * out may be base.  scale (A fp32) may be null (1).
+ * forward:  writes h (2, T, R) of dtype: scale * x down^T as hi + lo, rows without an adapter left as they were
+ * backward: reads dy, x, h and the factors; writes dx (T, K), ddown (A, R, K), dup (A, N, R), contiguous; each may be null;
+ *           g is scratch like h (needed for dx and ddown); workspace: nb_lora_workspace_bytes() for the same arguments,
+ *           256-byte aligned (needed for ddown and dup).  Sums over rows are taken in a fixed order.
+ * R a multiple of 16 up to NB_LORA_MAX_RANK, K and N multiples of 8 (else NB_ERR_UNSUPPORTED); every row 16-byte aligned.
+ */
+#define NB_LORA_MAX_RANK 128
+typedef struct nb_lora_args {
+    const void* x; const void* base; const void* down; const void* up;
+    const int32_t* offsets; const int32_t* adapters; const float* scale;
+    void* out; void* h;
+    const void* dy;
+    void* dx; void* ddown; void* dup; void* g;
+    void* workspace; int64_t workspace_bytes;
+    int64_t stride_x, stride_base, stride_out, stride_dy;
+    int32_t T, K, N, R, A, requests, dtype;
+} nb_lora_args;
+int nb_lora_forward(const nb_lora_args* args, void* stream);
+int nb_lora_backward(const nb_lora_args* args, void* stream);
+int64_t nb_lora_workspace_bytes(const nb_lora_args* args);
+
+/*
  * Layer norm with a weight and a bias and its backward pass.  NO COUNTERPART IN THE REFERENCE as an operator (it runs
  * torch's layer norm and modulates its output); the weight may be one row for all rows (`groups` 1) or one per group of
  * `rows` rows (`groups` samples: the scale and shift of an adaptive norm, with weight_add = 1).

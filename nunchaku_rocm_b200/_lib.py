@@ -91,6 +91,24 @@ class AttnArgs(C.Structure):
     )
 
 
+class LoraArgs(C.Structure):
+    _fields_ = (
+        [
+            (n, C.c_void_p)
+            for n in (
+                "x", "base", "down", "up", "offsets", "adapters", "scale", "out", "h", "dy", "dx", "ddown", "dup", "g",
+                "workspace",
+            )
+        ]
+        + [("workspace_bytes", C.c_int64)]
+        + [(n, C.c_int64) for n in ("stride_x", "stride_base", "stride_out", "stride_dy")]
+        + [(n, C.c_int32) for n in ("T", "K", "N", "R", "A", "requests", "dtype")]
+    )
+
+
+LORA_MAX_RANK = 128  # NB_LORA_MAX_RANK
+
+
 class LayerNormArgs(C.Structure):
     _fields_ = (
         [(n, C.c_void_p) for n in ("x", "w", "b", "y", "mean", "rstd", "dy", "dx", "dw", "db", "workspace")]
@@ -170,6 +188,10 @@ def lib() -> C.CDLL:
                 l.nb_qk_norm_rope.argtypes = [
                     C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.POINTER(QKArgs), C.c_void_p,
                 ]
+                l.nb_lora_forward.argtypes = [C.POINTER(LoraArgs), C.c_void_p]
+                l.nb_lora_backward.argtypes = [C.POINTER(LoraArgs), C.c_void_p]
+                l.nb_lora_workspace_bytes.argtypes = [C.POINTER(LoraArgs)]
+                l.nb_lora_workspace_bytes.restype = C.c_int64
                 l.nb_layer_norm.argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
                 l.nb_layer_norm_backward.argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
                 l.nb_layer_norm_workspace_bytes.argtypes = [C.c_int32] * 4

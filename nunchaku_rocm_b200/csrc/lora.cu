@@ -1,0 +1,725 @@
+// Low-rank adapters of many requests at once beside a shared projection, forward and backward.
+//
+// Rows [offsets[i], offsets[i+1]) of x belong to request i, which uses adapter a = adapters[i] (outside 0 .. A-1: none):
+//
+//     h   = x D_a^T               D (A, R, K)      (shrink)
+//     out = base + s_a h U_a^T    U (A, N, R)      (expand)
+//     g   = s_a dy U_a                             (shrink)
+//     dx  = g D_a                                  (expand)
+//     dD_a = sum of g^T x,  dU_a = sum of s_a dy^T h   over the rows of all requests of a   (outer, then join)
+//
+// Three kernels, each with either order of its factor's elements, cover the six products.  Work is cut into ITEMS: the
+// intervals between neighbouring borders, borders being the requests' offsets and every BM-th row.  An item therefore has one
+// adapter and at most BM rows, there are at most T / BM + requests + 2 of them however ragged the requests are (so the
+// grid is known without reading the offsets on the host), every row is in exactly one, and a CTA finds its item with one
+// pass over the offsets: border j of the offsets has floor(offset / BM) + 1 tile borders before it.
+//
+// h and g are sums in fp32.  Where they are operands again they are held as TWO 16-bit numbers, v = hi + lo (hi = v rounded
+// to T, lo = v - hi rounded to T): 16 significant bits for bf16 and 22 for fp16, so the second product loses nothing that
+// the final rounding would show; one rounding alone would add an error as large as that of the output itself.  It doubles
+// the matrix instructions of the second products, which move more bytes than they compute.
+//
+// Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out).
+#include <cooperative_groups.h>
+
+#include "nb_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace nb {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kRows = 64;  // rows of an item (shrink, expand)
+
+struct LoraParams {
+    const void* x;        // shrink: (T, K) operand; expand: base (T, C) or null; outer: (T, K) operand
+    void* out;            // expand: (T, C)
+    const void* factor;   // shrink: (A, R, K) or (A, K, R); expand: (A, C, R) or (A, R, C)
+    void* hi; void* lo;   // (T, R) each
+    float* part;          // outer: (items, R, K) or (items, K, R)
+    int* item_adapter;    // outer: (items)
+    const int* offsets; const int* adapters; const float* scale;
+    long long stride_x, stride_out;
+    int T, K, R, A, requests;  // K: length of the contraction (shrink), columns (expand, outer)
+    int rows_per_item, cols_per_cta;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// 16 bytes to shared memory, or 16 zero bytes (nothing is read then)
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+struct Item {
+    int first, rows, adapter;  // rows 0: nothing to do; adapter -1: rows without one
+};
+__host__ __device__ inline int item_count(int T, int requests, int bm) { return (T + bm - 1) / bm + requests + 1; }
+
+// The `w`-th interval of the merged borders (tile borders before equal offsets).  All threads of the CTA call it.
+__device__ __forceinline__ Item find_item(const LoraParams& p, int w) {
+    const int bm = p.rows_per_item, tiles = (p.T + bm - 1) / bm;
+    auto offset = [&](int j) { return min(max(__ldg(p.offsets + j), 0), p.T); };
+    int before = 0;  // offsets among the first w borders
+    for (int j0 = 0; j0 <= p.requests; j0 += kThreads) {
+        const int j = j0 + (int)threadIdx.x;
+        before += __syncthreads_count(j <= p.requests && j + min(offset(j) / bm + 1, tiles) < w);
+    }
+    int i = w - before, j = before;
+    Item it = {0, 0, -1};
+    const int tile = i < tiles ? i * bm : p.T, off = j <= p.requests ? offset(j) : p.T;
+    int next_tile = tile, next_off = off;
+    if (i < 0) return it;  // (offsets that go down)
+    if (i < tiles && tile <= off) {
+        it.first = tile;
+        next_tile = i + 1 < tiles ? (i + 1) * bm : p.T;
+    } else if (j <= p.requests) {
+        it.first = off;
+        ++j;
+        next_off = j <= p.requests ? offset(j) : p.T;
+    } else {
+        return it;
+    }
+    it.rows = min(max(min(next_tile, next_off) - it.first, 0), bm);
+    if (it.rows && j >= 1 && j <= p.requests) {
+        const int a = __ldg(p.adapters + j - 1);
+        it.adapter = a >= 0 && a < p.A ? a : -1;
+    }
+    return it;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ shrink
+// v[t, r] = s_a sum_k X[t, k] F_a[r, k], written as hi + lo.  A CTA has one item and one slice of K; the slices of an item
+// are a cluster, whose sums meet in shared memory (in a fixed order), so a few rows of a long K still use many SMs and no
+// partial sums go through memory.  The tiles of X and F travel by cp.async, ST stages deep.  With fewer than 64 rows the
+// warps that have no rows take a share of K instead.
+template <int RM, bool RCONTIG>
+struct ShrinkTile {
+    static constexpr int ST = RM >= 8 ? 3 : 4;
+    static constexpr int XROW = 64 * 2 + 16;                                     // 64 of K; 16 bytes of padding: ldmatrix rows on different banks
+    static constexpr int FROW = RCONTIG ? RM * 32 + 16 : XROW;
+    static constexpr int XBYTES = kRows * XROW, FBYTES = (RCONTIG ? 64 : RM * 16) * FROW;
+    static constexpr int PIPE = ST * (XBYTES + FBYTES), SUMS = kRows * RM * 16 * 4;
+    static constexpr int BYTES = PIPE > SUMS ? PIPE : SUMS;
+};
+template <typename T, int RM, bool RCONTIG>
+__global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraParams p) {
+    using S = ShrinkTile<RM, RCONTIG>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const Item it = find_item(p, blockIdx.x);
+    if (it.rows == 0 || it.adapter < 0) return;  // every CTA of the cluster
+    const int splits = gridDim.y, split = blockIdx.y;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const uint32_t sx = smem_u32(smem), sf = sx + S::ST * S::XBYTES;
+    const T* x = static_cast<const T*>(p.x) + (long long)it.first * p.stride_x;
+    const T* f = static_cast<const T*>(p.factor) + (long long)it.adapter * p.R * p.K;
+    const int mt = (it.rows + 15) / 16;
+    const int wm = mt > 2 ? 4 : mt, wk = 4 / wm;  // warps along the rows, along K
+    const int m = warp % wm, phase = warp / wm;
+    const int steps = (p.K + 63) / 64, per = (steps + splits - 1) / splits;
+    const int step0 = min(split * per, steps), n = min(per, steps - step0);
+
+    auto load = [&](int s) {
+        if (s < n) {
+            const int k0 = (step0 + s) * 64, st = s % S::ST;
+            for (int c = t; c < mt * 16 * 8; c += kThreads) {
+                const int row = c >> 3, k = k0 + (c & 7) * 8;
+                const bool real = row < it.rows && k < p.K;
+                cp16(sx + st * S::XBYTES + row * S::XROW + (c & 7) * 16, real ? x + row * p.stride_x + k : x, real);
+            }
+            if constexpr (RCONTIG) {
+                for (int c = t; c < 64 * RM * 2; c += kThreads) {
+                    const int k = c / (RM * 2), r = (c % (RM * 2)) * 8;
+                    const bool real = k0 + k < p.K && r < p.R;
+                    cp16(sf + st * S::FBYTES + k * S::FROW + r * 2, real ? f + (long long)(k0 + k) * p.R + r : f, real);
+                }
+            } else {
+                for (int c = t; c < RM * 16 * 8; c += kThreads) {
+                    const int r = c >> 3, k = k0 + (c & 7) * 8;
+                    const bool real = k < p.K && r < p.R;
+                    cp16(sf + st * S::FBYTES + r * S::FROW + (c & 7) * 16, real ? f + (long long)r * p.K + k : f, real);
+                }
+            }
+        }
+        cp_commit();
+    };
+
+    float acc[RM * 2][4];
+#pragma unroll
+    for (int i = 0; i < RM * 2; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll
+    for (int s = 0; s < S::ST - 1; ++s) load(s);
+    for (int s = 0; s < n; ++s) {
+        cp_wait<S::ST - 2>();
+        __syncthreads();
+        load(s + S::ST - 1);
+        const uint32_t xs = sx + (s % S::ST) * S::XBYTES, fs = sf + (s % S::ST) * S::FBYTES;
+        if (m < mt)
+            for (int kk = phase; kk < 4; kk += wk) {
+                uint32_t a[4];
+                ldsm4(a, xs + (m * 16 + (lane & 15)) * S::XROW + kk * 32 + (lane >> 4) * 16);
+#pragma unroll
+                for (int r = 0; r < RM; ++r) {
+                    uint32_t b[4];
+                    if constexpr (RCONTIG)
+                        ldsm4t(b, fs + (kk * 16 + (lane & 15)) * S::FROW + r * 32 + (lane >> 4) * 16);
+                    else
+                        ldsm4(b, fs + (r * 16 + (lane & 7) + (lane >> 4) * 8) * S::FROW + kk * 32 + ((lane >> 3) & 1) * 16);
+                    mma16816<T>(acc[2 * r], a, b[0], b[1]);
+                    mma16816<T>(acc[2 * r + 1], a, b[2], b[3]);
+                }
+            }
+    }
+    cp_wait<0>();
+    __syncthreads();
+
+    // the warps' shares of K, then the cluster's
+    float* sums = reinterpret_cast<float*>(smem);  // [rows][RM * 16]
+    constexpr int LD = RM * 16;
+    for (int q = 0; q < wk; ++q) {
+        if (q == phase && m < mt) {
+#pragma unroll
+            for (int i = 0; i < RM * 2; ++i) {
+                float* at = sums + (m * 16 + (lane >> 2)) * LD + i * 8 + (lane & 3) * 2;
+                float2* up = reinterpret_cast<float2*>(at);
+                float2* dn = reinterpret_cast<float2*>(at + 8 * LD);
+                float2 u = make_float2(acc[i][0], acc[i][1]), d = make_float2(acc[i][2], acc[i][3]);
+                if (q) {
+                    u.x += up->x; u.y += up->y;
+                    d.x += dn->x; d.y += dn->y;
+                }
+                *up = u;
+                *dn = d;
+            }
+        }
+        __syncthreads();
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (splits > 1) cluster.sync();
+    const float scale = p.scale ? __ldg(p.scale + it.adapter) : 1.f;
+    const int half = p.R / 2;  // pairs of a row
+    for (int e = split * kThreads + t; e < it.rows * half; e += splits * kThreads) {
+        const int row = e / half, r = (e - row * half) * 2;
+        float2 v = make_float2(0.f, 0.f);
+        for (int q = 0; q < splits; ++q) {
+            const float* from = splits > 1 ? cluster.map_shared_rank(sums, q) : sums;
+            const float2 u = *reinterpret_cast<const float2*>(from + row * LD + r);
+            v.x += u.x; v.y += u.y;
+        }
+        v.x *= scale; v.y *= scale;
+        const uint32_t hi = pack2<T>(v.x, v.y);
+        const float2 back = unpack2<T>(hi);
+        // a value beyond T's range is infinite in hi; its remainder is then left out (inf - inf)
+        const uint32_t lo = pack2<T>(isfinite(back.x) ? v.x - back.x : 0.f, isfinite(back.y) ? v.y - back.y : 0.f);
+        const long long at = ((long long)(it.first + row) * p.R + r) * 2;
+        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.hi) + at) = hi;
+        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.lo) + at) = lo;
+    }
+    if (splits > 1) cluster.sync();  // nobody's shared memory goes while others read it
+}
+
+// ------------------------------------------------------------------------------------------------------------------ expand
+// out[t, c] = base[t, c] + sum_r v[t, r] G_a[c, r], v = hi + lo.  A CTA keeps its item's v as matrix operands in registers
+// and walks over its columns, BN at a time, two tiles of G in shared memory.  The columns of a matrix instruction are
+// permuted (its operand rows may come from anywhere) so that a thread's results are eight neighbours: base and out are then
+// read and written 16 bytes at a time straight from and to memory.  Warps without rows take a share of the columns.
+template <int RM, bool CCONTIG>
+struct ExpandTile {
+    static constexpr int BN = RM >= 8 ? 64 : 128;
+    static constexpr int GROW = CCONTIG ? BN * 2 + 16 : RM * 32 + 16;
+    // [c][r] rows: 32 bytes more every eight rows, because a matrix operand's rows are 0, 1, 8, 9, 16, 17, 24, 25
+    static constexpr int GBYTES = CCONTIG ? RM * 16 * GROW : BN * GROW + BN / 8 * 32;
+    static constexpr int BYTES = 2 * GBYTES;
+    static constexpr int CHUNKS = RM * 16 * BN / 8 / kThreads;  // 16-byte pieces per thread and tile
+};
+template <typename T, int RM, bool CCONTIG>
+__global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams p) {
+    using S = ExpandTile<RM, CCONTIG>;
+    constexpr int BN = S::BN;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const Item it = find_item(p, blockIdx.y);
+    if (it.rows == 0) return;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int col0 = blockIdx.x * p.cols_per_cta, col1 = min(col0 + p.cols_per_cta, p.K);
+    const T* base = static_cast<const T*>(p.x);
+    T* out = static_cast<T*>(p.out);
+    if (it.adapter < 0) {  // base alone (zeros without one)
+        if (base == out) return;
+        const int n = (col1 - col0) / 8;
+        for (int e = t; e < it.rows * n; e += kThreads) {
+            const int row = e / n, c = col0 + (e - row * n) * 8;
+            const uint4 v = base ? *reinterpret_cast<const uint4*>(base + (it.first + row) * p.stride_x + c) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out + (it.first + row) * p.stride_out + c) = v;
+        }
+        return;
+    }
+    const T* g = static_cast<const T*>(p.factor) + (long long)it.adapter * p.R * p.K;
+    const uint32_t sg = smem_u32(smem);
+    const int mt = (it.rows + 15) / 16;
+    const int wm = mt > 2 ? 4 : mt, wn = 4 / wm;
+    const int m = warp % wm, share = warp / wm;
+    const int tiles = (col1 - col0 + BN - 1) / BN;
+
+    uint4 held[CCONTIG ? S::CHUNKS : 1];
+    auto issue = [&](int tile) {  // [c][r]: straight to shared memory; [r][c]: to registers
+        if (tile < tiles) {
+            const int c0 = col0 + tile * BN;
+#pragma unroll
+            for (int i = 0; i < S::CHUNKS; ++i) {
+                const int e = i * kThreads + t;
+                if constexpr (CCONTIG) {
+                    const int r = e / (BN / 8), c = c0 + e % (BN / 8) * 8;
+                    held[i] = r < p.R && c < col1 ? __ldg(reinterpret_cast<const uint4*>(g + (long long)r * p.K + c)) : make_uint4(0, 0, 0, 0);
+                } else {
+                    const int c = e / (RM * 2), r = e % (RM * 2) * 8;
+                    const bool real = r < p.R && c0 + c < col1;
+                    cp16(sg + (tile & 1) * S::GBYTES + c * S::GROW + (c >> 3) * 32 + r * 2, real ? g + (long long)(c0 + c) * p.R + r : g, real);
+                }
+            }
+        }
+        if constexpr (!CCONTIG) cp_commit();
+    };
+    auto land = [&](int tile) {
+        if constexpr (CCONTIG) {
+            // column pair j of the 16-byte piece q of a group of 32 goes to word 4 j + q: the permutation of the columns
+#pragma unroll
+            for (int i = 0; i < S::CHUNKS; ++i) {
+                const int e = i * kThreads + t, r = e / (BN / 8), q = e % (BN / 8);
+                uint32_t* w = reinterpret_cast<uint32_t*>(smem + (tile & 1) * S::GBYTES + r * S::GROW) + q / 4 * 16 + q % 4;
+                w[0] = held[i].x; w[4] = held[i].y; w[8] = held[i].z; w[12] = held[i].w;
+            }
+        } else {
+            cp_wait<0>();
+        }
+    };
+    issue(0);
+
+    uint32_t hi[RM][4], lo[RM][4];
+    const int row0 = m * 16 + (lane >> 2), row1 = row0 + 8;
+    {
+        const char* ph = static_cast<const char*>(p.hi);
+        const char* pl = static_cast<const char*>(p.lo);
+#pragma unroll
+        for (int k = 0; k < RM; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = i & 1 ? row1 : row0, r = k * 16 + (i >> 1) * 8 + (lane & 3) * 2;
+                const bool real = row < it.rows && r < p.R;
+                const long long at = ((long long)(it.first + row) * p.R + r) * 2;
+                hi[k][i] = real ? *reinterpret_cast<const uint32_t*>(ph + at) : 0u;
+                lo[k][i] = real ? *reinterpret_cast<const uint32_t*>(pl + at) : 0u;
+            }
+    }
+    const long long at0 = (long long)(it.first + row0), at1 = (long long)(it.first + row1);
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int c0 = col0 + tile * BN;
+        land(tile);
+        __syncthreads();
+        issue(tile + 1);
+        if (m < mt) {
+            const unsigned char* gs = smem + (tile & 1) * S::GBYTES;
+            for (int q = share; q < BN / 32; q += wn) {
+                const int c = c0 + q * 32 + (lane & 3) * 8;
+                const bool on0 = row0 < it.rows && c < col1, on1 = row1 < it.rows && c < col1;
+                uint4 b0 = make_uint4(0, 0, 0, 0), b1 = b0;
+                if (base && on0) b0 = *reinterpret_cast<const uint4*>(base + at0 * p.stride_x + c);
+                if (base && on1) b1 = *reinterpret_cast<const uint4*>(base + at1 * p.stride_x + c);
+                float acc[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < RM; ++k) {
+                    uint32_t b[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {  // instructions 2h and 2h + 1 of the four
+                        if constexpr (CCONTIG) {
+                            ldsm4t(b[h], smem_u32(gs) + (k * 16 + (lane & 15)) * S::GROW + q * 64 + h * 32 + (lane >> 4) * 16);
+                        } else {
+                            const int j = 2 * h + (lane >> 4), i = lane & 7;
+                            const int n = q * 32 + (i >> 1) * 8 + j * 2 + (i & 1);
+                            ldsm4(b[h], smem_u32(gs) + n * S::GROW + (n >> 3) * 32 + k * 32 + ((lane >> 3) & 1) * 16);
+                        }
+                        mma16816<T>(acc[2 * h], hi[k], b[h][0], b[h][1]);
+                        mma16816<T>(acc[2 * h + 1], hi[k], b[h][2], b[h][3]);
+                        mma16816<T>(acc[2 * h], lo[k], b[h][0], b[h][1]);
+                        mma16816<T>(acc[2 * h + 1], lo[k], b[h][2], b[h][3]);
+                    }
+                }
+                auto joined = [&](const uint4& b, int o) {
+                    const float2 f0 = unpack2<T>(b.x), f1 = unpack2<T>(b.y), f2 = unpack2<T>(b.z), f3 = unpack2<T>(b.w);
+                    return make_uint4(pack2<T>(f0.x + acc[0][o], f0.y + acc[0][o + 1]), pack2<T>(f1.x + acc[1][o], f1.y + acc[1][o + 1]),
+                                      pack2<T>(f2.x + acc[2][o], f2.y + acc[2][o + 1]), pack2<T>(f3.x + acc[3][o], f3.y + acc[3][o + 1]));
+                };
+                if (on0) *reinterpret_cast<uint4*>(out + at0 * p.stride_out + c) = joined(b0, 0);
+                if (on1) *reinterpret_cast<uint4*>(out + at1 * p.stride_out + c) = joined(b1, 2);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------- outer
+// part[item][r, k] = sum over the item's rows of v[t, r] X[t, k] (or [k, r] with KROWS), fp32, for one item of up to
+// rows_per_item rows and 128 columns.  Both operands are transposed on the way from shared memory to registers.
+template <int RM>
+struct OuterTile {
+    static constexpr int ST = RM >= 8 ? 3 : 4, BT = 32;
+    static constexpr int XROW = 128 * 2 + 16, VROW = RM * 32 + 16;
+    static constexpr int XBYTES = BT * XROW, VBYTES = BT * VROW;
+    static constexpr int STAGE = XBYTES + 2 * VBYTES, BYTES = ST * STAGE;
+};
+template <typename T, int RM, bool KROWS>
+__global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p) {
+    using S = OuterTile<RM>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
+    const int w = gridDim.y - 1 - blockIdx.y;
+    const Item it = find_item(p, w);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    if (blockIdx.x == 0 && t == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
+    if (it.rows == 0 || it.adapter < 0) return;
+    const int c0 = blockIdx.x * 128;
+    const T* x = static_cast<const T*>(p.x) + (long long)it.first * p.stride_x;
+    const char* hi = static_cast<const char*>(p.hi) + (long long)it.first * p.R * 2;
+    const char* lo = static_cast<const char*>(p.lo) + (long long)it.first * p.R * 2;
+    const uint32_t sm = smem_u32(smem);
+    const int n = (it.rows + S::BT - 1) / S::BT;
+
+    auto load = [&](int s) {
+        if (s < n) {
+            const int r0 = s * S::BT;
+            const uint32_t st = sm + (s % S::ST) * S::STAGE;
+#pragma unroll
+            for (int i = 0; i < S::BT * 16 / kThreads; ++i) {
+                const int e = i * kThreads + t, row = e >> 4, c = c0 + (e & 15) * 8;
+                const bool real = r0 + row < it.rows && c < p.K;
+                cp16(st + row * S::XROW + (e & 15) * 16, real ? x + (r0 + row) * p.stride_x + c : x, real);
+            }
+            for (int e = t; e < S::BT * RM * 2; e += kThreads) {
+                const int row = e / (RM * 2), r = e % (RM * 2) * 8;
+                const bool real = r0 + row < it.rows && r < p.R;
+                const long long at = real ? ((long long)(r0 + row) * p.R + r) * 2 : 0;
+                cp16(st + S::XBYTES + row * S::VROW + r * 2, hi + at, real);
+                cp16(st + S::XBYTES + S::VBYTES + row * S::VROW + r * 2, lo + at, real);
+            }
+        }
+        cp_commit();
+    };
+
+    // !KROWS: rows of the accumulator are r (RM tiles of 16), columns the warp's 32 of X (4 tiles of 8)
+    //  KROWS: rows are the warp's 32 columns of X (2 tiles of 16), columns are r (2 RM tiles of 8)
+    constexpr int MI = KROWS ? 2 : RM, NI = KROWS ? 2 * RM : 4;
+    float acc[MI][NI][4];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+#pragma unroll
+    for (int s = 0; s < S::ST - 1; ++s) load(s);
+    for (int s = 0; s < n; ++s) {
+        cp_wait<S::ST - 2>();
+        __syncthreads();
+        load(s + S::ST - 1);
+        const uint32_t xs = sm + (s % S::ST) * S::STAGE + warp * 64, vs = sm + (s % S::ST) * S::STAGE + S::XBYTES;
+#pragma unroll
+        for (int tt = 0; tt < S::BT; tt += 16) {
+            // operand with rows = columns of shared memory: matrices (t 0-7, c 0-7), (t 0-7, c 8-15), (t 8-15, ...) transposed
+            const int arow = tt + (lane & 7) + (lane >> 4) * 8, acol = ((lane >> 3) & 1) * 16;
+            const int brow = tt + (lane & 15), bcol = (lane >> 4) * 16;
+            if constexpr (KROWS) {
+                uint32_t a[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) ldsm4t(a[i], xs + arow * S::XROW + i * 32 + acol);
+#pragma unroll
+                for (int r = 0; r < RM; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t b[4];
+                        ldsm4t(b, vs + h * S::VBYTES + brow * S::VROW + r * 32 + bcol);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            mma16816<T>(acc[i][2 * r], a[i], b[0], b[1]);
+                            mma16816<T>(acc[i][2 * r + 1], a[i], b[2], b[3]);
+                        }
+                    }
+            } else {
+                uint32_t b[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) ldsm4t(b[j], xs + brow * S::XROW + j * 32 + bcol);
+#pragma unroll
+                for (int r = 0; r < RM; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t a[4];
+                        ldsm4t(a, vs + h * S::VBYTES + arow * S::VROW + r * 32 + acol);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            mma16816<T>(acc[r][2 * j], a, b[j][0], b[j][1]);
+                            mma16816<T>(acc[r][2 * j + 1], a, b[j][2], b[j][3]);
+                        }
+                    }
+            }
+        }
+    }
+    cp_wait<0>();
+    float* part = p.part + (long long)w * p.R * p.K;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const int mrow = i * 16 + (lane >> 2) + o * 8, ncol = j * 8 + (lane & 3) * 2;
+                const float2 v = make_float2(acc[i][j][2 * o], acc[i][j][2 * o + 1]);
+                if constexpr (KROWS) {
+                    const int k = c0 + warp * 32 + mrow;
+                    if (k < p.K && ncol < p.R) *reinterpret_cast<float2*>(part + (long long)k * p.R + ncol) = v;
+                } else {
+                    const int k = c0 + warp * 32 + ncol;
+                    if (k < p.K && mrow < p.R) *reinterpret_cast<float2*>(part + (long long)mrow * p.K + k) = v;
+                }
+            }
+}
+
+// dF[a] = sum of the partial products of a's items, in the items' order; zero for an adapter without rows
+template <typename T>
+__global__ void __launch_bounds__(256) lora_join_kernel(const float* part, const int* item_adapter, int items, long long size, T* out) {
+    __shared__ int mine[256];
+    __shared__ int count;
+    const int a = blockIdx.y, t = threadIdx.x;
+    const long long at = ((long long)blockIdx.x * 256 + t) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w0 = 0; w0 < items; w0 += 256) {
+        __syncthreads();
+        if (t < 32) {  // the items of this adapter, in order
+            int n = 0;
+            for (int w = w0; w < min(w0 + 256, items); w += 32) {
+                const bool hit = w + t < items && __ldg(item_adapter + w + t) == a;
+                const unsigned b = __ballot_sync(0xffffffffu, hit);
+                if (hit) mine[n + __popc(b & ((1u << t) - 1))] = w + t;
+                n += __popc(b);
+            }
+            if (t == 0) count = n;
+        }
+        __syncthreads();
+        if (at < size)
+            for (int i = 0; i < count; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(part + (long long)mine[i] * size + at);
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+    }
+    if (at < size) *reinterpret_cast<uint2*>(out + (long long)a * size + at) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+}
+
+// --------------------------------------------------------------------------------------------------------------- launchers
+int sms() {
+    const int n = nb_num_sms();
+    return n > 0 ? n : 148;
+}
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// rows of the gradients' items: long enough that the partial products stay small beside the operands, short enough that the
+// CTAs (one per item and 128 columns) cover the SMs about four times
+int outer_rows(int T, int cols) {
+    const int tiles = ceil_div(cols, 128), want = ceil_div(4ll * sms(), tiles);
+    const int rows = ceil_div(ceil_div(T, want), 64) * 64;
+    return rows < 128 ? 128 : rows;
+}
+
+template <typename K>
+int allow_smem(K kernel, int bytes) {
+    if (bytes > 48 * 1024) NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return NB_OK;
+}
+
+template <typename T, int RM, bool RCONTIG>
+int shrink(const LoraParams& p, cudaStream_t s) {
+    using S = ShrinkTile<RM, RCONTIG>;
+    const int items = item_count(p.T, p.requests, kRows);
+    // CTAs of an item: a power of two up to eight (a portable cluster), until the items cover the SMs twice, each with at
+    // least two steps of 64 of K
+    const int live = ceil_div(p.T, kRows) > p.requests ? ceil_div(p.T, kRows) : (p.requests < p.T ? p.requests : p.T);
+    int splits = 1;
+    while (splits < 8 && live * splits < 2 * sms() && ceil_div(p.K, 64) >= 4 * splits) splits *= 2;
+    auto* kernel = lora_shrink_kernel<T, RM, RCONTIG>;
+    if (int rc = allow_smem(kernel, S::BYTES)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(items, splits);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 1;
+    at.val.clusterDim.y = splits;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    NB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
+    return NB_OK;
+}
+template <typename T, int RM, bool CCONTIG>
+int expand(LoraParams p, cudaStream_t s) {
+    using S = ExpandTile<RM, CCONTIG>;
+    const int items = item_count(p.T, p.requests, kRows);
+    const int live = ceil_div(p.T, kRows) > p.requests ? ceil_div(p.T, kRows) : (p.requests < p.T ? p.requests : p.T);
+    // columns of a CTA: whole tiles, as many as leave about eight CTAs per SM
+    const int tiles = ceil_div(p.K, S::BN), per = ceil_div(8ll * sms(), live);
+    p.cols_per_cta = ceil_div(tiles, per < tiles ? per : tiles) * S::BN;
+    auto* kernel = lora_expand_kernel<T, RM, CCONTIG>;
+    if (int rc = allow_smem(kernel, S::BYTES)) return rc;
+    kernel<<<dim3(ceil_div(p.K, p.cols_per_cta), items), kThreads, S::BYTES, s>>>(p);
+    NB_CUDA_CHECK(cudaGetLastError());
+    return NB_OK;
+}
+template <typename T, int RM, bool KROWS>
+int outer(LoraParams p, T* grad, cudaStream_t s) {
+    using S = OuterTile<RM>;
+    p.rows_per_item = outer_rows(p.T, p.K);
+    const int items = item_count(p.T, p.requests, p.rows_per_item);
+    auto* kernel = lora_outer_kernel<T, RM, KROWS>;
+    if (int rc = allow_smem(kernel, S::BYTES)) return rc;
+    kernel<<<dim3(ceil_div(p.K, 128), items), kThreads, S::BYTES, s>>>(p);
+    NB_CUDA_CHECK(cudaGetLastError());
+    const long long size = (long long)p.R * p.K;
+    lora_join_kernel<T><<<dim3(ceil_div(size, 1024), p.A), 256, 0, s>>>(p.part, p.item_adapter, items, size, grad);
+    NB_CUDA_CHECK(cudaGetLastError());
+    return NB_OK;
+}
+
+LoraParams params_of(const nb_lora_args* a) {
+    LoraParams p = {};
+    p.offsets = a->offsets; p.adapters = a->adapters; p.scale = a->scale;
+    p.T = a->T; p.R = a->R; p.A = a->A; p.requests = a->requests;
+    p.rows_per_item = kRows;
+    return p;
+}
+char* plane(void* h, const nb_lora_args* a, int which) { return static_cast<char*>(h) + (long long)which * a->T * a->R * 2; }
+
+template <typename T, int RM>
+int forward_t(const nb_lora_args* a, cudaStream_t s) {
+    LoraParams p = params_of(a);
+    p.hi = plane(a->h, a, 0);
+    p.lo = plane(a->h, a, 1);
+    p.x = a->x; p.stride_x = a->stride_x; p.factor = a->down; p.K = a->K;
+    if (int rc = shrink<T, RM, false>(p, s)) return rc;
+    p.x = a->base; p.stride_x = a->stride_base; p.out = a->out; p.stride_out = a->stride_out; p.factor = a->up; p.K = a->N;
+    return expand<T, RM, false>(p, s);
+}
+template <typename T, int RM>
+int backward_t(const nb_lora_args* a, cudaStream_t s) {
+    LoraParams p = params_of(a);
+    char* ws = static_cast<char*>(a->workspace);
+    p.item_adapter = reinterpret_cast<int*>(ws);
+    ws += ((int64_t)item_count(a->T, a->requests, 128) * 4 + 255) / 256 * 256;
+    p.part = reinterpret_cast<float*>(ws);
+    LoraParams g = p;
+    if (a->dx || a->ddown) {
+        g.hi = plane(a->g, a, 0);
+        g.lo = plane(a->g, a, 1);
+        g.x = a->dy; g.stride_x = a->stride_dy; g.factor = a->up; g.K = a->N;
+        if (int rc = shrink<T, RM, true>(g, s)) return rc;
+    }
+    if (a->dup) {
+        p.x = a->dy; p.stride_x = a->stride_dy; p.K = a->N;
+        p.hi = plane(a->h, a, 0);
+        p.lo = plane(a->h, a, 1);
+        if (int rc = outer<T, RM, true>(p, static_cast<T*>(a->dup), s)) return rc;
+    }
+    g.K = a->K;
+    if (a->ddown) {
+        g.x = a->x; g.stride_x = a->stride_x;
+        if (int rc = outer<T, RM, false>(g, static_cast<T*>(a->ddown), s)) return rc;
+    }
+    if (a->dx) {
+        g.x = nullptr; g.out = a->dx; g.stride_out = a->K; g.factor = a->down;
+        return expand<T, RM, true>(g, s);
+    }
+    return NB_OK;
+}
+template <typename T>
+int dispatch(const nb_lora_args* a, bool backward, cudaStream_t s) {
+    const int rm = a->R / 16;
+    if (rm <= 1) return backward ? backward_t<T, 1>(a, s) : forward_t<T, 1>(a, s);
+    if (rm <= 2) return backward ? backward_t<T, 2>(a, s) : forward_t<T, 2>(a, s);
+    if (rm <= 4) return backward ? backward_t<T, 4>(a, s) : forward_t<T, 4>(a, s);
+    return backward ? backward_t<T, 8>(a, s) : forward_t<T, 8>(a, s);
+}
+
+int check(const nb_lora_args* a) {
+    NB_REQUIRE(a && a->T >= 0 && a->K > 0 && a->N > 0 && a->R > 0 && a->A > 0 && a->requests >= 0);
+    NB_REQUIRE(a->dtype == NB_DTYPE_BF16 || a->dtype == NB_DTYPE_FP16);
+    if (a->R % 16 || a->R > NB_LORA_MAX_RANK) return fail_with(NB_ERR_UNSUPPORTED, "the rank must be a multiple of 16 up to NB_LORA_MAX_RANK");
+    if (a->K % 8 || a->N % 8) return fail_with(NB_ERR_UNSUPPORTED, "K and N must be multiples of 8");
+    if (a->T > (1 << 30) || a->requests > 65535 || a->A > 65535 || item_count(a->T, a->requests, kRows) > 65535 || a->K > (1 << 24) || a->N > (1 << 24))
+        return fail_with(NB_ERR_TOO_LARGE, "rows / 64 + requests or adapters above 65535, or more than 2^24 columns");
+    if (a->T == 0) return NB_OK;
+    NB_REQUIRE(a->offsets && (a->adapters || a->requests == 0) && a->down && a->up && aligned16(a->down) && aligned16(a->up));
+    return NB_OK;
+}
+
+}  // namespace
+}  // namespace nb
+
+extern "C" int64_t nb_lora_workspace_bytes(const nb_lora_args* a) {
+    using namespace nb;
+    if (check(a) != NB_OK || a->T == 0) return 0;
+    int64_t most = 0;
+    for (int cols : {a->dup ? a->N : 0, a->ddown ? a->K : 0}) {
+        if (!cols) continue;
+        const int64_t n = (int64_t)item_count(a->T, a->requests, outer_rows(a->T, cols)) * a->R * cols * 4;
+        if (n > most) most = n;
+    }
+    return most ? ((int64_t)item_count(a->T, a->requests, 128) * 4 + 255) / 256 * 256 + most : 0;
+}
+
+extern "C" int nb_lora_forward(const nb_lora_args* a, void* stream) {
+    using namespace nb;
+    if (int rc = check(a)) return rc;
+    if (a->T == 0) return NB_OK;
+    NB_REQUIRE(a->x && a->out && a->h && aligned16(a->x) && aligned16(a->out) && aligned16(a->h) && aligned16(a->base));
+    NB_REQUIRE(a->stride_x % 8 == 0 && a->stride_out % 8 == 0 && (!a->base || a->stride_base % 8 == 0));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return a->dtype == NB_DTYPE_BF16 ? dispatch<__nv_bfloat16>(a, false, s) : dispatch<__half>(a, false, s);
+}
+
+extern "C" int nb_lora_backward(const nb_lora_args* a, void* stream) {
+    using namespace nb;
+    if (int rc = check(a)) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->T == 0) {  // empty sums
+        if (a->ddown) NB_CUDA_CHECK(cudaMemsetAsync(a->ddown, 0, (size_t)a->A * a->R * a->K * 2, s));
+        if (a->dup) NB_CUDA_CHECK(cudaMemsetAsync(a->dup, 0, (size_t)a->A * a->R * a->N * 2, s));
+        return NB_OK;
+    }
+    if (!a->dx && !a->ddown && !a->dup) return NB_OK;
+    NB_REQUIRE(a->dy && aligned16(a->dy) && a->stride_dy % 8 == 0);
+    NB_REQUIRE(!(a->dx || a->ddown) || (a->g && aligned16(a->g)));
+    NB_REQUIRE(!a->ddown || (a->x && aligned16(a->x) && a->stride_x % 8 == 0 && aligned16(a->ddown)));
+    NB_REQUIRE(!a->dup || (a->h && aligned16(a->h) && aligned16(a->dup)));
+    NB_REQUIRE(aligned16(a->dx));
+    if (a->dup || a->ddown) {
+        NB_REQUIRE(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 255) == 0);
+        if (a->workspace_bytes < nb_lora_workspace_bytes(a)) return fail_with(NB_ERR_INVALID, "workspace smaller than nb_lora_workspace_bytes()");
+    }
+    return a->dtype == NB_DTYPE_BF16 ? dispatch<__nv_bfloat16>(a, true, s) : dispatch<__half>(a, true, s);
+}

@@ -1,0 +1,163 @@
+"""
+Low-rank adapters of many requests at once beside a shared projection (``csrc/lora.cu``).
+
+The reference serves one LoRA set at a time (nunchaku/lora/runtime.py:475-535: the factors become part of the layer).  Here
+every request of a batch names its own adapter, and the projection's output gets each row's ``scale (x D^T) U^T``.
+:mod:`nunchaku_rocm_b200.lora` attaches stacks of adapters to layers; this is the operator under it.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib as L
+from .elementwise import _strided_rows
+
+__all__ = ["lora_batched"]
+
+
+def _aligned_rows(t: torch.Tensor):
+    """``t (..., C)`` with rows evenly strided on 16-byte boundaries, and their stride (a copy only if they are not)."""
+    t, stride = _strided_rows(t)
+    if stride % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        stride = t.shape[-1]
+    return t, stride
+
+
+def _args(T, K, N, down, up, offsets, adapters, scale):
+    a = L.LoraArgs()
+    a.down, a.up = down.data_ptr(), up.data_ptr()
+    a.offsets, a.adapters = offsets.data_ptr(), adapters.data_ptr()
+    if scale is not None:
+        a.scale = scale.data_ptr()
+    a.T, a.K, a.N, a.R, a.A = T, K, N, down.shape[1], down.shape[0]
+    a.requests, a.dtype = adapters.shape[0], L.DTYPE_CODE[down.dtype]
+    return a
+
+
+def _forward(x, base, down, up, offsets, adapters, scale, out):
+    """``out`` and the two 16-bit parts of ``scale x down^T``; the arguments are checked already."""
+    K, N = down.shape[2], up.shape[1]
+    T = x.numel() // K
+    h = torch.empty(2, T, down.shape[1], dtype=x.dtype, device=x.device)
+    if T == 0:
+        return h
+    x, stride_x = _aligned_rows(x)
+    a = _args(T, K, N, down, up, offsets, adapters, scale)
+    a.x, a.stride_x = x.data_ptr(), stride_x
+    if base is not None:
+        base, a.stride_base = _aligned_rows(base)
+        a.base = base.data_ptr()
+    a.out, a.stride_out = out.data_ptr(), _strided_rows(out)[1]
+    a.h = h.data_ptr()
+    with L.on_device(x.device):
+        L.check(L.lib().nb_lora_forward(a, L.stream_of(x)), "lora_batched")
+    return h
+
+
+class _LoraBatched(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, base, down, up, offsets, adapters, scale):
+        out = torch.empty(*x.shape[:-1], up.shape[1], dtype=x.dtype, device=x.device)
+        h = _forward(x, base, down, up, offsets, adapters, scale, out)
+        need = ctx.needs_input_grad
+        ctx.save_for_backward(x if need[2] else None, down, up, h if need[3] else None, offsets, adapters, scale)
+        ctx.x_shape = x.shape
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, down, up, h, offsets, adapters, scale = ctx.saved_tensors
+        need_x, need_base, need_down, need_up = ctx.needs_input_grad[:4]
+        new = lambda shape: torch.empty(shape, dtype=down.dtype, device=down.device)  # noqa: E731
+        dx = new(ctx.x_shape) if need_x else None
+        ddown = new(down.shape) if need_down else None
+        dup = new(up.shape) if need_up else None
+        K, N = down.shape[2], up.shape[1]
+        T = dy.numel() // N
+        if T == 0:
+            for t in (ddown, dup):
+                if t is not None:
+                    t.zero_()
+        elif need_x or need_down or need_up:
+            rows, stride_dy = _aligned_rows(dy)
+            a = _args(T, K, N, down, up, offsets, adapters, scale)
+            a.dy, a.stride_dy = rows.data_ptr(), stride_dy
+            if need_x:
+                a.dx = dx.data_ptr()
+            if need_down:
+                x, a.stride_x = _aligned_rows(x)
+                a.x, a.ddown = x.data_ptr(), ddown.data_ptr()
+            if need_x or need_down:
+                g = new((2, T, down.shape[1]))
+                a.g = g.data_ptr()
+            if need_up:
+                a.h, a.dup = h.data_ptr(), dup.data_ptr()
+            lib = L.lib()
+            with L.on_device(down.device):
+                n = lib.nb_lora_workspace_bytes(a)
+                if n:
+                    ws = torch.empty(n, dtype=torch.uint8, device=down.device)
+                    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+                L.check(lib.nb_lora_backward(a, L.stream_of(down)), "lora_batched backward")
+        return dx, (dy if need_base else None), ddown, dup, None, None, None
+
+
+def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor, adapters: torch.Tensor,
+                 base: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """
+    ``out[t] = base[t] + scale[a] * (x[t] @ down[a]^T) @ up[a]^T`` with ``a`` the adapter of row ``t``'s request.
+
+    ``x (..., K)`` and ``base (..., N)`` (zeros when ``None``) are taken as rows, bfloat16 or float16.  Request ``i`` has the
+    rows ``offsets[i] .. offsets[i + 1] - 1`` (``offsets (requests + 1,)`` int32, not going down, zero-length requests
+    allowed) and uses adapter ``adapters[i]`` (int32); a value outside ``0 .. A - 1``, -1 by convention, is no adapter.
+    Rows outside every request have none either: ``out`` is ``base`` there.  Both index tensors stay on the device, so they
+    may change between replays of a captured graph (as many requests as at capture).
+
+    ``down (A, R, K)`` and ``up (A, N, R)`` are contiguous stacks of adapters (``R`` a multiple of 16 up to 128, ``K`` and
+    ``N`` multiples of 8; smaller ranks are padded with zeros, see :func:`nunchaku_rocm_b200.lora.stack_loras`); ``scale
+    (A,)`` is float32.  ``out`` may be given where no gradient is asked for, and may be ``base``.
+
+    Differentiable in ``x``, ``base``, ``down`` and ``up`` (not in ``scale``); gradients of adapters that several requests
+    share are summed in a fixed order.
+    """
+    if x.dtype not in L.DTYPE_CODE or any(t is not None and t.dtype != x.dtype for t in (down, up, base, out)):
+        raise ValueError("x, base, down, up and out must share one dtype, bfloat16 or float16")
+    if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2] or down.shape[0] == 0:
+        raise ValueError(f"down must be (A, R, K) and up (A, N, R); got {tuple(down.shape)} and {tuple(up.shape)}")
+    A, R, K = down.shape
+    N = up.shape[1]
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError(f"x must be (..., {K}), got {tuple(x.shape)}")
+    for name, t in (("base", base), ("out", out)):
+        if t is not None and t.shape != (*x.shape[:-1], N):
+            raise ValueError(f"{name} must be {(*x.shape[:-1], N)}, got {tuple(t.shape)}")
+    if R == 0 or R % 16 or R > L.LORA_MAX_RANK or K == 0 or K % 8 or N == 0 or N % 8:
+        raise NotImplementedError(f"rank {R} must be a multiple of 16 up to {L.LORA_MAX_RANK}, K={K} and N={N} multiples of 8")
+    for name, t in (("offsets", offsets), ("adapters", adapters)):
+        if t.dtype != torch.int32 or t.dim() != 1:
+            raise ValueError(f"{name} must be a 1-D int32 tensor, got {tuple(t.shape)} {t.dtype}")
+    if offsets.shape[0] != adapters.shape[0] + 1:
+        raise ValueError(f"{adapters.shape[0]} adapters need {adapters.shape[0] + 1} offsets, got {offsets.shape[0]}")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (A,)):
+        raise ValueError(f"scale must be ({A},) float32, got {tuple(scale.shape)} {scale.dtype}")
+    grad = torch.is_grad_enabled()
+    if grad and scale is not None and scale.requires_grad:
+        raise ValueError("lora_batched has no gradient for scale")
+    if out is not None:
+        if out.stride(-1) != 1 or out.data_ptr() % 16 or (out.numel() and _strided_rows(out)[0] is not out) or _strided_rows(out)[1] % 8:
+            raise ValueError("out must have evenly strided rows on 16-byte boundaries")
+    L.require_cuda(x, down, up, offsets, adapters, base, scale, out)
+    down, up, offsets, adapters = down.contiguous(), up.contiguous(), offsets.contiguous(), adapters.contiguous()
+    scale = None if scale is None else scale.contiguous()
+    if grad and any(t is not None and t.requires_grad for t in (x, base, down, up)):
+        if out is not None:
+            raise ValueError("out cannot be given where a gradient is asked for")
+        return _LoraBatched.apply(x, base, down, up, offsets, adapters, scale)
+    if out is None:
+        out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    _forward(x, base, down, up, offsets, adapters, scale, out)
+    return out
