@@ -9,7 +9,6 @@ There is no fallback: a missing library or a non-zero status raises.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 import threading
@@ -232,13 +231,28 @@ def stream_of(t: torch.Tensor) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-_here = contextlib.nullcontext()
+def launch(fn, what: str, like: torch.Tensor, *args) -> None:
+    """``fn(*args, stream)`` on ``like``'s device and that device's current stream; raises for a non-zero status.  The small
+    calls are bound by the host, so the device is entered only where it is not the current one already."""
+    i = like.get_device()
+    if i == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if status:
+        check(status, what)
 
 
-def on_device(dev: torch.device):
-    """``torch.cuda.device(dev)``, or nothing to enter where it is the current device already (the common case, and
-    entering costs more than a small launch)."""
-    return _here if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def once_differentiable(backward):
+    """A ``backward`` whose results have no graph of their own: as ``torch.autograd.function.once_differentiable`` where the
+    caller asked for a graph, at no cost where not."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 _selftested: set[int] = set()

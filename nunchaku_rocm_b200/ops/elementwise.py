@@ -152,7 +152,7 @@ def _ln_prepare(x, weight, bias, weight_add):
 
 
 def _ln_forward(x, weight, bias, eps, weight_add, y, stats):
-    """``y`` and / or the rows' (mean, rstd) into the given tensors; the arguments are prepared already."""
+    """``y`` and / or the rows' (mean, rstd) into the given tensors; the arguments are checked already."""
     if x.numel() == 0:
         return
     x, stride_x = _strided_rows(x)
@@ -161,52 +161,50 @@ def _ln_forward(x, weight, bias, eps, weight_add, y, stats):
         a.y = y.data_ptr()
     if stats is not None:
         a.mean = stats.data_ptr()
-        a.rstd = a.mean + 4 * (stats.numel() // 2)
-    with L.on_device(x.device):
-        L.check(L.lib().nb_layer_norm(a, L.stream_of(x)), "layer_norm")
+        a.rstd = a.mean + 2 * stats.numel()
+    L.launch(L.lib().nb_layer_norm, "layer_norm", x, a)
 
 
 def _ln_backward(x, weight, bias, stats, dy, eps, weight_add, need):
     """(dx, dweight, dbias), ``None`` where ``need`` says so."""
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if need[1] else None
-    db = torch.empty(bias.shape, dtype=bias.dtype, device=x.device) if need[2] else None
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = weight.new_empty(weight.shape) if need[1] else None
+    db = bias.new_empty(bias.shape) if need[2] else None
     if x.numel() == 0:
         return dx, (dw.zero_() if need[1] else None), (db.zero_() if need[2] else None)
     x, stride_x = _strided_rows(x)
     dy, stride_dy = _strided_rows(dy)
     a = _ln_args(x, stride_x, weight, bias, eps, weight_add)
     a.mean = stats.data_ptr()
-    a.rstd = a.mean + 4 * (stats.numel() // 2)
+    a.rstd = a.mean + 2 * stats.numel()
     a.dy, a.stride_dy = dy.data_ptr(), stride_dy
     if need[0]:
         a.dx = dx.data_ptr()
     lib = L.lib()
-    with L.on_device(x.device):
-        if need[1] or need[2]:
-            n = lib.nb_layer_norm_workspace_bytes(a.groups, a.rows, a.dim, a.dtype)
-            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), n
-            if need[1]:
-                a.dw = dw.data_ptr()
-            if need[2]:
-                a.db = db.data_ptr()
-        L.check(lib.nb_layer_norm_backward(a, L.stream_of(x)), "layer_norm backward")
+    if need[1] or need[2]:
+        n = lib.nb_layer_norm_workspace_bytes(a.groups, a.rows, a.dim, a.dtype)
+        ws = stats.new_empty(n // 4)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+        if need[1]:
+            a.dw = dw.data_ptr()
+        if need[2]:
+            a.db = db.data_ptr()
+    L.launch(lib.nb_layer_norm_backward, "layer_norm backward", x, a)
     return dx, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, weight_add):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty(2, x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        y = x.new_empty(x.shape)
+        stats = x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
         _ln_forward(x, weight, bias, eps, weight_add, y, stats)
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.consts = eps, weight_add
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
         return (*_ln_backward(x, weight, bias, stats, dy, *ctx.consts, ctx.needs_input_grad), None, None)
@@ -222,12 +220,12 @@ class _LayerNormModulate(torch.autograd.Function):
         return _layernorm_modulate(x, scale, shift, scale_add, eps)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.once_differentiable
     def backward(ctx, dy):
         eps, scale_add = ctx.consts
         x, scale, shift = ctx.saved_tensors
         scale, shift = _ln_prepare(x, scale, shift, scale_add)
-        stats = torch.empty(2, x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        stats = x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
         _ln_forward(x, None, None, eps, 0.0, None, stats)
         return (*_ln_backward(x, scale, shift, stats, dy, eps, scale_add, ctx.needs_input_grad), None, None)
 
@@ -243,11 +241,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     are summed over the rows in fp32, in a fixed order.  ``D`` is at most 16384.
     """
     weight, bias = _ln_prepare(x, weight, bias, weight_add)
-    dev = L.require_cuda(x, weight, bias)
+    L.require_cuda(x, weight, bias)
     grad = torch.is_grad_enabled() and (
         x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
     if grad:
         return _LayerNorm.apply(x, weight, bias, eps, weight_add)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = x.new_empty(x.shape)
     _ln_forward(x, weight, bias, eps, weight_add, y, None)
     return y

@@ -40,7 +40,7 @@ def _forward(x, base, down, up, offsets, adapters, scale, out):
     """``out`` and the two 16-bit parts of ``scale x down^T``; the arguments are checked already."""
     K, N = down.shape[2], up.shape[1]
     T = x.numel() // K
-    h = torch.empty(2, T, down.shape[1], dtype=x.dtype, device=x.device)
+    h = x.new_empty((2, T, down.shape[1]))
     if T == 0:
         return h
     x, stride_x = _aligned_rows(x)
@@ -51,15 +51,14 @@ def _forward(x, base, down, up, offsets, adapters, scale, out):
         a.base = base.data_ptr()
     a.out, a.stride_out = out.data_ptr(), _strided_rows(out)[1]
     a.h = h.data_ptr()
-    with L.on_device(x.device):
-        L.check(L.lib().nb_lora_forward(a, L.stream_of(x)), "lora_batched")
+    L.launch(L.lib().nb_lora_forward, "lora_batched", x, a)
     return h
 
 
 class _LoraBatched(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, base, down, up, offsets, adapters, scale):
-        out = torch.empty(*x.shape[:-1], up.shape[1], dtype=x.dtype, device=x.device)
+        out = x.new_empty((*x.shape[:-1], up.shape[1]))
         h = _forward(x, base, down, up, offsets, adapters, scale, out)
         need = ctx.needs_input_grad
         ctx.save_for_backward(x if need[2] else None, down, up, h if need[3] else None, offsets, adapters, scale)
@@ -67,11 +66,11 @@ class _LoraBatched(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.once_differentiable
     def backward(ctx, dy):
         x, down, up, h, offsets, adapters, scale = ctx.saved_tensors
         need_x, need_base, need_down, need_up = ctx.needs_input_grad[:4]
-        new = lambda shape: torch.empty(shape, dtype=down.dtype, device=down.device)  # noqa: E731
+        new = down.new_empty
         dx = new(ctx.x_shape) if need_x else None
         ddown = new(down.shape) if need_down else None
         dup = new(up.shape) if need_up else None
@@ -96,12 +95,11 @@ class _LoraBatched(torch.autograd.Function):
             if need_up:
                 a.h, a.dup = h.data_ptr(), dup.data_ptr()
             lib = L.lib()
-            with L.on_device(down.device):
-                n = lib.nb_lora_workspace_bytes(a)
-                if n:
-                    ws = torch.empty(n, dtype=torch.uint8, device=down.device)
-                    a.workspace, a.workspace_bytes = ws.data_ptr(), n
-                L.check(lib.nb_lora_backward(a, L.stream_of(down)), "lora_batched backward")
+            n = lib.nb_lora_workspace_bytes(a) if need_down or need_up else 0
+            if n:
+                ws = new((n + 1) // 2)
+                a.workspace, a.workspace_bytes = ws.data_ptr(), n
+            L.launch(lib.nb_lora_backward, "lora_batched backward", down, a)
         return dx, (dy if need_base else None), ddown, dup, None, None, None
 
 
@@ -124,7 +122,9 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     Differentiable in ``x``, ``base``, ``down`` and ``up`` (not in ``scale``); gradients of adapters that several requests
     share are summed in a fixed order.
     """
-    if x.dtype not in L.DTYPE_CODE or any(t is not None and t.dtype != x.dtype for t in (down, up, base, out)):
+    dt = x.dtype
+    if (dt not in L.DTYPE_CODE or down.dtype != dt or up.dtype != dt or (base is not None and base.dtype != dt)
+            or (out is not None and out.dtype != dt)):
         raise ValueError("x, base, down, up and out must share one dtype, bfloat16 or float16")
     if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2] or down.shape[0] == 0:
         raise ValueError(f"down must be (A, R, K) and up (A, N, R); got {tuple(down.shape)} and {tuple(up.shape)}")
@@ -132,14 +132,14 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     N = up.shape[1]
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"x must be (..., {K}), got {tuple(x.shape)}")
+    out_shape = (*x.shape[:-1], N)
     for name, t in (("base", base), ("out", out)):
-        if t is not None and t.shape != (*x.shape[:-1], N):
-            raise ValueError(f"{name} must be {(*x.shape[:-1], N)}, got {tuple(t.shape)}")
+        if t is not None and t.shape != out_shape:
+            raise ValueError(f"{name} must be {out_shape}, got {tuple(t.shape)}")
     if R == 0 or R % 16 or R > L.LORA_MAX_RANK or K == 0 or K % 8 or N == 0 or N % 8:
         raise NotImplementedError(f"rank {R} must be a multiple of 16 up to {L.LORA_MAX_RANK}, K={K} and N={N} multiples of 8")
-    for name, t in (("offsets", offsets), ("adapters", adapters)):
-        if t.dtype != torch.int32 or t.dim() != 1:
-            raise ValueError(f"{name} must be a 1-D int32 tensor, got {tuple(t.shape)} {t.dtype}")
+    if offsets.dtype != torch.int32 or adapters.dtype != torch.int32 or offsets.dim() != 1 or adapters.dim() != 1:
+        raise ValueError("offsets and adapters must be 1-D int32 tensors")
     if offsets.shape[0] != adapters.shape[0] + 1:
         raise ValueError(f"{adapters.shape[0]} adapters need {adapters.shape[0] + 1} offsets, got {offsets.shape[0]}")
     if scale is not None and (scale.dtype != torch.float32 or scale.shape != (A,)):
@@ -148,16 +148,17 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     if grad and scale is not None and scale.requires_grad:
         raise ValueError("lora_batched has no gradient for scale")
     if out is not None:
-        if out.stride(-1) != 1 or out.data_ptr() % 16 or (out.numel() and _strided_rows(out)[0] is not out) or _strided_rows(out)[1] % 8:
+        rows, stride = _strided_rows(out)
+        if rows is not out or stride % 8 or out.data_ptr() % 16:
             raise ValueError("out must have evenly strided rows on 16-byte boundaries")
     L.require_cuda(x, down, up, offsets, adapters, base, scale, out)
     down, up, offsets, adapters = down.contiguous(), up.contiguous(), offsets.contiguous(), adapters.contiguous()
     scale = None if scale is None else scale.contiguous()
-    if grad and any(t is not None and t.requires_grad for t in (x, base, down, up)):
+    if grad and (x.requires_grad or down.requires_grad or up.requires_grad or (base is not None and base.requires_grad)):
         if out is not None:
             raise ValueError("out cannot be given where a gradient is asked for")
         return _LoraBatched.apply(x, base, down, up, offsets, adapters, scale)
     if out is None:
-        out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+        out = x.new_empty((*x.shape[:-1], N))
     _forward(x, base, down, up, offsets, adapters, scale, out)
     return out

@@ -46,8 +46,8 @@ def _rotate(q, k, ids, ladder, half, inverse):
     if k is not None and k.stride(3) != 1:
         k = k.contiguous()
     B, S, H, D = q.shape
-    qo = torch.empty((B, S, H, D), dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    qo = q.new_empty(q.shape)
+    ko = None if k is None else q.new_empty(k.shape)
     a = L.RotaryArgs()
     a.q, a.q_out, a.ids = q.data_ptr(), qo.data_ptr(), ids.data_ptr()
     a.stride_qb, a.stride_qs, a.stride_qh, _ = q.stride()
@@ -58,8 +58,7 @@ def _rotate(q, k, ids, ladder, half, inverse):
     a.stride_ib, a.stride_is, a.stride_ia = _ids_strides(ids, ladder.n_axes, B, S)
     a.dtype, a.ids_type = L.DTYPE_CODE_32[q.dtype], L.IDS_CODE[ids.dtype]
     a.half, a.inverse = half, inverse
-    with L.on_device(q.device):
-        L.check(L.lib().nb_rotary_axes(a, ladder, L.stream_of(q)), "rotary_axes")
+    L.launch(L.lib().nb_rotary_axes, "rotary_axes", q, a, ladder)
     return qo, ko
 
 
@@ -72,7 +71,7 @@ class _RotaryAxes(torch.autograd.Function):
         return _rotate(q, k, ids, ladder, half, inverse)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.once_differentiable
     def backward(ctx, dq, dk):
         (ids,) = ctx.saved_tensors
         ladder, half, inverse = ctx.consts
@@ -133,10 +132,6 @@ def rotary_table(ids: torch.Tensor, axes_dim, theta: float = 10000.0) -> torch.T
     st = _ids_strides(ids, ladder.n_axes, B, S)
     pairs = ladder.pair_end[ladder.n_axes - 1]
     L.require_cuda(ids)
-    out = torch.empty((*ids.shape[:-1], pairs, 1, 2), dtype=torch.float32, device=ids.device)
-    with L.on_device(ids.device):
-        L.check(
-            L.lib().nb_rotary_table(ids.data_ptr(), L.IDS_CODE[ids.dtype], B, S, *st, out.data_ptr(), ladder, L.stream_of(out)),
-            "rotary_table",
-        )
+    out = ids.new_empty((*ids.shape[:-1], pairs, 1, 2), dtype=torch.float32)
+    L.launch(L.lib().nb_rotary_table, "rotary_table", out, ids.data_ptr(), L.IDS_CODE[ids.dtype], B, S, *st, out.data_ptr(), ladder)
     return out
