@@ -401,10 +401,10 @@ struct Ring {
     __device__ __forceinline__ uint32_t at(int i, int which, int u, int k, int t, int team) const {
         return base + (i % ST) * slot + which * half + ((k * U + u) * team + t) * 16;
     }
-    __device__ __forceinline__ void fill(int i, int which, const T* row, const bool (&on)[U], int t, int team) const {
+    __device__ __forceinline__ void fill(int i, int which, const T* row, bool last, int t, int team) const {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (!on[u]) continue;
+            if (u == U - 1 && !last) continue;
             const T* src = row + col<true>(u, 0, t, team);
 #pragma unroll
             for (int k = 0; k < PIECES; ++k)
@@ -438,18 +438,14 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
     const long long first = (long long)blockIdx.y * p.rows;
     if (row0 >= p.rows) return;  // a whole team
     const Ring<T, U, ST, false> ring(smem, team);
-    bool on[U];
-    float count = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        on[u] = col<true>(u, 0, t, team) < p.dim;
-        count += on[u] ? 8.f : 0.f;
-    }
+    // all groups but the last are whole: a team of U > 1 groups has at most dim / 8 / (U - 1) threads
+    const bool last = col<true>(U - 1, 0, t, team) < p.dim;
+    const float count = 8.f * (U - 1) + (last ? 8.f : 0.f);
     const int mine = (p.rows - row0 + step - 1) / step;  // rows of this team
     const T* next = static_cast<const T*>(p.x) + (first + row0) * p.stride_x;
     const long long ahead = step * p.stride_x, along = (long long)step * p.dim;
     auto fill = [&](int i) {
-        if (i < mine) ring.fill(i, 0, next, on, t, team);
+        if (i < mine) ring.fill(i, 0, next, last, t, team);
         next += ahead;
         commit();
     };
@@ -459,7 +455,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
     Eight w[U], b[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if (!on[u]) continue;
+        if (u == U - 1 && !last) continue;
         w[u] = get_pairs<W>(p.w, blockIdx.y * p.stride_w, col<true>(u, 0, t, team), 1.f, p.add);
         b[u] = get_pairs<W>(p.b, blockIdx.y * p.stride_w, col<true>(u, 0, t, team), 0.f, 0.f);
     }
@@ -483,7 +479,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
             uint64_t a = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (!on[u]) continue;
+                if (u == U - 1 && !last) continue;
                 d[u] = ring.read(i + r, 0, u, t, team);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) a = add_f32x2(a, d[u].v[k]);
@@ -494,7 +490,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
             a = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (!on[u]) continue;
+                if (u == U - 1 && !last) continue;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint64_t off = add_f32x2(d[u].v[k], m);
@@ -546,13 +542,13 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
             if (t == 0 && p.mean) p.mean[first + row0 + (i + r) * step] = mean[r];
             if (t == 0 && p.rstd) p.rstd[first + row0 + (i + r) * step] = rstd[r];
             if (!p.y) continue;
-            const uint64_t scale = both(rstd[r]), off = both(-mean[r]);
+            const uint64_t scale = both(rstd[r]), off = both(-mean[r] * rstd[r]);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (!on[u]) continue;
+                if (u == U - 1 && !last) continue;
                 Eight o = ring.read(i + r, 0, u, t, team);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o.v[k] = fma_f32x2(mul_f32x2(add_f32x2(o.v[k], off), scale), w[u].v[k], b[u].v[k]);
+                for (int k = 0; k < 4; ++k) o.v[k] = fma_f32x2(fma_f32x2(o.v[k], scale, off), w[u].v[k], b[u].v[k]);
                 put_pairs<T>(y + col<true>(u, 0, t, team), o);
             }
             y += along;
@@ -573,17 +569,15 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
     const int step = gridDim.x * blockDim.y, row0 = blockIdx.x * blockDim.y + threadIdx.y;
     const long long first = (long long)blockIdx.y * p.rows;
     const Ring<T, U, ST, true> ring(smem, team);
-    bool on[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) on[u] = col<true>(u, 0, t, team) < p.dim;
+    const bool last = col<true>(U - 1, 0, t, team) < p.dim;  // (all groups before it are whole)
     const int mine = row0 < p.rows ? (p.rows - row0 + step - 1) / step : 0;  // rows of this team
     const T* next_x = static_cast<const T*>(p.x) + (first + row0) * p.stride_x;
     const T* next_dy = static_cast<const T*>(p.dy) + (first + row0) * p.stride_dy;
     const long long ahead_x = step * p.stride_x, ahead_dy = step * p.stride_dy, along = (long long)step * p.dim;
     auto fill = [&](int i) {
         if (i < mine) {
-            ring.fill(i, 0, next_x, on, t, team);
-            ring.fill(i, 1, next_dy, on, t, team);
+            ring.fill(i, 0, next_x, last, t, team);
+            ring.fill(i, 1, next_dy, last, t, team);
         }
         next_x += ahead_x;
         next_dy += ahead_dy;
@@ -597,7 +591,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
     for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) dw[u].v[k] = db[u].v[k] = 0;
-        if (on[u]) w[u] = get_pairs<W>(p.w, blockIdx.y * p.stride_w, col<true>(u, 0, t, team), 1.f, p.add);
+        if (u < U - 1 || last) w[u] = get_pairs<W>(p.w, blockIdx.y * p.stride_w, col<true>(u, 0, t, team), 1.f, p.add);
     }
     const float per_row = 1.f / (float)p.dim;
     float nm[RB], nr[RB];
@@ -618,15 +612,15 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
             s[2 * r] = s[2 * r + 1] = 0.f;
             mean[r] = nm[r], rstd[r] = nr[r];
             if (i + r >= mine) continue;  // (its slot holds an older row)
-            const uint64_t scale = both(nr[r]), off = both(-nm[r]);
+            const uint64_t scale = both(nr[r]), off = both(-nm[r] * nr[r]);
             uint64_t a0 = 0, a1 = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (!on[u]) continue;
+                if (u == U - 1 && !last) continue;
                 const Eight xv = ring.read(i + r, 0, u, t, team), dv = ring.read(i + r, 1, u, t, team);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint64_t h = mul_f32x2(add_f32x2(xv.v[k], off), scale), g = dv.v[k];
+                    const uint64_t h = fma_f32x2(xv.v[k], scale, off), g = dv.v[k];
                     if constexpr (SUMS) {
                         dw[u].v[k] = fma_f32x2(g, h, dw[u].v[k]);
                         db[u].v[k] = add_f32x2(g, db[u].v[k]);
@@ -660,17 +654,16 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
             if (i + r >= mine || !p.dx) continue;
-            const uint64_t scale = both(rstd[r]), off = both(-mean[r]), c0 = both(-m[2 * r]), c1 = both(-m[2 * r + 1]);
+            // v - mean(v) - xh mean(v xh) as a line in x beside v
+            const float slope = -rstd[r] * m[2 * r + 1];
+            const uint64_t scale = both(rstd[r]), c1 = both(slope), c0 = both(fmaf(-mean[r], slope, -m[2 * r]));
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (!on[u]) continue;
+                if (u == U - 1 && !last) continue;
                 const Eight xv = ring.read(i + r, 0, u, t, team);
                 Eight o = ring.read(i + r, 1, u, t, team);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint64_t h = mul_f32x2(add_f32x2(xv.v[k], off), scale);
-                    o.v[k] = mul_f32x2(fma_f32x2(h, c1, fma_f32x2(o.v[k], w[u].v[k], c0)), scale);
-                }
+                for (int k = 0; k < 4; ++k) o.v[k] = mul_f32x2(fma_f32x2(o.v[k], w[u].v[k], fma_f32x2(xv.v[k], c1, c0)), scale);
                 put_pairs<T>(dx + col<true>(u, 0, t, team), o);
             }
             dx += along;
@@ -690,6 +683,9 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
                 fw[u][2 * k] = a.x; fw[u][2 * k + 1] = a.y;
                 fb[u][2 * k] = c.x; fb[u][2 * k + 1] = c.y;
             }
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) on[u] = u < U - 1 || last;
         leave_sums<U, true>(p, fw, fb, on, reinterpret_cast<float*>(smem));
     }
 }
