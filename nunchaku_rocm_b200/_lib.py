@@ -101,7 +101,8 @@ class LoraArgs(C.Structure):
         ]
         + [("workspace_bytes", C.c_int64)]
         + [(n, C.c_int64) for n in ("stride_x", "stride_base", "stride_out", "stride_dy")]
-        + [(n, C.c_int32) for n in ("T", "K", "N", "R", "A", "requests", "dtype")]
+        + [(n, C.c_int32) for n in ("T", "K", "N", "R", "A", "requests", "dtype", "impl")]
+        + [("status", C.c_void_p)]
     )
 
 

@@ -22,28 +22,16 @@
 // Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out).
 #include <cooperative_groups.h>
 
-#include "nb_common.cuh"
+#include "lora.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace nb {
+namespace lora {
 namespace {
 
 constexpr int kThreads = 128;
 constexpr int kRows = 64;  // rows of an item (shrink, expand)
-
-struct LoraParams {
-    const void* x;        // shrink: (T, K) operand; expand: base (T, C) or null; outer: (T, K) operand
-    void* out;            // expand: (T, C)
-    const void* factor;   // shrink: (A, R, K) or (A, K, R); expand: (A, C, R) or (A, R, C)
-    void* hi; void* lo;   // (T, R) each
-    float* part;          // outer: (items, R, K) or (items, K, R)
-    int* item_adapter;    // outer: (items)
-    const int* offsets; const int* adapters; const float* scale;
-    long long stride_x, stride_out;
-    int T, K, R, A, requests;  // K: length of the contraction (shrink), columns (expand, outer)
-    int rows_per_item, cols_per_cta;
-};
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -71,43 +59,6 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-struct Item {
-    int first, rows, adapter;  // rows 0: nothing to do; adapter -1: rows without one
-};
-__host__ __device__ inline int item_count(int T, int requests, int bm) { return (T + bm - 1) / bm + requests + 1; }
-
-// The `w`-th interval of the merged borders (tile borders before equal offsets).  All threads of the CTA call it.
-__device__ __forceinline__ Item find_item(const LoraParams& p, int w) {
-    const int bm = p.rows_per_item, tiles = (p.T + bm - 1) / bm;
-    auto offset = [&](int j) { return min(max(__ldg(p.offsets + j), 0), p.T); };
-    int before = 0;  // offsets among the first w borders
-    for (int j0 = 0; j0 <= p.requests; j0 += kThreads) {
-        const int j = j0 + (int)threadIdx.x;
-        before += __syncthreads_count(j <= p.requests && j + min(offset(j) / bm + 1, tiles) < w);
-    }
-    int i = w - before, j = before;
-    Item it = {0, 0, -1};
-    const int tile = i < tiles ? i * bm : p.T, off = j <= p.requests ? offset(j) : p.T;
-    int next_tile = tile, next_off = off;
-    if (i < 0) return it;  // (offsets that go down)
-    if (i < tiles && tile <= off) {
-        it.first = tile;
-        next_tile = i + 1 < tiles ? (i + 1) * bm : p.T;
-    } else if (j <= p.requests) {
-        it.first = off;
-        ++j;
-        next_off = j <= p.requests ? offset(j) : p.T;
-    } else {
-        return it;
-    }
-    it.rows = min(max(min(next_tile, next_off) - it.first, 0), bm);
-    if (it.rows && j >= 1 && j <= p.requests) {
-        const int a = __ldg(p.adapters + j - 1);
-        it.adapter = a >= 0 && a < p.A ? a : -1;
-    }
-    return it;
-}
-
 // ------------------------------------------------------------------------------------------------------------------ shrink
 // v[t, r] = s_a sum_k X[t, k] F_a[r, k], written as hi + lo.  A CTA has one item and one slice of K; the slices of an item
 // are a cluster, whose sums meet in shared memory (in a fixed order), so a few rows of a long K still use many SMs and no
@@ -126,7 +77,7 @@ template <typename T, int RM, bool RCONTIG>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraParams p) {
     using S = ShrinkTile<RM, RCONTIG>;
     extern __shared__ __align__(128) unsigned char smem[];
-    const Item it = find_item(p, blockIdx.x);
+    const Item it = find_item<kThreads>(p, blockIdx.x);
     if (it.rows == 0 || it.adapter < 0) return;  // every CTA of the cluster
     const int splits = gridDim.y, split = blockIdx.y;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -257,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
     using S = ExpandTile<RM, CCONTIG>;
     constexpr int BN = S::BN;
     extern __shared__ __align__(128) unsigned char smem[];
-    const Item it = find_item(p, blockIdx.y);
+    const Item it = find_item<kThreads>(p, blockIdx.y);
     if (it.rows == 0) return;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int col0 = blockIdx.x * p.cols_per_cta, col1 = min(col0 + p.cols_per_cta, p.K);
@@ -393,7 +344,7 @@ __global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p
     extern __shared__ __align__(128) unsigned char smem[];
     // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
     const int w = gridDim.y - 1 - blockIdx.y;
-    const Item it = find_item(p, w);
+    const Item it = find_item<kThreads>(p, w);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     if (blockIdx.x == 0 && t == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
     if (it.rows == 0 || it.adapter < 0) return;
@@ -531,17 +482,25 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const float* part, const
 }
 
 // --------------------------------------------------------------------------------------------------------------- launchers
-int sms() {
-    const int n = nb_num_sms();
-    return n > 0 ? n : 148;
+// Whether a call runs on the tcgen05 kernels: their tiles are 128 rows, so the requests have to be that long on the whole.
+bool use_tc(const nb_lora_args* a) {
+    if (a->impl != NB_IMPL_AUTO) return a->impl == NB_IMPL_TCGEN05;
+    return a->T >= 512 && a->T >= 64ll * a->requests;
 }
-int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
-
+// A tcgen05 launch, or the mma.sync one where there is no tensor map for the operands (rows a stride of zero apart) and the
+// caller did not insist.
+#define NB_TC_OR(a, tc_call, call)                                                                             \
+    ([&]() -> int {                                                                                            \
+        if (!use_tc(a)) return call;                                                                           \
+        const int rc_ = tc_call;                                                                               \
+        return rc_ == NB_ERR_UNSUPPORTED && (a)->impl == NB_IMPL_AUTO ? call : rc_;                            \
+    }())
 // rows of the gradients' items: long enough that the partial products stay small beside the operands, short enough that the
-// CTAs (one per item and 128 columns) cover the SMs about four times
-int outer_rows(int T, int cols) {
-    const int tiles = ceil_div(cols, 128), want = ceil_div(4ll * sms(), tiles);
-    const int rows = ceil_div(ceil_div(T, want), 64) * 64;
+// CTAs (one per item and 128 columns) cover the SMs: twice with the tcgen05 kernels, about four times with the small ones
+int outer_rows(const nb_lora_args* a, int cols) {
+    const bool tc = use_tc(a);
+    const int tiles = ceil_div(cols, 128), want = ceil_div((tc ? 2ll : 4ll) * sms(), tiles);
+    const int rows = ceil_div(ceil_div(a->T, want), 64) * 64;
     return rows < 128 ? 128 : rows;
 }
 
@@ -592,14 +551,18 @@ int expand(LoraParams p, cudaStream_t s) {
     return NB_OK;
 }
 template <typename T, int RM, bool KROWS>
-int outer(LoraParams p, T* grad, cudaStream_t s) {
+int outer(const nb_lora_args* a, LoraParams p, T* grad, cudaStream_t s) {
     using S = OuterTile<RM>;
-    p.rows_per_item = outer_rows(p.T, p.K);
+    p.rows_per_item = outer_rows(a, p.K);
     const int items = item_count(p.T, p.requests, p.rows_per_item);
-    auto* kernel = lora_outer_kernel<T, RM, KROWS>;
-    if (int rc = allow_smem(kernel, S::BYTES)) return rc;
-    kernel<<<dim3(ceil_div(p.K, 128), items), kThreads, S::BYTES, s>>>(p);
-    NB_CUDA_CHECK(cudaGetLastError());
+    auto small = [&]() -> int {
+        auto* kernel = lora_outer_kernel<T, RM, KROWS>;
+        if (int rc = allow_smem(kernel, S::BYTES)) return rc;
+        kernel<<<dim3(ceil_div(p.K, 128), items), kThreads, S::BYTES, s>>>(p);
+        NB_CUDA_CHECK(cudaGetLastError());
+        return NB_OK;
+    };
+    if (int rc = NB_TC_OR(a, tc_outer(p, KROWS, a->dtype, s), small())) return rc;
     const long long size = (long long)p.R * p.K;
     lora_join_kernel<T><<<dim3(ceil_div(size, 1024), p.A), 256, 0, s>>>(p.part, p.item_adapter, items, size, grad);
     NB_CUDA_CHECK(cudaGetLastError());
@@ -611,6 +574,7 @@ LoraParams params_of(const nb_lora_args* a) {
     p.offsets = a->offsets; p.adapters = a->adapters; p.scale = a->scale;
     p.T = a->T; p.R = a->R; p.A = a->A; p.requests = a->requests;
     p.rows_per_item = kRows;
+    p.status = static_cast<int*>(a->status);
     return p;
 }
 char* plane(void* h, const nb_lora_args* a, int which) { return static_cast<char*>(h) + (long long)which * a->T * a->R * 2; }
@@ -621,9 +585,9 @@ int forward_t(const nb_lora_args* a, cudaStream_t s) {
     p.hi = plane(a->h, a, 0);
     p.lo = plane(a->h, a, 1);
     p.x = a->x; p.stride_x = a->stride_x; p.factor = a->down; p.K = a->K;
-    if (int rc = shrink<T, RM, false>(p, s)) return rc;
+    if (int rc = NB_TC_OR(a, tc_shrink(p, false, a->dtype, s), (shrink<T, RM, false>(p, s)))) return rc;
     p.x = a->base; p.stride_x = a->stride_base; p.out = a->out; p.stride_out = a->stride_out; p.factor = a->up; p.K = a->N;
-    return expand<T, RM, false>(p, s);
+    return NB_TC_OR(a, tc_expand(p, false, a->dtype, s), (expand<T, RM, false>(p, s)));
 }
 template <typename T, int RM>
 int backward_t(const nb_lora_args* a, cudaStream_t s) {
@@ -637,22 +601,22 @@ int backward_t(const nb_lora_args* a, cudaStream_t s) {
         g.hi = plane(a->g, a, 0);
         g.lo = plane(a->g, a, 1);
         g.x = a->dy; g.stride_x = a->stride_dy; g.factor = a->up; g.K = a->N;
-        if (int rc = shrink<T, RM, true>(g, s)) return rc;
+        if (int rc = NB_TC_OR(a, tc_shrink(g, true, a->dtype, s), (shrink<T, RM, true>(g, s)))) return rc;
     }
     if (a->dup) {
         p.x = a->dy; p.stride_x = a->stride_dy; p.K = a->N;
         p.hi = plane(a->h, a, 0);
         p.lo = plane(a->h, a, 1);
-        if (int rc = outer<T, RM, true>(p, static_cast<T*>(a->dup), s)) return rc;
+        if (int rc = outer<T, RM, true>(a, p, static_cast<T*>(a->dup), s)) return rc;
     }
     g.K = a->K;
     if (a->ddown) {
         g.x = a->x; g.stride_x = a->stride_x;
-        if (int rc = outer<T, RM, false>(g, static_cast<T*>(a->ddown), s)) return rc;
+        if (int rc = outer<T, RM, false>(a, g, static_cast<T*>(a->ddown), s)) return rc;
     }
     if (a->dx) {
         g.x = nullptr; g.out = a->dx; g.stride_out = a->K; g.factor = a->down;
-        return expand<T, RM, true>(g, s);
+        return NB_TC_OR(a, tc_expand(g, true, a->dtype, s), (expand<T, RM, true>(g, s)));
     }
     return NB_OK;
 }
@@ -668,6 +632,7 @@ int dispatch(const nb_lora_args* a, bool backward, cudaStream_t s) {
 int check(const nb_lora_args* a) {
     NB_REQUIRE(a && a->T >= 0 && a->K > 0 && a->N > 0 && a->R > 0 && a->A > 0 && a->requests >= 0);
     NB_REQUIRE(a->dtype == NB_DTYPE_BF16 || a->dtype == NB_DTYPE_FP16);
+    NB_REQUIRE(a->impl == NB_IMPL_AUTO || a->impl == NB_IMPL_TCGEN05 || a->impl == NB_IMPL_GENERIC);
     if (a->R % 16 || a->R > NB_LORA_MAX_RANK) return fail_with(NB_ERR_UNSUPPORTED, "the rank must be a multiple of 16 up to NB_LORA_MAX_RANK");
     if (a->K % 8 || a->N % 8) return fail_with(NB_ERR_UNSUPPORTED, "K and N must be multiples of 8");
     if (a->T > (1 << 30) || a->requests > 65535 || a->A > 65535 || item_count(a->T, a->requests, kRows) > 65535 || a->K > (1 << 24) || a->N > (1 << 24))
@@ -678,15 +643,17 @@ int check(const nb_lora_args* a) {
 }
 
 }  // namespace
+}  // namespace lora
 }  // namespace nb
 
 extern "C" int64_t nb_lora_workspace_bytes(const nb_lora_args* a) {
     using namespace nb;
+    using namespace nb::lora;
     if (check(a) != NB_OK || a->T == 0) return 0;
     int64_t most = 0;
     for (int cols : {a->dup ? a->N : 0, a->ddown ? a->K : 0}) {
         if (!cols) continue;
-        const int64_t n = (int64_t)item_count(a->T, a->requests, outer_rows(a->T, cols)) * a->R * cols * 4;
+        const int64_t n = (int64_t)item_count(a->T, a->requests, outer_rows(a, cols)) * a->R * cols * 4;
         if (n > most) most = n;
     }
     return most ? ((int64_t)item_count(a->T, a->requests, 128) * 4 + 255) / 256 * 256 + most : 0;
@@ -694,6 +661,7 @@ extern "C" int64_t nb_lora_workspace_bytes(const nb_lora_args* a) {
 
 extern "C" int nb_lora_forward(const nb_lora_args* a, void* stream) {
     using namespace nb;
+    using namespace nb::lora;
     if (int rc = check(a)) return rc;
     if (a->T == 0) return NB_OK;
     NB_REQUIRE(a->x && a->out && a->h && aligned16(a->x) && aligned16(a->out) && aligned16(a->h) && aligned16(a->base));
@@ -704,6 +672,7 @@ extern "C" int nb_lora_forward(const nb_lora_args* a, void* stream) {
 
 extern "C" int nb_lora_backward(const nb_lora_args* a, void* stream) {
     using namespace nb;
+    using namespace nb::lora;
     if (int rc = check(a)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->T == 0) {  // empty sums

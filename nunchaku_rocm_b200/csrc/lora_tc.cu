@@ -1,0 +1,672 @@
+// The products of the batched adapters (lora.cu has the mathematics and the items) on the tcgen05 tensor cores, for calls
+// with many rows per request: operands by TMA into 128-byte-swizzled tiles, accumulators in tensor memory, an epilogue
+// that overlaps the next tiles.  The products move many bytes per multiplication (rank 64: 32 multiply-adds per byte of x,
+// base, out or dy), so what the tensor cores give here is not arithmetic but the absence of it elsewhere: no operand passes
+// through registers, and the bytes in flight are the size of the shared-memory ring.
+//
+// A tile is loaded whole even where its item has fewer rows: the rows behind belong to other requests (or are filled with
+// zeros behind the last row).  They are multiplied along and not stored; where rows are summed (outer) they are set to zero
+// in shared memory first.  Every mbarrier wait is bounded; on expiry the CTA records a code in the status word and unwinds.
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "lora.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace nb {
+namespace lora {
+namespace {
+
+constexpr int KB = 64;  // values of a 128-byte row of a tile
+
+enum { E_SHRINK = 0x310, E_EXPAND = 0x330, E_OUTER = 0x350 };
+
+// K-major operand (rows along M or N, the 64 values of a 128-byte row along K): 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// MN-major operand (the 64 values of a 128-byte row along M or N, rows along K): 8-row groups 1024 bytes apart along K,
+// `half` bytes between 64-wide halves along M or N
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t half) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(half >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+constexpr uint32_t A_MN = 1u << 15, B_MN = 1u << 16;
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+// after a wait that expired: copies in flight land before the CTA's shared memory goes (bounded)
+__device__ __forceinline__ void let_copies_land() {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 100000000ull) {}
+}
+template <typename T>
+struct Fmt { static constexpr uint32_t value = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u; };
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(tmap),
+                 "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ uint8_t* align1k(unsigned char* p) {
+    return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
+}
+
+// ------------------------------------------------------------------------------------------------------------------ shrink
+// 128 rows x R over one slice of K; the slices of an item are a cluster whose sums meet in shared memory.
+// Warps: TMA producer, MMA issuer, four for the sums.
+template <int RP>  // R rounded up to 16, 32, 64 or 128
+struct ShrinkTc {
+    static constexpr int XB = kTcRows * 128;
+    static constexpr int FB = RP <= 64 ? 64 * 128 : 2 * 64 * 128;  // [64 of K][64 r] tiles, or RP rows of 64 of K
+    static constexpr int STAGE = XB + FB, ST = RP <= 64 ? 4 : 3;
+    static constexpr int LD = RP + 4;  // floats of a row of sums: 16-byte accesses of eight rows on different banks
+    static constexpr int PIPE = ST * STAGE, SUMS = kTcRows * LD * 4;
+    static constexpr int OFF_BAR = PIPE > SUMS ? PIPE : SUMS;
+    static constexpr int BYTES = OFF_BAR + 256 + 1024;
+    static constexpr int COLS = RP < 32 ? 32 : RP;
+    static constexpr int THREADS = 192;
+};
+template <typename T, int RP, bool RCONTIG>
+__global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_f,
+                                                              const LoraParams p) {
+    using S = ShrinkTc<RP>;
+    extern __shared__ unsigned char raw[];
+    const Item it = find_item<S::THREADS>(p, blockIdx.x);
+    if (it.rows == 0 || it.adapter < 0) return;  // every CTA of the cluster
+    uint8_t* smem = align1k(raw);
+    const uint32_t base = smem_u32(smem), bars = base + S::OFF_BAR;
+    auto full = [&](int i) { return bars + 8u * i; };
+    auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
+    const uint32_t done = bars + 8u * (2 * S::ST);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 128);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 136);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::ST; ++i) {
+            mbar_init(full(i), 1);
+            mbar_init(empty(i), 1);
+        }
+        mbar_init(done, 1);
+        *abort_s = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_at), S::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+    const int splits = gridDim.y, split = blockIdx.y;
+    const int steps = (p.K + KB - 1) / KB, per = (steps + splits - 1) / splits;
+    const int step0 = min(split * per, steps), n = min(per, steps - step0);
+    // bytes that land per stage (the part of a box outside the tensor arrives as zeros and counts)
+    const int fhalves = RP <= 64 ? 1 : 2;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tm_x);
+            tma_prefetch_desc(&tm_f);
+            bool ok = true;
+            for (int s = 0; s < n; ++s) {
+                const int st = s % S::ST;
+                if (s >= S::ST && !mbar_wait(empty(st), ((s / S::ST) & 1) ^ 1, abort_s, E_SHRINK | 1, 50)) { ok = false; break; }
+                const uint32_t x = base + st * S::STAGE, f = x + S::XB;
+                const int k0 = (step0 + s) * KB;
+                mbar_expect_tx(full(st), S::XB + (RCONTIG ? fhalves * 64 * 128 : p.R * 128));
+                tma_load_2d(x, &tm_x, full(st), k0, it.first);
+                if constexpr (RCONTIG) {
+                    for (int h = 0; h < fhalves; ++h) tma_load_3d(f + h * 64 * 128, &tm_f, full(st), h * 64, k0, it.adapter);
+                } else {
+                    tma_load_3d(f, &tm_f, full(st), k0, 0, it.adapter);
+                }
+            }
+            if (!ok) let_copies_land();
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = umma_idesc(1u, Fmt<T>::value, Fmt<T>::value, p.R) | (RCONTIG ? B_MN : 0u);
+        bool ok = true;
+        for (int s = 0; s < n && ok; ++s) {
+            const int st = s % S::ST;
+            if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_SHRINK | 2)) { ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t a = desc_k(base + st * S::STAGE);
+                const uint64_t b = RCONTIG ? desc_mn(base + st * S::STAGE + S::XB, 64 * 128) : desc_k(base + st * S::STAGE + S::XB);
+                const int k16 = min(4, (p.K - (step0 + s) * KB + 15) / 16);
+                for (int k = 0; k < k16; ++k) mma_f16(tmem, a + k * 2, b + k * (RCONTIG ? 16 * 128 >> 4 : 2), idesc, (s || k) ? 1u : 0u);
+                tc_commit(empty(st));
+                if (s == n - 1) tc_commit(done);
+            }
+            __syncwarp();
+        }
+    }
+    const float scale = p.scale ? __ldg(p.scale + it.adapter) : 1.f;
+    float* sums = reinterpret_cast<float*>(smem);
+    bool ok = true;
+    if (warp >= 2) {
+        const int row = (warp & 3) * 32 + lane;
+        if (n > 0) ok = mbar_wait_warp(done, 0, abort_s, E_SHRINK | 3);
+        tc_fence_after();
+        for (int c = 0; c < RP && ok; c += 32) {
+            float v[32];
+            if (n > 0) {
+                tmem_ld32(tmem + ((warp & 3) * 32 << 16) + c, v);
+                tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < (RP < 32 ? RP : 32); i += 4)
+                *reinterpret_cast<float4*>(sums + row * S::LD + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    cg::cluster_group cluster = cg::this_cluster();
+    if (splits > 1) cluster.sync();
+    const int half = p.R / 2;
+    for (int e = split * S::THREADS + threadIdx.x; e < it.rows * half; e += splits * S::THREADS) {
+        const int row = e / half, r = (e - row * half) * 2;
+        float2 v = make_float2(0.f, 0.f);
+        for (int q = 0; q < splits; ++q) {
+            const float* from = splits > 1 ? cluster.map_shared_rank(sums, q) : sums;
+            const float2 u = *reinterpret_cast<const float2*>(from + row * S::LD + r);
+            v.x += u.x; v.y += u.y;
+        }
+        v.x *= scale; v.y *= scale;
+        const uint32_t hi = pack2<T>(v.x, v.y);
+        const float2 back = unpack2<T>(hi);
+        const uint32_t lo = pack2<T>(isfinite(back.x) ? v.x - back.x : 0.f, isfinite(back.y) ? v.y - back.y : 0.f);
+        const long long at = ((long long)(it.first + row) * p.R + r) * 2;
+        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.hi) + at) = hi;
+        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.lo) + at) = lo;
+    }
+    if (splits > 1) cluster.sync();
+    else __syncthreads();
+    if (threadIdx.x == 0 && *abort_s && p.status) atomicCAS(p.status, 0, *abort_s);
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::COLS);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ expand
+// out[128 rows, columns col0 .. col1) = base + (hi + lo) G^T, 64 columns at a time.  The item's hi and lo stay in shared
+// memory; a ring of SLOTS 16 KB tiles carries base in and out back: TMA load, tensor-memory result added in place, TMA
+// store (row by row where the item has fewer than 128 rows).  Warps: TMA producer, MMA issuer, two groups of four that take
+// every second tile.
+template <int RP>
+struct ExpandTc {
+    static constexpr int HALVES = RP <= 64 ? 1 : 2;
+    static constexpr int VB = HALVES * kTcRows * 128;   // hi or lo
+    static constexpr int GB = HALVES * 64 * 128, GST = 3;
+    static constexpr int SLOT = kTcRows * 128, SLOTS = 5;
+    static constexpr int OFF_G = 2 * VB, OFF_S = OFF_G + GST * GB, OFF_BAR = OFF_S + SLOTS * SLOT;
+    static constexpr int BYTES = OFF_BAR + 256 + 1024;
+    static constexpr int THREADS = 320;
+};
+template <typename T, int RP, bool CCONTIG>
+__global__ void __launch_bounds__(320) lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tm_hi, const __grid_constant__ CUtensorMap tm_lo,
+                                                              const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_base,
+                                                              const __grid_constant__ CUtensorMap tm_out, const LoraParams p) {
+    using S = ExpandTc<RP>;
+    extern __shared__ unsigned char raw[];
+    const Item it = find_item<S::THREADS>(p, blockIdx.y);
+    if (it.rows == 0) return;
+    const int col0 = blockIdx.x * p.cols_per_cta, col1 = min(col0 + p.cols_per_cta, p.K);
+    const T* in = static_cast<const T*>(p.x);
+    T* out = static_cast<T*>(p.out);
+    if (it.adapter < 0) {  // base alone (zeros without one)
+        if (in == out) return;
+        const int n = (col1 - col0) / 8;
+        for (int e = threadIdx.x; e < it.rows * n; e += S::THREADS) {
+            const int row = e / n, c = col0 + (e - row * n) * 8;
+            const uint4 v = in ? *reinterpret_cast<const uint4*>(in + (it.first + row) * p.stride_x + c) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out + (it.first + row) * p.stride_out + c) = v;
+        }
+        return;
+    }
+    uint8_t* smem = align1k(raw);
+    const uint32_t sb = smem_u32(smem), bars = sb + S::OFF_BAR;
+    auto bar = [&](int i) { return bars + 8u * i; };
+    enum { V = 0, GF = 1, GE = GF + S::GST, DF = GE + S::GST, DE = DF + 2, LF = DE + 2, LE = LF + S::SLOTS, COUNT = LE + S::SLOTS };
+    static_assert(COUNT * 8 <= 192, "barriers");
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(bar(V), 1);
+        for (int i = 0; i < S::GST; ++i) { mbar_init(bar(GF + i), 1); mbar_init(bar(GE + i), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(DF + i), 1); mbar_init(bar(DE + i), 4); }
+        for (int i = 0; i < S::SLOTS; ++i) { mbar_init(bar(LF + i), 1); mbar_init(bar(LE + i), 1); }
+        *abort_s = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_at), 128);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+    const int tiles = (col1 - col0 + 63) / 64;
+    const bool has_base = in != nullptr;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tm_g);
+            tma_prefetch_desc(&tm_base);
+            tma_prefetch_desc(&tm_out);
+            mbar_expect_tx(bar(V), 2 * S::VB);
+            for (int h = 0; h < S::HALVES; ++h) {
+                tma_load_2d(sb + h * kTcRows * 128, &tm_hi, bar(V), h * 64, it.first);
+                tma_load_2d(sb + S::VB + h * kTcRows * 128, &tm_lo, bar(V), h * 64, it.first);
+            }
+            bool ok = true;
+            for (int i = 0; i < tiles; ++i) {
+                const int c = col0 + i * 64, gs = i % S::GST, ls = i % S::SLOTS;
+                if (i >= S::GST && !mbar_wait(bar(GE + gs), ((i / S::GST) & 1) ^ 1, abort_s, E_EXPAND | 1, 50)) { ok = false; break; }
+                const uint32_t g = sb + S::OFF_G + gs * S::GB;
+                if constexpr (CCONTIG) {  // R rows of 64 columns
+                    mbar_expect_tx(bar(GF + gs), p.R * 128);
+                    tma_load_3d(g, &tm_g, bar(GF + gs), c, 0, it.adapter);
+                } else {  // 64 rows (columns of out) of R
+                    mbar_expect_tx(bar(GF + gs), S::GB);
+                    for (int h = 0; h < S::HALVES; ++h) tma_load_3d(g + h * 64 * 128, &tm_g, bar(GF + gs), h * 64, c, it.adapter);
+                }
+                if (has_base) {
+                    if (i >= S::SLOTS && !mbar_wait(bar(LE + ls), ((i / S::SLOTS) & 1) ^ 1, abort_s, E_EXPAND | 2, 50)) { ok = false; break; }
+                    mbar_expect_tx(bar(LF + ls), S::SLOT);
+                    tma_load_2d(sb + S::OFF_S + ls * S::SLOT, &tm_base, bar(LF + ls), c, it.first);
+                }
+            }
+            if (!ok) let_copies_land();
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = umma_idesc(1u, Fmt<T>::value, Fmt<T>::value, 64) | (CCONTIG ? B_MN : 0u);
+        const int k16 = p.R / 16;
+        bool ok = mbar_wait_warp(bar(V), 0, abort_s, E_EXPAND | 3);
+        for (int i = 0; i < tiles && ok; ++i) {
+            const int gs = i % S::GST, d = i & 1;
+            if (!mbar_wait_warp(bar(GF + gs), (i / S::GST) & 1, abort_s, E_EXPAND | 4)) { ok = false; break; }
+            if (i >= 2 && !mbar_wait_warp(bar(DE + d), ((i >> 1) & 1) ^ 1, abort_s, E_EXPAND | 5)) { ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t g = sb + S::OFF_G + gs * S::GB;
+                for (int v = 0; v < 2; ++v)  // hi, lo
+                    for (int k = 0; k < k16; ++k) {
+                        const uint64_t a = desc_k(sb + v * S::VB + (k >> 2) * kTcRows * 128) + (k & 3) * 2;
+                        const uint64_t b = CCONTIG ? desc_mn(g + k * 16 * 128, 64 * 128) : desc_k(g + (k >> 2) * 64 * 128) + (k & 3) * 2;
+                        mma_f16(tmem + d * 64, a, b, idesc, (v || k) ? 1u : 0u);
+                    }
+                tc_commit(bar(GE + gs));
+                tc_commit(bar(DF + d));
+            }
+            __syncwarp();
+        }
+    } else {
+        const int group = (warp - 2) >> 2, q = warp & 3, row = q * 32 + lane;
+        const bool whole = it.rows == kTcRows, leader = ((warp - 2) & 3) == 0 && lane == 0;
+        const int gt = ((warp - 2) & 3) * 32 + lane;  // thread of the group
+        bool ok = true;  // after a wait that expired a warp only keeps its group's barriers going
+        int held = -1;   // leader: a slot whose store may still be reading
+        for (int i = group; i < tiles; i += 2) {
+            const int c = col0 + i * 64, ls = i % S::SLOTS, d = i & 1;  // (group and buffer are the same number)
+            const uint32_t slot = sb + S::OFF_S + ls * S::SLOT;
+            ok = ok && mbar_wait_warp(bar(DF + d), (i >> 1) & 1, abort_s, E_EXPAND | 6);
+            tc_fence_after();
+            float v[2][32];
+            tmem_ld32(tmem + (q * 32 << 16) + d * 64, v[0]);
+            tmem_ld32(tmem + (q * 32 << 16) + d * 64 + 32, v[1]);
+            tmem_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(DE + d));
+            if (has_base)
+                ok = ok && mbar_wait_warp(bar(LF + ls), (i / S::SLOTS) & 1, abort_s, E_EXPAND | 7);
+            else if (i >= S::SLOTS)  // nobody loads into the slot, but its last store has to have read it
+                ok = ok && mbar_wait_warp(bar(LE + ls), ((i / S::SLOTS) & 1) ^ 1, abort_s, E_EXPAND | 8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t at = slot + row * 128 + ((j ^ (row & 7)) << 4);
+                const float* f = v[j >> 2] + (j & 3) * 8;
+                uint4 o;
+                if (has_base) {
+                    uint4 b;
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "r"(at) : "memory");
+                    const float2 b0 = unpack2<T>(b.x), b1 = unpack2<T>(b.y), b2 = unpack2<T>(b.z), b3 = unpack2<T>(b.w);
+                    o = make_uint4(pack2<T>(f[0] + b0.x, f[1] + b0.y), pack2<T>(f[2] + b1.x, f[3] + b1.y), pack2<T>(f[4] + b2.x, f[5] + b2.y),
+                                   pack2<T>(f[6] + b3.x, f[7] + b3.y));
+                } else {
+                    o = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+                }
+                if (ok) asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w) : "memory");
+            }
+            fence_proxy_async_smem();
+            named_sync(1 + group, 128);
+            if (whole) {
+                if (leader && ok) {
+                    tma_store_2d(&tm_out, slot, c, it.first);
+                    bulk_commit();
+                    bulk_wait_read<1>();  // the store before this one has read its slot
+                    if (held >= 0) mbar_arrive(bar(LE + held));
+                    held = ls;
+                }
+            } else {
+                const int chunks = min(8, (col1 - c) / 8);
+                for (int e = gt; e < it.rows * 8 && ok; e += 128) {
+                    const int r = e >> 3, j = e & 7;
+                    if (j >= chunks) continue;
+                    uint4 o;
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                                 : "r"(slot + r * 128 + ((j ^ (r & 7)) << 4)) : "memory");
+                    *reinterpret_cast<uint4*>(out + (it.first + r) * p.stride_out + c + j * 8) = o;
+                }
+                fence_proxy_async_smem();  // the next load into this slot comes after these reads
+                named_sync(1 + group, 128);
+                if (leader) mbar_arrive(bar(LE + ls));
+            }
+        }
+        if (leader) bulk_wait_all();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_s && p.status) atomicCAS(p.status, 0, *abort_s);
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 128);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------- outer
+// part[item][r, k] (or [k, r] with KROWS) = sum over the item's rows of (hi + lo)[t, r] X[t, k], 128 columns of X per CTA:
+// both operands run along the rows (MN-major), so they are used as they lie.
+template <int RP>
+struct OuterTc {
+    static constexpr int HALVES = RP <= 64 ? 1 : 2;
+    static constexpr int TILE = KB * 128;  // 64 rows of 64 values
+    static constexpr int STAGE = (2 + 2 * HALVES) * TILE, ST = RP <= 64 ? 3 : 4;
+    static constexpr int OFF_BAR = ST * STAGE;
+    static constexpr int BYTES = OFF_BAR + 256 + 1024;
+    static constexpr int COLS = RP < 32 ? 32 : RP;
+    static constexpr int THREADS = 192;
+};
+template <typename T, int RP, bool KROWS>
+__global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_hi,
+                                                             const __grid_constant__ CUtensorMap tm_lo, const LoraParams p) {
+    using S = OuterTc<RP>;
+    extern __shared__ unsigned char raw[];
+    // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
+    const int w = gridDim.y - 1 - blockIdx.y;
+    const Item it = find_item<S::THREADS>(p, w);
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
+    if (it.rows == 0 || it.adapter < 0) return;
+    uint8_t* smem = align1k(raw);
+    const uint32_t sb = smem_u32(smem), bars = sb + S::OFF_BAR;
+    auto full = [&](int i) { return bars + 8u * i; };
+    auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
+    const uint32_t done = bars + 8u * (2 * S::ST);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 128);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 136);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::ST; ++i) {
+            mbar_init(full(i), 1);
+            mbar_init(empty(i), 1);
+        }
+        mbar_init(done, 1);
+        *abort_s = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_at), S::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+    const int c0 = blockIdx.x * 128, n = (it.rows + KB - 1) / KB;
+    const bool second = c0 + 64 < p.K;  // the second half of the columns exists
+
+    if (warp == 0) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tm_x);
+            tma_prefetch_desc(&tm_hi);
+            tma_prefetch_desc(&tm_lo);
+            bool ok = true;
+            for (int s = 0; s < n; ++s) {
+                const int st = s % S::ST, t0 = it.first + s * KB;
+                if (s >= S::ST && !mbar_wait(empty(st), ((s / S::ST) & 1) ^ 1, abort_s, E_OUTER | 1, 50)) { ok = false; break; }
+                const uint32_t at = sb + st * S::STAGE;
+                mbar_expect_tx(full(st), ((second ? 2 : 1) + 2 * S::HALVES) * S::TILE);
+                tma_load_2d(at, &tm_x, full(st), c0, t0);
+                if (second) tma_load_2d(at + S::TILE, &tm_x, full(st), c0 + 64, t0);
+                for (int h = 0; h < S::HALVES; ++h) {
+                    tma_load_2d(at + (2 + h) * S::TILE, &tm_hi, full(st), h * 64, t0);
+                    tma_load_2d(at + (2 + S::HALVES + h) * S::TILE, &tm_lo, full(st), h * 64, t0);
+                }
+            }
+            if (!ok) let_copies_land();
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = umma_idesc(1u, Fmt<T>::value, Fmt<T>::value, p.R) | A_MN | B_MN;
+        bool ok = true;
+        for (int s = 0; s < n && ok; ++s) {
+            const int st = s % S::ST, rows = min(KB, it.rows - s * KB), k16 = (rows + 15) / 16;
+            const uint32_t at = sb + st * S::STAGE;
+            if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_OUTER | 2)) { ok = false; break; }
+            if (rows < k16 * 16) {  // rows behind the item's last one: zeros in every tile
+                for (int tile = 0; tile < 2 + 2 * S::HALVES; ++tile)
+                    for (int e = rows * 8 + lane; e < k16 * 16 * 8; e += 32)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + tile * S::TILE + e * 16), "r"(0) : "memory");
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            tc_fence_after();
+            if (elect_one()) {
+                for (int k = 0; k < k16; ++k) {
+                    const uint64_t a = desc_mn(at + k * 16 * 128, S::TILE);
+                    mma_f16(tmem, a, desc_mn(at + 2 * S::TILE + k * 16 * 128, S::TILE), idesc, (s || k) ? 1u : 0u);
+                    mma_f16(tmem, a, desc_mn(at + (2 + S::HALVES) * S::TILE + k * 16 * 128, S::TILE), idesc, 1u);
+                }
+                tc_commit(empty(st));
+                if (s == n - 1) tc_commit(done);
+            }
+            __syncwarp();
+        }
+    } else {
+        const int q = warp & 3, k = c0 + q * 32 + lane;
+        float* part = p.part + (long long)w * p.R * p.K;
+        if (mbar_wait_warp(done, 0, abort_s, E_OUTER | 3)) {
+            tc_fence_after();
+            for (int c = 0; c < p.R; c += 32) {
+                float v[32];
+                tmem_ld32(tmem + (q * 32 << 16) + c, v);
+                tmem_wait_ld();
+                if (k < p.K) {
+                    const int left = p.R - c;  // 16 or more
+                    if constexpr (KROWS) {
+                        float* to = part + (long long)k * p.R + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            if (i < left)
+                                asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]),
+                                             "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7]) : "memory");
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < left) part[(long long)(c + i) * p.K + k] = v[i];
+                    }
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_s && p.status) atomicCAS(p.status, 0, *abort_s);
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::COLS);
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------- launchers
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = [] {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<EncodeTiledFn>(sym)
+                   : nullptr;
+    }();
+    return fn;
+}
+// `depth` matrices (0: one, as a 2-D map) of (rows, cols) 16-bit values one behind the other, `stride` elements between rows;
+// boxes of 64 columns by `box_rows` rows of one matrix, zeros outside it
+template <typename T>
+bool make_map(CUtensorMap* m, const void* base, long long rows, long long cols, long long stride, int box_rows, int depth = 0) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)depth};
+    const cuuint64_t strides[2] = {(cuuint64_t)stride * 2, (cuuint64_t)(stride * rows) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+    return fn(m, std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth > 0 ? 3 : 2,
+              const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int RP, bool RCONTIG>
+int shrink(LoraParams p, cudaStream_t s) {
+    using S = ShrinkTc<RP>;
+    p.rows_per_item = kTcRows;
+    CUtensorMap x, f;
+    const bool ok = make_map<T>(&x, p.x, p.T, p.K, p.stride_x, kTcRows) &&
+                    (RCONTIG ? make_map<T>(&f, p.factor, p.K, p.R, p.R, KB, p.A) : make_map<T>(&f, p.factor, p.R, p.K, p.K, p.R, p.A));
+    if (!ok) return NB_ERR_UNSUPPORTED;
+    const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
+    // CTAs of an item: a power of two up to eight (a portable cluster), until the items cover the SMs twice, each with at
+    // least four steps of 64 of K
+    int splits = 1;
+    while (splits < 8 && live * splits < 2 * sms() && ceil_div(p.K, KB) >= 8 * splits) splits *= 2;
+    auto* kernel = lora_shrink_tc_kernel<T, RP, RCONTIG>;
+    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(items, splits);
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 1;
+    at.val.clusterDim.y = splits;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    NB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, x, f, p));
+    return NB_OK;
+}
+template <typename T, int RP, bool CCONTIG>
+int expand(LoraParams p, cudaStream_t s) {
+    using S = ExpandTc<RP>;
+    p.rows_per_item = kTcRows;
+    CUtensorMap hi, lo, g, base, out;
+    bool ok = make_map<T>(&hi, p.hi, p.T, p.R, p.R, kTcRows) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, kTcRows) &&
+              make_map<T>(&out, p.out, p.T, p.K, p.stride_out, kTcRows) &&
+              (CCONTIG ? make_map<T>(&g, p.factor, p.R, p.K, p.K, p.R, p.A) : make_map<T>(&g, p.factor, p.K, p.R, p.R, 64, p.A));
+    if (ok && p.x) ok = make_map<T>(&base, p.x, p.T, p.K, p.stride_x, kTcRows);
+    else base = out;
+    if (!ok) return NB_ERR_UNSUPPORTED;
+    const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
+    // columns of a CTA: whole tiles, as few as leave about four CTAs per SM over the call, but at least four tiles where the
+    // row has them (an item's hi and lo are loaded once per CTA)
+    const int tiles = ceil_div(p.K, 64);
+    int per = ceil_div((long long)tiles * live, 4ll * sms());
+    if (per < 4) per = 4;
+    if (per > tiles) per = tiles;
+    p.cols_per_cta = per * 64;
+    auto* kernel = lora_expand_tc_kernel<T, RP, CCONTIG>;
+    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+    kernel<<<dim3(ceil_div(tiles, per), items), S::THREADS, S::BYTES, s>>>(hi, lo, g, base, out, p);
+    NB_CUDA_CHECK(cudaGetLastError());
+    return NB_OK;
+}
+template <typename T, int RP, bool KROWS>
+int outer(const LoraParams& p, cudaStream_t s) {
+    using S = OuterTc<RP>;
+    CUtensorMap x, hi, lo;
+    if (!(make_map<T>(&x, p.x, p.T, p.K, p.stride_x, KB) && make_map<T>(&hi, p.hi, p.T, p.R, p.R, KB) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, KB)))
+        return NB_ERR_UNSUPPORTED;
+    auto* kernel = lora_outer_tc_kernel<T, RP, KROWS>;
+    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+    kernel<<<dim3(ceil_div(p.K, 128), item_count(p.T, p.requests, p.rows_per_item)), S::THREADS, S::BYTES, s>>>(x, hi, lo, p);
+    NB_CUDA_CHECK(cudaGetLastError());
+    return NB_OK;
+}
+
+#define NB_LORA_RP(CALL)                         \
+    if (p.R <= 16) return CALL(16);              \
+    if (p.R <= 32) return CALL(32);              \
+    if (p.R <= 64) return CALL(64);              \
+    return CALL(128)
+
+template <typename T>
+int shrink_t(const LoraParams& p, bool rcontig, cudaStream_t s) {
+#define NB_CALL(RP) (rcontig ? shrink<T, RP, true>(p, s) : shrink<T, RP, false>(p, s))
+    NB_LORA_RP(NB_CALL);
+#undef NB_CALL
+}
+template <typename T>
+int expand_t(const LoraParams& p, bool ccontig, cudaStream_t s) {
+#define NB_CALL(RP) (ccontig ? expand<T, RP, true>(p, s) : expand<T, RP, false>(p, s))
+    NB_LORA_RP(NB_CALL);
+#undef NB_CALL
+}
+template <typename T>
+int outer_t(const LoraParams& p, bool krows, cudaStream_t s) {
+#define NB_CALL(RP) (krows ? outer<T, RP, true>(p, s) : outer<T, RP, false>(p, s))
+    NB_LORA_RP(NB_CALL);
+#undef NB_CALL
+}
+
+}  // namespace
+
+int tc_shrink(LoraParams p, bool rcontig, int dtype, cudaStream_t s) {
+    return dtype == NB_DTYPE_BF16 ? shrink_t<__nv_bfloat16>(p, rcontig, s) : shrink_t<__half>(p, rcontig, s);
+}
+int tc_expand(LoraParams p, bool ccontig, int dtype, cudaStream_t s) {
+    return dtype == NB_DTYPE_BF16 ? expand_t<__nv_bfloat16>(p, ccontig, s) : expand_t<__half>(p, ccontig, s);
+}
+int tc_outer(const LoraParams& p, bool krows, int dtype, cudaStream_t s) {
+    return dtype == NB_DTYPE_BF16 ? outer_t<__nv_bfloat16>(p, krows, s) : outer_t<__half>(p, krows, s);
+}
+
+}  // namespace lora
+}  // namespace nb

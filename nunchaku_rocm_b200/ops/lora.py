@@ -25,18 +25,19 @@ def _aligned_rows(t: torch.Tensor):
     return t, stride
 
 
-def _args(T, K, N, down, up, offsets, adapters, scale):
+def _args(T, K, N, down, up, offsets, adapters, scale, impl):
     a = L.LoraArgs()
     a.down, a.up = down.data_ptr(), up.data_ptr()
     a.offsets, a.adapters = offsets.data_ptr(), adapters.data_ptr()
     if scale is not None:
         a.scale = scale.data_ptr()
     a.T, a.K, a.N, a.R, a.A = T, K, N, down.shape[1], down.shape[0]
-    a.requests, a.dtype = adapters.shape[0], L.DTYPE_CODE[down.dtype]
+    a.requests, a.dtype, a.impl = adapters.shape[0], L.DTYPE_CODE[down.dtype], impl
+    a.status = L.status_word(down.device).data_ptr()
     return a
 
 
-def _forward(x, base, down, up, offsets, adapters, scale, out):
+def _forward(x, base, down, up, offsets, adapters, scale, out, impl):
     """``out`` and the two 16-bit parts of ``scale x down^T``; the arguments are checked already."""
     K, N = down.shape[2], up.shape[1]
     T = x.numel() // K
@@ -44,7 +45,7 @@ def _forward(x, base, down, up, offsets, adapters, scale, out):
     if T == 0:
         return h
     x, stride_x = _aligned_rows(x)
-    a = _args(T, K, N, down, up, offsets, adapters, scale)
+    a = _args(T, K, N, down, up, offsets, adapters, scale, impl)
     a.x, a.stride_x = x.data_ptr(), stride_x
     if base is not None:
         base, a.stride_base = _aligned_rows(base)
@@ -57,12 +58,12 @@ def _forward(x, base, down, up, offsets, adapters, scale, out):
 
 class _LoraBatched(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, base, down, up, offsets, adapters, scale):
+    def forward(ctx, x, base, down, up, offsets, adapters, scale, impl):
         out = x.new_empty((*x.shape[:-1], up.shape[1]))
-        h = _forward(x, base, down, up, offsets, adapters, scale, out)
+        h = _forward(x, base, down, up, offsets, adapters, scale, out, impl)
         need = ctx.needs_input_grad
         ctx.save_for_backward(x if need[2] else None, down, up, h if need[3] else None, offsets, adapters, scale)
-        ctx.x_shape = x.shape
+        ctx.x_shape, ctx.impl = x.shape, impl
         return out
 
     @staticmethod
@@ -82,7 +83,7 @@ class _LoraBatched(torch.autograd.Function):
                     t.zero_()
         elif need_x or need_down or need_up:
             rows, stride_dy = _aligned_rows(dy)
-            a = _args(T, K, N, down, up, offsets, adapters, scale)
+            a = _args(T, K, N, down, up, offsets, adapters, scale, ctx.impl)
             a.dy, a.stride_dy = rows.data_ptr(), stride_dy
             if need_x:
                 a.dx = dx.data_ptr()
@@ -100,12 +101,12 @@ class _LoraBatched(torch.autograd.Function):
                 ws = new((n + 1) // 2)
                 a.workspace, a.workspace_bytes = ws.data_ptr(), n
             L.launch(lib.nb_lora_backward, "lora_batched backward", down, a)
-        return dx, (dy if need_base else None), ddown, dup, None, None, None
+        return dx, (dy if need_base else None), ddown, dup, None, None, None, None
 
 
 def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor, adapters: torch.Tensor,
                  base: torch.Tensor | None = None, scale: torch.Tensor | None = None,
-                 out: torch.Tensor | None = None) -> torch.Tensor:
+                 out: torch.Tensor | None = None, _impl: int = L.IMPL_AUTO) -> torch.Tensor:
     """
     ``out[t] = base[t] + scale[a] * (x[t] @ down[a]^T) @ up[a]^T`` with ``a`` the adapter of row ``t``'s request.
 
@@ -157,8 +158,8 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     if grad and (x.requires_grad or down.requires_grad or up.requires_grad or (base is not None and base.requires_grad)):
         if out is not None:
             raise ValueError("out cannot be given where a gradient is asked for")
-        return _LoraBatched.apply(x, base, down, up, offsets, adapters, scale)
+        return _LoraBatched.apply(x, base, down, up, offsets, adapters, scale, _impl)
     if out is None:
         out = x.new_empty((*x.shape[:-1], N))
-    _forward(x, base, down, up, offsets, adapters, scale, out)
+    _forward(x, base, down, up, offsets, adapters, scale, out, _impl)
     return out

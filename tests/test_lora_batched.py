@@ -66,10 +66,19 @@ def reference(p, offsets, adapters, scale=True, base=True):
     return {k: (v, t[k] + half(dt) * (v.abs() + t[k]) + torch.finfo(dt).smallest_normal) for k, v in {"out": out, "dx": dx, "ddown": dd, "dup": du}.items()}
 
 
+IMPLS = {"generic": L.IMPL_GENERIC, "tcgen05": L.IMPL_TCGEN05}
+
+
 def check(dev, p, offsets, adapters, scale=True, base=True):
+    for impl in IMPLS.values():
+        check_impl(dev, p, offsets, adapters, scale, base, impl)
+    assert L.device_status(dev) == 0
+
+
+def check_impl(dev, p, offsets, adapters, scale, base, impl):
     off, ad = index(dev, offsets, adapters)
     ref = reference(p, offsets, adapters, scale, base)
-    kw = {"base": p["base"] if base else None, "scale": p["scale"] if scale else None}
+    kw = {"base": p["base"] if base else None, "scale": p["scale"] if scale else None, "_impl": impl}
     plain = lora_batched(p["x"], p["down"], p["up"], off, ad, **kw)
     within(plain, *ref["out"])
     leaves = [p[k].detach().requires_grad_(True) for k in ("x", "down", "up")]
