@@ -56,7 +56,6 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 template <int N>
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // after a wait that expired: copies in flight land before the CTA's shared memory goes (bounded)
 __device__ __forceinline__ void let_copies_land() {
     const uint64_t t0 = globaltimer_ns();
@@ -207,6 +206,7 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
     }
     if (splits > 1) cluster.sync();
     else __syncthreads();
+    if (*abort_s) let_copies_land();
     if (threadIdx.x == 0 && *abort_s && p.status) atomicCAS(p.status, 0, *abort_s);
     if (warp == 1) {
         tc_fence_after();
@@ -217,20 +217,23 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
 // ------------------------------------------------------------------------------------------------------------------ expand
 // out[128 rows, columns col0 .. col1) = base + (hi + lo) G^T, 64 columns at a time.  The item's hi and lo stay in shared
 // memory; a ring of SLOTS 16 KB tiles carries base in and out back: TMA load, tensor-memory result added in place, TMA
-// store (row by row where the item has fewer than 128 rows).  Warps: TMA producer, MMA issuer, two groups of four that take
-// every second tile.
+// store (straight from registers where the item has fewer than 128 rows).  Warps: TMA producer, MMA issuer, eight that add
+// (a lane has a row, a warp half of a tile's columns), one that stores.  All of them take every tile, in order: a barrier of
+// the ring is then never more than one phase ahead of anybody who waits on it.
 template <int RP>
 struct ExpandTc {
     static constexpr int HALVES = RP <= 64 ? 1 : 2;
     static constexpr int VB = HALVES * kTcRows * 128;   // hi or lo
-    static constexpr int GB = HALVES * 64 * 128, GST = 3;
-    static constexpr int SLOT = kTcRows * 128, SLOTS = 5;
+    // up to rank 64 two CTAs share an SM, so that one starts and drains under the other's tiles
+    static constexpr int PER_SM = RP <= 64 ? 2 : 1;
+    static constexpr int GB = HALVES * 64 * 128, GST = RP <= 64 ? 2 : 3;
+    static constexpr int SLOT = kTcRows * 128, SLOTS = RP <= 64 ? 3 : 5;
     static constexpr int OFF_G = 2 * VB, OFF_S = OFF_G + GST * GB, OFF_BAR = OFF_S + SLOTS * SLOT;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
-    static constexpr int THREADS = 320;
+    static constexpr int THREADS = 352;
 };
 template <typename T, int RP, bool CCONTIG>
-__global__ void __launch_bounds__(320) lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tm_hi, const __grid_constant__ CUtensorMap tm_lo,
+__global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tm_hi, const __grid_constant__ CUtensorMap tm_lo,
                                                               const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_base,
                                                               const __grid_constant__ CUtensorMap tm_out, const LoraParams p) {
     using S = ExpandTc<RP>;
@@ -253,16 +256,17 @@ __global__ void __launch_bounds__(320) lora_expand_tc_kernel(const __grid_consta
     uint8_t* smem = align1k(raw);
     const uint32_t sb = smem_u32(smem), bars = sb + S::OFF_BAR;
     auto bar = [&](int i) { return bars + 8u * i; };
-    enum { V = 0, GF = 1, GE = GF + S::GST, DF = GE + S::GST, DE = DF + 2, LF = DE + 2, LE = LF + S::SLOTS, COUNT = LE + S::SLOTS };
-    static_assert(COUNT * 8 <= 192, "barriers");
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
-    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
+    enum { V = 0, GF = 1, GE = GF + S::GST, DF = GE + S::GST, DE = DF + 2, LF = DE + 2, LE = LF + S::SLOTS, WF = LE + S::SLOTS, COUNT = WF + S::SLOTS };
+    // V, G: operands landed / free; D: accumulator done / read; L: a slot's base landed / the slot free; W: its result written
+    static_assert(COUNT * 8 <= 224, "barriers");
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 224);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 232);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(bar(V), 1);
         for (int i = 0; i < S::GST; ++i) { mbar_init(bar(GF + i), 1); mbar_init(bar(GE + i), 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar(DF + i), 1); mbar_init(bar(DE + i), 4); }
-        for (int i = 0; i < S::SLOTS; ++i) { mbar_init(bar(LF + i), 1); mbar_init(bar(LE + i), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(DF + i), 1); mbar_init(bar(DE + i), 8); }
+        for (int i = 0; i < S::SLOTS; ++i) { mbar_init(bar(LF + i), 1); mbar_init(bar(LE + i), 1); mbar_init(bar(WF + i), 8); }
         *abort_s = 0;
         fence_barrier_init();
     }
@@ -329,32 +333,30 @@ __global__ void __launch_bounds__(320) lora_expand_tc_kernel(const __grid_consta
             }
             __syncwarp();
         }
-    } else {
-        const int group = (warp - 2) >> 2, q = warp & 3, row = q * 32 + lane;
-        const bool whole = it.rows == kTcRows, leader = ((warp - 2) & 3) == 0 && lane == 0;
-        const int gt = ((warp - 2) & 3) * 32 + lane;  // thread of the group
-        bool ok = true;  // after a wait that expired a warp only keeps its group's barriers going
-        int held = -1;   // leader: a slot whose store may still be reading
-        for (int i = group; i < tiles; i += 2) {
-            const int c = col0 + i * 64, ls = i % S::SLOTS, d = i & 1;  // (group and buffer are the same number)
-            const uint32_t slot = sb + S::OFF_S + ls * S::SLOT;
-            ok = ok && mbar_wait_warp(bar(DF + d), (i >> 1) & 1, abort_s, E_EXPAND | 6);
+    } else if (warp < 10) {
+        const int q = warp & 3, half = (warp - 2) >> 2, row = q * 32 + lane;
+        const bool whole = it.rows == kTcRows;
+        for (int i = 0; i < tiles; ++i) {
+            const int ls = i % S::SLOTS, d = i & 1, c = col0 + i * 64 + half * 32;
+            const uint32_t line = sb + S::OFF_S + ls * S::SLOT + row * 128;
+            if (!mbar_wait_warp(bar(DF + d), (i >> 1) & 1, abort_s, E_EXPAND | 6)) break;
             tc_fence_after();
-            float v[2][32];
-            tmem_ld32(tmem + (q * 32 << 16) + d * 64, v[0]);
-            tmem_ld32(tmem + (q * 32 << 16) + d * 64 + 32, v[1]);
+            float v[32];
+            tmem_ld32(tmem + (q * 32 << 16) + d * 64 + half * 32, v);
             tmem_wait_ld();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(DE + d));
-            if (has_base)
-                ok = ok && mbar_wait_warp(bar(LF + ls), (i / S::SLOTS) & 1, abort_s, E_EXPAND | 7);
-            else if (i >= S::SLOTS)  // nobody loads into the slot, but its last store has to have read it
-                ok = ok && mbar_wait_warp(bar(LE + ls), ((i / S::SLOTS) & 1) ^ 1, abort_s, E_EXPAND | 8);
+            __syncwarp();
+            if (has_base) {
+                if (!mbar_wait_warp(bar(LF + ls), (i / S::SLOTS) & 1, abort_s, E_EXPAND | 7)) break;
+            } else if (i >= S::SLOTS) {  // nobody loads into the slot, but its last store has to have read it
+                if (!mbar_wait_warp(bar(LE + ls), ((i / S::SLOTS) & 1) ^ 1, abort_s, E_EXPAND | 8)) break;
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t at = slot + row * 128 + ((j ^ (row & 7)) << 4);
-                const float* f = v[j >> 2] + (j & 3) * 8;
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t at = line + (((half * 4 + j) ^ (row & 7)) << 4);
+                const float* f = v + j * 8;
                 uint4 o;
                 if (has_base) {
                     uint4 b;
@@ -365,37 +367,32 @@ __global__ void __launch_bounds__(320) lora_expand_tc_kernel(const __grid_consta
                 } else {
                     o = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
                 }
-                if (ok) asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w) : "memory");
+                if (whole)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w) : "memory");
+                else if (row < it.rows && c + j * 8 < col1)
+                    *reinterpret_cast<uint4*>(out + (it.first + row) * p.stride_out + c + j * 8) = o;
             }
-            fence_proxy_async_smem();
-            named_sync(1 + group, 128);
-            if (whole) {
-                if (leader && ok) {
-                    tma_store_2d(&tm_out, slot, c, it.first);
-                    bulk_commit();
-                    bulk_wait_read<1>();  // the store before this one has read its slot
-                    if (held >= 0) mbar_arrive(bar(LE + held));
-                    held = ls;
-                }
-            } else {
-                const int chunks = min(8, (col1 - c) / 8);
-                for (int e = gt; e < it.rows * 8 && ok; e += 128) {
-                    const int r = e >> 3, j = e & 7;
-                    if (j >= chunks) continue;
-                    uint4 o;
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
-                                 : "r"(slot + r * 128 + ((j ^ (r & 7)) << 4)) : "memory");
-                    *reinterpret_cast<uint4*>(out + (it.first + r) * p.stride_out + c + j * 8) = o;
-                }
-                fence_proxy_async_smem();  // the next load into this slot comes after these reads
-                named_sync(1 + group, 128);
-                if (leader) mbar_arrive(bar(LE + ls));
-            }
+            fence_proxy_async_smem();  // what was written is stored, and what was read is loaded over, by the async proxy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(WF + ls));
+            __syncwarp();
         }
-        if (leader) bulk_wait_all();
+    } else if (lane == 0) {
+        for (int i = 0; i < tiles; ++i) {
+            const int ls = i % S::SLOTS;
+            if (!mbar_wait(bar(WF + ls), (i / S::SLOTS) & 1, abort_s, E_EXPAND | 9, 50)) break;
+            if (it.rows == kTcRows) {
+                tma_store_2d(&tm_out, sb + S::OFF_S + ls * S::SLOT, col0 + i * 64, it.first);
+                bulk_commit();
+                bulk_wait_read<0>();
+            }
+            mbar_arrive(bar(LE + ls));
+        }
+        bulk_wait_all();
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_s) let_copies_land();
     if (threadIdx.x == 0 && *abort_s && p.status) atomicCAS(p.status, 0, *abort_s);
     if (warp == 1) {
         tc_fence_after();
@@ -529,6 +526,7 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         }
     }
     __syncthreads();
+    if (*abort_s) let_copies_land();
     if (threadIdx.x == 0 && *abort_s && p.status) atomicCAS(p.status, 0, *abort_s);
     if (warp == 1) {
         tc_fence_after();
@@ -567,17 +565,20 @@ template <typename T, int RP, bool RCONTIG>
 int shrink(LoraParams p, cudaStream_t s) {
     using S = ShrinkTc<RP>;
     p.rows_per_item = kTcRows;
+    auto* kernel = lora_shrink_tc_kernel<T, RP, RCONTIG>;
+    // (before the tensor maps: it makes the device's context current in a thread that has not used it yet)
+    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
     CUtensorMap x, f;
     const bool ok = make_map<T>(&x, p.x, p.T, p.K, p.stride_x, kTcRows) &&
                     (RCONTIG ? make_map<T>(&f, p.factor, p.K, p.R, p.R, KB, p.A) : make_map<T>(&f, p.factor, p.R, p.K, p.K, p.R, p.A));
     if (!ok) return NB_ERR_UNSUPPORTED;
     const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
-    // CTAs of an item: a power of two up to eight (a portable cluster), until the items cover the SMs twice, each with at
-    // least four steps of 64 of K
-    int splits = 1;
-    while (splits < 8 && live * splits < 2 * sms() && ceil_div(p.K, KB) >= 8 * splits) splits *= 2;
-    auto* kernel = lora_shrink_tc_kernel<T, RP, RCONTIG>;
-    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+    // CTAs of an item: as many as fit the SMs in one wave (two per SM), up to eight (a portable cluster), each with at least
+    // four steps of 64 of K
+    int splits = 2 * sms() / live;
+    if (splits > ceil_div(p.K, 4 * KB)) splits = ceil_div(p.K, 4 * KB);
+    if (splits > 8) splits = 8;
+    if (splits < 1) splits = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(items, splits);
     cfg.blockDim = dim3(S::THREADS);
@@ -597,6 +598,8 @@ template <typename T, int RP, bool CCONTIG>
 int expand(LoraParams p, cudaStream_t s) {
     using S = ExpandTc<RP>;
     p.rows_per_item = kTcRows;
+    auto* kernel = lora_expand_tc_kernel<T, RP, CCONTIG>;
+    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
     CUtensorMap hi, lo, g, base, out;
     bool ok = make_map<T>(&hi, p.hi, p.T, p.R, p.R, kTcRows) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, kTcRows) &&
               make_map<T>(&out, p.out, p.T, p.K, p.stride_out, kTcRows) &&
@@ -605,15 +608,18 @@ int expand(LoraParams p, cudaStream_t s) {
     else base = out;
     if (!ok) return NB_ERR_UNSUPPORTED;
     const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
-    // columns of a CTA: whole tiles, as few as leave about four CTAs per SM over the call, but at least four tiles where the
-    // row has them (an item's hi and lo are loaded once per CTA)
-    const int tiles = ceil_div(p.K, 64);
-    int per = ceil_div((long long)tiles * live, 4ll * sms());
-    if (per < 4) per = 4;
-    if (per > tiles) per = tiles;
+    // columns of a CTA: the cut of a row into `cuts` pieces that is done soonest, a CTA's cost being its tiles (0.7 us of an
+    // SM's share of HBM each) and about three microseconds to start and to load the item's hi and lo, waves of the CTAs that
+    // are resident together taking turns
+    const int tiles = ceil_div(p.K, 64), slots = S::PER_SM * sms();
+    int per = tiles;
+    float best = 1e30f;
+    for (int cuts = 1; cuts <= 16 && cuts <= tiles; ++cuts) {
+        const int t = ceil_div(tiles, cuts);
+        const float cost = (float)ceil_div((long long)live * ceil_div(tiles, t), slots) * (0.7f * S::PER_SM * t + 3.f);
+        if (cost < best) best = cost, per = t;
+    }
     p.cols_per_cta = per * 64;
-    auto* kernel = lora_expand_tc_kernel<T, RP, CCONTIG>;
-    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
     kernel<<<dim3(ceil_div(tiles, per), items), S::THREADS, S::BYTES, s>>>(hi, lo, g, base, out, p);
     NB_CUDA_CHECK(cudaGetLastError());
     return NB_OK;
@@ -621,11 +627,11 @@ int expand(LoraParams p, cudaStream_t s) {
 template <typename T, int RP, bool KROWS>
 int outer(const LoraParams& p, cudaStream_t s) {
     using S = OuterTc<RP>;
+    auto* kernel = lora_outer_tc_kernel<T, RP, KROWS>;
+    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
     CUtensorMap x, hi, lo;
     if (!(make_map<T>(&x, p.x, p.T, p.K, p.stride_x, KB) && make_map<T>(&hi, p.hi, p.T, p.R, p.R, KB) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, KB)))
         return NB_ERR_UNSUPPORTED;
-    auto* kernel = lora_outer_tc_kernel<T, RP, KROWS>;
-    NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
     kernel<<<dim3(ceil_div(p.K, 128), item_count(p.T, p.requests, p.rows_per_item)), S::THREADS, S::BYTES, s>>>(x, hi, lo, p);
     NB_CUDA_CHECK(cudaGetLastError());
     return NB_OK;

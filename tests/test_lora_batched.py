@@ -171,6 +171,16 @@ def test_many_rows_and_requests(cuda_dev, T, requests):
 
 
 @gpu
+@pytest.mark.parametrize("R,K,N,offsets,adapters", [
+    (16, 64, 6016, [0, 2944, 6000], [1, 0]),         # long walks over the columns, whole and partial tiles
+    (64, 4096, 72, [0, 1000, 1003, 6000], [0, -1, 1]),  # long contractions
+    (128, 72, 4104, [0, 6000], [0]),
+])
+def test_long_rows_and_columns(cuda_dev, R, K, N, offsets, adapters):
+    check(cuda_dev, make(cuda_dev, 6000, K, N, R, 2, BF16, seed=R), offsets, adapters)
+
+
+@gpu
 def test_without_base_and_scale(cuda_dev):
     p = make(cuda_dev, 90, 128, 256, 64, 2, BF16)
     check(cuda_dev, p, [10, 50, 80], [1, 0], scale=False, base=False)
