@@ -573,9 +573,11 @@ int shrink(LoraParams p, cudaStream_t s) {
                     (RCONTIG ? make_map<T>(&f, p.factor, p.K, p.R, p.R, KB, p.A) : make_map<T>(&f, p.factor, p.R, p.K, p.K, p.R, p.A));
     if (!ok) return NB_ERR_UNSUPPORTED;
     const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
-    // CTAs of an item: as many as fit the SMs in one wave (two per SM), up to eight (a portable cluster), each with at least
-    // four steps of 64 of K
+    // CTAs of an item: as many as fit the SMs in one wave, up to eight (a portable cluster), each with at least four steps of
+    // 64 of K.  An SM holds two, but clusters do not fill the groups of SMs that they have to stay within: of 296 places,
+    // clusters of 3 to 8 get 259 to 284 (a wave of 72 clusters of 4 ran as 71 and one: 49 us for what takes 35 with 3).
     int splits = 2 * sms() / live;
+    if (splits > 2) splits = (int)(0.87f * 2 * sms()) / live > 2 ? (int)(0.87f * 2 * sms()) / live : 2;
     if (splits > ceil_div(p.K, 4 * KB)) splits = ceil_div(p.K, 4 * KB);
     if (splits > 8) splits = 8;
     if (splits < 1) splits = 1;
