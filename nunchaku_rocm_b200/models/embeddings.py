@@ -25,6 +25,18 @@ def flux_pos_embed(ids: torch.Tensor, axes_dim=(16, 56, 56), theta: int = 10000)
     return torch.cat(parts, dim=2)[0].contiguous()
 
 
+def qwen_image_ids(txt_tokens: int, frames: int, height: int, width: int, device=None) -> torch.Tensor:
+    """Position ids of ``txt_tokens`` text rows followed by a ``frames x height x width`` latent grid, as Qwen-Image numbers
+    them: rows and columns of the grid count from its centre, the text runs along the diagonal behind the grid."""
+    ids = torch.zeros(txt_tokens + frames * height * width, 3, device=device)
+    first = max(height // 2, width // 2)
+    ids[:txt_tokens] = torch.arange(first, first + txt_tokens, device=device)[:, None]
+    f, y, x = torch.meshgrid(torch.arange(frames, device=device), torch.arange(height, device=device) - (height - height // 2),
+                             torch.arange(width, device=device) - (width - width // 2), indexing="ij")
+    ids[txt_tokens:] = torch.stack([f, y, x], -1).reshape(-1, 3).to(ids.dtype)
+    return ids
+
+
 def flux_image_ids(txt_tokens: int, height: int, width: int, device=None) -> torch.Tensor:
     """Position ids of ``txt_tokens`` text rows (0, 0, 0) followed by a ``height x width`` latent grid (0, y, x)."""
     ids = torch.zeros(txt_tokens + height * width, 3, device=device)

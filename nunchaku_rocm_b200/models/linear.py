@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from ..lora.batched import add_lora_batch, has_lora_batch
 from ..ops.gemm import svdq_gemm_w4a4_cuda
 from ..ops.gemv import awq_gemv_w4a16_cuda
 from ..ops.quantize import svdq_quantize_w4a4_act_fuse_lora_cuda
@@ -70,6 +71,8 @@ class SVDQW4A4Linear(nn.Module):
             output = torch.empty(batch_size * seq_len, self.out_features, dtype=x.dtype, device=x.device)
         quantized_x, ascales, lora_act_out = self.quantize(x)
         output = self.forward_quant(quantized_x, ascales, lora_act_out, output)
+        if has_lora_batch(self):
+            output = add_lora_batch(self, x, output, samples=batch_size)
         return output.reshape(batch_size, seq_len, -1)
 
     def quantize(self, x: torch.Tensor, pad_size: int = 256):

@@ -28,6 +28,8 @@ import torch.nn.functional as F
 from ..ops.dispatch import scaled_dot_product_attention
 from ..ops.elementwise import gated_residual, layernorm_modulate
 from ..ops.fused import fused_gelu_mlp, fused_qkv_norm_rottary
+from ..ops.rotary import rotary_table as three_axis_table
+from .embeddings import qwen_image_ids
 from .flux_dit import _side_stream, join_modulations, modulations_ahead
 from .linear import AWQW4A16Linear, SVDQW4A4Linear
 
@@ -43,6 +45,8 @@ class QwenDiTConfig:
     in_channels: int = 64
     text_dim: int = 3584       # Qwen2.5-VL hidden size
     dtype: torch.dtype = torch.bfloat16
+    axes_dim: tuple = (16, 56, 56)
+    theta: float = 10000.0
 
 
 def _rms(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
@@ -208,6 +212,13 @@ class QwenDiT(nn.Module):
         inv = 1.0 / theta ** (torch.arange(0, head_dim, 2, dtype=torch.float32, device=device) / head_dim)
         ang = torch.arange(n, dtype=torch.float32, device=device)[:, None] * inv[None]
         return torch.polar(torch.ones_like(ang), ang)
+
+    def rotary_tables(self, txt_tokens: int, frames: int, height: int, width: int, device=None):
+        """``(img_freqs, txt_freqs)`` of a ``frames x height x width`` latent grid and its text: the model's three-axis
+        positions (time, row, column) as the tables that the fused Q/K epilogue reads."""
+        ids = qwen_image_ids(txt_tokens, frames, height, width, device or self.proj_out.weight.device)
+        table = three_axis_table(ids, self.cfg.axes_dim, self.cfg.theta)
+        return table[txt_tokens:], table[:txt_tokens]
 
     def forward(self, hidden_states, encoder_hidden_states, timestep, img_freqs, txt_freqs):
         from .flux_dit import _timestep_embedding

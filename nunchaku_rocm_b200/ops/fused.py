@@ -21,7 +21,11 @@ def fused_gelu_mlp(x: torch.Tensor, fc1, fc2, pad_size: int = 256) -> torch.Tens
     ``fc2(gelu_tanh(fc1(x)))`` for two ``SVDQW4A4Linear`` layers: quantize, fc1 GEMM whose epilogue applies the GELU,
     the ``+0.171875`` shift and fc2's unsigned int4 quantisation and LoRA-down, then fc2's GEMM.  ``x (B, S, C_in)``.
     """
+    from ..lora.batched import add_lora_batch, has_lora_batch
+
     batch_size, seq_len, channels = x.shape
+    if has_lora_batch(fc1) or has_lora_batch(fc2):
+        return _gelu_mlp_lora_batch(x, fc1, fc2, pad_size, add_lora_batch, has_lora_batch)
     x = x.view(batch_size * seq_len, channels)
     quantized_x, ascales, lora_act = fc1.quantize(x)
     batch_size_pad = ceil_divide(batch_size * seq_len, pad_size) * pad_size
@@ -38,6 +42,29 @@ def fused_gelu_mlp(x: torch.Tensor, fc1, fc2, pad_size: int = 256) -> torch.Tens
     )
     output = torch.empty(batch_size * seq_len, fc2.out_features, dtype=x.dtype, device=x.device)
     output = fc2.forward_quant(qout_act, qout_ascales, qout_lora_act, output=output)
+    return output.view(batch_size, seq_len, -1)
+
+
+def _gelu_mlp_lora_batch(x, fc1, fc2, pad_size, add_lora_batch, has_lora_batch):
+    """:func:`fused_gelu_mlp` with adapters of the active requests: fc1's are added to its 16-bit output before the
+    quantizer applies the GELU, fc2's see the GELU's 16-bit output."""
+    from .triton.gemm_w4a4 import GELU_SHIFT, quantize_w4a4_act_fuse_lora
+
+    batch_size, seq_len, _ = x.shape
+    rows = batch_size * seq_len
+    hidden = fc1(x).view(rows, fc1.out_features)
+    if hidden.requires_grad:
+        raise NotImplementedError("no backward pass: a fused operator")
+    padded, fp4 = ceil_divide(rows, pad_size) * pad_size, fc2.precision == "nvfp4"
+    act = torch.empty(padded, fc1.out_features // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(fc1.out_features // (16 if fp4 else 64), padded, dtype=torch.float8_e4m3fn if fp4 else x.dtype, device=x.device)
+    lora_act = torch.empty(padded, fc2.proj_down.shape[1], dtype=torch.float32, device=x.device)
+    quantize_w4a4_act_fuse_lora(hidden, act, scales, fc2.proj_down, lora_act, fc2.smooth_factor, fp4=fp4, fuse_gelu=True,
+                                shift_value=0.0 if fp4 else GELU_SHIFT, unsigned=not fp4)
+    output = torch.empty(rows, fc2.out_features, dtype=x.dtype, device=x.device)
+    output = fc2.forward_quant(act, scales, lora_act, output=output)
+    if has_lora_batch(fc2):
+        output = add_lora_batch(fc2, torch.nn.functional.gelu(hidden, approximate="tanh"), output, samples=batch_size, fused=True)
     return output.view(batch_size, seq_len, -1)
 
 
@@ -62,8 +89,11 @@ def interleave_swiglu_linear_(linear, up_first: bool = False) -> None:
 
 def fused_swiglu_mlp(x: torch.Tensor, fc1, fc2, pad_size: int = 256) -> torch.Tensor:
     """``fc2(silu(gate) * up)`` with ``[gate | up] = fc1(x)``; ``fc1`` must have been interleaved (int4 only)."""
+    from ..lora.batched import has_lora_batch
     from .triton.gemm_w4a4 import gemm_w4a4
 
+    if has_lora_batch(fc1) or has_lora_batch(fc2):
+        raise NotImplementedError("adapters of several requests on an interleaved SwiGLU projection")
     shape = x.shape
     x = x.reshape(-1, shape[-1])
     M = x.shape[0]
@@ -92,6 +122,8 @@ def fused_qkv_norm_rottary(x: torch.Tensor, proj, norm_q=None, norm_k=None, rota
     serves every batch element.  A tuple ``output`` (packed Q/K/V of the ``nunchaku-fp16`` processor) raises
     ``NotImplementedError`` as in the reference's natural-layout backend.
     """
+    from ..lora.batched import add_lora_batch, has_lora_batch
+
     assert _is_rmsnorm(norm_q) and _is_rmsnorm(norm_k)
     batch_size, seq_len, channels = x.shape
     x = x.view(batch_size * seq_len, channels)
@@ -109,5 +141,18 @@ def fused_qkv_norm_rottary(x: torch.Tensor, proj, norm_q=None, norm_k=None, rota
         output_q, output_k, output_v = output
         svdq_gemm_w4a4_cuda(**common, out_q=output_q, out_k=output_k, out_v=output_v, attn_tokens=attn_tokens)
         return output_q, output_k, output_v
+    if has_lora_batch(proj):
+        # adapters of the active requests: they are added to the projection before Q and K are normalised and rotated
+        from .triton.gemm_w4a4 import _apply_rmsnorm_rope_qk
+
+        qk = {name: common.pop(name) for name in ("norm_q", "norm_k", "rotary_emb")}
+        svdq_gemm_w4a4_cuda(**common, out=output)
+        rows = output.view(batch_size * seq_len, proj.out_features)
+        added = add_lora_batch(proj, x, rows, samples=batch_size, fused=True)
+        if added is not rows:
+            rows.copy_(added)
+        if all(v is not None for v in qk.values()):
+            _apply_rmsnorm_rope_qk(rows, qk["norm_q"], qk["norm_k"], qk["rotary_emb"])
+        return output.view(batch_size, seq_len, -1)
     svdq_gemm_w4a4_cuda(**common, out=output)
     return output.view(batch_size, seq_len, -1)
