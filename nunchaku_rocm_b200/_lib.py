@@ -205,6 +205,31 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The extension module with torch's side of the differentiable operators (``csrc/binding/``), bound to :func:`lib`."""
+    global _binding
+    if _binding is None:
+        l = lib()
+        with _lock:
+            if _binding is None:
+                try:
+                    from . import _binding as b
+                except ImportError as e:
+                    raise NativeLibraryError(
+                        f"the extension module _binding does not load ({e}): build it with "
+                        "`python -m nunchaku_rocm_b200.build`. There is no fallback path."
+                    ) from e
+                names = ["layer_norm", "layer_norm_backward", "layer_norm_workspace_bytes", "rotary_ladder_init", "rotary_axes", "rotary_table",
+                         "lora_forward", "lora_backward", "lora_workspace_bytes", "strerror", "last_error_detail", "last_cuda_error",
+                         "last_cuda_error_string"]
+                b.bind({f"nb_{n}": C.cast(getattr(l, f"nb_{n}"), C.c_void_p).value for n in names})
+                _binding = b
+    return _binding
+
+
 def check(status: int, what: str) -> None:
     """Raise for a non-zero status (error convention of nunchaku/ops/triton/native/hip.py:110-116)."""
     if status == NB_OK:
@@ -230,19 +255,6 @@ def ptr(t: torch.Tensor | None):
 
 def stream_of(t: torch.Tensor) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
-
-
-def launch(fn, what: str, like: torch.Tensor, *args) -> None:
-    """``fn(*args, stream)`` on ``like``'s device and that device's current stream; raises for a non-zero status.  The small
-    calls are bound by the host, so the device is entered only where it is not the current one already."""
-    i = like.get_device()
-    if i == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    else:
-        with torch.cuda.device(i):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    if status:
-        check(status, what)
 
 
 def once_differentiable(backward):

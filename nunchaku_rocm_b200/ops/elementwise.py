@@ -85,19 +85,6 @@ def gated_residual(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, y2: tor
     return out
 
 
-def _strided_rows(x: torch.Tensor):
-    """``x (..., D)`` and the stride between its rows: a copy only where the rows are not evenly strided."""
-    D = x.shape[-1]
-    if not x.is_contiguous():
-        try:
-            if x.stride(-1) == 1:
-                return x, x.detach().view(-1, D).stride(0)
-        except RuntimeError:
-            pass
-        x = x.contiguous()
-    return x, D
-
-
 def _ln_weight(name, w, x, groups):
     """``w`` as the kernel reads it, with the stride between its groups' rows."""
     D = x.shape[-1]
@@ -106,26 +93,6 @@ def _ln_weight(name, w, x, groups):
     if w.shape != ((D,) if w.dim() == 1 else (groups, D)) or (w.dim() == 2 and x.dim() != 3):
         raise ValueError(f"{name} must be ({D},), or (B, {D}) for x (B, T, {D}); got {tuple(w.shape)} for {tuple(x.shape)}")
     return w if w.stride(-1) == 1 else w.contiguous()
-
-
-def _ln_args(x, stride_x, weight, bias, eps, weight_add):
-    D, a = x.shape[-1], L.LayerNormArgs()
-    first = weight if weight is not None else bias
-    grouped = first is not None and first.dim() == 2
-    rows = x.numel() // D
-    a.groups = x.shape[0] if grouped else 1
-    a.rows = rows // a.groups if a.groups else 0
-    a.dim, a.dtype = D, L.DTYPE_CODE_32[x.dtype]
-    a.x, a.stride_x = x.data_ptr(), stride_x
-    if weight is not None:
-        a.w = weight.data_ptr()
-    if bias is not None:
-        a.b = bias.data_ptr()
-    if first is not None:
-        a.w_fp32 = first.dtype == torch.float32
-        a.stride_w = first.stride(0) if grouped else 0
-    a.eps, a.weight_add = eps, weight_add
-    return a
 
 
 def _ln_prepare(x, weight, bias, weight_add):
@@ -151,65 +118,6 @@ def _ln_prepare(x, weight, bias, weight_add):
     return weight, bias
 
 
-def _ln_forward(x, weight, bias, eps, weight_add, y, stats):
-    """``y`` and / or the rows' (mean, rstd) into the given tensors; the arguments are checked already."""
-    if x.numel() == 0:
-        return
-    x, stride_x = _strided_rows(x)
-    a = _ln_args(x, stride_x, weight, bias, eps, weight_add)
-    if y is not None:
-        a.y = y.data_ptr()
-    if stats is not None:
-        a.mean = stats.data_ptr()
-        a.rstd = a.mean + 2 * stats.numel()
-    L.launch(L.lib().nb_layer_norm, "layer_norm", x, a)
-
-
-def _ln_backward(x, weight, bias, stats, dy, eps, weight_add, need):
-    """(dx, dweight, dbias), ``None`` where ``need`` says so."""
-    dx = x.new_empty(x.shape) if need[0] else None
-    dw = weight.new_empty(weight.shape) if need[1] else None
-    db = bias.new_empty(bias.shape) if need[2] else None
-    if x.numel() == 0:
-        return dx, (dw.zero_() if need[1] else None), (db.zero_() if need[2] else None)
-    x, stride_x = _strided_rows(x)
-    dy, stride_dy = _strided_rows(dy)
-    a = _ln_args(x, stride_x, weight, bias, eps, weight_add)
-    a.mean = stats.data_ptr()
-    a.rstd = a.mean + 2 * stats.numel()
-    a.dy, a.stride_dy = dy.data_ptr(), stride_dy
-    if need[0]:
-        a.dx = dx.data_ptr()
-    lib = L.lib()
-    if need[1] or need[2]:
-        n = lib.nb_layer_norm_workspace_bytes(a.groups, a.rows, a.dim, a.dtype)
-        ws = stats.new_empty(n // 4)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n
-        if need[1]:
-            a.dw = dw.data_ptr()
-        if need[2]:
-            a.db = db.data_ptr()
-    L.launch(lib.nb_layer_norm_backward, "layer_norm backward", x, a)
-    return dx, dw, db
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, weight_add):
-        y = x.new_empty(x.shape)
-        stats = x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
-        _ln_forward(x, weight, bias, eps, weight_add, y, stats)
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.consts = eps, weight_add
-        return y
-
-    @staticmethod
-    @L.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        return (*_ln_backward(x, weight, bias, stats, dy, *ctx.consts, ctx.needs_input_grad), None, None)
-
-
 class _LayerNormModulate(torch.autograd.Function):
     """:func:`layernorm_modulate` as it is without gradients, and the backward pass of the function that it rounds."""
 
@@ -226,8 +134,9 @@ class _LayerNormModulate(torch.autograd.Function):
         x, scale, shift = ctx.saved_tensors
         scale, shift = _ln_prepare(x, scale, shift, scale_add)
         stats = x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
-        _ln_forward(x, None, None, eps, 0.0, None, stats)
-        return (*_ln_backward(x, scale, shift, stats, dy, eps, scale_add, ctx.needs_input_grad), None, None)
+        b = L.binding()
+        b.layer_norm_forward(x, None, None, eps, 0.0, None, stats)
+        return (*b.layer_norm_backward(x, scale, shift, stats, dy, eps, scale_add, *ctx.needs_input_grad[:3]), None, None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-6,
@@ -242,10 +151,4 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """
     weight, bias = _ln_prepare(x, weight, bias, weight_add)
     L.require_cuda(x, weight, bias)
-    grad = torch.is_grad_enabled() and (
-        x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
-    if grad:
-        return _LayerNorm.apply(x, weight, bias, eps, weight_add)
-    y = x.new_empty(x.shape)
-    _ln_forward(x, weight, bias, eps, weight_add, y, None)
-    return y
+    return L.binding().layer_norm(x, weight, bias, eps, weight_add)

@@ -11,97 +11,23 @@ from __future__ import annotations
 import torch
 
 from .. import _lib as L
-from .elementwise import _strided_rows
 
 __all__ = ["lora_batched"]
 
 
-def _aligned_rows(t: torch.Tensor):
-    """``t (..., C)`` with rows evenly strided on 16-byte boundaries, and their stride (a copy only if they are not)."""
-    t, stride = _strided_rows(t)
-    if stride % 8 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        stride = t.shape[-1]
-    return t, stride
-
-
-def _args(T, K, N, down, up, offsets, adapters, scale, impl):
-    a = L.LoraArgs()
-    a.down, a.up = down.data_ptr(), up.data_ptr()
-    a.offsets, a.adapters = offsets.data_ptr(), adapters.data_ptr()
-    if scale is not None:
-        a.scale = scale.data_ptr()
-    a.T, a.K, a.N, a.R, a.A = T, K, N, down.shape[1], down.shape[0]
-    a.requests, a.dtype, a.impl = adapters.shape[0], L.DTYPE_CODE[down.dtype], impl
-    a.status = L.status_word(down.device).data_ptr()
-    return a
-
-
-def _forward(x, base, down, up, offsets, adapters, scale, out, impl):
-    """``out`` and the two 16-bit parts of ``scale x down^T``; the arguments are checked already."""
-    K, N = down.shape[2], up.shape[1]
-    T = x.numel() // K
-    h = x.new_empty((2, T, down.shape[1]))
-    if T == 0:
-        return h
-    x, stride_x = _aligned_rows(x)
-    a = _args(T, K, N, down, up, offsets, adapters, scale, impl)
-    a.x, a.stride_x = x.data_ptr(), stride_x
-    if base is not None:
-        base, a.stride_base = _aligned_rows(base)
-        a.base = base.data_ptr()
-    a.out, a.stride_out = out.data_ptr(), _strided_rows(out)[1]
-    a.h = h.data_ptr()
-    L.launch(L.lib().nb_lora_forward, "lora_batched", x, a)
-    return h
-
-
-class _LoraBatched(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, base, down, up, offsets, adapters, scale, impl):
-        out = x.new_empty((*x.shape[:-1], up.shape[1]))
-        h = _forward(x, base, down, up, offsets, adapters, scale, out, impl)
-        need = ctx.needs_input_grad
-        ctx.save_for_backward(x if need[2] else None, down, up, h if need[3] else None, offsets, adapters, scale)
-        ctx.x_shape, ctx.impl = x.shape, impl
-        return out
-
-    @staticmethod
-    @L.once_differentiable
-    def backward(ctx, dy):
-        x, down, up, h, offsets, adapters, scale = ctx.saved_tensors
-        need_x, need_base, need_down, need_up = ctx.needs_input_grad[:4]
-        new = down.new_empty
-        dx = new(ctx.x_shape) if need_x else None
-        ddown = new(down.shape) if need_down else None
-        dup = new(up.shape) if need_up else None
-        K, N = down.shape[2], up.shape[1]
-        T = dy.numel() // N
-        if T == 0:
-            for t in (ddown, dup):
-                if t is not None:
-                    t.zero_()
-        elif need_x or need_down or need_up:
-            rows, stride_dy = _aligned_rows(dy)
-            a = _args(T, K, N, down, up, offsets, adapters, scale, ctx.impl)
-            a.dy, a.stride_dy = rows.data_ptr(), stride_dy
-            if need_x:
-                a.dx = dx.data_ptr()
-            if need_down:
-                x, a.stride_x = _aligned_rows(x)
-                a.x, a.ddown = x.data_ptr(), ddown.data_ptr()
-            if need_x or need_down:
-                g = new((2, T, down.shape[1]))
-                a.g = g.data_ptr()
-            if need_up:
-                a.h, a.dup = h.data_ptr(), dup.data_ptr()
-            lib = L.lib()
-            n = lib.nb_lora_workspace_bytes(a) if need_down or need_up else 0
-            if n:
-                ws = new((n + 1) // 2)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), n
-            L.launch(lib.nb_lora_backward, "lora_batched backward", down, a)
-        return dx, (dy if need_base else None), ddown, dup, None, None, None, None
+def _rows_ok(t: torch.Tensor) -> bool:
+    """Whether the kernel can write ``t (..., C)`` in place: rows evenly strided, each on a 16-byte boundary."""
+    if t.data_ptr() % 16 or t.stride(-1) != 1:
+        return False
+    run, step = 1, t.shape[-1]
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size != 1:
+            if run == 1:
+                step = stride
+            elif stride != run * step:
+                return False
+            run *= size
+    return step % 8 == 0
 
 
 def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor, adapters: torch.Tensor,
@@ -148,18 +74,11 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     grad = torch.is_grad_enabled()
     if grad and scale is not None and scale.requires_grad:
         raise ValueError("lora_batched has no gradient for scale")
-    if out is not None:
-        rows, stride = _strided_rows(out)
-        if rows is not out or stride % 8 or out.data_ptr() % 16:
-            raise ValueError("out must have evenly strided rows on 16-byte boundaries")
+    if out is not None and not _rows_ok(out):
+        raise ValueError("out must have evenly strided rows on 16-byte boundaries")
     L.require_cuda(x, down, up, offsets, adapters, base, scale, out)
-    down, up, offsets, adapters = down.contiguous(), up.contiguous(), offsets.contiguous(), adapters.contiguous()
-    scale = None if scale is None else scale.contiguous()
-    if grad and (x.requires_grad or down.requires_grad or up.requires_grad or (base is not None and base.requires_grad)):
-        if out is not None:
-            raise ValueError("out cannot be given where a gradient is asked for")
-        return _LoraBatched.apply(x, base, down, up, offsets, adapters, scale, _impl)
-    if out is None:
-        out = x.new_empty((*x.shape[:-1], N))
-    _forward(x, base, down, up, offsets, adapters, scale, out, _impl)
-    return out
+    if out is not None and grad and (x.requires_grad or down.requires_grad or up.requires_grad or (base is not None and base.requires_grad)):
+        raise ValueError("out cannot be given where a gradient is asked for")
+    return L.binding().lora_batched(
+        x, down.contiguous(), up.contiguous(), offsets.contiguous(), adapters.contiguous(), base,
+        None if scale is None else scale.contiguous(), out, _impl, L.status_word(x.device).data_ptr())

@@ -9,7 +9,6 @@ with torch operators (``rope`` / ``NunchakuFluxPosEmbed``, nunchaku/models/embed
 
 from __future__ import annotations
 
-import ctypes as C
 import functools
 
 import torch
@@ -20,70 +19,21 @@ __all__ = ["rotary_axes", "rotary_table"]
 
 
 @functools.lru_cache(maxsize=64)
-def _ladder(axes_dim: tuple, theta: float) -> L.RotaryLadder:
+def _ladder(axes_dim: tuple, theta: float):
+    """The rates of the axes' pairs, made once per (axes, theta)."""
     if not 1 <= len(axes_dim) <= L.ROTARY_MAX_AXES:
         raise ValueError(f"1 to {L.ROTARY_MAX_AXES} axes, got {len(axes_dim)}")
     if any(d <= 0 or d % 2 for d in axes_dim) or sum(axes_dim) > 2 * L.ROTARY_MAX_PAIRS:
         raise ValueError(f"the axes' channels must be even, positive and at most {2 * L.ROTARY_MAX_PAIRS} together: {axes_dim}")
-    ladder = L.RotaryLadder()
-    L.check(L.lib().nb_rotary_ladder_init(ladder, (C.c_int32 * len(axes_dim))(*axes_dim), len(axes_dim), theta), "rotary ladder")
-    return ladder
+    return L.binding().Ladder(axes_dim, theta)
 
 
-def _ids_strides(ids: torch.Tensor, n_axes: int, batch: int, rows: int):
+def _check_ids(ids: torch.Tensor, n_axes: int, batch: int, rows: int) -> None:
     if ids.dtype not in L.IDS_CODE:
         raise ValueError(f"ids must be float32, float64, int32 or int64, got {ids.dtype}")
-    if ids.shape not in ((rows, n_axes), (batch, rows, n_axes)):
-        raise ValueError(f"ids must be ({rows}, {n_axes}) or ({batch}, {rows}, {n_axes}), got {tuple(ids.shape)}")
-    st = ids.stride()
-    return st if len(st) == 3 else (0, *st)
-
-
-def _rotate(q, k, ids, ladder, half, inverse):
-    """(rotated q, rotated k): one launch over the heads of both; ``k`` may be ``None``."""
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if k is not None and k.stride(3) != 1:
-        k = k.contiguous()
-    B, S, H, D = q.shape
-    qo = q.new_empty(q.shape)
-    ko = None if k is None else q.new_empty(k.shape)
-    a = L.RotaryArgs()
-    a.q, a.q_out, a.ids = q.data_ptr(), qo.data_ptr(), ids.data_ptr()
-    a.stride_qb, a.stride_qs, a.stride_qh, _ = q.stride()
-    a.B, a.S, a.H, a.D = B, S, H, D
-    if k is not None:
-        a.k, a.k_out, a.Hk = k.data_ptr(), ko.data_ptr(), k.shape[2]
-        a.stride_kb, a.stride_ks, a.stride_kh, _ = k.stride()
-    a.stride_ib, a.stride_is, a.stride_ia = _ids_strides(ids, ladder.n_axes, B, S)
-    a.dtype, a.ids_type = L.DTYPE_CODE_32[q.dtype], L.IDS_CODE[ids.dtype]
-    a.half, a.inverse = half, inverse
-    L.launch(L.lib().nb_rotary_axes, "rotary_axes", q, a, ladder)
-    return qo, ko
-
-
-class _RotaryAxes(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, ids, ladder, half, inverse):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(ids)
-        ctx.consts = ladder, half, inverse
-        return _rotate(q, k, ids, ladder, half, inverse)
-
-    @staticmethod
-    @L.once_differentiable
-    def backward(ctx, dq, dk):
-        (ids,) = ctx.saved_tensors
-        ladder, half, inverse = ctx.consts
-        if not ctx.needs_input_grad[0]:
-            dq = None
-        if not ctx.needs_input_grad[1]:
-            dk = None
-        if dq is not None:
-            dq, dk = _rotate(dq, dk, ids, ladder, half, not inverse)
-        elif dk is not None:
-            dk, _ = _rotate(dk, None, ids, ladder, half, not inverse)
-        return dq, dk, None, None, None, None
+    shape = ids.shape
+    if shape != (rows, n_axes) and shape != (batch, rows, n_axes):
+        raise ValueError(f"ids must be ({rows}, {n_axes}) or ({batch}, {rows}, {n_axes}), got {tuple(shape)}")
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes_dim, theta: float = 10000.0,
@@ -107,17 +57,14 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes
         raise ValueError(f"k must be (B, S, Hk, D) beside q, got {tuple(k.shape)} {k.dtype} for {tuple(q.shape)} {q.dtype}")
     ladder = _ladder(tuple(axes_dim), float(theta))
     B, S, H, D = q.shape
-    _ids_strides(ids, ladder.n_axes, B, S)
-    if 2 * ladder.pair_end[ladder.n_axes - 1] > D:
+    _check_ids(ids, ladder.n_axes, B, S)
+    if 2 * ladder.pairs > D:
         raise ValueError(f"axes {tuple(axes_dim)} have more channels than a head ({D})")
     if H == 0 or (k is not None and k.shape[2] == 0):
         raise ValueError("no heads")
     L.require_cuda(q, k, ids)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        out = _RotaryAxes.apply(q, k, ids, ladder, not interleaved, inverse)
-    else:
-        out = _rotate(q, k, ids, ladder, not interleaved, inverse)
-    return out[0] if k is None else out
+    out = L.binding().rotary_axes(q, k, ids, ladder, not interleaved, inverse)
+    return out[0] if k is None else (out[0], out[1])
 
 
 def rotary_table(ids: torch.Tensor, axes_dim, theta: float = 10000.0) -> torch.Tensor:
@@ -129,9 +76,6 @@ def rotary_table(ids: torch.Tensor, axes_dim, theta: float = 10000.0) -> torch.T
         raise ValueError(f"ids must be (S, axes) or (B, S, axes), got {tuple(ids.shape)}")
     ladder = _ladder(tuple(axes_dim), float(theta))
     B, S = (1, ids.shape[0]) if ids.dim() == 2 else ids.shape[:2]
-    st = _ids_strides(ids, ladder.n_axes, B, S)
-    pairs = ladder.pair_end[ladder.n_axes - 1]
+    _check_ids(ids, ladder.n_axes, B, S)
     L.require_cuda(ids)
-    out = ids.new_empty((*ids.shape[:-1], pairs, 1, 2), dtype=torch.float32)
-    L.launch(L.lib().nb_rotary_table, "rotary_table", out, ids.data_ptr(), L.IDS_CODE[ids.dtype], B, S, *st, out.data_ptr(), ladder)
-    return out
+    return L.binding().rotary_table(ids, ladder)

@@ -226,11 +226,11 @@ def test_layernorm_modulate_keeps_its_values_and_has_gradients(cuda_dev, dtype):
 def test_layer_norm_captured_on_another_stream(cuda_dev):
     x = torch.randn(64, 768, device=cuda_dev).to(BF16)
     w, b, dy = torch.randn(768, device=cuda_dev), torch.randn(768, device=cuda_dev), torch.randn(64, 768, device=cuda_dev).to(BF16)
-    from nunchaku_rocm_b200.ops.elementwise import _ln_backward, _ln_forward
-
+    ops = L.binding()
     stats = torch.empty(2, 64, device=cuda_dev)
     y = torch.empty_like(x)
-    _ln_forward(x, w, b, 1e-6, 0.0, y, stats)
+    ops.layer_norm_forward(x, w, b, 1e-6, 0.0, y, stats)
+    backward = lambda: ops.layer_norm_backward(x, w, b, stats, dy, 1e-6, 0.0, True, True, True)  # noqa: E731
     s = torch.cuda.Stream()
     graphs, outs = [], []
     s.wait_stream(torch.cuda.current_stream())
@@ -238,18 +238,18 @@ def test_layer_norm_captured_on_another_stream(cuda_dev):
         for _ in range(2):  # two graphs, each with a workspace of its own
             gr = torch.cuda.CUDAGraph()
             with torch.cuda.graph(gr, stream=s):
-                outs.append((layer_norm(x, w, b), *_ln_backward(x, w, b, stats, dy, 1e-6, 0.0, (True, True, True))))
+                outs.append((layer_norm(x, w, b), *backward()))
             graphs.append(gr)
     torch.cuda.current_stream().wait_stream(s)
     x.copy_(torch.randn(64, 768, device=cuda_dev))
-    _ln_forward(x, w, b, 1e-6, 0.0, None, stats)
+    ops.layer_norm_forward(x, w, b, 1e-6, 0.0, None, stats)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
     for gr, st in zip(graphs, streams):
         with torch.cuda.stream(st):
             gr.replay()
     torch.cuda.synchronize()
-    want = (layer_norm(x, w, b), *_ln_backward(x, w, b, stats, dy, 1e-6, 0.0, (True, True, True)))
+    want = (layer_norm(x, w, b), *backward())
     for out in outs:
         assert all(torch.equal(p, q) for p, q in zip(out, want))
 
