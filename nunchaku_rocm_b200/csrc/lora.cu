@@ -77,6 +77,7 @@ template <typename T, int RM, bool RCONTIG>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraParams p) {
     using S = ShrinkTile<RM, RCONTIG>;
     extern __shared__ __align__(128) unsigned char smem[];
+    chain_next();
     const Item it = find_item<kThreads>(p, blockIdx.x);
     if (it.rows == 0 || it.adapter < 0) return;  // every CTA of the cluster
     const int splits = gridDim.y, split = blockIdx.y;
@@ -215,6 +216,7 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
     const T* base = static_cast<const T*>(p.x);
     T* out = static_cast<T*>(p.out);
     if (it.adapter < 0) {  // base alone (zeros without one)
+        chain_wait();
         if (base == out) return;
         const int n = (col1 - col0) / 8;
         for (int e = t; e < it.rows * n; e += kThreads) {
@@ -265,8 +267,23 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
     };
     issue(0);
 
-    uint32_t hi[RM][4], lo[RM][4];
     const int row0 = m * 16 + (lane >> 2), row1 = row0 + 8;
+    const long long at0 = (long long)(it.first + row0), at1 = (long long)(it.first + row1);
+    // base of the warp's groups of 32 columns of a tile, fetched a tile ahead
+    constexpr int GROUPS = BN / 32;
+    uint4 b0[GROUPS], b1[GROUPS];
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const int q = share + i * wn, c = col0 + tile * BN + q * 32 + (lane & 3) * 8;
+            const bool on = base && tile < tiles && q < GROUPS && c < col1;
+            b0[i] = on && row0 < it.rows ? *reinterpret_cast<const uint4*>(base + at0 * p.stride_x + c) : make_uint4(0, 0, 0, 0);
+            b1[i] = on && row1 < it.rows ? *reinterpret_cast<const uint4*>(base + at1 * p.stride_x + c) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    fetch(0);
+    chain_wait();
+    uint32_t hi[RM][4], lo[RM][4];
     {
         const char* ph = static_cast<const char*>(p.hi);
         const char* pl = static_cast<const char*>(p.lo);
@@ -281,50 +298,47 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
                 lo[k][i] = real ? *reinterpret_cast<const uint32_t*>(pl + at) : 0u;
             }
     }
-    const long long at0 = (long long)(it.first + row0), at1 = (long long)(it.first + row1);
     for (int tile = 0; tile < tiles; ++tile) {
         const int c0 = col0 + tile * BN;
         land(tile);
         __syncthreads();
         issue(tile + 1);
-        if (m < mt) {
-            const unsigned char* gs = smem + (tile & 1) * S::GBYTES;
-            for (int q = share; q < BN / 32; q += wn) {
-                const int c = c0 + q * 32 + (lane & 3) * 8;
-                const bool on0 = row0 < it.rows && c < col1, on1 = row1 < it.rows && c < col1;
-                uint4 b0 = make_uint4(0, 0, 0, 0), b1 = b0;
-                if (base && on0) b0 = *reinterpret_cast<const uint4*>(base + at0 * p.stride_x + c);
-                if (base && on1) b1 = *reinterpret_cast<const uint4*>(base + at1 * p.stride_x + c);
-                float acc[4][4];
+        const unsigned char* gs = smem + (tile & 1) * S::GBYTES;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        for (int g32 = 0; g32 < GROUPS; ++g32) {
+            const int q = share + g32 * wn;
+            if (m >= mt || q >= GROUPS) break;
+            const int c = c0 + q * 32 + (lane & 3) * 8;
+            float acc[4][4];
 #pragma unroll
-                for (int k = 0; k < RM; ++k) {
-                    uint32_t b[2][4];
+            for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {  // instructions 2h and 2h + 1 of the four
-                        if constexpr (CCONTIG) {
-                            ldsm4t(b[h], smem_u32(gs) + (k * 16 + (lane & 15)) * S::GROW + q * 64 + h * 32 + (lane >> 4) * 16);
-                        } else {
-                            const int j = 2 * h + (lane >> 4), i = lane & 7;
-                            const int n = q * 32 + (i >> 1) * 8 + j * 2 + (i & 1);
-                            ldsm4(b[h], smem_u32(gs) + n * S::GROW + (n >> 3) * 32 + k * 32 + ((lane >> 3) & 1) * 16);
-                        }
-                        mma16816<T>(acc[2 * h], hi[k], b[h][0], b[h][1]);
-                        mma16816<T>(acc[2 * h + 1], hi[k], b[h][2], b[h][3]);
-                        mma16816<T>(acc[2 * h], lo[k], b[h][0], b[h][1]);
-                        mma16816<T>(acc[2 * h + 1], lo[k], b[h][2], b[h][3]);
+            for (int k = 0; k < RM; ++k) {
+                uint32_t b[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // instructions 2h and 2h + 1 of the four
+                    if constexpr (CCONTIG) {
+                        ldsm4t(b[h], smem_u32(gs) + (k * 16 + (lane & 15)) * S::GROW + q * 64 + h * 32 + (lane >> 4) * 16);
+                    } else {
+                        const int j = 2 * h + (lane >> 4), i = lane & 7;
+                        const int n = q * 32 + (i >> 1) * 8 + j * 2 + (i & 1);
+                        ldsm4(b[h], smem_u32(gs) + n * S::GROW + (n >> 3) * 32 + k * 32 + ((lane >> 3) & 1) * 16);
                     }
+                    mma16816<T>(acc[2 * h], hi[k], b[h][0], b[h][1]);
+                    mma16816<T>(acc[2 * h + 1], hi[k], b[h][2], b[h][3]);
+                    mma16816<T>(acc[2 * h], lo[k], b[h][0], b[h][1]);
+                    mma16816<T>(acc[2 * h + 1], lo[k], b[h][2], b[h][3]);
                 }
-                auto joined = [&](const uint4& b, int o) {
-                    const float2 f0 = unpack2<T>(b.x), f1 = unpack2<T>(b.y), f2 = unpack2<T>(b.z), f3 = unpack2<T>(b.w);
-                    return make_uint4(pack2<T>(f0.x + acc[0][o], f0.y + acc[0][o + 1]), pack2<T>(f1.x + acc[1][o], f1.y + acc[1][o + 1]),
-                                      pack2<T>(f2.x + acc[2][o], f2.y + acc[2][o + 1]), pack2<T>(f3.x + acc[3][o], f3.y + acc[3][o + 1]));
-                };
-                if (on0) *reinterpret_cast<uint4*>(out + at0 * p.stride_out + c) = joined(b0, 0);
-                if (on1) *reinterpret_cast<uint4*>(out + at1 * p.stride_out + c) = joined(b1, 2);
             }
+            auto joined = [&](const uint4& b, int o) {
+                const float2 f0 = unpack2<T>(b.x), f1 = unpack2<T>(b.y), f2 = unpack2<T>(b.z), f3 = unpack2<T>(b.w);
+                return make_uint4(pack2<T>(f0.x + acc[0][o], f0.y + acc[0][o + 1]), pack2<T>(f1.x + acc[1][o], f1.y + acc[1][o + 1]),
+                                  pack2<T>(f2.x + acc[2][o], f2.y + acc[2][o + 1]), pack2<T>(f3.x + acc[3][o], f3.y + acc[3][o + 1]));
+            };
+            if (row0 < it.rows && c < col1) *reinterpret_cast<uint4*>(out + at0 * p.stride_out + c) = joined(b0[g32], 0);
+            if (row1 < it.rows && c < col1) *reinterpret_cast<uint4*>(out + at1 * p.stride_out + c) = joined(b1[g32], 2);
         }
+        fetch(tile + 1);
     }
 }
 
@@ -344,7 +358,9 @@ __global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p
     extern __shared__ __align__(128) unsigned char smem[];
     // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
     const int w = gridDim.y - 1 - blockIdx.y;
+    chain_next();
     const Item it = find_item<kThreads>(p, w);
+    chain_wait();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     if (blockIdx.x == 0 && t == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
     if (it.rows == 0 || it.adapter < 0) return;
@@ -456,6 +472,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) lora_join_kernel(const float* part, const int* item_adapter, int items, long long size, T* out) {
     __shared__ int mine[256];
     __shared__ int count;
+    chain_next();
+    chain_wait();
     const int a = blockIdx.y, t = threadIdx.x;
     const long long at = ((long long)blockIdx.x * 256 + t) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -523,20 +541,7 @@ int shrink(const LoraParams& p, cudaStream_t s) {
     while (splits < 8 && live * splits < 2 * sms() && ceil_div(p.K, 64) >= 4 * splits) splits *= 2;
     auto* kernel = lora_shrink_kernel<T, RM, RCONTIG>;
     if (int rc = allow_smem(kernel, S::BYTES)) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(items, splits);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = S::BYTES;
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = 1;
-    at.val.clusterDim.y = splits;
-    at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    NB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
-    return NB_OK;
+    return launch(kernel, dim3(items, splits), kThreads, S::BYTES, splits, p.chained, s, p);
 }
 template <typename T, int RM, bool CCONTIG>
 int expand(LoraParams p, cudaStream_t s) {
@@ -548,9 +553,7 @@ int expand(LoraParams p, cudaStream_t s) {
     p.cols_per_cta = ceil_div(tiles, per < tiles ? per : tiles) * S::BN;
     auto* kernel = lora_expand_kernel<T, RM, CCONTIG>;
     if (int rc = allow_smem(kernel, S::BYTES)) return rc;
-    kernel<<<dim3(ceil_div(p.K, p.cols_per_cta), items), kThreads, S::BYTES, s>>>(p);
-    NB_CUDA_CHECK(cudaGetLastError());
-    return NB_OK;
+    return launch(kernel, dim3(ceil_div(p.K, p.cols_per_cta), items), kThreads, S::BYTES, 1, p.chained, s, p);
 }
 template <typename T, int RM, bool KROWS>
 int outer(const nb_lora_args* a, LoraParams p, T* grad, cudaStream_t s) {
@@ -560,15 +563,11 @@ int outer(const nb_lora_args* a, LoraParams p, T* grad, cudaStream_t s) {
     auto small = [&]() -> int {
         auto* kernel = lora_outer_kernel<T, RM, KROWS>;
         if (int rc = allow_smem(kernel, S::BYTES)) return rc;
-        kernel<<<dim3(ceil_div(p.K, 128), items), kThreads, S::BYTES, s>>>(p);
-        NB_CUDA_CHECK(cudaGetLastError());
-        return NB_OK;
+        return launch(kernel, dim3(ceil_div(p.K, 128), items), kThreads, S::BYTES, 1, p.chained, s, p);
     };
     if (int rc = NB_TC_OR(a, tc_outer(p, KROWS, a->dtype, s), small())) return rc;
     const long long size = (long long)p.R * p.K;
-    lora_join_kernel<T><<<dim3(ceil_div(size, 1024), p.A), 256, 0, s>>>(p.part, p.item_adapter, items, size, grad);
-    NB_CUDA_CHECK(cudaGetLastError());
-    return NB_OK;
+    return launch(lora_join_kernel<T>, dim3(ceil_div(size, 1024), p.A), 256, 0, 1, true, s, p.part, p.item_adapter, items, size, grad);
 }
 
 LoraParams params_of(const nb_lora_args* a) {
@@ -588,6 +587,7 @@ int forward_t(const nb_lora_args* a, cudaStream_t s) {
     p.lo = plane(a->h, a, 1);
     p.x = a->x; p.stride_x = a->stride_x; p.factor = a->down; p.K = a->K;
     if (int rc = NB_TC_OR(a, tc_shrink(p, false, a->dtype, s), (shrink<T, RM, false>(p, s)))) return rc;
+    p.chained = true;
     p.x = a->base; p.stride_x = a->stride_base; p.out = a->out; p.stride_out = a->stride_out; p.factor = a->up; p.K = a->N;
     return NB_TC_OR(a, tc_expand(p, false, a->dtype, s), (expand<T, RM, false>(p, s)));
 }
@@ -605,6 +605,7 @@ int backward_t(const nb_lora_args* a, cudaStream_t s) {
         g.x = a->dy; g.stride_x = a->stride_dy; g.factor = a->up; g.K = a->N;
         if (int rc = NB_TC_OR(a, tc_shrink(g, true, a->dtype, s), (shrink<T, RM, true>(g, s)))) return rc;
     }
+    p.chained = a->dx || a->ddown;
     if (a->dup) {
         p.x = a->dy; p.stride_x = a->stride_dy; p.K = a->N;
         p.hi = plane(a->h, a, 0);
@@ -612,6 +613,7 @@ int backward_t(const nb_lora_args* a, cudaStream_t s) {
         if (int rc = outer<T, RM, true>(a, p, static_cast<T*>(a->dup), s)) return rc;
     }
     g.K = a->K;
+    g.chained = true;
     if (a->ddown) {
         g.x = a->x; g.stride_x = a->stride_x;
         if (int rc = outer<T, RM, false>(a, g, static_cast<T*>(a->ddown), s)) return rc;

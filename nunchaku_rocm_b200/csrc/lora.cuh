@@ -17,6 +17,7 @@ struct LoraParams {
     long long stride_x, stride_out;
     int T, K, R, A, requests;  // K: length of the contraction (shrink), columns (expand, outer)
     int rows_per_item, cols_per_cta;
+    bool chained;         // launched behind a kernel of the same call
     int* status;          // device int32, set non-zero when a bounded wait expires; may be null
 };
 
@@ -56,6 +57,37 @@ __device__ __forceinline__ Item find_item(const LoraParams& p, int w) {
         it.adapter = a >= 0 && a < p.A ? a : -1;
     }
     return it;
+}
+
+// The kernels of a call form a chain: each is launched while the one before it still runs (programmatic stream
+// serialization), does what does not depend on it - finding its item, loading the factor and base - and waits for its end
+// before it reads what it wrote, or writes what it may still read.  A kernel that has ended has waited for the one before
+// it, so the wait covers all of the chain; its first kernel is launched as usual, after everything before the call.
+__device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster_y, bool chained, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (cluster_y > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = 1;
+        at[n].val.clusterDim.y = cluster_y;
+        at[n++].val.clusterDim.z = 1;
+    }
+    if (chained) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    NB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+    return NB_OK;
 }
 
 inline int sms() {

@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
                                                               const LoraParams p) {
     using S = ShrinkTc<RP>;
     extern __shared__ unsigned char raw[];
+    chain_next();
     const Item it = find_item<S::THREADS>(p, blockIdx.x);
     if (it.rows == 0 || it.adapter < 0) return;  // every CTA of the cluster
     uint8_t* smem = align1k(raw);
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
     const T* in = static_cast<const T*>(p.x);
     T* out = static_cast<T*>(p.out);
     if (it.adapter < 0) {  // base alone (zeros without one)
+        chain_wait();
         if (in == out) return;
         const int n = (col1 - col0) / 8;
         for (int e = threadIdx.x; e < it.rows * n; e += S::THREADS) {
@@ -286,11 +288,6 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
             tma_prefetch_desc(&tm_g);
             tma_prefetch_desc(&tm_base);
             tma_prefetch_desc(&tm_out);
-            mbar_expect_tx(bar(V), 2 * S::VB);
-            for (int h = 0; h < S::HALVES; ++h) {
-                tma_load_2d(sb + h * kTcRows * 128, &tm_hi, bar(V), h * 64, it.first);
-                tma_load_2d(sb + S::VB + h * kTcRows * 128, &tm_lo, bar(V), h * 64, it.first);
-            }
             bool ok = true;
             for (int i = 0; i < tiles; ++i) {
                 const int c = col0 + i * 64, gs = i % S::GST, ls = i % S::SLOTS;
@@ -307,6 +304,14 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
                     if (i >= S::SLOTS && !mbar_wait(bar(LE + ls), ((i / S::SLOTS) & 1) ^ 1, abort_s, E_EXPAND | 2, 50)) { ok = false; break; }
                     mbar_expect_tx(bar(LF + ls), S::SLOT);
                     tma_load_2d(sb + S::OFF_S + ls * S::SLOT, &tm_base, bar(LF + ls), c, it.first);
+                }
+                if (i == min(S::GST, tiles) - 1) {  // the ring is filled as far as it goes without the kernel before this one
+                    chain_wait();
+                    mbar_expect_tx(bar(V), 2 * S::VB);
+                    for (int h = 0; h < S::HALVES; ++h) {
+                        tma_load_2d(sb + h * kTcRows * 128, &tm_hi, bar(V), h * 64, it.first);
+                        tma_load_2d(sb + S::VB + h * kTcRows * 128, &tm_lo, bar(V), h * 64, it.first);
+                    }
                 }
             }
             if (!ok) let_copies_land();
@@ -420,7 +425,9 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
     extern __shared__ unsigned char raw[];
     // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
     const int w = gridDim.y - 1 - blockIdx.y;
+    chain_next();
     const Item it = find_item<S::THREADS>(p, w);
+    chain_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
     if (it.rows == 0 || it.adapter < 0) return;
     uint8_t* smem = align1k(raw);
@@ -581,20 +588,7 @@ int shrink(LoraParams p, cudaStream_t s) {
     if (splits > ceil_div(p.K, 4 * KB)) splits = ceil_div(p.K, 4 * KB);
     if (splits > 8) splits = 8;
     if (splits < 1) splits = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(items, splits);
-    cfg.blockDim = dim3(S::THREADS);
-    cfg.dynamicSmemBytes = S::BYTES;
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = 1;
-    at.val.clusterDim.y = splits;
-    at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    NB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, x, f, p));
-    return NB_OK;
+    return launch(kernel, dim3(items, splits), S::THREADS, S::BYTES, splits, p.chained, s, x, f, p);
 }
 template <typename T, int RP, bool CCONTIG>
 int expand(LoraParams p, cudaStream_t s) {
@@ -622,9 +616,7 @@ int expand(LoraParams p, cudaStream_t s) {
         if (cost < best) best = cost, per = t;
     }
     p.cols_per_cta = per * 64;
-    kernel<<<dim3(ceil_div(tiles, per), items), S::THREADS, S::BYTES, s>>>(hi, lo, g, base, out, p);
-    NB_CUDA_CHECK(cudaGetLastError());
-    return NB_OK;
+    return launch(kernel, dim3(ceil_div(tiles, per), items), S::THREADS, S::BYTES, 1, p.chained, s, hi, lo, g, base, out, p);
 }
 template <typename T, int RP, bool KROWS>
 int outer(const LoraParams& p, cudaStream_t s) {
@@ -634,9 +626,7 @@ int outer(const LoraParams& p, cudaStream_t s) {
     CUtensorMap x, hi, lo;
     if (!(make_map<T>(&x, p.x, p.T, p.K, p.stride_x, KB) && make_map<T>(&hi, p.hi, p.T, p.R, p.R, KB) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, KB)))
         return NB_ERR_UNSUPPORTED;
-    kernel<<<dim3(ceil_div(p.K, 128), item_count(p.T, p.requests, p.rows_per_item)), S::THREADS, S::BYTES, s>>>(x, hi, lo, p);
-    NB_CUDA_CHECK(cudaGetLastError());
-    return NB_OK;
+    return launch(kernel, dim3(ceil_div(p.K, 128), item_count(p.T, p.requests, p.rows_per_item)), S::THREADS, S::BYTES, 1, p.chained, s, x, hi, lo, p);
 }
 
 #define NB_LORA_RP(CALL)                         \
