@@ -737,7 +737,7 @@ Shape shape_of(int groups, int rows, int dim, int size, bool backward, bool ring
         s.teams = 1;
     }
     const int slot = s.team * s.teams * s.u * 8 * size * (backward ? 2 : 1);
-    s.st = !ring ? 0 : slot * 8 <= kSmemPerSm / 2 ? 8 : slot * 4 <= kSmemPerSm ? 4 : 0;
+    s.st = !ring ? 0 : slot * 8 <= kSmemPerSm / (backward ? 3 : 2) ? 8 : slot * 4 <= kSmemPerSm ? 4 : 0;
     s.smem = s.st * slot;
     const int joined = backward && s.teams > 1 ? s.teams * 2 * dim * 4 : 0;  // at most 8 x 2 x 512 x 4 = 32 KB
     if (s.smem < joined) s.smem = joined;

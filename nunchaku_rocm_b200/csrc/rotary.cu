@@ -70,12 +70,19 @@ __device__ __forceinline__ int axis_of(const nb_rotary_ladder& l, int pair) {
     return a;
 }
 
-// (cos, sin) of `turns` whole turns
+// (cos, sin) of `turns` whole turns.  Whole turns and then the nearest quarter are taken off in fp64; what is left, y of at
+// most pi / 4, goes through the Taylor series in fp32 (first terms left out: y^11 / 11! and y^12 / 12!, under 2^-28), and
+// the quarter turns it by swaps and signs.  (The library's sincospif reduces once more and took twice as long; where there
+// are few heads per token the angles are what the kernel waits for.)
 __device__ __forceinline__ float2 cos_sin_turns(double turns) {
-    const double part = turns - rint(turns);  // [-1/2, 1/2]
-    const double quarter = rint(4.0 * part);
-    float s, c;
-    sincospif((float)(2.0 * (part - 0.25 * quarter)), &s, &c);  // |argument| <= 1/4
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    const double part = turns - __dadd_rn(__dadd_rn(turns, kRound), -kRound);  // [-1/2, 1/2]
+    const float quarter = rintf(4.f * (float)part);
+    const float f = (float)fma(-0.25, (double)quarter, part);
+    const float y = fmaf(f, -1.7484556e-7f, f * 6.2831855f);  // f * 2 pi, the constant in two parts
+    const float z = y * y;
+    const float s = fmaf(y * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), y);
+    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
     const int n = (int)quarter & 3;
     const float cs = (n & 1) ? s : c, sn = (n & 1) ? c : s;
     return make_float2((n == 1 || n == 2) ? -cs : cs, (n >= 2) ? -sn : sn);
@@ -143,7 +150,7 @@ __device__ __forceinline__ Item locate(const RotParams& p, uint32_t row0, uint32
 // VEC: an item is 16 bytes of a head (interleaved), two 16-byte pieces R/2 apart (HALF), or 16 bytes that pass through.
 // Otherwise an item is one channel pair or one channel that passes through: every size and alignment.
 template <typename T, bool HALF, bool VEC>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotParams p) {
+__global__ void __launch_bounds__(kThreads, HALF ? 4 : 5) rotary_kernel(const __grid_constant__ RotParams p) {
     extern __shared__ float2 cs[];  // [tok][pairs]
     const uint32_t row0 = blockIdx.x * (uint32_t)p.tok;
     const int ntok = (int)min((uint32_t)p.tok, p.rows - row0);
@@ -152,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     // The first items' loads are issued before the angles are computed, so that they travel meanwhile.
     constexpr int N = Vec<T>::N;
     constexpr int PER = HALF ? N : N / 2;  // pairs of an item
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = HALF ? 4 : 3;
     const int steps = p.pairs / PER;
     Item it[AHEAD];
     uint4 r0[AHEAD], r1[AHEAD];
@@ -176,14 +183,19 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     };
     fetch(threadIdx.x);
 
-    for (int i = threadIdx.x; i < ntok * p.pairs; i += kThreads) {
-        const int tok = i / p.pairs, pair = i - tok * p.pairs;
-        const uint32_t row = row0 + tok, b = fastdiv(row, p.div_s), s = row - b * p.div_s.d;
-        const double pos = load_id(p.ids, p.ids_type, b * p.si_b + s * p.si_s + axis_of(p.ladder, pair) * p.si_a);
-        float2 v = cos_sin_turns(pos * p.ladder.turns[pair]);
-        v.y *= p.sign;
+    // a thread keeps its pair (one rate, one axis) and walks over the tokens
+    const int pair = threadIdx.x % p.pairs, per = kThreads / p.pairs;
+    if (threadIdx.x < per * p.pairs) {
+        const double rate = p.ladder.turns[pair];
+        const long long axis = axis_of(p.ladder, pair) * p.si_a;
         // VEC: the PER pairs of an item lie pairs / PER apart, so that the lanes of a warp read neighbouring words
-        cs[VEC ? tok * p.pairs + (pair % PER) * steps + pair / PER : i] = v;
+        const int at = VEC ? (pair % PER) * steps + pair / PER : pair;
+        for (int tok = threadIdx.x / p.pairs; tok < ntok; tok += per) {
+            const uint32_t row = row0 + tok, b = fastdiv(row, p.div_s), s = row - b * p.div_s.d;
+            float2 v = cos_sin_turns(load_id(p.ids, p.ids_type, b * p.si_b + s * p.si_s + axis) * rate);
+            v.y *= p.sign;
+            cs[tok * p.pairs + at] = v;
+        }
     }
     __syncthreads();
 
