@@ -467,22 +467,33 @@ __global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p
             }
 }
 
-// dF[a] = sum of the partial products of a's items, in the items' order; zero for an adapter without rows
+// dF[a] = sum of the partial products of a's items, in the items' order; zero for an adapter without rows.  One launch for
+// both factors: `blocks` CTAs (of 1024 values each) for the first, the rest for the second.
 template <typename T>
-__global__ void __launch_bounds__(256) lora_join_kernel(const float* part, const int* item_adapter, int items, long long size, T* out) {
+struct Join {
+    const float* part;
+    const int* item_adapter;
+    T* out;
+    long long size;
+    int items, blocks;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) lora_join_kernel(const Join<T> first, const Join<T> second) {
     __shared__ int mine[256];
     __shared__ int count;
     chain_next();
     chain_wait();
+    const bool one = (int)blockIdx.x < first.blocks;
+    const Join<T>& j = one ? first : second;
     const int a = blockIdx.y, t = threadIdx.x;
-    const long long at = ((long long)blockIdx.x * 256 + t) * 4;
+    const long long at = ((long long)(one ? blockIdx.x : blockIdx.x - first.blocks) * 256 + t) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w0 = 0; w0 < items; w0 += 256) {
+    for (int w0 = 0; w0 < j.items; w0 += 256) {
         __syncthreads();
         if (t < 32) {  // the items of this adapter, in order
             int n = 0;
-            for (int w = w0; w < min(w0 + 256, items); w += 32) {
-                const bool hit = w + t < items && __ldg(item_adapter + w + t) == a;
+            for (int w = w0; w < min(w0 + 256, j.items); w += 32) {
+                const bool hit = w + t < j.items && j.item_adapter[w + t] == a;
                 const unsigned b = __ballot_sync(0xffffffffu, hit);
                 if (hit) mine[n + __popc(b & ((1u << t) - 1))] = w + t;
                 n += __popc(b);
@@ -490,13 +501,15 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const float* part, const
             if (t == 0) count = n;
         }
         __syncthreads();
-        if (at < size)
+        if (at < j.size) {
+#pragma unroll 4
             for (int i = 0; i < count; ++i) {
-                const float4 v = *reinterpret_cast<const float4*>(part + (long long)mine[i] * size + at);
+                const float4 v = *reinterpret_cast<const float4*>(j.part + (long long)mine[i] * j.size + at);
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
+        }
     }
-    if (at < size) *reinterpret_cast<uint2*>(out + (long long)a * size + at) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+    if (at < j.size) *reinterpret_cast<uint2*>(j.out + (long long)a * j.size + at) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
 }
 
 // --------------------------------------------------------------------------------------------------------------- launchers
@@ -556,7 +569,7 @@ int expand(LoraParams p, cudaStream_t s) {
     return launch(kernel, dim3(ceil_div(p.K, p.cols_per_cta), items), kThreads, S::BYTES, 1, p.chained, s, p);
 }
 template <typename T, int RM, bool KROWS>
-int outer(const nb_lora_args* a, LoraParams p, T* grad, cudaStream_t s) {
+int outer(const nb_lora_args* a, LoraParams p, cudaStream_t s) {
     using S = OuterTile<RM>;
     p.rows_per_item = outer_rows(a, p.K);
     const int items = item_count(p.T, p.requests, p.rows_per_item);
@@ -565,9 +578,21 @@ int outer(const nb_lora_args* a, LoraParams p, T* grad, cudaStream_t s) {
         if (int rc = allow_smem(kernel, S::BYTES)) return rc;
         return launch(kernel, dim3(ceil_div(p.K, 128), items), kThreads, S::BYTES, 1, p.chained, s, p);
     };
-    if (int rc = NB_TC_OR(a, tc_outer(p, KROWS, a->dtype, s), small())) return rc;
-    const long long size = (long long)p.R * p.K;
-    return launch(lora_join_kernel<T>, dim3(ceil_div(size, 1024), p.A), 256, 0, 1, true, s, p.part, p.item_adapter, items, size, grad);
+    return NB_TC_OR(a, tc_outer(p, KROWS, a->dtype, s), small());
+}
+
+// The gradients' workspace: for each of the two factors asked for, the items' adapters and their partial products.
+struct Piece {
+    int64_t table, part, end;
+    int items;
+};
+Piece piece_of(const nb_lora_args* a, int cols, int64_t at) {
+    Piece p;
+    p.items = item_count(a->T, a->requests, outer_rows(a, cols));
+    p.table = at;
+    p.part = at + ((int64_t)p.items * 4 + 255) / 256 * 256;
+    p.end = p.part + ((int64_t)p.items * a->R * cols * 4 + 255) / 256 * 256;
+    return p;
 }
 
 LoraParams params_of(const nb_lora_args* a) {
@@ -594,10 +619,6 @@ int forward_t(const nb_lora_args* a, cudaStream_t s) {
 template <typename T, int RM>
 int backward_t(const nb_lora_args* a, cudaStream_t s) {
     LoraParams p = params_of(a);
-    char* ws = static_cast<char*>(a->workspace);
-    p.item_adapter = reinterpret_cast<int*>(ws);
-    ws += ((int64_t)item_count(a->T, a->requests, 128) * 4 + 255) / 256 * 256;
-    p.part = reinterpret_cast<float*>(ws);
     LoraParams g = p;
     if (a->dx || a->ddown) {
         g.hi = plane(a->g, a, 0);
@@ -605,19 +626,35 @@ int backward_t(const nb_lora_args* a, cudaStream_t s) {
         g.x = a->dy; g.stride_x = a->stride_dy; g.factor = a->up; g.K = a->N;
         if (int rc = NB_TC_OR(a, tc_shrink(g, true, a->dtype, s), (shrink<T, RM, true>(g, s)))) return rc;
     }
+    char* ws = static_cast<char*>(a->workspace);
+    int64_t used = 0;
+    Join<T> joins[2] = {};
+    int n = 0;
+    auto join_of = [&](LoraParams& q, int cols, void* grad) {
+        const Piece w = piece_of(a, cols, used);
+        used = w.end;
+        q.item_adapter = reinterpret_cast<int*>(ws + w.table);
+        q.part = reinterpret_cast<float*>(ws + w.part);
+        const long long size = (long long)a->R * cols;
+        joins[n++] = {q.part, q.item_adapter, static_cast<T*>(grad), size, w.items, ceil_div(size, 1024)};
+    };
     p.chained = a->dx || a->ddown;
     if (a->dup) {
         p.x = a->dy; p.stride_x = a->stride_dy; p.K = a->N;
         p.hi = plane(a->h, a, 0);
         p.lo = plane(a->h, a, 1);
-        if (int rc = outer<T, RM, true>(a, p, static_cast<T*>(a->dup), s)) return rc;
+        join_of(p, a->N, a->dup);
+        if (int rc = outer<T, RM, true>(a, p, s)) return rc;
     }
     g.K = a->K;
     g.chained = true;
     if (a->ddown) {
         g.x = a->x; g.stride_x = a->stride_x;
-        if (int rc = outer<T, RM, false>(a, g, static_cast<T*>(a->ddown), s)) return rc;
+        join_of(g, a->K, a->ddown);
+        if (int rc = outer<T, RM, false>(a, g, s)) return rc;
     }
+    if (n)
+        if (int rc = launch(lora_join_kernel<T>, dim3(joins[0].blocks + joins[1].blocks, a->A), 256, 0, 1, true, s, joins[0], joins[1])) return rc;
     if (a->dx) {
         g.x = nullptr; g.out = a->dx; g.stride_out = a->K; g.factor = a->down;
         return NB_TC_OR(a, tc_expand(g, true, a->dtype, s), (expand<T, RM, true>(g, s)));
@@ -654,13 +691,10 @@ extern "C" int64_t nb_lora_workspace_bytes(const nb_lora_args* a) {
     using namespace nb;
     using namespace nb::lora;
     if (check(a) != NB_OK || a->T == 0) return 0;
-    int64_t most = 0;
-    for (int cols : {a->dup ? a->N : 0, a->ddown ? a->K : 0}) {
-        if (!cols) continue;
-        const int64_t n = (int64_t)item_count(a->T, a->requests, outer_rows(a, cols)) * a->R * cols * 4;
-        if (n > most) most = n;
-    }
-    return most ? ((int64_t)item_count(a->T, a->requests, 128) * 4 + 255) / 256 * 256 + most : 0;
+    int64_t bytes = 0;
+    if (a->dup) bytes = piece_of(a, a->N, bytes).end;
+    if (a->ddown) bytes = piece_of(a, a->K, bytes).end;
+    return bytes;
 }
 
 extern "C" int nb_lora_forward(const nb_lora_args* a, void* stream) {

@@ -92,8 +92,6 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
     using S = ShrinkTc<RP>;
     extern __shared__ unsigned char raw[];
     chain_next();
-    const Item it = find_item<S::THREADS>(p, blockIdx.x);
-    if (it.rows == 0 || it.adapter < 0) return;  // every CTA of the cluster
     uint8_t* smem = align1k(raw);
     const uint32_t base = smem_u32(smem), bars = base + S::OFF_BAR;
     auto full = [&](int i) { return bars + 8u * i; };
@@ -102,7 +100,10 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 128);
     volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 136);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (set up while the offsets are on their way)
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tm_x);
+        tma_prefetch_desc(&tm_f);
         for (int i = 0; i < S::ST; ++i) {
             mbar_init(full(i), 1);
             mbar_init(empty(i), 1);
@@ -115,10 +116,15 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
         tmem_alloc(smem_u32(tmem_at), S::COLS);
         tmem_relinquish();
     }
+    const Item it = find_item<S::THREADS>(p, blockIdx.x);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
+    if (it.rows == 0 || it.adapter < 0) {  // every CTA of the cluster
+        if (warp == 1) tmem_dealloc(tmem, S::COLS);
+        return;
+    }
     const int splits = gridDim.y, split = blockIdx.y;
     const int steps = (p.K + KB - 1) / KB, per = (steps + splits - 1) / splits;
     const int step0 = min(split * per, steps), n = min(per, steps - step0);
@@ -127,8 +133,6 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
 
     if (warp == 0) {
         if (lane == 0) {
-            tma_prefetch_desc(&tm_x);
-            tma_prefetch_desc(&tm_f);
             bool ok = true;
             for (int s = 0; s < n; ++s) {
                 const int st = s % S::ST;
@@ -188,22 +192,25 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
     __syncthreads();
     cg::cluster_group cluster = cg::this_cluster();
     if (splits > 1) cluster.sync();
-    const int half = p.R / 2;
-    for (int e = split * S::THREADS + threadIdx.x; e < it.rows * half; e += splits * S::THREADS) {
-        const int row = e / half, r = (e - row * half) * 2;
-        float2 v = make_float2(0.f, 0.f);
-        for (int q = 0; q < splits; ++q) {
-            const float* from = splits > 1 ? cluster.map_shared_rank(sums, q) : sums;
-            const float2 u = *reinterpret_cast<const float2*>(from + row * S::LD + r);
-            v.x += u.x; v.y += u.y;
-        }
-        v.x *= scale; v.y *= scale;
-        const uint32_t hi = pack2<T>(v.x, v.y);
-        const float2 back = unpack2<T>(hi);
-        const uint32_t lo = pack2<T>(isfinite(back.x) ? v.x - back.x : 0.f, isfinite(back.y) ? v.y - back.y : 0.f);
+    // four values of r at a time, the slices' sums in order; all the loads of a value are on their way together
+    const int quads = p.R / 4;
+    for (int e = split * S::THREADS + threadIdx.x; e < it.rows * quads; e += splits * S::THREADS) {
+        const int row = e / quads, r = (e - row * quads) * 4;
+        float4 u[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < splits) u[q] = *reinterpret_cast<const float4*>((splits > 1 ? cluster.map_shared_rank(sums, q) : sums) + row * S::LD + r);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < splits) { v.x += u[q].x; v.y += u[q].y; v.z += u[q].z; v.w += u[q].w; }
+        v.x *= scale; v.y *= scale; v.z *= scale; v.w *= scale;
+        const uint2 hi = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+        const float2 b0 = unpack2<T>(hi.x), b1 = unpack2<T>(hi.y);
+        auto rest = [](float value, float back) { return isfinite(back) ? value - back : 0.f; };  // (beyond T: infinite in hi alone)
+        const uint2 lo = make_uint2(pack2<T>(rest(v.x, b0.x), rest(v.y, b0.y)), pack2<T>(rest(v.z, b1.x), rest(v.w, b1.y)));
         const long long at = ((long long)(it.first + row) * p.R + r) * 2;
-        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.hi) + at) = hi;
-        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.lo) + at) = lo;
+        *reinterpret_cast<uint2*>(static_cast<char*>(p.hi) + at) = hi;
+        *reinterpret_cast<uint2*>(static_cast<char*>(p.lo) + at) = lo;
     }
     if (splits > 1) cluster.sync();
     else __syncthreads();
@@ -285,9 +292,6 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
 
     if (warp == 0) {
         if (lane == 0) {
-            tma_prefetch_desc(&tm_g);
-            tma_prefetch_desc(&tm_base);
-            tma_prefetch_desc(&tm_out);
             bool ok = true;
             for (int i = 0; i < tiles; ++i) {
                 const int c = col0 + i * 64, gs = i % S::GST, ls = i % S::SLOTS;
@@ -423,13 +427,7 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                                                              const __grid_constant__ CUtensorMap tm_lo, const LoraParams p) {
     using S = OuterTc<RP>;
     extern __shared__ unsigned char raw[];
-    // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
-    const int w = gridDim.y - 1 - blockIdx.y;
     chain_next();
-    const Item it = find_item<S::THREADS>(p, w);
-    chain_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
-    if (it.rows == 0 || it.adapter < 0) return;
     uint8_t* smem = align1k(raw);
     const uint32_t sb = smem_u32(smem), bars = sb + S::OFF_BAR;
     auto full = [&](int i) { return bars + 8u * i; };
@@ -438,7 +436,11 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 128);
     volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 136);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (set up while the offsets are on their way)
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tm_x);
+        tma_prefetch_desc(&tm_hi);
+        tma_prefetch_desc(&tm_lo);
         for (int i = 0; i < S::ST; ++i) {
             mbar_init(full(i), 1);
             mbar_init(empty(i), 1);
@@ -451,18 +453,24 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         tmem_alloc(smem_u32(tmem_at), S::COLS);
         tmem_relinquish();
     }
+    // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
+    const int w = gridDim.y - 1 - blockIdx.y;
+    const Item it = find_item<S::THREADS>(p, w);
+    chain_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
+    if (it.rows == 0 || it.adapter < 0) {
+        if (warp == 1) tmem_dealloc(tmem, S::COLS);
+        return;
+    }
     const int c0 = blockIdx.x * 128, n = (it.rows + KB - 1) / KB;
     const bool second = c0 + 64 < p.K;  // the second half of the columns exists
 
     if (warp == 0) {
         if (lane == 0) {
-            tma_prefetch_desc(&tm_x);
-            tma_prefetch_desc(&tm_hi);
-            tma_prefetch_desc(&tm_lo);
             bool ok = true;
             for (int s = 0; s < n; ++s) {
                 const int st = s % S::ST, t0 = it.first + s * KB;
