@@ -527,11 +527,10 @@ bool use_tc(const nb_lora_args* a) {
         return rc_ == NB_ERR_UNSUPPORTED && (a)->impl == NB_IMPL_AUTO ? call : rc_;                            \
     }())
 // rows of the gradients' items: long enough that the partial products stay small beside the operands, short enough that the
-// CTAs (one per item and 128 columns) cover the SMs: one wave of two per SM with the tcgen05 kernels, about four per SM with
-// the small ones
+// CTAs cover the SMs: one wave of one per SM (an item and 256 columns each) with the tcgen05 kernels, about four per SM (128
+// columns) with the small ones
 int outer_rows(const nb_lora_args* a, int cols) {
-    const int tiles = ceil_div(cols, 128);
-    int want = use_tc(a) ? 2 * sms() / tiles : ceil_div(4ll * sms(), tiles);
+    int want = use_tc(a) ? sms() / ceil_div(cols, kTcCols) : ceil_div(4ll * sms(), ceil_div(cols, 128));
     if (want < 1) want = 1;
     const int rows = ceil_div(ceil_div(a->T, want), 64) * 64;
     return rows < 128 ? 128 : rows;

@@ -98,7 +98,7 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // The tcgen05 kernels (lora_tc.cu): the same three products for calls with many rows per request.  `p` as for the kernels in
 // lora.cu, with rows_per_item set by these (kTcRows for shrink and expand).  NB_ERR_UNSUPPORTED: no tensor map, nothing ran.
-constexpr int kTcRows = 128;
+constexpr int kTcRows = 128, kTcCols = 256;  // rows of an item (shrink, expand), columns of a CTA (outer)
 int tc_shrink(LoraParams p, bool rcontig, int dtype, cudaStream_t s);
 int tc_expand(LoraParams p, bool ccontig, int dtype, cudaStream_t s);
 int tc_outer(const LoraParams& p, bool krows, int dtype, cudaStream_t s);

@@ -410,16 +410,18 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------------------------- outer
-// part[item][r, k] (or [k, r] with KROWS) = sum over the item's rows of (hi + lo)[t, r] X[t, k], 128 columns of X per CTA:
-// both operands run along the rows (MN-major), so they are used as they lie.
+// part[item][r, k] (or [k, r] with KROWS) = sum over the item's rows of (hi + lo)[t, r] X[t, k], 256 columns of X per CTA
+// (two accumulators of 128: hi and lo come from the L2 cache once for both, 16 KB beside 32 KB of X at rank 64; with 128
+// columns the cache delivered as much of them as HBM of X).  Both operands run along the rows (MN-major), so they are used
+// as they lie.
 template <int RP>
 struct OuterTc {
     static constexpr int HALVES = RP <= 64 ? 1 : 2;
     static constexpr int TILE = KB * 128;  // 64 rows of 64 values
-    static constexpr int STAGE = (2 + 2 * HALVES) * TILE, ST = RP <= 64 ? 3 : 4;
+    static constexpr int STAGE = (4 + 2 * HALVES) * TILE, ST = RP <= 64 ? 4 : 3;
     static constexpr int OFF_BAR = ST * STAGE;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
-    static constexpr int COLS = RP < 32 ? 32 : RP;
+    static constexpr int ACC = RP < 32 ? 32 : RP, COLS = 2 * ACC;  // tensor-memory columns: read 32 at a time
     static constexpr int THREADS = 192;
 };
 template <typename T, int RP, bool KROWS>
@@ -466,8 +468,8 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         if (warp == 1) tmem_dealloc(tmem, S::COLS);
         return;
     }
-    const int c0 = blockIdx.x * 128, n = (it.rows + KB - 1) / KB;
-    const bool second = c0 + 64 < p.K;  // the second half of the columns exists
+    const int c0 = blockIdx.x * kTcCols, n = (it.rows + KB - 1) / KB;
+    const int quarters = min(4, (p.K - c0 + 63) / 64);  // tiles of 64 columns that exist
 
     if (warp == 0) {
         if (lane == 0) {
@@ -476,12 +478,11 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                 const int st = s % S::ST, t0 = it.first + s * KB;
                 if (s >= S::ST && !mbar_wait(empty(st), ((s / S::ST) & 1) ^ 1, abort_s, E_OUTER | 1, 50)) { ok = false; break; }
                 const uint32_t at = sb + st * S::STAGE;
-                mbar_expect_tx(full(st), ((second ? 2 : 1) + 2 * S::HALVES) * S::TILE);
-                tma_load_2d(at, &tm_x, full(st), c0, t0);
-                if (second) tma_load_2d(at + S::TILE, &tm_x, full(st), c0 + 64, t0);
+                mbar_expect_tx(full(st), (quarters + 2 * S::HALVES) * S::TILE);
+                for (int q = 0; q < quarters; ++q) tma_load_2d(at + q * S::TILE, &tm_x, full(st), c0 + q * 64, t0);
                 for (int h = 0; h < S::HALVES; ++h) {
-                    tma_load_2d(at + (2 + h) * S::TILE, &tm_hi, full(st), h * 64, t0);
-                    tma_load_2d(at + (2 + S::HALVES + h) * S::TILE, &tm_lo, full(st), h * 64, t0);
+                    tma_load_2d(at + (4 + h) * S::TILE, &tm_hi, full(st), h * 64, t0);
+                    tma_load_2d(at + (4 + S::HALVES + h) * S::TILE, &tm_lo, full(st), h * 64, t0);
                 }
             }
             if (!ok) let_copies_land();
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
             const uint32_t at = sb + st * S::STAGE;
             if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_OUTER | 2)) { ok = false; break; }
             if (rows < k16 * 16) {  // rows behind the item's last one: zeros in every tile
-                for (int tile = 0; tile < 2 + 2 * S::HALVES; ++tile)
+                for (int tile = 0; tile < 4 + 2 * S::HALVES; ++tile)
                     for (int e = rows * 8 + lane; e < k16 * 16 * 8; e += 32)
                         asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + tile * S::TILE + e * 16), "r"(0) : "memory");
                 fence_proxy_async_smem();
@@ -503,9 +504,13 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
             tc_fence_after();
             if (elect_one()) {
                 for (int k = 0; k < k16; ++k) {
-                    const uint64_t a = desc_mn(at + k * 16 * 128, S::TILE);
-                    mma_f16(tmem, a, desc_mn(at + 2 * S::TILE + k * 16 * 128, S::TILE), idesc, (s || k) ? 1u : 0u);
-                    mma_f16(tmem, a, desc_mn(at + (2 + S::HALVES) * S::TILE + k * 16 * 128, S::TILE), idesc, 1u);
+                    const uint64_t hi = desc_mn(at + 4 * S::TILE + k * 16 * 128, S::TILE);
+                    const uint64_t lo = desc_mn(at + (4 + S::HALVES) * S::TILE + k * 16 * 128, S::TILE);
+                    for (int h = 0; 2 * h < quarters; ++h) {
+                        const uint64_t a = desc_mn(at + 2 * h * S::TILE + k * 16 * 128, S::TILE);
+                        mma_f16(tmem + h * S::ACC, a, hi, idesc, (s || k) ? 1u : 0u);
+                        mma_f16(tmem + h * S::ACC, a, lo, idesc, 1u);
+                    }
                 }
                 tc_commit(empty(st));
                 if (s == n - 1) tc_commit(done);
@@ -513,27 +518,30 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
             __syncwarp();
         }
     } else {
-        const int q = warp & 3, k = c0 + q * 32 + lane;
+        const int q = warp & 3;
         float* part = p.part + (long long)w * p.R * p.K;
         if (mbar_wait_warp(done, 0, abort_s, E_OUTER | 3)) {
             tc_fence_after();
-            for (int c = 0; c < p.R; c += 32) {
-                float v[32];
-                tmem_ld32(tmem + (q * 32 << 16) + c, v);
-                tmem_wait_ld();
-                if (k < p.K) {
-                    const int left = p.R - c;  // 16 or more
-                    if constexpr (KROWS) {
-                        float* to = part + (long long)k * p.R + c;
+            for (int h = 0; 2 * h < quarters; ++h) {
+                const int k = c0 + h * 128 + q * 32 + lane;
+                for (int c = 0; c < p.R; c += 32) {
+                    float v[32];
+                    tmem_ld32(tmem + (q * 32 << 16) + h * S::ACC + c, v);
+                    tmem_wait_ld();
+                    if (k < p.K) {
+                        const int left = p.R - c;  // 16 or more
+                        if constexpr (KROWS) {
+                            float* to = part + (long long)k * p.R + c;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            if (i < left)
-                                asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]),
-                                             "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7]) : "memory");
-                    } else {
+                            for (int i = 0; i < 32; i += 8)
+                                if (i < left)
+                                    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + i), "f"(v[i]), "f"(v[i + 1]),
+                                                 "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7]) : "memory");
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i < left) part[(long long)(c + i) * p.K + k] = v[i];
+                            for (int i = 0; i < 32; ++i)
+                                if (i < left) part[(long long)(c + i) * p.K + k] = v[i];
+                        }
                     }
                 }
             }
@@ -634,7 +642,7 @@ int outer(const LoraParams& p, cudaStream_t s) {
     CUtensorMap x, hi, lo;
     if (!(make_map<T>(&x, p.x, p.T, p.K, p.stride_x, KB) && make_map<T>(&hi, p.hi, p.T, p.R, p.R, KB) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, KB)))
         return NB_ERR_UNSUPPORTED;
-    return launch(kernel, dim3(ceil_div(p.K, 128), item_count(p.T, p.requests, p.rows_per_item)), S::THREADS, S::BYTES, 1, p.chained, s, x, hi, lo, p);
+    return launch(kernel, dim3(ceil_div(p.K, kTcCols), item_count(p.T, p.requests, p.rows_per_item)), S::THREADS, S::BYTES, 1, p.chained, s, x, hi, lo, p);
 }
 
 #define NB_LORA_RP(CALL)                         \
