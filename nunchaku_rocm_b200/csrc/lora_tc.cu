@@ -78,7 +78,7 @@ template <int RP>  // R rounded up to 16, 32, 64 or 128
 struct ShrinkTc {
     static constexpr int XB = kTcRows * 128;
     static constexpr int FB = RP <= 64 ? 64 * 128 : 2 * 64 * 128;  // [64 of K][64 r] tiles, or RP rows of 64 of K
-    static constexpr int STAGE = XB + FB, ST = RP <= 64 ? 4 : 3;
+    static constexpr int STAGE = XB + FB, ST = RP <= 64 ? 8 : 6;  // 192 KB: one CTA per SM
     static constexpr int LD = RP + 4;  // floats of a row of sums: 16-byte accesses of eight rows on different banks
     static constexpr int PIPE = ST * STAGE, SUMS = kTcRows * LD * 4;
     static constexpr int OFF_BAR = PIPE > SUMS ? PIPE : SUMS;
@@ -97,8 +97,9 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
     auto full = [&](int i) { return bars + 8u * i; };
     auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
     const uint32_t done = bars + 8u * (2 * S::ST);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 128);
-    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 136);
+    static_assert(8 * (2 * S::ST + 1) <= 192, "barriers");
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // (set up while the offsets are on their way)
     if (threadIdx.x == 0) {
@@ -435,8 +436,9 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
     auto full = [&](int i) { return bars + 8u * i; };
     auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
     const uint32_t done = bars + 8u * (2 * S::ST);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 128);
-    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 136);
+    static_assert(8 * (2 * S::ST + 1) <= 192, "barriers");
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // (set up while the offsets are on their way)
     if (threadIdx.x == 0) {
@@ -581,7 +583,7 @@ bool make_map(CUtensorMap* m, const void* base, long long rows, long long cols, 
     const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
     return fn(m, std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth > 0 ? 3 : 2,
               const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int RP, bool RCONTIG>
@@ -596,11 +598,9 @@ int shrink(LoraParams p, cudaStream_t s) {
                     (RCONTIG ? make_map<T>(&f, p.factor, p.K, p.R, p.R, KB, p.A) : make_map<T>(&f, p.factor, p.R, p.K, p.K, p.R, p.A));
     if (!ok) return NB_ERR_UNSUPPORTED;
     const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
-    // CTAs of an item: as many as fit the SMs in one wave, up to eight (a portable cluster), each with at least four steps of
-    // 64 of K.  An SM holds two, but clusters do not fill the groups of SMs that they have to stay within: of 296 places,
-    // clusters of 3 to 8 get 259 to 284 (a wave of 72 clusters of 4 ran as 71 and one: 49 us for what takes 35 with 3).
-    int splits = 2 * sms() / live;
-    if (splits > 2) splits = (int)(0.87f * 2 * sms()) / live > 2 ? (int)(0.87f * 2 * sms()) / live : 2;
+    // CTAs of an item: as many as fit the SMs in one wave of one each, up to eight (a portable cluster), each with at least four
+    // steps of 64 of K
+    int splits = sms() / live;
     if (splits > ceil_div(p.K, 4 * KB)) splits = ceil_div(p.K, 4 * KB);
     if (splits > 8) splits = 8;
     if (splits < 1) splits = 1;
