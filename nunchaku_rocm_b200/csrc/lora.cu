@@ -513,10 +513,17 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const Join<T> first, con
 }
 
 // --------------------------------------------------------------------------------------------------------------- launchers
-// Whether a call runs on the tcgen05 kernels: their tiles are 128 rows, so the requests have to be that long on the whole.
+// Whether a call runs on the tcgen05 kernels.  Their tiles are 128 rows and a launch costs some 3 us more, so the requests
+// have to be long on the whole, and there has to be work: the mma.sync kernels fall behind with the rank (shared memory
+// feeds their instructions) and, having 64-row items in clusters of eight, with a long contraction over few rows.  Measured,
+// mma.sync / tcgen05, forward, K = 2048, N = 6144: rank 16: 512 rows 9.0 / 13.3 us, 8192 rows 50.9 / 48.8; rank 64: 512 rows
+// 15.6 / 12.2, 1024 rows 22.7 / 16.3; 64 requests of 32 rows 38.5 / 42.6, of 64 rows 57.0 / 54.6.  K = 12288, N = 3072: rank 32,
+// 128 rows 22.9 / 15.1 us; rank 64, 128 rows of 4 requests 26.6 / 16.6, 16 single rows 24.3 / 28.3.
 bool use_tc(const nb_lora_args* a) {
     if (a->impl != NB_IMPL_AUTO) return a->impl == NB_IMPL_TCGEN05;
-    return a->T >= 512 && a->T >= 64ll * a->requests;
+    const int contraction = a->dy ? a->N : a->K;
+    if (a->R >= 32 && contraction >= 8192 && a->T >= 16ll * a->requests) return true;
+    return a->T >= 96ll * a->requests && (double)a->T * a->R * a->R * ((double)a->K + a->N) >= 1e10;
 }
 // A tcgen05 launch, or the mma.sync one where there is no tensor map for the operands (rows a stride of zero apart) and the
 // caller did not insist.
@@ -548,7 +555,7 @@ int shrink(const LoraParams& p, cudaStream_t s) {
     const int items = item_count(p.T, p.requests, kRows);
     // CTAs of an item: a power of two up to eight (a portable cluster), until the items cover the SMs twice, each with at
     // least two steps of 64 of K
-    const int live = ceil_div(p.T, kRows) > p.requests ? ceil_div(p.T, kRows) : (p.requests < p.T ? p.requests : p.T);
+    const int live = live_items(p, kRows);
     int splits = 1;
     while (splits < 8 && live * splits < 2 * sms() && ceil_div(p.K, 64) >= 4 * splits) splits *= 2;
     auto* kernel = lora_shrink_kernel<T, RM, RCONTIG>;
@@ -559,7 +566,7 @@ template <typename T, int RM, bool CCONTIG>
 int expand(LoraParams p, cudaStream_t s) {
     using S = ExpandTile<RM, CCONTIG>;
     const int items = item_count(p.T, p.requests, kRows);
-    const int live = ceil_div(p.T, kRows) > p.requests ? ceil_div(p.T, kRows) : (p.requests < p.T ? p.requests : p.T);
+    const int live = live_items(p, kRows);
     // columns of a CTA: whole tiles, as many as leave about eight CTAs per SM
     const int tiles = ceil_div(p.K, S::BN), per = ceil_div(8ll * sms(), live);
     p.cols_per_cta = ceil_div(tiles, per < tiles ? per : tiles) * S::BN;

@@ -59,6 +59,12 @@ __device__ __forceinline__ Item find_item(const LoraParams& p, int w) {
     return it;
 }
 
+// about how many of them have rows
+inline int live_items(const LoraParams& p, int bm) {
+    const int tiles = (p.T + bm - 1) / bm, requests = p.requests < p.T ? p.requests : p.T;
+    return tiles > requests ? tiles : requests;
+}
+
 // The kernels of a call form a chain: each is launched while the one before it still runs (programmatic stream
 // serialization), does what does not depend on it - finding its item, loading the factor and base - and waits for its end
 // before it reads what it wrote, or writes what it may still read.  A kernel that has ended has waited for the one before

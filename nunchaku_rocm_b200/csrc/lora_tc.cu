@@ -597,7 +597,7 @@ int shrink(LoraParams p, cudaStream_t s) {
     const bool ok = make_map<T>(&x, p.x, p.T, p.K, p.stride_x, kTcRows) &&
                     (RCONTIG ? make_map<T>(&f, p.factor, p.K, p.R, p.R, KB, p.A) : make_map<T>(&f, p.factor, p.R, p.K, p.K, p.R, p.A));
     if (!ok) return NB_ERR_UNSUPPORTED;
-    const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
+    const int items = item_count(p.T, p.requests, kTcRows), live = live_items(p, kTcRows);
     // CTAs of an item: as many as fit the SMs in one wave of one each, up to eight (a portable cluster), each with at least four
     // steps of 64 of K
     int splits = sms() / live;
@@ -619,14 +619,14 @@ int expand(LoraParams p, cudaStream_t s) {
     if (ok && p.x) ok = make_map<T>(&base, p.x, p.T, p.K, p.stride_x, kTcRows);
     else base = out;
     if (!ok) return NB_ERR_UNSUPPORTED;
-    const int items = item_count(p.T, p.requests, kTcRows), live = ceil_div(p.T, kTcRows);
+    const int items = item_count(p.T, p.requests, kTcRows), live = live_items(p, kTcRows);
     // columns of a CTA: the cut of a row into `cuts` pieces that is done soonest, a CTA's cost being its tiles (0.7 us of an
     // SM's share of HBM each) and about three microseconds to start and to load the item's hi and lo, waves of the CTAs that
     // are resident together taking turns
     const int tiles = ceil_div(p.K, 64), slots = S::PER_SM * sms();
     int per = tiles;
     float best = 1e30f;
-    for (int cuts = 1; cuts <= 16 && cuts <= tiles; ++cuts) {
+    for (int cuts = 1; cuts <= 64 && cuts <= tiles; ++cuts) {
         const int t = ceil_div(tiles, cuts);
         const float cost = (float)ceil_div((long long)live * ceil_div(tiles, t), slots) * (0.7f * S::PER_SM * t + 3.f);
         if (cost < best) best = cost, per = t;
