@@ -302,19 +302,21 @@ def ensure_selftest(dev: torch.device) -> None:
 
 def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
     """All given tensors must live on one CUDA device; there is no CPU path.  First use of a device runs the self-test."""
-    dev = None
+    first, index = None, -1
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError("nunchaku_rocm_b200 kernels need CUDA tensors (there is no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
             raise ValueError("tensors on different devices")
-    if dev is not None:
-        ensure_selftest(dev)
-    return dev
+    if first is None:
+        return None
+    if index not in _selftested:
+        ensure_selftest(first.device)
+    return first.device
 
 
 _status_words: dict[int, torch.Tensor] = {}

@@ -377,7 +377,7 @@ struct Lora : torch::autograd::Function<Lora> {
         const bool need_x = ctx->needs_input_grad(0), need_down = ctx->needs_input_grad(1), need_up = ctx->needs_input_grad(2);
         const c10::cuda::CUDAGuard guard(down.device());
         const int64_t rows = dy.numel() / up.size(1);
-        Tensor dx, ddown, dup, g, ws, xr, dyr;
+        Tensor dx, ddown, dup, ws, xr, dyr;
         if (need_x) dx = at::empty(shape, down.options());
         if (need_down) ddown = rows ? at::empty(down.sizes(), down.options()) : at::zeros(down.sizes(), down.options());
         if (need_up) dup = rows ? at::empty(up.sizes(), up.options()) : at::zeros(up.sizes(), up.options());
@@ -391,19 +391,16 @@ struct Lora : torch::autograd::Function<Lora> {
                 a.x = xr.const_data_ptr();
                 a.ddown = ddown.data_ptr();
             }
-            if (need_x || need_down) {
-                g = at::empty({2, rows, down.size(1)}, down.options());
-                a.g = g.data_ptr();
-            }
             if (need_up) {
                 a.h = h.data_ptr();
                 a.dup = dup.data_ptr();
             }
-            if (need_down || need_up) {
-                a.workspace_bytes = lib.lora_workspace_bytes(&a);
-                ws = at::empty({a.workspace_bytes}, down.options().dtype(at::kByte));
-                a.workspace = ws.data_ptr();
-            }
+            // the workspace and g in one allocation (each costs the worker thread some microseconds)
+            a.workspace_bytes = need_down || need_up ? lib.lora_workspace_bytes(&a) : 0;
+            const int64_t at_g = (a.workspace_bytes + 255) / 256 * 256;
+            ws = at::empty({at_g + (need_x || need_down ? 4 * rows * down.size(1) : 0)}, down.options().dtype(at::kByte));
+            if (a.workspace_bytes) a.workspace = ws.data_ptr();
+            if (need_x || need_down) a.g = ws.data_ptr<uint8_t>() + at_g;
             check(lib.lora_backward(&a, stream_of(down)), "lora_batched backward");
         }
         variable_list r = once({dx, ddown, dup});
