@@ -19,7 +19,8 @@
 // the final rounding would show; one rounding alone would add an error as large as that of the output itself.  It doubles
 // the matrix instructions of the second products, which move more bytes than they compute.
 //
-// Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out).
+// Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out); for a few rows the latency of two
+// dependent kernels, 24 single rows of 24 requests, 3072 -> 18432, rank 16: 6.3 + 9.9 us, of which one overlaps.
 #include <cooperative_groups.h>
 
 #include "lora.cuh"

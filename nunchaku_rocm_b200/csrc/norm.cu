@@ -13,6 +13,11 @@
 // CTA.  What has to be covered is the latency of a row's load and of its reductions (shuffles, a barrier): the RING kernels
 // keep several rows of every team on their way into shared memory (cp.async; a thread copies just the columns that it reads
 // itself, so no barrier guards a row) and reduce RB rows together.
+//
+// Measured on a B200: 32761 x 5120 fp16, forward 115 us (5.8 TB/s; a copy of the tensor takes 109), backward 207 (4.9 TB/s; a
+// sum of two such tensors takes 146); 9216 x 3072 bf16 with a scale and shift per sample, 27.5 and 42.5 us (a copy 24.3, a sum
+// 28.8).  The long backward pass runs at two CTAs per SM (registers of the column sums and the ring both allow no third) with
+// 53 % of the issue slots and 49 % of DRAM busy: what remains are the waits of a row's own reductions.
 #include "nb_common.cuh"
 
 namespace nb {
@@ -722,7 +727,8 @@ int ctas_per_group(int resident, int groups) {
     const int sms = nb_num_sms(), per = resident * (sms > 0 ? sms : 148) / groups;
     return per < 1 ? 1 : per;
 }
-// `ring`: the rows are whole 16-byte pieces.  The ring has 8 slots while two CTAs of it fit an SM, else 4; rows too long for
+// `ring`: the rows are whole 16-byte pieces.  The ring has 8 slots while two CTAs of it (three in the
+// backward pass) fit an SM, else 4; rows too long for
 // that (over 27 KB a slot: 13 K channels of 16 bits in the backward pass) go to the kernel without one.
 Shape shape_of(int groups, int rows, int dim, int size, bool backward, bool ring) {
     Shape s;
