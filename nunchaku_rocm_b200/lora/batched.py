@@ -78,14 +78,18 @@ def lora_requests(adapters: torch.Tensor):
 
 
 @functools.lru_cache(maxsize=256)
-def _even_offsets(samples: int, rows: int, device: torch.device) -> torch.Tensor:
-    return torch.arange(samples + 1, dtype=torch.int32, device=device) * rows
+def _even_offsets(samples: int, rows: int, device: torch.device, stream: int) -> torch.Tensor:
+    with torch.inference_mode(False):  # (a training step may save it)
+        return torch.arange(0, samples * rows + 1, rows, dtype=torch.int32, device=device)
 
 
 def _offsets(samples, rows, device):
-    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():  # (a tensor made here belongs to the graph)
-        return _even_offsets.__wrapped__(samples, rows, device)
-    return _even_offsets(samples, rows, device)
+    if device.type != "cuda":
+        return _even_offsets(samples, rows, device, 0)
+    if torch.cuda.is_current_stream_capturing():  # (a tensor made here belongs to the graph)
+        return _even_offsets.__wrapped__(samples, rows, device, 0)
+    # one per stream: another stream would not wait for the kernel that fills it
+    return _even_offsets(samples, rows, device, torch.cuda.current_stream(device).cuda_stream)
 
 
 def has_lora_batch(module: nn.Module) -> bool:

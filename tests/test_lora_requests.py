@@ -10,6 +10,7 @@ import torch
 from torch import nn
 
 from nunchaku_rocm_b200.lora import attach_lora, attach_lora_batch, detach_lora_batch, lora_requests, stack_loras
+from nunchaku_rocm_b200.lora import batched
 from nunchaku_rocm_b200.models.embeddings import flux_pos_embed, qwen_image_ids
 from nunchaku_rocm_b200.models.linear import AWQW4A16Linear, SVDQW4A4Linear
 
@@ -94,6 +95,14 @@ def test_qwen_image_ids():
     ids = qwen_image_ids(3, 2, 5, 4)
     assert ids.shape == (43, 3) and ids[:3].tolist() == [[2, 2, 2], [3, 3, 3], [4, 4, 4]]
     assert ids[3].tolist() == [0, -3, -2] and ids[-1].tolist() == [1, 1, 1]
+
+
+def test_offsets_are_kept_for_each_stream_and_may_be_saved():
+    cpu = torch.device("cpu")
+    with torch.inference_mode():
+        a = batched._even_offsets(3, 7, cpu, 1)
+    assert a.tolist() == [0, 7, 14, 21] and a.dtype == torch.int32 and not a.is_inference()
+    assert batched._even_offsets(3, 7, cpu, 1) is a and batched._even_offsets(3, 7, cpu, 2) is not a
 
 
 # ------------------------------------------------------------------------------------------------------------------- GPU
@@ -308,3 +317,20 @@ def test_operators_in_a_run_together(cuda_dev, dtype):
     for name, a, b in zip(["y", *leaves], got, want):
         err = ((a.double() - b).norm() / b.norm()).item()
         assert err <= bound, (name, err, bound)
+
+
+@gpu
+def test_training_after_serving_in_inference_mode(cuda_dev):
+    lin = nn.Linear(64, 48, dtype=BF16, device=cuda_dev).requires_grad_(False)
+    down, up = stack_loras([pair(16, 64, 48, 1, cuda_dev), pair(16, 64, 48, 2, cuda_dev)])
+    down, up = down.requires_grad_(True), up.requires_grad_(True)
+    attach_lora_batch(lin, (down, up))
+    x = torch.randn(2, 29, 64, generator=torch.Generator().manual_seed(3)).to(BF16).to(cuda_dev)
+    ids = torch.tensor([1, 0], dtype=torch.int32, device=cuda_dev)
+    with torch.inference_mode(), lora_requests(ids):
+        served = lin(x)
+    with lora_requests(ids):
+        y = lin(x)
+    assert torch.equal(y, served)
+    y.float().sum().backward()
+    assert down.grad.any() and up.grad.any()
