@@ -97,6 +97,20 @@ def has_lora_batch(module: nn.Module) -> bool:
     return getattr(module, "_lora_stack", None) is not None and getattr(_active, "adapters", None) is not None
 
 
+def _stack_on(module: nn.Module, x: torch.Tensor):
+    """The module's stack and scale where ``x`` is and in its dtype (the module may have moved after the attachment)."""
+    (down, up), scale = module._lora_stack, module._lora_stack_scale
+    if down.device == x.device and down.dtype == x.dtype:
+        return down, up, scale
+    with torch.inference_mode(False):
+        down, up = down.to(x.device, x.dtype), up.to(x.device, x.dtype)
+        scale = None if scale is None else scale.to(x.device)
+    trained = any(t.requires_grad for t in module._lora_stack)  # (each step converts the leaves anew)
+    if not trained and not (x.is_cuda and torch.cuda.is_current_stream_capturing()):
+        module._lora_stack, module._lora_stack_scale = (down, up), scale
+    return down, up, scale
+
+
 def add_lora_batch(module: nn.Module, x: torch.Tensor, out: torch.Tensor, samples: int | None = None,
                    fused: bool = False) -> torch.Tensor:
     """
@@ -109,9 +123,7 @@ def add_lora_batch(module: nn.Module, x: torch.Tensor, out: torch.Tensor, sample
     samples = x.shape[0] if samples is None else samples
     if adapters.shape[0] != samples:
         raise ValueError(f"lora_requests has {adapters.shape[0]} samples, the layer's input {samples}")
-    down, up = module._lora_stack
-    if down.device != x.device or down.dtype != x.dtype:  # the module moved after the attachment
-        module._lora_stack = down, up = down.to(x.device, x.dtype), up.to(x.device, x.dtype)
+    down, up, scale = _stack_on(module, x)
     rows = x.numel() // x.shape[-1]
     if rows == 0:
         return out
@@ -120,7 +132,7 @@ def add_lora_batch(module: nn.Module, x: torch.Tensor, out: torch.Tensor, sample
     if graph and (fused or (x.requires_grad and _is_svdq(module))):
         raise NotImplementedError("no backward pass: " + ("a fused operator" if fused else "the input of a quantised layer"))
     in_place = not graph and out.is_contiguous() and out.data_ptr() % 16 == 0
-    return lora_batched(x, down, up, offsets, adapters, base=out, scale=getattr(module, "_lora_stack_scale", None),
+    return lora_batched(x, down, up, offsets, adapters, base=out, scale=scale,
                         out=out if in_place else None)
 
 

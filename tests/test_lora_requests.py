@@ -97,6 +97,23 @@ def test_qwen_image_ids():
     assert ids[3].tolist() == [0, -3, -2] and ids[-1].tolist() == [1, 1, 1]
 
 
+def test_a_stack_follows_its_module():
+    lin = nn.Linear(16, 8)
+    attach_lora_batch(lin, [pair(2, 16, 8, 1, dtype=torch.float32)], scale=[0.5])
+    x = torch.zeros(3, 16, dtype=torch.float64, device="cpu")
+    with torch.inference_mode():
+        down, up, scale = batched._stack_on(lin, x)
+    assert lin._lora_stack == (down, up) and down.dtype == up.dtype == x.dtype and not down.is_inference() and scale is lin._lora_stack_scale
+    assert batched._stack_on(lin, torch.zeros(1, 16, device="meta", dtype=BF16))[2].device.type == "meta"  # the scale moves too
+    # leaves that are trained stay the module's stack: every step converts them with a graph of its own
+    leaves = tuple(torch.zeros(s, requires_grad=True) for s in ((1, 16, 16), (1, 8, 16)))
+    attach_lora_batch(lin, leaves)
+    for _ in range(2):
+        down, up, _ = batched._stack_on(lin, x)
+        (down.sum() + up.sum()).backward()
+    assert lin._lora_stack[0] is leaves[0] and (leaves[0].grad == 2).all() and (leaves[1].grad == 2).all()
+
+
 def test_offsets_are_kept_for_each_stream_and_may_be_saved():
     cpu = torch.device("cpu")
     with torch.inference_mode():
