@@ -136,8 +136,8 @@ def add_lora_batch(module: nn.Module, x: torch.Tensor, out: torch.Tensor, sample
                         out=out if in_place else None)
 
 
-def _hook(module, args, output):
-    return add_lora_batch(module, args[0], output) if has_lora_batch(module) else None
+def _hook(module, args, kwargs, output):
+    return add_lora_batch(module, args[0] if args else next(iter(kwargs.values())), output) if has_lora_batch(module) else None
 
 
 def attach_lora_batch(module: nn.Module, adapters, scale=None) -> None:
@@ -168,7 +168,7 @@ def attach_lora_batch(module: nn.Module, adapters, scale=None) -> None:
     detach_lora_batch(module)
     module._lora_stack, module._lora_stack_scale = (down, up), scale
     if not svdq:  # (SVDQW4A4Linear and the fused operators look for the stack themselves)
-        module._lora_stack_hook = module.register_forward_hook(_hook)
+        module._lora_stack_hook = module.register_forward_hook(_hook, with_kwargs=True)
 
 
 def detach_lora_batch(module: nn.Module) -> None:

@@ -85,6 +85,8 @@ def test_attach_and_requests_refuse():
     y = plain(x)  # no requests are active: the stack is not used
     with pytest.raises(ValueError, match="samples"), lora_requests(torch.zeros(2, dtype=torch.int32)):
         plain(x)
+    with pytest.raises(ValueError, match="samples"), lora_requests(torch.zeros(2, dtype=torch.int32)):
+        plain(input=x)  # found by name too
     detach_lora_batch(plain)
     detach_lora_batch(plain)
     with lora_requests(torch.zeros(2, dtype=torch.int32)):
