@@ -413,6 +413,7 @@ Tensor lora_batched(const Tensor& x, const Tensor& down, const Tensor& up, const
         return Lora::apply(x, down, up, base, offsets, adapters, scale, impl, status);
     const Tensor to = defined(out) ? *out : new_out(x, up);
     run_lora(x, or_none(base), down, up, offsets, adapters, or_none(scale), to, impl, status);
+    if (defined(out) && !to.is_inference()) to.unsafeGetTensorImpl()->bump_version();  // a graph that saved it must notice
     return to;
 }
 

@@ -16,7 +16,7 @@ __all__ = ["lora_batched"]
 
 
 def _rows_ok(t: torch.Tensor) -> bool:
-    """Whether the kernel can write ``t (..., C)`` in place: rows evenly strided, each on a 16-byte boundary."""
+    """Whether the kernel can write ``t (..., C)`` in place: rows evenly strided and apart, each on a 16-byte boundary."""
     if t.data_ptr() % 16 or t.stride(-1) != 1:
         return False
     run, step = 1, t.shape[-1]
@@ -27,7 +27,7 @@ def _rows_ok(t: torch.Tensor) -> bool:
             elif stride != run * step:
                 return False
             run *= size
-    return step % 8 == 0
+    return step % 8 == 0 and (step >= t.shape[-1] or run <= 1)
 
 
 def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor, adapters: torch.Tensor,
@@ -44,7 +44,9 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
 
     ``down (A, R, K)`` and ``up (A, N, R)`` are contiguous stacks of adapters (``R`` a multiple of 16 up to 128, ``K`` and
     ``N`` multiples of 8; smaller ranks are padded with zeros, see :func:`nunchaku_rocm_b200.lora.stack_loras`); ``scale
-    (A,)`` is float32.  ``out`` may be given where no gradient is asked for, and may be ``base``.
+    (A,)`` is float32.  ``out`` may be given where no gradient is asked for; it may be ``base`` itself, and shares no memory
+    with the inputs otherwise.  At most 65535 adapters, and ``rows / 64 + requests`` at most 65000.  A backward pass needs a
+    workspace of ``R (K + N)`` floats for every request and every few hundred rows.
 
     Differentiable in ``x``, ``base``, ``down`` and ``up`` (not in ``scale``); gradients of adapters that several requests
     share are summed in a fixed order.
@@ -75,9 +77,9 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     if grad and scale is not None and scale.requires_grad:
         raise ValueError("lora_batched has no gradient for scale")
     if out is not None and not _rows_ok(out):
-        raise ValueError("out must have evenly strided rows on 16-byte boundaries")
+        raise ValueError("out must have evenly strided rows on 16-byte boundaries that do not overlap")
     L.require_cuda(x, down, up, offsets, adapters, base, scale, out)
-    if out is not None and grad and (x.requires_grad or down.requires_grad or up.requires_grad or (base is not None and base.requires_grad)):
+    if out is not None and grad and (out.requires_grad or x.requires_grad or down.requires_grad or up.requires_grad or (base is not None and base.requires_grad)):
         raise ValueError("out cannot be given where a gradient is asked for")
     return L.binding().lora_batched(
         x, down.contiguous(), up.contiguous(), offsets.contiguous(), adapters.contiguous(), base,

@@ -116,6 +116,8 @@ def test_refuses():
                {"scale": torch.ones(2, requires_grad=True)}, {"out": torch.zeros(4, 40, dtype=BF16)}, {"out": torch.zeros(4, 34, dtype=BF16)[:, :32]}):
         with pytest.raises(ValueError):
             lora_batched(x, down, up, off, ad, **kw)
+    with pytest.raises(ValueError, match="overlap"):
+        lora_batched(x, down, up, off, ad, out=torch.zeros(1, 32, dtype=BF16).expand(4, 32))
     for r, k, n in ((8, 64, 32), (144, 64, 32), (16, 60, 32), (16, 64, 36), (0, 64, 32)):
         with pytest.raises(NotImplementedError):
             lora_batched(torch.zeros(4, k, dtype=BF16), torch.zeros(1, r, k, dtype=BF16), torch.zeros(1, n, r, dtype=BF16), off, ad)
@@ -215,6 +217,47 @@ def test_layouts_and_out(cuda_dev):
     ones = {**p, "dy": torch.ones_like(p["dy"])}
     within(dx[:, 128:256], *reference(ones, [0, 33, 96], [1, 0], scale=False)["dx"])
     assert not dx[:, :128].any() and (drow == 96).all()
+
+
+@gpu
+def test_out_is_an_in_place_change(cuda_dev):
+    p = make(cuda_dev, 40, 64, 64, 16, 1, BF16)
+    off, ad = index(cuda_dev, [0, 40], [0])
+    w = torch.ones(40, 64, dtype=BF16, device=cuda_dev, requires_grad=True)
+    y = (w * p["base"]).sum()  # keeps base for w's gradient
+    lora_batched(p["x"], p["down"], p["up"], off, ad, base=p["base"], out=p["base"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with pytest.raises(ValueError, match="gradient"):
+        lora_batched(p["x"], p["down"], p["up"], off, ad, out=w)
+
+
+@gpu
+def test_captured_training_step(cuda_dev):
+    p = make(cuda_dev, 300, 256, 384, 32, 3, FP16)
+    off, ad = index(cuda_dev, [0, 120, 120, 300], [0, 1, 2])
+
+    def step():
+        leaves = [p[k].detach().requires_grad_(True) for k in ("x", "down", "up")]
+        out = lora_batched(*leaves, off, ad, base=p["base"], scale=p["scale"])
+        return (out.detach(), *torch.autograd.grad(out, leaves, p["dy"]))
+
+    step()
+    s, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.cuda.graph(gr, stream=s):
+        got = step()
+    torch.cuda.current_stream().wait_stream(s)
+    ad.copy_(torch.tensor([2, 0, 2], dtype=torch.int32))
+    off.copy_(torch.tensor([0, 7, 190, 290], dtype=torch.int32))
+    p["dy"].neg_()
+    for _ in range(2):
+        gr.replay()
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ref = reference(p, [0, 7, 190, 290], [2, 0, 2])
+    for name, t in zip(("out", "dx", "ddown", "dup"), got):
+        within(t, *ref[name])
 
 
 @gpu
