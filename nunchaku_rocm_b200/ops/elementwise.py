@@ -147,7 +147,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
     ``weight`` and ``bias`` are ``(D,)``, or ``(B, D)`` for ``x (B, T, D)`` (one row per sample, as an adaptive norm's scale
     and shift, then with ``weight_add=1``), both of ``x``'s dtype or both float32; either may be ``None``.  Their gradients
-    are summed over the rows in fp32, in a fixed order.  ``D`` is at most 16384.
+    are summed over the rows in fp32, in a fixed order.  ``D`` is at most 16384, ``B`` with a row per sample at most 65535.
     """
     weight, bias = _ln_prepare(x, weight, bias, weight_add)
     L.require_cuda(x, weight, bias)

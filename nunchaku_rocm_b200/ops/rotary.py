@@ -62,6 +62,8 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes
         raise ValueError(f"axes {tuple(axes_dim)} have more channels than a head ({D})")
     if H == 0 or (k is not None and k.shape[2] == 0):
         raise ValueError("no heads")
+    if ids.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rotary_axes has no gradient for ids")
     L.require_cuda(q, k, ids)
     out = L.binding().rotary_axes(q, k, ids, ladder, not interleaved, inverse)
     return out[0] if k is None else (out[0], out[1])
@@ -77,5 +79,7 @@ def rotary_table(ids: torch.Tensor, axes_dim, theta: float = 10000.0) -> torch.T
     ladder = _ladder(tuple(axes_dim), float(theta))
     B, S = (1, ids.shape[0]) if ids.dim() == 2 else ids.shape[:2]
     _check_ids(ids, ladder.n_axes, B, S)
+    if ids.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rotary_table has no gradient for ids")
     L.require_cuda(ids)
     return L.binding().rotary_table(ids, ladder)

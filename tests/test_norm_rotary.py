@@ -53,6 +53,11 @@ def test_rotary_refuses():
             rotary_axes(*args, **kw)
     with pytest.raises(ValueError):
         rotary_table(torch.zeros(5), (64,))
+    learned = torch.zeros(5, 2, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        rotary_axes(q, None, learned, (32, 32))
+    with pytest.raises(ValueError, match="gradient"):
+        rotary_table(learned, (32, 32))
     with pytest.raises(RuntimeError, match="no CPU path"):
         rotary_axes(q, None, ids, (32, 32))
     with pytest.raises(RuntimeError, match="no CPU path"):
@@ -380,3 +385,16 @@ def test_rotary_captured(cuda_dev):
     torch.cuda.synchronize()
     assert torch.equal(a, rotary_axes(q, None, ids, (16, 56, 56))) and torch.equal(a, b)
     assert torch.equal(t, rotary_table(ids, (16, 56, 56)))
+
+
+def test_struct_fields_match_the_header():
+    import pathlib
+    import re
+
+    text = (pathlib.Path(__file__).parent.parent / "include" / "nunchaku_b200.h").read_text()
+    text = re.sub(r"/\*.*?\*/|//[^\n]*", "", text, flags=re.S)
+    for name, ctype in (("nb_lora_args", L.LoraArgs), ("nb_layer_norm_args", L.LayerNormArgs), ("nb_rotary_args", L.RotaryArgs),
+                        ("nb_rotary_ladder", L.RotaryLadder)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+        fields = [re.search(r"(\w+)\s*(\[[^\]]*\])?$", f.strip()).group(1) for line in body.split(";") if line.strip() for f in line.split(",")]
+        assert fields == [f[0] for f in ctype._fields_], name
