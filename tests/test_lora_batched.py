@@ -341,3 +341,24 @@ def test_on_a_stream_of_its_own(cuda_dev):
         got = [lora_batched(p["x"], p["down"], p["up"], off, ad, base=p["base"]) for _ in range(8)]
     s.synchronize()
     assert all(torch.equal(t, want) for t in got)
+
+
+@gpu
+@pytest.mark.parametrize("impl", IMPLS.values(), ids=IMPLS)
+def test_more_than_2_31_elements(cuda_dev, impl):
+    # the last rows, whose offsets pass 32 bits, against 64 bits
+    T, K, N, tail = 3_000_000, 16, 728, 200
+    assert T * N > 1 << 31
+    g = torch.Generator(device=cuda_dev).manual_seed(0)
+    p = make(cuda_dev, tail, K, N, 16, 2, BF16)
+    x, dy = torch.zeros(T, K, dtype=BF16, device=cuda_dev), torch.zeros(T, N, dtype=BF16, device=cuda_dev)
+    x[:-tail].normal_(generator=g)
+    x[-tail:], dy[-tail:] = p["x"], p["dy"]
+    off, ad = index(cuda_dev, [0, 1_000_001, T - 90, T], [1, 0, 1])
+    x.requires_grad_(True)
+    out = lora_batched(x, p["down"], p["up"], off, ad, _impl=impl)
+    dx, = torch.autograd.grad(out, x, dy)
+    ref = reference(p, [0, tail - 90, tail], [0, 1], scale=False, base=False)
+    within(out[-tail:], *ref["out"])
+    within(dx[-tail:], *ref["dx"])
+    assert L.device_status(cuda_dev) == 0

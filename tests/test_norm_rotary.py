@@ -398,3 +398,49 @@ def test_struct_fields_match_the_header():
         body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
         fields = [re.search(r"(\w+)\s*(\[[^\]]*\])?$", f.strip()).group(1) for line in body.split(";") if line.strip() for f in line.split(",")]
         assert fields == [f[0] for f in ctype._fields_], name
+
+
+@gpu
+def test_norm_and_rotary_training_steps_captured(cuda_dev):
+    x, w, b, dy = (torch.randn(s, device=cuda_dev).to(FP16) for s in ((2, 50, 320), (2, 320), (2, 320), (2, 50, 320)))
+    q, k, dq, dk = (torch.randn(2, 50, h, 64, device=cuda_dev).to(FP16) for h in (4, 1, 4, 1))
+    ids = torch.randint(0, 90, (50, 2), device=cuda_dev).float()
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b, q, k)]
+        y = layer_norm(*leaves[:3], weight_add=1.0)
+        r = rotary_axes(*leaves[3:], ids, (32, 32), interleaved=False)
+        return (y.detach(), *(t.detach() for t in r), *torch.autograd.grad((y, *r), leaves, (dy, dq, dk)))
+
+    step()
+    s, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.cuda.graph(gr, stream=s):
+        got = step()
+    torch.cuda.current_stream().wait_stream(s)
+    ids.add_(3)
+    for t in (x, w, dy, q, dk):
+        t.mul_(-0.5)
+    for _ in range(2):
+        gr.replay()
+    assert all(torch.equal(a, c) for a, c in zip(got, step()))
+
+
+@gpu
+def test_more_than_2_31_elements(cuda_dev):
+    # the last rows, whose offsets pass 32 bits, are those of a call on these rows alone
+    T, D, tail = (1 << 19) + 5, 4104, 37
+    assert T * D > 1 << 31
+    x, dy = torch.empty(T, D, dtype=FP16, device=cuda_dev).normal_(), torch.empty(T, D, dtype=FP16, device=cuda_dev).normal_()
+    y, dx = [], []
+    for rows in (slice(None), slice(T - tail, None)):
+        leaf = x[rows].detach().requires_grad_(True)
+        y.append(layer_norm(leaf))
+        dx += torch.autograd.grad(y[-1], leaf, dy[rows])
+    assert torch.equal(y[0][-tail:], y[1]) and torch.equal(dx[0][-tail:], dx[1])
+    del dy, y, dx
+    H = 4104 // 8
+    q = x.view(T, 1, H, 8)  # more than 2^19 samples of one token
+    ids = torch.randint(0, 500, (T, 1, 2), device=cuda_dev)
+    got = rotary_axes(q, None, ids, (4, 4))
+    assert torch.equal(got[-tail:], rotary_axes(q[-tail:], None, ids[-tail:], (4, 4)))
