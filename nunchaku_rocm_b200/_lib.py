@@ -208,6 +208,13 @@ def lib() -> C.CDLL:
 _binding = None
 
 
+def _first_use(index: int) -> int:
+    """A device's self-test and the address of its status word, for the extension module."""
+    dev = torch.device("cuda", index)
+    ensure_selftest(dev)
+    return status_word(dev).data_ptr()
+
+
 def binding():
     """The extension module with torch's side of the differentiable operators (``csrc/binding/``), bound to :func:`lib`."""
     global _binding
@@ -225,7 +232,7 @@ def binding():
                 names = ["layer_norm", "layer_norm_backward", "layer_norm_workspace_bytes", "rotary_ladder_init", "rotary_axes", "rotary_table",
                          "lora_forward", "lora_backward", "lora_workspace_bytes", "strerror", "last_error_detail", "last_cuda_error",
                          "last_cuda_error_string"]
-                b.bind({f"nb_{n}": C.cast(getattr(l, f"nb_{n}"), C.c_void_p).value for n in names})
+                b.bind({f"nb_{n}": C.cast(getattr(l, f"nb_{n}"), C.c_void_p).value for n in names}, _first_use)
                 _binding = b
     return _binding
 

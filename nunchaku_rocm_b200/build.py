@@ -71,9 +71,11 @@ def _binding_command(force: bool) -> list[str] | None:
     made = open(stamp).read() if os.path.exists(stamp) else ""
     if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest and made == _binding_versions():
         return None
-    cxx = shutil.which(os.environ.get("CXX", "g++"))
+    # the compiler that nvcc takes too, whatever $CXX is: one that links a C++ library of its own in brings a second copy of
+    # its locale into torch's process, and the first number printed into an error message ends it
+    cxx = shutil.which("g++")
     if cxx is None:
-        raise RuntimeError("no C++ compiler found; set CXX")
+        raise RuntimeError("g++ not found on PATH")
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),

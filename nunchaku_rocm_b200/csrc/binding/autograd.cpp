@@ -3,10 +3,11 @@
 // These operators run inside training steps, where a Python autograd function costs more than the kernels of a small call:
 // the engine's worker thread has to take the interpreter lock and interpret the backward pass on another core.  Measured on
 // a B200's host for a layer norm of 154 x 1152, forward and backward: 120 us a step with Python functions (23 forward, about
-// 45 the engine itself), 82 with these (torch's own layer norm: 72).  The arguments' checks stay in Python
-// (ops/elementwise.py, ops/rotary.py, ops/lora.py): what arrives here is valid.
+// 45 the engine itself), 82 with these (torch's own layer norm: 72).  The arguments' checks are here for the same reason:
+// they took a third of a small call in Python.
 //
 // The library's functions are bound by address, so that this module calls the very library that ctypes loaded.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -37,7 +38,11 @@ struct Library {
     decltype(&nb_last_cuda_error_string) last_cuda_error_string;
 } lib;
 
-void bind(const std::map<std::string, uintptr_t>& at) {
+// (device index) -> address of its status word, after the device's self-test; called once per device
+PyObject* first_use = nullptr;
+
+void bind(const std::map<std::string, uintptr_t>& at, py::function on_first_use) {
+    first_use = on_first_use.release().ptr();
 #define NB_BIND(name) lib.name = reinterpret_cast<decltype(lib.name)>(at.at("nb_" #name))
     NB_BIND(layer_norm); NB_BIND(layer_norm_backward); NB_BIND(layer_norm_workspace_bytes);
     NB_BIND(rotary_ladder_init); NB_BIND(rotary_axes); NB_BIND(rotary_table);
@@ -61,6 +66,32 @@ void check(int status, const char* what) {
     TORCH_CHECK(false, message);
 }
 
+int64_t status_of(int device) {
+    static std::array<int64_t, 64> known = {};
+    TORCH_CHECK(device >= 0 && device < (int)known.size(), "device index ", device);
+    if (!known[device]) {  // (the caller is Python: it holds the interpreter lock)
+        known[device] = py::reinterpret_borrow<py::function>(first_use)(device).cast<int64_t>();
+    }
+    return known[device];
+}
+// All given tensors live on one CUDA device; its status word.
+template <typename... Rest>
+int64_t require_cuda(const Tensor& first, const Rest&... rest) {
+    const auto one = [&](const Tensor& t) {
+        if (!t.defined()) return;
+        TORCH_CHECK(t.is_cuda(), "nunchaku_rocm_b200 kernels need CUDA tensors (there is no CPU path)");
+        TORCH_CHECK_VALUE(t.get_device() == first.get_device(), "tensors on different devices");
+    };
+    one(first);
+    (one(rest), ...);
+    return status_of(first.get_device());
+}
+// An uninitialised contiguous tensor beside `like`, without the dispatcher.
+Tensor empty_of(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+Tensor empty_of(at::IntArrayRef sizes, const Tensor& like) { return empty_of(sizes, like.scalar_type(), like); }
+
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 bool defined(const OptTensor& t) { return t.has_value() && t->defined(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -72,24 +103,28 @@ int dtype_of(const Tensor& t) {
     return t.scalar_type() == at::kBFloat16 ? NB_DTYPE_BF16 : t.scalar_type() == at::kHalf ? NB_DTYPE_FP16 : NB_DTYPE_FP32;
 }
 
-// `t (..., C)` and the stride between its rows: a copy only where the rows are not evenly strided (and, with `aligned`, not
-// on 16-byte boundaries)
+// Whether the rows of `t (..., C)` are evenly strided: every outer dimension steps over whole runs of the ones inside it.
+bool even_rows(const Tensor& t, int64_t* stride) {
+    *stride = t.size(-1);
+    if (t.is_contiguous()) return true;
+    if (t.stride(-1) != 1) return false;
+    int64_t run = 1;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (run == 1) *stride = t.stride(d);
+        else if (t.stride(d) != run * *stride) return false;
+        run *= t.size(d);
+    }
+    return true;
+}
+// `t` and the stride between its rows: a copy only where the rows are not evenly strided (and, with `aligned`, not on
+// 16-byte boundaries)
 Tensor strided_rows(const Tensor& t, int64_t* stride, bool aligned) {
     const int64_t c = t.size(-1);
     Tensor r = t;
-    *stride = c;
-    if (!t.is_contiguous()) {
-        // rows are evenly strided when every outer dimension steps over whole runs of the ones inside it
-        bool even = t.stride(-1) == 1;
-        int64_t step = 0, run = 1;
-        for (int64_t d = t.dim() - 2; even && d >= 0; --d) {
-            if (t.size(d) == 1) continue;
-            if (run == 1) step = t.stride(d);
-            else even = t.stride(d) == run * step;
-            run *= t.size(d);
-        }
-        if (even) *stride = run == 1 ? c : step;
-        else r = t.contiguous();
+    if (!even_rows(t, stride)) {
+        r = t.contiguous();
+        *stride = c;
     }
     if (aligned && ((*stride % 8) != 0 || (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15))) {
         r = r.clone(at::MemoryFormat::Contiguous);
@@ -140,6 +175,31 @@ nb_layer_norm_args ln_args(const Tensor& x, int64_t stride, const Tensor& weight
     a.weight_add = (float)add;
     return a;
 }
+bool known_type(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat; }
+Tensor ln_weight(const char* name, const Tensor& w, const Tensor& x) {
+    const int64_t dim = x.size(-1);
+    TORCH_CHECK_VALUE(w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, name, " must be ", x.scalar_type(), " or Float, got ",
+                      w.scalar_type());
+    const bool one = w.dim() == 1 && w.size(0) == dim, each = w.dim() == 2 && x.dim() == 3 && w.size(0) == x.size(0) && w.size(1) == dim;
+    TORCH_CHECK_VALUE(one || each, name, " must be (", dim, ",), or (B, ", dim, ") for x (B, T, ", dim, "); got ", w.sizes(), " for ", x.sizes());
+    return w.stride(-1) == 1 ? w : w.contiguous();
+}
+// The checks of the arguments; weight and bias with one stride and unit inner stride.
+void ln_prepare(const Tensor& x, Tensor& weight, Tensor& bias, double add) {
+    TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm needs at least one channel, got x ", x.sizes());
+    TORCH_CHECK_NOT_IMPLEMENTED(x.size(-1) <= NB_LAYER_NORM_MAX_DIM, "layer_norm takes up to ", NB_LAYER_NORM_MAX_DIM, " channels, got ", x.size(-1));
+    TORCH_CHECK_VALUE(known_type(x), "layer_norm takes bfloat16, float16 and float32, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(weight.defined() || add == 0, "weight_add without a weight");
+    if (weight.defined()) weight = ln_weight("weight", weight, x);
+    if (!bias.defined()) return;
+    bias = ln_weight("bias", bias, x);
+    if (!weight.defined()) return;
+    TORCH_CHECK_VALUE(bias.scalar_type() == weight.scalar_type() && bias.dim() == weight.dim(), "weight and bias must have one shape and one dtype");
+    if (bias.dim() == 2 && bias.stride(0) != weight.stride(0)) {
+        weight = weight.contiguous();
+        bias = bias.contiguous();
+    }
+}
 // y and / or the rows' (mean, rstd) into the given tensors
 void ln_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, double add, const Tensor& y, const Tensor& stats) {
     if (x.numel() == 0) return;
@@ -159,9 +219,9 @@ variable_list ln_backward(const Tensor& x, const Tensor& weight, const Tensor& b
     variable_list out(3);
     const c10::cuda::CUDAGuard guard(x.device());
     const bool empty = x.numel() == 0;
-    if (need_x) out[0] = at::empty(x.sizes(), x.options());
-    if (need_w) out[1] = empty ? at::zeros(weight.sizes(), weight.options()) : at::empty(weight.sizes(), weight.options());
-    if (need_b) out[2] = empty ? at::zeros(bias.sizes(), bias.options()) : at::empty(bias.sizes(), bias.options());
+    if (need_x) out[0] = empty_of(x.sizes(), x);
+    if (need_w) out[1] = empty ? at::zeros(weight.sizes(), weight.options()) : empty_of(weight.sizes(), weight);
+    if (need_b) out[2] = empty ? at::zeros(bias.sizes(), bias.options()) : empty_of(bias.sizes(), bias);
     if (empty) return out;
     int64_t stride_x, stride_dy;
     const Tensor rows = strided_rows(x, &stride_x, false), grad = strided_rows(dy, &stride_dy, false);
@@ -176,17 +236,17 @@ variable_list ln_backward(const Tensor& x, const Tensor& weight, const Tensor& b
     Tensor ws;
     if (need_w || need_b) {
         a.workspace_bytes = lib.layer_norm_workspace_bytes(a.groups, a.rows, a.dim, a.dtype);
-        ws = at::empty({a.workspace_bytes}, x.options().dtype(at::kByte));
+        ws = empty_of({a.workspace_bytes}, at::kByte, x);
         a.workspace = ws.data_ptr();
     }
     check(lib.layer_norm_backward(&a, stream_of(x)), "layer_norm backward");
     return out;
 }
-Tensor new_stats(const Tensor& x) { return at::empty({2, x.numel() / x.size(-1)}, x.options().dtype(at::kFloat)); }
+Tensor new_stats(const Tensor& x) { return empty_of({2, x.numel() / x.size(-1)}, at::kFloat, x); }
 
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, double add) {
-        const Tensor y = at::empty(x.sizes(), x.options()), stats = new_stats(x), w = or_none(weight), b = or_none(bias);
+        const Tensor y = empty_of(x.sizes(), x), stats = new_stats(x), w = or_none(weight), b = or_none(bias);
         ln_forward(x, w, b, eps, add, y, stats);
         ctx->save_for_backward({x, w, b, stats});
         ctx->saved_data["consts"] = std::vector<double>{eps, add};
@@ -201,17 +261,25 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 };
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, double add) {
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias))) return LayerNorm::apply(x, weight, bias, eps, add);
-    const Tensor y = at::empty(x.sizes(), x.options());
-    ln_forward(x, or_none(weight), or_none(bias), eps, add, y, Tensor());
+    Tensor w = or_none(weight), b = or_none(bias);
+    ln_prepare(x, w, b, add);
+    require_cuda(x, w, b);
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) return LayerNorm::apply(x, or_none(w), or_none(b), eps, add);
+    const Tensor y = empty_of(x.sizes(), x);
+    ln_forward(x, w, b, eps, add, y, Tensor());
     return y;
 }
+// without autograd: y and / or the statistics, and the gradients from these
 void layer_norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, double add, const OptTensor& y, const OptTensor& stats) {
-    ln_forward(x, or_none(weight), or_none(bias), eps, add, or_none(y), or_none(stats));
+    Tensor w = or_none(weight), b = or_none(bias);
+    ln_prepare(x, w, b, add);
+    ln_forward(x, w, b, eps, add, or_none(y), or_none(stats));
 }
 std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, const Tensor& stats,
                                                                 const Tensor& dy, double eps, double add, bool need_x, bool need_w, bool need_b) {
-    const auto g = ln_backward(x, or_none(weight), or_none(bias), stats, dy, eps, add, need_x, need_w, need_b);
+    Tensor w = or_none(weight), b = or_none(bias);
+    ln_prepare(x, w, b, add);
+    const auto g = ln_backward(x, w, b, stats, dy, eps, add, need_x, need_w, need_b);
     return {or_none(g[0]), or_none(g[1]), or_none(g[2])};
 }
 
@@ -228,15 +296,23 @@ int ids_type(const Tensor& ids) {
         case at::kFloat: return NB_IDS_F32;
         case at::kInt: return NB_IDS_I32;
         case at::kLong: return NB_IDS_I64;
-        default: return NB_IDS_F64;
+        case at::kDouble: return NB_IDS_F64;
+        default: TORCH_CHECK_VALUE(false, "ids must be float32, float64, int32 or int64, got ", ids.scalar_type());
     }
+}
+void check_ids(const char* what, const Tensor& ids, int64_t axes, int64_t batch, int64_t rows) {
+    ids_type(ids);
+    const int64_t d = ids.dim();
+    TORCH_CHECK_VALUE((d == 2 || (d == 3 && ids.size(0) == batch)) && ids.size(d - 2) == rows && ids.size(d - 1) == axes, "ids must be (", rows, ", ", axes,
+                      ") or (", batch, ", ", rows, ", ", axes, "), got ", ids.sizes());
+    TORCH_CHECK_VALUE(!(ids.requires_grad() && at::GradMode::is_enabled()), what, " has no gradient for ids");
 }
 // (q', k'): one launch over the heads of both; k may be undefined
 variable_list rotate(const Tensor& q_in, const Tensor& k_in, const Tensor& ids, const Ladder& ladder, bool half, bool inverse) {
     const c10::cuda::CUDAGuard guard(q_in.device());
     const Tensor q = q_in.stride(3) == 1 ? q_in : q_in.contiguous();
     const Tensor k = !k_in.defined() || k_in.stride(3) == 1 ? k_in : k_in.contiguous();
-    variable_list out = {at::empty(q.sizes(), q.options()), k.defined() ? at::empty(k.sizes(), k.options()) : Tensor()};
+    variable_list out = {empty_of(q.sizes(), q), k.defined() ? empty_of(k.sizes(), k) : Tensor()};
     nb_rotary_args a = {};
     a.q = q.const_data_ptr();
     a.q_out = out[0].data_ptr();
@@ -286,20 +362,32 @@ struct Rotary : torch::autograd::Function<Rotary> {
         return {g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-variable_list rotary_axes(const Tensor& q, const OptTensor& k, const Tensor& ids, const LadderPtr& ladder, bool half, bool inverse) {
-    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k))) return Rotary::apply(q, k, ids, ladder, half, inverse);
-    variable_list out = rotate(q, or_none(k), ids, *ladder, half, inverse);
-    if (!defined(k)) out.pop_back();
-    return out;
+// q', or (q', k')
+py::object rotary_axes(const Tensor& q, const OptTensor& k, const Tensor& ids, const LadderPtr& ladder, bool half, bool inverse) {
+    TORCH_CHECK_VALUE(known_type(q), "rotary_axes takes bfloat16, float16 and float32, got ", q.scalar_type());
+    TORCH_CHECK_VALUE(q.dim() == 4, "q must be (B, S, H, D), got ", q.sizes());
+    if (defined(k))
+        TORCH_CHECK_VALUE(k->dim() == 4 && k->scalar_type() == q.scalar_type() && k->size(0) == q.size(0) && k->size(1) == q.size(1) && k->size(3) == q.size(3),
+                          "k must be (B, S, Hk, D) beside q, got ", k->sizes(), " ", k->scalar_type(), " for ", q.sizes(), " ", q.scalar_type());
+    check_ids("rotary_axes", ids, ladder->l.n_axes, q.size(0), q.size(1));
+    TORCH_CHECK_VALUE(2 * ladder->pairs() <= q.size(3), "the axes have ", 2 * ladder->pairs(), " channels, more than a head (", q.size(3), ")");
+    TORCH_CHECK_VALUE(q.size(2) > 0 && (!defined(k) || k->size(2) > 0), "no heads");
+    require_cuda(q, or_none(k), ids);
+    const bool graph = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k));
+    const variable_list out = graph ? Rotary::apply(q, k, ids, ladder, half, inverse) : rotate(q, or_none(k), ids, *ladder, half, inverse);
+    return defined(k) ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
 }
 Tensor rotary_table(const Tensor& ids, const LadderPtr& ladder) {
+    TORCH_CHECK_VALUE(ids.dim() == 2 || ids.dim() == 3, "ids must be (S, axes) or (B, S, axes), got ", ids.sizes());
+    check_ids("rotary_table", ids, ladder->l.n_axes, ids.size(0), ids.size(-2));
+    require_cuda(ids);
     const c10::cuda::CUDAGuard guard(ids.device());
     const bool batched = ids.dim() == 3;
     auto shape = ids.sizes().vec();
     shape.back() = ladder->pairs();
     shape.push_back(1);
     shape.push_back(2);
-    const Tensor out = at::empty(shape, ids.options().dtype(at::kFloat));
+    const Tensor out = empty_of(shape, at::kFloat, ids);
     check(lib.rotary_table(ids.const_data_ptr(), ids_type(ids), batched ? (int32_t)ids.size(0) : 1, (int32_t)ids.size(batched), batched ? ids.stride(0) : 0,
                            ids.stride(batched), ids.stride(batched + 1), out.data_ptr<float>(), &ladder->l, stream_of(out)),
           "rotary_table");
@@ -328,7 +416,7 @@ nb_lora_args lora_args(int64_t rows, const Tensor& down, const Tensor& up, const
 Tensor run_lora(const Tensor& x, const Tensor& base, const Tensor& down, const Tensor& up, const Tensor& offsets, const Tensor& adapters, const Tensor& scale,
                 const Tensor& out, int64_t impl, int64_t status) {
     const int64_t rows = x.numel() / down.size(2);
-    const Tensor h = at::empty({2, rows, down.size(1)}, x.options());
+    const Tensor h = empty_of({2, rows, down.size(1)}, x);
     if (rows == 0) return h;
     const c10::cuda::CUDAGuard guard(x.device());
     nb_lora_args a = lora_args(rows, down, up, offsets, adapters, scale, impl, status);
@@ -348,7 +436,7 @@ Tensor run_lora(const Tensor& x, const Tensor& base, const Tensor& down, const T
 Tensor new_out(const Tensor& x, const Tensor& up) {
     auto shape = x.sizes().vec();
     shape.back() = up.size(1);
-    return at::empty(shape, x.options());
+    return empty_of(shape, x);
 }
 struct Lora : torch::autograd::Function<Lora> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& down, const Tensor& up, const OptTensor& base, const Tensor& offsets,
@@ -378,9 +466,9 @@ struct Lora : torch::autograd::Function<Lora> {
         const c10::cuda::CUDAGuard guard(down.device());
         const int64_t rows = dy.numel() / up.size(1);
         Tensor dx, ddown, dup, ws, xr, dyr;
-        if (need_x) dx = at::empty(shape, down.options());
-        if (need_down) ddown = rows ? at::empty(down.sizes(), down.options()) : at::zeros(down.sizes(), down.options());
-        if (need_up) dup = rows ? at::empty(up.sizes(), up.options()) : at::zeros(up.sizes(), up.options());
+        if (need_x) dx = empty_of(shape, down);
+        if (need_down) ddown = rows ? empty_of(down.sizes(), down) : at::zeros(down.sizes(), down.options());
+        if (need_up) dup = rows ? empty_of(up.sizes(), up) : at::zeros(up.sizes(), up.options());
         if (rows && (need_x || need_down || need_up)) {
             nb_lora_args a = lora_args(rows, down, up, saved[4], saved[5], saved[6], impl, status);
             dyr = strided_rows(dy, &a.stride_dy, true);
@@ -398,7 +486,7 @@ struct Lora : torch::autograd::Function<Lora> {
             // the workspace and g in one allocation (each costs the worker thread some microseconds)
             a.workspace_bytes = need_down || need_up ? lib.lora_workspace_bytes(&a) : 0;
             const int64_t at_g = (a.workspace_bytes + 255) / 256 * 256;
-            ws = at::empty({at_g + (need_x || need_down ? 4 * rows * down.size(1) : 0)}, down.options().dtype(at::kByte));
+            ws = empty_of({at_g + (need_x || need_down ? 4 * rows * down.size(1) : 0)}, at::kByte, down);
             if (a.workspace_bytes) a.workspace = ws.data_ptr();
             if (need_x || need_down) a.g = ws.data_ptr<uint8_t>() + at_g;
             check(lib.lora_backward(&a, stream_of(down)), "lora_batched backward");
@@ -407,10 +495,44 @@ struct Lora : torch::autograd::Function<Lora> {
         return {r[0], r[1], r[2], has_base && ctx->needs_input_grad(3) ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-Tensor lora_batched(const Tensor& x, const Tensor& down, const Tensor& up, const Tensor& offsets, const Tensor& adapters, const OptTensor& base,
-                    const OptTensor& scale, const OptTensor& out, int64_t impl, int64_t status) {
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(down) || wants_grad(up) || wants_grad(base)))
-        return Lora::apply(x, down, up, base, offsets, adapters, scale, impl, status);
+// Whether the kernels can write `t (..., C)` in place: rows evenly strided and apart, each on a 16-byte boundary.
+bool writable_rows(const Tensor& t) {
+    int64_t stride;
+    return even_rows(t, &stride) && stride % 8 == 0 && (stride >= t.size(-1) || t.numel() <= t.size(-1)) &&
+           (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0;
+}
+Tensor lora_batched(const Tensor& x, const Tensor& down_, const Tensor& up_, const Tensor& offsets_, const Tensor& adapters_, const OptTensor& base,
+                    const OptTensor& scale_, const OptTensor& out, int64_t impl) {
+    const auto type = x.scalar_type();
+    const auto other = [&](const Tensor& t) { return t.defined() && t.scalar_type() != type; };
+    TORCH_CHECK_VALUE((type == at::kBFloat16 || type == at::kHalf) && !other(down_) && !other(up_) && !other(or_none(base)) && !other(or_none(out)),
+                      "x, base, down, up and out must share one dtype, bfloat16 or float16");
+    TORCH_CHECK_VALUE(down_.dim() == 3 && up_.dim() == 3 && down_.size(0) == up_.size(0) && down_.size(1) == up_.size(2) && down_.size(0) > 0,
+                      "down must be (A, R, K) and up (A, N, R); got ", down_.sizes(), " and ", up_.sizes());
+    const int64_t A = down_.size(0), R = down_.size(1), K = down_.size(2), N = up_.size(1);
+    TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) == K, "x must be (..., ", K, "), got ", x.sizes());
+    const auto fits = [&](const OptTensor& t) {
+        return !defined(t) || (t->dim() == x.dim() && t->size(-1) == N && t->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1));
+    };
+    TORCH_CHECK_VALUE(fits(base), "base must be (..., ", N, ") beside x ", x.sizes(), ", got ", base->sizes());
+    TORCH_CHECK_VALUE(fits(out), "out must be (..., ", N, ") beside x ", x.sizes(), ", got ", out->sizes());
+    TORCH_CHECK_NOT_IMPLEMENTED(R > 0 && R % 16 == 0 && R <= NB_LORA_MAX_RANK && K > 0 && K % 8 == 0 && N > 0 && N % 8 == 0, "rank ", R,
+                                " must be a multiple of 16 up to ", NB_LORA_MAX_RANK, ", K=", K, " and N=", N, " multiples of 8");
+    TORCH_CHECK_VALUE(offsets_.scalar_type() == at::kInt && adapters_.scalar_type() == at::kInt && offsets_.dim() == 1 && adapters_.dim() == 1,
+                      "offsets and adapters must be 1-D int32 tensors");
+    TORCH_CHECK_VALUE(offsets_.size(0) == adapters_.size(0) + 1, adapters_.size(0), " adapters need ", adapters_.size(0) + 1, " offsets, got ",
+                      offsets_.size(0));
+    TORCH_CHECK_VALUE(!defined(scale_) || (scale_->scalar_type() == at::kFloat && scale_->dim() == 1 && scale_->size(0) == A), "scale must be (", A,
+                      ",) float32");
+    const bool grad = at::GradMode::is_enabled();
+    TORCH_CHECK_VALUE(!grad || !wants_grad(scale_), "lora_batched has no gradient for scale");
+    TORCH_CHECK_VALUE(!defined(out) || writable_rows(*out), "out must have evenly strided rows on 16-byte boundaries that do not overlap");
+    const int64_t status = require_cuda(x, down_, up_, offsets_, adapters_, or_none(base), or_none(scale_), or_none(out));
+    const bool graph = grad && (wants_grad(x) || wants_grad(down_) || wants_grad(up_) || wants_grad(base));
+    TORCH_CHECK_VALUE(!defined(out) || !(graph || (grad && wants_grad(out))), "out cannot be given where a gradient is asked for");
+    const Tensor down = down_.contiguous(), up = up_.contiguous(), offsets = offsets_.contiguous(), adapters = adapters_.contiguous();
+    const OptTensor scale = defined(scale_) ? OptTensor(scale_->contiguous()) : std::nullopt;
+    if (graph) return Lora::apply(x, down, up, base, offsets, adapters, scale, impl, status);
     const Tensor to = defined(out) ? *out : new_out(x, up);
     run_lora(x, or_none(base), down, up, offsets, adapters, or_none(scale), to, impl, status);
     if (defined(out) && !to.is_inference()) to.unsafeGetTensorImpl()->bump_version();  // a graph that saved it must notice

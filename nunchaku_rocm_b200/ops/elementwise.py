@@ -85,39 +85,6 @@ def gated_residual(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, y2: tor
     return out
 
 
-def _ln_weight(name, w, x, groups):
-    """``w`` as the kernel reads it, with the stride between its groups' rows."""
-    D = x.shape[-1]
-    if w.dtype != x.dtype and w.dtype != torch.float32:
-        raise ValueError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
-    if w.shape != ((D,) if w.dim() == 1 else (groups, D)) or (w.dim() == 2 and x.dim() != 3):
-        raise ValueError(f"{name} must be ({D},), or (B, {D}) for x (B, T, {D}); got {tuple(w.shape)} for {tuple(x.shape)}")
-    return w if w.stride(-1) == 1 else w.contiguous()
-
-
-def _ln_prepare(x, weight, bias, weight_add):
-    """The checks of the arguments; weight and bias with one stride and unit inner stride."""
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"layer_norm needs at least one channel, got x {tuple(x.shape)}")
-    if x.shape[-1] > 16384:
-        raise NotImplementedError(f"layer_norm takes up to 16384 channels, got {x.shape[-1]}")
-    if x.dtype not in L.DTYPE_CODE_32:
-        raise ValueError(f"layer_norm takes bfloat16, float16 and float32, got {x.dtype}")
-    if weight is None and weight_add:
-        raise ValueError("weight_add without a weight")
-    groups = x.shape[0] if x.dim() == 3 else 1
-    if weight is not None:
-        weight = _ln_weight("weight", weight, x, groups)
-    if bias is not None:
-        bias = _ln_weight("bias", bias, x, groups)
-        if weight is not None:
-            if bias.dtype != weight.dtype or bias.dim() != weight.dim():
-                raise ValueError("weight and bias must have one shape and one dtype")
-            if bias.dim() == 2 and bias.stride(0) != weight.stride(0):
-                weight, bias = weight.contiguous(), bias.contiguous()
-    return weight, bias
-
-
 class _LayerNormModulate(torch.autograd.Function):
     """:func:`layernorm_modulate` as it is without gradients, and the backward pass of the function that it rounds."""
 
@@ -132,7 +99,6 @@ class _LayerNormModulate(torch.autograd.Function):
     def backward(ctx, dy):
         eps, scale_add = ctx.consts
         x, scale, shift = ctx.saved_tensors
-        scale, shift = _ln_prepare(x, scale, shift, scale_add)
         stats = x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
         b = L.binding()
         b.layer_norm_forward(x, None, None, eps, 0.0, None, stats)
@@ -149,6 +115,4 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     and shift, then with ``weight_add=1``), both of ``x``'s dtype or both float32; either may be ``None``.  Their gradients
     are summed over the rows in fp32, in a fixed order.  ``D`` is at most 16384, ``B`` with a row per sample at most 65535.
     """
-    weight, bias = _ln_prepare(x, weight, bias, weight_add)
-    L.require_cuda(x, weight, bias)
     return L.binding().layer_norm(x, weight, bias, eps, weight_add)

@@ -28,14 +28,6 @@ def _ladder(axes_dim: tuple, theta: float):
     return L.binding().Ladder(axes_dim, theta)
 
 
-def _check_ids(ids: torch.Tensor, n_axes: int, batch: int, rows: int) -> None:
-    if ids.dtype not in L.IDS_CODE:
-        raise ValueError(f"ids must be float32, float64, int32 or int64, got {ids.dtype}")
-    shape = ids.shape
-    if shape != (rows, n_axes) and shape != (batch, rows, n_axes):
-        raise ValueError(f"ids must be ({rows}, {n_axes}) or ({batch}, {rows}, {n_axes}), got {tuple(shape)}")
-
-
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes_dim, theta: float = 10000.0,
                 interleaved: bool = True, inverse: bool = False):
     """
@@ -49,24 +41,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes
 
     bfloat16, float16 or float32; any strides; ``ids`` float32, float64, int32 or int64.
     """
-    if q.dtype not in L.DTYPE_CODE_32:
-        raise ValueError(f"rotary_axes takes bfloat16, float16 and float32, got {q.dtype}")
-    if q.dim() != 4:
-        raise ValueError(f"q must be (B, S, H, D), got {tuple(q.shape)}")
-    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]):
-        raise ValueError(f"k must be (B, S, Hk, D) beside q, got {tuple(k.shape)} {k.dtype} for {tuple(q.shape)} {q.dtype}")
-    ladder = _ladder(tuple(axes_dim), float(theta))
-    B, S, H, D = q.shape
-    _check_ids(ids, ladder.n_axes, B, S)
-    if 2 * ladder.pairs > D:
-        raise ValueError(f"axes {tuple(axes_dim)} have more channels than a head ({D})")
-    if H == 0 or (k is not None and k.shape[2] == 0):
-        raise ValueError("no heads")
-    if ids.requires_grad and torch.is_grad_enabled():
-        raise ValueError("rotary_axes has no gradient for ids")
-    L.require_cuda(q, k, ids)
-    out = L.binding().rotary_axes(q, k, ids, ladder, not interleaved, inverse)
-    return out[0] if k is None else (out[0], out[1])
+    return L.binding().rotary_axes(q, k, ids, _ladder(tuple(axes_dim), float(theta)), not interleaved, inverse)
 
 
 def rotary_table(ids: torch.Tensor, axes_dim, theta: float = 10000.0) -> torch.Tensor:
@@ -74,12 +49,4 @@ def rotary_table(ids: torch.Tensor, axes_dim, theta: float = 10000.0) -> torch.T
     The ``(sin, cos)`` table of ``ids (S, axes)`` -> ``(S, sum(axes_dim) / 2, 1, 2)`` fp32 (or with a leading ``B``): what
     the fused QKV epilogue reads as ``rotary_emb``, with the angles of :func:`rotary_axes`.
     """
-    if ids.dim() not in (2, 3):
-        raise ValueError(f"ids must be (S, axes) or (B, S, axes), got {tuple(ids.shape)}")
-    ladder = _ladder(tuple(axes_dim), float(theta))
-    B, S = (1, ids.shape[0]) if ids.dim() == 2 else ids.shape[:2]
-    _check_ids(ids, ladder.n_axes, B, S)
-    if ids.requires_grad and torch.is_grad_enabled():
-        raise ValueError("rotary_table has no gradient for ids")
-    L.require_cuda(ids)
-    return L.binding().rotary_table(ids, ladder)
+    return L.binding().rotary_table(ids, _ladder(tuple(axes_dim), float(theta)))
