@@ -20,7 +20,8 @@
 // the matrix instructions of the second products, which move more bytes than they compute.
 //
 // Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out); for a few rows the latency of two
-// dependent kernels, 24 single rows of 24 requests, 3072 -> 18432, rank 16: 6.3 + 9.9 us, of which one overlaps.
+// dependent kernels, 24 single rows of 24 requests, 3072 -> 18432, rank 16: 12.9 us back to back in a graph.  The forward
+// pass of so few rows is one kernel therefore (9.3 us; the floor by bytes is 2).
 #include <cooperative_groups.h>
 
 #include "lora.cuh"
@@ -343,6 +344,205 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- few rows
+// Both products of the forward pass in one kernel, for items of at most 16 rows.  A cluster of eight CTAs has an item: each
+// CTA takes an eighth of the contraction of h, the eight sums meet through shared memory, and each CTA multiplies the whole
+// h with its own columns' part of U, which has been on its way into shared memory since the kernel began.  Both products run
+// on m16n8k16 with the order of k chosen so that a thread's operands are 16 (8) consecutive bytes: any order will do as long
+// as both operands have the same.  The columns of four neighbouring tiles are dealt out so that a thread ends with eight
+// consecutive ones.
+// Bound: latency (index, operands, two cluster barriers, store); what is read again is read from L2.
+struct FewParams {
+    LoraParams l;  // x, K: of h; factor: D; out
+    const void* base; const void* up;
+    long long stride_base;
+    int N, cols;  // columns of a CTA, a multiple of 32
+};
+constexpr int kFewRows = 16, kFewWarps = 8, kFewCluster = 8;
+template <int R>
+struct FewTile {
+    static constexpr int LDH = R + 8;
+    // ranks of a warp in the first product (its sums and its steps of D in registers, two CTAs per SM), warps along k
+    static constexpr int RW = R <= 32 ? R : R / 2, KW = kFewWarps * RW / R;
+    static constexpr int RED = KW * 16 * R * 4, PART = 16 * R * 4, H = 2 * 16 * LDH * 2;
+    static int bytes(int cols) { return cols * R * 2 + RED + PART + H; }
+    // 16-byte piece of U's row: pieces that half a warp reads together are on different banks
+    static __device__ __forceinline__ int piece(int row, int ch) {
+        const int far = (row >> 3) & 1;
+        if (R == 16) return (row ^ (far << 1)) * 2 + ch;
+        if (R == 32) return row * 4 + (ch ^ (far << 1));
+        if (R == 64) return row * 8 + (ch ^ ((row & 1) << 1) ^ (far << 2));
+        return row * (R / 8) + ch;
+    }
+};
+template <typename T, int R>
+__global__ void __launch_bounds__(kFewWarps * 32, 2) lora_few_kernel(const FewParams f) {
+    using S = FewTile<R>;
+    extern __shared__ __align__(16) unsigned char few_smem[];
+    const LoraParams& p = f.l;
+    const Item it = find_item<kFewWarps * 32>(p, blockIdx.x);
+    if (it.rows == 0) return;  // every CTA of the cluster
+    const int col0 = blockIdx.y * f.cols, ncols = max(0, min(f.cols, f.N - col0));
+    const T* base = f.base ? static_cast<const T*>(f.base) + it.first * f.stride_base + col0 : nullptr;
+    T* out = static_cast<T*>(p.out) + it.first * p.stride_out + col0;
+    if (it.adapter < 0) {  // base alone (zeros without one)
+        if (base == out) return;
+        for (int e = threadIdx.x; e < it.rows * (ncols / 8); e += kFewWarps * 32) {
+            const int row = e / (ncols / 8), c = (e - row * (ncols / 8)) * 8;
+            const uint4 v = base ? *reinterpret_cast<const uint4*>(base + row * f.stride_base + c) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out + row * p.stride_out + c) = v;
+        }
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    unsigned char* us = few_smem;
+    float* red = reinterpret_cast<float*>(few_smem + (size_t)f.cols * R * 2);
+    float* part = red + S::RED / 4;
+    T* hs = reinterpret_cast<T*>(part + S::PART / 4);
+    const bool on0 = g < it.rows, on1 = g + 8 < it.rows;
+    // this CTA's part of h: 32 values of k per step
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank();
+    const int slice = (p.K + 32 * kFewCluster - 1) / (32 * kFewCluster) * 32, k1 = min((rank + 1) * slice, p.K);
+    const T* x0 = static_cast<const T*>(p.x) + (it.first + g) * p.stride_x;
+    const T* x1 = x0 + 8 * p.stride_x;
+    const int kw = warp % S::KW, r0 = warp / S::KW * S::RW;
+    const T* d0 = static_cast<const T*>(p.factor) + ((long long)it.adapter * R + r0 + g) * p.K;
+    constexpr int DEPTH = R == 16 ? 3 : 2, STEP = S::KW * 32, NT = S::RW / 8;  // steps on their way; tiles of r
+    uint4 xa[DEPTH], xb[DEPTH], d[DEPTH][NT];
+    auto load = [&](int i, int k0) {
+        const int k = k0 + t * 8;
+        const bool in = k < k1;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        xa[i] = in && on0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+        xb[i] = in && on1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) d[i][n] = in ? __ldg(reinterpret_cast<const uint4*>(d0 + (long long)n * 8 * p.K + k)) : zero;
+    };
+    const int first = rank * slice + kw * 32;
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) load(i, first + i * STEP);
+    // U and base under their latency
+    {
+        const T* u = static_cast<const T*>(f.up) + ((long long)it.adapter * f.N + col0) * R;
+        const uint32_t to = smem_u32(us);
+        for (int e = threadIdx.x; e < ncols * (R / 8); e += kFewWarps * 32) {
+            const int row = e / (R / 8), ch = e % (R / 8);
+            cp16(to + S::piece(row, ch) * 16, u + (long long)e * 8, true);
+        }
+        cp_commit();
+    }
+    // the first blocks of base: a warp has every eighth block of 32 columns
+    constexpr int AHEAD = 3;
+    const int blocks = (ncols + 31) / 32;
+    uint4 b0[AHEAD], b1[AHEAD];
+    auto fetch = [&](int i, int blk) {
+        const int c = blk * 32 + t * 8;
+        const bool in = base && c < ncols;
+        b0[i] = in && on0 ? *reinterpret_cast<const uint4*>(base + g * f.stride_base + c) : make_uint4(0, 0, 0, 0);
+        b1[i] = in && on1 ? *reinterpret_cast<const uint4*>(base + (g + 8) * f.stride_base + c) : make_uint4(0, 0, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(i, warp + i * kFewWarps);
+
+    float acc[NT][4] = {};
+    for (int k0 = first; k0 < k1; k0 += DEPTH * STEP) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+            if (k0 + i * STEP >= k1) break;
+            const uint32_t a0[4] = {xa[i].x, xb[i].x, xa[i].y, xb[i].y}, a1[4] = {xa[i].z, xb[i].z, xa[i].w, xb[i].w};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma16816<T>(acc[n], a0, d[i][n].x, d[i][n].y);
+                mma16816<T>(acc[n], a1, d[i][n].z, d[i][n].w);
+            }
+            load(i, k0 + (i + DEPTH) * STEP);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float* at = red + (kw * 16 + g) * R + r0 + n * 8 + t * 2;
+        *reinterpret_cast<float2*>(at) = make_float2(acc[n][0], acc[n][1]);
+        *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[n][2], acc[n][3]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * R; e += kFewWarps * 32) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < S::KW; ++w) s += red[w * 16 * R + e];
+        part[e] = s;
+    }
+    const float scale = p.scale ? __ldg(p.scale + it.adapter) : 1.f;
+    cluster.sync();
+    for (int e = threadIdx.x; e < 16 * R; e += kFewWarps * 32) {
+        float v[kFewCluster], h = 0.f;
+#pragma unroll
+        for (int q = 0; q < kFewCluster; ++q) v[q] = cluster.map_shared_rank(part, q)[e];
+#pragma unroll
+        for (int q = 0; q < kFewCluster; ++q) h += v[q];
+        h *= scale;
+        const int row = e / R, r = e % R;
+        const T hi = from_f32<T>(h);
+        const float back = to_f32(hi);
+        const T lo = from_f32<T>(isfinite(back) ? h - back : 0.f);  // (beyond T: infinite in hi alone)
+        hs[row * S::LDH + r] = hi;
+        hs[(16 + row) * S::LDH + r] = lo;
+        if (blockIdx.y == 0 && row < it.rows) {  // for the backward pass
+            const long long at = (long long)(it.first + row) * R + r;
+            static_cast<T*>(p.hi)[at] = hi;
+            static_cast<T*>(p.lo)[at] = lo;
+        }
+    }
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // the others' sums have been read
+    cp_wait<0>();
+    __syncthreads();
+
+    uint32_t a[2][R / 16][4];
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int s = 0; s < R / 16; ++s) {
+            const uint2 lo8 = *reinterpret_cast<const uint2*>(hs + (v * 16 + g) * S::LDH + s * 16 + t * 4);
+            const uint2 hi8 = *reinterpret_cast<const uint2*>(hs + (v * 16 + g + 8) * S::LDH + s * 16 + t * 4);
+            a[v][s][0] = lo8.x; a[v][s][1] = hi8.x; a[v][s][2] = lo8.y; a[v][s][3] = hi8.y;
+        }
+    for (int blk0 = warp; blk0 < blocks; blk0 += AHEAD * kFewWarps) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int blk = blk0 + i * kFewWarps;
+            if (blk >= blocks) break;
+            float o[4][4] = {};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // column n of tile j; behind the last column: some other row of U, whose result is not stored
+                const int row = min(blk * 32 + (g >> 1) * 8 + j * 2 + (g & 1), ncols - 1);
+#pragma unroll
+                for (int s = 0; s < R / 16; ++s) {
+                    const uint2 b = *reinterpret_cast<const uint2*>(us + S::piece(row, s * 2 + (t >> 1)) * 16 + (t & 1) * 8);
+                    mma16816<T>(o[j], a[0][s], b.x, b.y);
+                    mma16816<T>(o[j], a[1][s], b.x, b.y);
+                }
+            }
+            auto joined = [&](const uint4& b, int at) {
+                const uint32_t in[4] = {b.x, b.y, b.z, b.w};
+                uint32_t r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 v = unpack2<T>(in[j]);
+                    r[j] = pack2<T>(v.x + o[j][at], v.y + o[j][at + 1]);
+                }
+                return make_uint4(r[0], r[1], r[2], r[3]);
+            };
+            const int c = blk * 32 + t * 8;
+            if (c < ncols && on0) *reinterpret_cast<uint4*>(out + g * p.stride_out + c) = joined(b0[i], 0);
+            if (c < ncols && on1) *reinterpret_cast<uint4*>(out + (g + 8) * p.stride_out + c) = joined(b1[i], 2);
+            fetch(i, blk + AHEAD * kFewWarps);
+        }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
 // ------------------------------------------------------------------------------------------------------------------- outer
 // part[item][r, k] = sum over the item's rows of v[t, r] X[t, k] (or [k, r] with KROWS), fp32, for one item of up to
 // rows_per_item rows and 128 columns.  Both operands are transposed on the way from shared memory to registers.
@@ -526,6 +726,21 @@ bool use_tc(const nb_lora_args* a) {
     if (a->R >= 32 && contraction >= 8192 && a->T >= 16ll * a->requests) return true;
     return a->T >= 96ll * a->requests && (double)a->T * a->R * a->R * ((double)a->K + a->N) >= 1e10;
 }
+// Whether the forward pass is the one kernel for few rows: where its clusters are resident together, or in two turns when
+// one cluster per item is enough (it then reads D once and still saves a kernel).  Two kernels / one, measured: rank 16, K =
+// 3072, N = 18432: 1 row 7.2 / 5.6 us, 24 rows of 24 requests 12.9 / 9.3, 64 of 64 (two turns) 25.3 / 17.2; rank 32, K =
+// 12288, N = 3072: 128 rows 22.9 / 7.6 (15.1 on tcgen05), 1024 rows of 64 requests (two turns) 26.6 / 22.5; K = 2048, N = 6144,
+// 1024 rows of 64 requests: rank 16 15.5 / 16.5, rank 32 20.4 / 19.9.  Not taken: rank 64, K = 3072, N = 18432 (four clusters
+// per item), 256 rows 19.1 / 22.6; rank 32, 24 rows of 24 requests (two clusters per item) 16.1 / 16.9.
+int few_need(const nb_lora_args* a) {  // clusters of an item that keep a CTA's part of U within 80 KB
+    return ceil_div((long long)a->N * a->R * 2, kFewCluster * 80 * 1024);
+}
+bool use_few(const nb_lora_args* a) {
+    if (a->impl == NB_IMPL_TCGEN05 || a->R > 64) return false;
+    const long long tiles = ceil_div(a->T, kFewRows), requests = a->requests < a->T ? a->requests : a->T;
+    const int need = few_need(a);
+    return (tiles > requests ? tiles : requests) * need * kFewCluster <= 2ll * sms() * (need == 1 ? 2 : 1);
+}
 // A tcgen05 launch, or the mma.sync one where there is no tensor map for the operands (rows a stride of zero apart) and the
 // caller did not insist.
 #define NB_TC_OR(a, tc_call, call)                                                                             \
@@ -568,13 +783,34 @@ int expand(LoraParams p, cudaStream_t s) {
     using S = ExpandTile<RM, CCONTIG>;
     const int items = item_count(p.T, p.requests, kRows);
     const int live = live_items(p, kRows);
-    // columns of a CTA: whole tiles, as many as leave about four CTAs per SM: they are resident together (24 rows of 24
-    // requests, 3072 -> 18432, rank 16: 12.8 us the call, 14.5 with eight per SM in two waves, 14.5 with two)
+    // columns of a CTA: whole tiles, as many as leave about four CTAs per SM: they are resident together (measured
+    // with 24 rows of 24 requests, 3072 -> 18432, rank 16: 12.8 us for both products, 14.5 with eight per SM in two waves, 14.5
+    // with two)
     const int tiles = ceil_div(p.K, S::BN), per = ceil_div(4ll * sms(), live);
     p.cols_per_cta = ceil_div(tiles, per < tiles ? per : tiles) * S::BN;
     auto* kernel = lora_expand_kernel<T, RM, CCONTIG>;
     if (int rc = allow_smem(kernel, S::BYTES)) return rc;
     return launch(kernel, dim3(ceil_div(p.K, p.cols_per_cta), items), kThreads, S::BYTES, 1, p.chained, s, p);
+}
+template <typename T, int R>
+int few(const nb_lora_args* a, const LoraParams& p, cudaStream_t s) {
+    FewParams f = {};
+    f.l = p;
+    f.l.rows_per_item = kFewRows;
+    f.l.x = a->x; f.l.stride_x = a->stride_x; f.l.factor = a->down; f.l.K = a->K;
+    f.l.out = a->out; f.l.stride_out = a->stride_out;
+    f.base = a->base; f.stride_base = a->stride_base; f.up = a->up; f.N = a->N;
+    // clusters of an item: more than it needs where few items leave SMs idle, each of which computes h anew, as long as that
+    // reads less than its columns
+    const int live = live_items(f.l, kFewRows), need = few_need(a);
+    int splits = 2 * sms() / (kFewCluster * live);
+    if (splits > ceil_div(a->N, a->K)) splits = ceil_div(a->N, a->K);
+    if (splits < need) splits = need;
+    f.cols = ceil_div(ceil_div(a->N, kFewCluster * splits), 32) * 32;
+    auto* kernel = lora_few_kernel<T, R>;
+    const int bytes = FewTile<R>::bytes(f.cols);
+    if (int rc = allow_smem(kernel, bytes)) return rc;
+    return launch(kernel, dim3(item_count(a->T, a->requests, kFewRows), kFewCluster * splits), kFewWarps * 32, bytes, kFewCluster, false, s, f);
 }
 template <typename T, int RM, bool KROWS>
 int outer(const nb_lora_args* a, LoraParams p, cudaStream_t s) {
@@ -618,6 +854,12 @@ int forward_t(const nb_lora_args* a, cudaStream_t s) {
     LoraParams p = params_of(a);
     p.hi = plane(a->h, a, 0);
     p.lo = plane(a->h, a, 1);
+    if (use_few(a)) switch (a->R) {
+            case 16: return few<T, 16>(a, p, s);
+            case 32: return few<T, 32>(a, p, s);
+            case 48: return few<T, 48>(a, p, s);
+            default: return few<T, 64>(a, p, s);
+        }
     p.x = a->x; p.stride_x = a->stride_x; p.factor = a->down; p.K = a->K;
     if (int rc = NB_TC_OR(a, tc_shrink(p, false, a->dtype, s), (shrink<T, RM, false>(p, s)))) return rc;
     p.chained = true;

@@ -362,3 +362,21 @@ def test_more_than_2_31_elements(cuda_dev, impl):
     within(out[-tail:], *ref["out"])
     within(dx[-tail:], *ref["dx"])
     assert L.device_status(cuda_dev) == 0
+
+
+@gpu
+@pytest.mark.parametrize("R", [16, 32, 48, 64])
+@pytest.mark.parametrize("K,N", [(8, 8), (40, 264), (2048, 18432), (12288, 72)])
+@pytest.mark.parametrize("T,offsets,adapters", [
+    (1, [0, 1], [0]),
+    (17, [0, 16, 17], [1, 0]),
+    (24, list(range(25)), [i % 4 - 1 for i in range(24)]),
+    (70, [2, 2, 3, 20, 20, 69], [2, 0, -1, 1, 2]),
+])
+def test_few_rows(cuda_dev, R, K, N, T, offsets, adapters):
+    # the forward pass in one kernel, and the adapters' part added in place
+    p = make(cuda_dev, T, K, N, R, 3, BF16 if R % 32 else FP16, seed=T + R)
+    check_impl(cuda_dev, p, offsets, adapters, True, True, L.IMPL_AUTO)
+    out = p["base"].clone()
+    lora_batched(p["x"], p["down"], p["up"], *index(cuda_dev, offsets, adapters), base=out, scale=p["scale"], out=out)
+    assert torch.equal(out, lora_batched(p["x"], p["down"], p["up"], *index(cuda_dev, offsets, adapters), base=p["base"], scale=p["scale"]))
