@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraParams 
     using S = ShrinkTile<RM, RCONTIG>;
     extern __shared__ __align__(128) unsigned char smem[];
     chain_next();
-    const Item it = find_item<kThreads>(p, blockIdx.x);
+    const Item it = find_item<kThreads>(p, blockIdx.x, p.rows_per_item);
     if (it.rows == 0 || it.adapter < 0) return;  // every CTA of the cluster
     const int splits = gridDim.y, split = blockIdx.y;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
     using S = ExpandTile<RM, CCONTIG>;
     constexpr int BN = S::BN;
     extern __shared__ __align__(128) unsigned char smem[];
-    const Item it = find_item<kThreads>(p, blockIdx.y);
+    const Item it = find_item<kThreads>(p, blockIdx.y, p.rows_per_item);
     if (it.rows == 0) return;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int col0 = blockIdx.x * p.cols_per_cta, col1 = min(col0 + p.cols_per_cta, p.K);
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) lora_few_kernel(const FewPa
     using S = FewTile<R>;
     extern __shared__ __align__(16) unsigned char few_smem[];
     const LoraParams& p = f.l;
-    const Item it = find_item<kFewWarps * 32>(p, blockIdx.x);
+    const Item it = find_item<kFewWarps * 32>(p, blockIdx.x, kFewRows);
     if (it.rows == 0) return;  // every CTA of the cluster
     const int col0 = blockIdx.y * f.cols, ncols = max(0, min(f.cols, f.N - col0));
     const T* base = f.base ? static_cast<const T*>(f.base) + it.first * f.stride_base + col0 : nullptr;
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) lora_few_kernel(const FewPa
 }
 
 // ------------------------------------------------------------------------------------------------------------------- outer
-// part[item][r, k] = sum over the item's rows of v[t, r] X[t, k] (or [k, r] with KROWS), fp32, for one item of up to
+// part[item][r, k] = sum over the item's rows of v[t, r] X[t, k] ([k, r] with KROWS, job 0), fp32, for one item of up to
 // rows_per_item rows and 128 columns.  Both operands are transposed on the way from shared memory to registers.
 template <int RM>
 struct OuterTile {
@@ -554,21 +554,12 @@ struct OuterTile {
     static constexpr int STAGE = XBYTES + 2 * VBYTES, BYTES = ST * STAGE;
 };
 template <typename T, int RM, bool KROWS>
-__global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p) {
+__device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJob& job, const Item& it, int w, int c0, unsigned char* smem) {
     using S = OuterTile<RM>;
-    extern __shared__ __align__(128) unsigned char smem[];
-    // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
-    const int w = gridDim.y - 1 - blockIdx.y;
-    chain_next();
-    const Item it = find_item<kThreads>(p, w);
-    chain_wait();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    if (blockIdx.x == 0 && t == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
-    if (it.rows == 0 || it.adapter < 0) return;
-    const int c0 = blockIdx.x * 128;
-    const T* x = static_cast<const T*>(p.x) + (long long)it.first * p.stride_x;
-    const char* hi = static_cast<const char*>(p.hi) + (long long)it.first * p.R * 2;
-    const char* lo = static_cast<const char*>(p.lo) + (long long)it.first * p.R * 2;
+    const T* x = static_cast<const T*>(job.x) + (long long)it.first * job.stride_x;
+    const char* hi = static_cast<const char*>(job.hi) + (long long)it.first * p.R * 2;
+    const char* lo = static_cast<const char*>(job.lo) + (long long)it.first * p.R * 2;
     const uint32_t sm = smem_u32(smem);
     const int n = (it.rows + S::BT - 1) / S::BT;
 
@@ -579,8 +570,8 @@ __global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p
 #pragma unroll
             for (int i = 0; i < S::BT * 16 / kThreads; ++i) {
                 const int e = i * kThreads + t, row = e >> 4, c = c0 + (e & 15) * 8;
-                const bool real = r0 + row < it.rows && c < p.K;
-                cp16(st + row * S::XROW + (e & 15) * 16, real ? x + (r0 + row) * p.stride_x + c : x, real);
+                const bool real = r0 + row < it.rows && c < job.K;
+                cp16(st + row * S::XROW + (e & 15) * 16, real ? x + (r0 + row) * job.stride_x + c : x, real);
             }
             for (int e = t; e < S::BT * RM * 2; e += kThreads) {
                 const int row = e / (RM * 2), r = e % (RM * 2) * 8;
@@ -649,7 +640,7 @@ __global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p
         }
     }
     cp_wait<0>();
-    float* part = p.part + (long long)w * p.R * p.K;
+    float* part = job.part + (long long)w * p.R * job.K;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -660,12 +651,28 @@ __global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p
                 const float2 v = make_float2(acc[i][j][2 * o], acc[i][j][2 * o + 1]);
                 if constexpr (KROWS) {
                     const int k = c0 + warp * 32 + mrow;
-                    if (k < p.K && ncol < p.R) *reinterpret_cast<float2*>(part + (long long)k * p.R + ncol) = v;
+                    if (k < job.K && ncol < p.R) *reinterpret_cast<float2*>(part + (long long)k * p.R + ncol) = v;
                 } else {
                     const int k = c0 + warp * 32 + ncol;
-                    if (k < p.K && mrow < p.R) *reinterpret_cast<float2*>(part + (long long)mrow * p.K + k) = v;
+                    if (k < job.K && mrow < p.R) *reinterpret_cast<float2*>(part + (long long)mrow * job.K + k) = v;
                 }
             }
+}
+
+template <typename T, int RM>
+__global__ void __launch_bounds__(kThreads) lora_outer_kernel(const LoraParams p, const __grid_constant__ OuterJobs jobs) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
+    const int group = (int)blockIdx.x - jobs.groups, which = group < 0 ? 0 : 1;
+    const int w = jobs.job[which].items - 1 - (int)blockIdx.y;
+    chain_next();
+    const Item it = find_item<kThreads>(p, w, jobs.job[which].rows);
+    chain_wait();
+    if (w < 0) return;  // (the other job has more items)
+    if ((blockIdx.x == 0 || group == 0) && threadIdx.x == 0) jobs.job[which].item_adapter[w] = it.rows ? it.adapter : -1;
+    if (it.rows == 0 || it.adapter < 0) return;
+    if (group < 0) outer_product<T, RM, true>(p, jobs.job[0], it, w, (int)blockIdx.x * 128, smem);
+    else outer_product<T, RM, false>(p, jobs.job[1], it, w, group * 128, smem);
 }
 
 // dF[a] = sum of the partial products of a's items, in the items' order; zero for an adapter without rows.  One launch for
@@ -719,11 +726,13 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const Join<T> first, con
 // feeds their instructions) and, having 64-row items in clusters of eight, with a long contraction over few rows.  Measured,
 // mma.sync / tcgen05, forward, K = 2048, N = 6144: rank 16: 512 rows 9.0 / 13.3 us, 8192 rows 50.9 / 48.8; rank 64: 512 rows
 // 15.6 / 12.2, 1024 rows 22.7 / 16.3; 64 requests of 32 rows 38.5 / 42.6, of 64 rows 57.0 / 54.6.  K = 12288, N = 3072: rank 32,
-// 128 rows 22.9 / 15.1 us; rank 64, 128 rows of 4 requests 26.6 / 16.6, 16 single rows 24.3 / 28.3.
+// 128 rows 22.9 / 15.1 us; rank 64, 128 rows of 4 requests 26.6 / 16.6, 16 single rows 24.3 / 28.3.  Rank 128, K = 2048, N =
+// 6144: 2048 rows of 32 requests 46.4 / 38.5 us, 512 rows of 16 25.9 / 27.3.
 bool use_tc(const nb_lora_args* a) {
     if (a->impl != NB_IMPL_AUTO) return a->impl == NB_IMPL_TCGEN05;
     const int contraction = a->dy ? a->N : a->K;
     if (a->R >= 32 && contraction >= 8192 && a->T >= 16ll * a->requests) return true;
+    if (a->R > 64 && a->T >= 48ll * a->requests) return true;
     return a->T >= 96ll * a->requests && (double)a->T * a->R * a->R * ((double)a->K + a->N) >= 1e10;
 }
 // Whether the forward pass is the one kernel for few rows: where its clusters are resident together, or in two turns when
@@ -796,7 +805,6 @@ template <typename T, int R>
 int few(const nb_lora_args* a, const LoraParams& p, cudaStream_t s) {
     FewParams f = {};
     f.l = p;
-    f.l.rows_per_item = kFewRows;
     f.l.x = a->x; f.l.stride_x = a->stride_x; f.l.factor = a->down; f.l.K = a->K;
     f.l.out = a->out; f.l.stride_out = a->stride_out;
     f.base = a->base; f.stride_base = a->stride_base; f.up = a->up; f.N = a->N;
@@ -812,27 +820,29 @@ int few(const nb_lora_args* a, const LoraParams& p, cudaStream_t s) {
     if (int rc = allow_smem(kernel, bytes)) return rc;
     return launch(kernel, dim3(item_count(a->T, a->requests, kFewRows), kFewCluster * splits), kFewWarps * 32, bytes, kFewCluster, false, s, f);
 }
-template <typename T, int RM, bool KROWS>
-int outer(const nb_lora_args* a, LoraParams p, cudaStream_t s) {
+template <typename T, int RM>
+int outer(const nb_lora_args* a, const LoraParams& p, OuterJobs j, cudaStream_t s) {
     using S = OuterTile<RM>;
-    p.rows_per_item = outer_rows(a, p.K);
-    const int items = item_count(p.T, p.requests, p.rows_per_item);
     auto small = [&]() -> int {
-        auto* kernel = lora_outer_kernel<T, RM, KROWS>;
+        auto* kernel = lora_outer_kernel<T, RM>;
         if (int rc = allow_smem(kernel, S::BYTES)) return rc;
-        return launch(kernel, dim3(ceil_div(p.K, 128), items), kThreads, S::BYTES, 1, p.chained, s, p);
+        j.groups = ceil_div(j.job[0].K, 128);
+        const int groups = j.groups + ceil_div(j.job[1].K, 128);
+        const int items = j.job[0].items > j.job[1].items ? j.job[0].items : j.job[1].items;
+        return launch(kernel, dim3(groups, items), kThreads, S::BYTES, 1, p.chained, s, p, j);
     };
-    return NB_TC_OR(a, tc_outer(p, KROWS, a->dtype, s), small());
+    return NB_TC_OR(a, tc_outer(p, j, a->dtype, s), small());
 }
 
 // The gradients' workspace: for each of the two factors asked for, the items' adapters and their partial products.
 struct Piece {
     int64_t table, part, end;
-    int items;
+    int rows, items;
 };
 Piece piece_of(const nb_lora_args* a, int cols, int64_t at) {
     Piece p;
-    p.items = item_count(a->T, a->requests, outer_rows(a, cols));
+    p.rows = outer_rows(a, cols);
+    p.items = item_count(a->T, a->requests, p.rows);
     p.table = at;
     p.part = at + ((int64_t)p.items * 4 + 255) / 256 * 256;
     p.end = p.part + ((int64_t)p.items * a->R * cols * 4 + 255) / 256 * 256;
@@ -868,45 +878,37 @@ int forward_t(const nb_lora_args* a, cudaStream_t s) {
 }
 template <typename T, int RM>
 int backward_t(const nb_lora_args* a, cudaStream_t s) {
-    LoraParams p = params_of(a);
-    LoraParams g = p;
+    LoraParams g = params_of(a);
     if (a->dx || a->ddown) {
         g.hi = plane(a->g, a, 0);
         g.lo = plane(a->g, a, 1);
         g.x = a->dy; g.stride_x = a->stride_dy; g.factor = a->up; g.K = a->N;
         if (int rc = NB_TC_OR(a, tc_shrink(g, true, a->dtype, s), (shrink<T, RM, true>(g, s)))) return rc;
     }
-    char* ws = static_cast<char*>(a->workspace);
-    int64_t used = 0;
-    Join<T> joins[2] = {};
-    int n = 0;
-    auto join_of = [&](LoraParams& q, int cols, void* grad) {
-        const Piece w = piece_of(a, cols, used);
-        used = w.end;
-        q.item_adapter = reinterpret_cast<int*>(ws + w.table);
-        q.part = reinterpret_cast<float*>(ws + w.part);
-        const long long size = (long long)a->R * cols;
-        joins[n++] = {q.part, q.item_adapter, static_cast<T*>(grad), size, w.items, ceil_div(size, 1024)};
-    };
-    p.chained = a->dx || a->ddown;
-    if (a->dup) {
-        p.x = a->dy; p.stride_x = a->stride_dy; p.K = a->N;
-        p.hi = plane(a->h, a, 0);
-        p.lo = plane(a->h, a, 1);
-        join_of(p, a->N, a->dup);
-        if (int rc = outer<T, RM, true>(a, p, s)) return rc;
-    }
-    g.K = a->K;
-    g.chained = true;
-    if (a->ddown) {
-        g.x = a->x; g.stride_x = a->stride_x;
-        join_of(g, a->K, a->ddown);
-        if (int rc = outer<T, RM, false>(a, g, s)) return rc;
-    }
-    if (n)
+    g.chained = a->dx || a->ddown;
+    if (a->dup || a->ddown) {
+        char* ws = static_cast<char*>(a->workspace);
+        int64_t used = 0;
+        OuterJobs j = {};
+        Join<T> joins[2] = {};
+        int n = 0;
+        auto job = [&](int i, const void* x, long long stride, int cols, void* planes, void* grad) {
+            const Piece w = piece_of(a, cols, used);
+            used = w.end;
+            float* part = reinterpret_cast<float*>(ws + w.part);
+            int* table = reinterpret_cast<int*>(ws + w.table);
+            j.job[i] = {x, plane(planes, a, 0), plane(planes, a, 1), part, table, stride, cols, w.rows, w.items};
+            const long long size = (long long)a->R * cols;
+            joins[n++] = {part, table, static_cast<T*>(grad), size, w.items, ceil_div(size, 1024)};
+        };
+        if (a->dup) job(0, a->dy, a->stride_dy, a->N, a->h, a->dup);
+        if (a->ddown) job(1, a->x, a->stride_x, a->K, a->g, a->ddown);
+        if (int rc = outer<T, RM>(a, g, j, s)) return rc;
         if (int rc = launch(lora_join_kernel<T>, dim3(joins[0].blocks + joins[1].blocks, a->A), 256, 0, 1, true, s, joins[0], joins[1])) return rc;
+        g.chained = true;
+    }
     if (a->dx) {
-        g.x = nullptr; g.out = a->dx; g.stride_out = a->K; g.factor = a->down;
+        g.x = nullptr; g.K = a->K; g.out = a->dx; g.stride_out = a->K; g.factor = a->down;
         return NB_TC_OR(a, tc_expand(g, true, a->dtype, s), (expand<T, RM, true>(g, s)));
     }
     return NB_OK;

@@ -7,18 +7,30 @@ namespace nb {
 namespace lora {
 
 struct LoraParams {
-    const void* x;        // shrink: (T, K) operand; expand: base (T, C) or null; outer: (T, K) operand
+    const void* x;        // shrink: (T, K) operand; expand: base (T, C) or null
     void* out;            // expand: (T, C)
     const void* factor;   // shrink: (A, R, K) or (A, K, R); expand: (A, C, R) or (A, R, C)
     void* hi; void* lo;   // (T, R) each
-    float* part;          // outer: (items, R, K) or (items, K, R)
-    int* item_adapter;    // outer: (items)
     const int* offsets; const int* adapters; const float* scale;
     long long stride_x, stride_out;
-    int T, K, R, A, requests;  // K: length of the contraction (shrink), columns (expand, outer)
-    int rows_per_item, cols_per_cta;
+    int T, K, R, A, requests;  // K: length of the contraction (shrink), columns (expand)
+    int rows_per_item, cols_per_cta;  // (shrink, expand)
     bool chained;         // launched behind a kernel of the same call
     int* status;          // device int32, set non-zero when a bounded wait expires; may be null
+};
+
+// The gradients of both factors are one launch: the first `groups` CTAs of a row of the grid are job 0's, U's, with partial
+// products (items, K, R); the others job 1's, D's, (items, R, K).
+struct OuterJob {
+    const void* x; const void* hi; const void* lo;  // (T, K) and (T, R) operands
+    float* part;
+    int* item_adapter;  // (items): -1 for an item without rows or adapter
+    long long stride_x;
+    int K, rows, items;  // columns (0: no such job), rows of an item
+};
+struct OuterJobs {
+    OuterJob job[2];
+    int groups;
 };
 
 struct Item {
@@ -26,10 +38,10 @@ struct Item {
 };
 __host__ __device__ inline int item_count(int T, int requests, int bm) { return (T + bm - 1) / bm + requests + 1; }
 
-// The `w`-th interval of the merged borders (tile borders before equal offsets).  All threads of the CTA call it.
+// The `w`-th interval of the merged borders (those of tiles of `bm` rows before equal offsets).  All threads of the CTA call it.
 template <int THREADS>
-__device__ __forceinline__ Item find_item(const LoraParams& p, int w) {
-    const int bm = p.rows_per_item, tiles = (p.T + bm - 1) / bm;
+__device__ __forceinline__ Item find_item(const LoraParams& p, int w, int bm) {
+    const int tiles = (p.T + bm - 1) / bm;
     auto offset = [&](int j) { return min(max(__ldg(p.offsets + j), 0), p.T); };
     int before = 0;  // offsets among the first w borders
     for (int j0 = 0; j0 <= p.requests; j0 += THREADS) {
@@ -107,7 +119,7 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 constexpr int kTcRows = 128, kTcCols = 256;  // rows of an item (shrink, expand), columns of a CTA (outer)
 int tc_shrink(LoraParams p, bool rcontig, int dtype, cudaStream_t s);
 int tc_expand(LoraParams p, bool ccontig, int dtype, cudaStream_t s);
-int tc_outer(const LoraParams& p, bool krows, int dtype, cudaStream_t s);
+int tc_outer(const LoraParams& p, OuterJobs j, int dtype, cudaStream_t s);
 
 }  // namespace lora
 }  // namespace nb

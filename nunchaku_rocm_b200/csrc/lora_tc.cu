@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
         tmem_alloc(smem_u32(tmem_at), S::COLS);
         tmem_relinquish();
     }
-    const Item it = find_item<S::THREADS>(p, blockIdx.x);
+    const Item it = find_item<S::THREADS>(p, blockIdx.x, p.rows_per_item);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
                                                               const __grid_constant__ CUtensorMap tm_out, const LoraParams p) {
     using S = ExpandTc<RP>;
     extern __shared__ unsigned char raw[];
-    const Item it = find_item<S::THREADS>(p, blockIdx.y);
+    const Item it = find_item<S::THREADS>(p, blockIdx.y, p.rows_per_item);
     if (it.rows == 0) return;
     const int col0 = blockIdx.x * p.cols_per_cta, col1 = min(col0 + p.cols_per_cta, p.K);
     const T* in = static_cast<const T*>(p.x);
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------------------------- outer
-// part[item][r, k] (or [k, r] with KROWS) = sum over the item's rows of (hi + lo)[t, r] X[t, k], 256 columns of X per CTA
+// part[item][r, k] (job 1; [k, r] for job 0) = sum over the item's rows of (hi + lo)[t, r] X[t, k], 256 columns of X per CTA
 // (two accumulators of 128: hi and lo come from the L2 cache once for both, 16 KB beside 32 KB of X at rank 64; with 128
 // columns the cache delivered as much of them as HBM of X).  Both operands run along the rows (MN-major), so they are used
 // as they lie.
@@ -427,10 +427,16 @@ struct OuterTc {
     static constexpr int ACC = RP < 32 ? 32 : RP, COLS = 2 * ACC;  // tensor-memory columns: read 32 at a time
     static constexpr int THREADS = 192;
 };
-template <typename T, int RP, bool KROWS>
-__global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_hi,
-                                                             const __grid_constant__ CUtensorMap tm_lo, const LoraParams p) {
+struct OuterMaps {
+    CUtensorMap x[2], hi[2], lo[2];  // of the two jobs
+};
+template <typename T, int RP>
+__global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constant__ OuterMaps maps, const LoraParams p,
+                                                            const __grid_constant__ OuterJobs jobs) {
     using S = OuterTc<RP>;
+    const bool krows = (int)blockIdx.x < jobs.groups;
+    const int which = krows ? 0 : 1, K = jobs.job[which].K;
+    const CUtensorMap &tm_x = maps.x[which], &tm_hi = maps.hi[which], &tm_lo = maps.lo[which];
     extern __shared__ unsigned char raw[];
     chain_next();
     uint8_t* smem = align1k(raw);
@@ -460,20 +466,20 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         tmem_relinquish();
     }
     // last items first: their rows are the ones that the kernel before this one read last and left in the L2 cache
-    const int w = gridDim.y - 1 - blockIdx.y;
-    const Item it = find_item<S::THREADS>(p, w);
+    const int w = jobs.job[which].items - 1 - (int)blockIdx.y;
+    const Item it = find_item<S::THREADS>(p, w, jobs.job[which].rows);
     chain_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.item_adapter[w] = it.rows ? it.adapter : -1;
+    if (blockIdx.x == (krows ? 0 : jobs.groups) && threadIdx.x == 0 && w >= 0) jobs.job[which].item_adapter[w] = it.rows ? it.adapter : -1;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
-    if (it.rows == 0 || it.adapter < 0) {
+    if (w < 0 || it.rows == 0 || it.adapter < 0) {  // (w: the other job has more items)
         if (warp == 1) tmem_dealloc(tmem, S::COLS);
         return;
     }
-    const int c0 = blockIdx.x * kTcCols, n = (it.rows + KB - 1) / KB;
-    const int quarters = min(4, (p.K - c0 + 63) / 64);  // tiles of 64 columns that exist
+    const int c0 = (blockIdx.x - (krows ? 0 : jobs.groups)) * kTcCols, n = (it.rows + KB - 1) / KB;
+    const int quarters = min(4, (K - c0 + 63) / 64);  // tiles of 64 columns that exist
 
     if (warp == 0) {
         if (lane == 0) {
@@ -523,7 +529,7 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         }
     } else {
         const int q = warp & 3;
-        float* part = p.part + (long long)w * p.R * p.K;
+        float* part = jobs.job[which].part + (long long)w * p.R * K;
         if (mbar_wait_warp(done, 0, abort_s, E_OUTER | 3)) {
             tc_fence_after();
             for (int h = 0; 2 * h < quarters; ++h) {
@@ -532,9 +538,9 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                     float v[32];
                     tmem_ld32(tmem + (q * 32 << 16) + h * S::ACC + c, v);
                     tmem_wait_ld();
-                    if (k < p.K) {
+                    if (k < K) {
                         const int left = p.R - c;  // 16 or more
-                        if constexpr (KROWS) {
+                        if (krows) {
                             float* to = part + (long long)k * p.R + c;
 #pragma unroll
                             for (int i = 0; i < 32; i += 8)
@@ -544,7 +550,7 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                         } else {
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (i < left) part[(long long)(c + i) * p.K + k] = v[i];
+                                if (i < left) part[(long long)(c + i) * K + k] = v[i];
                         }
                     }
                 }
@@ -636,15 +642,23 @@ int expand(LoraParams p, cudaStream_t s) {
     p.cols_per_cta = per * 64;
     return launch(kernel, dim3(ceil_div(tiles, per), items), S::THREADS, S::BYTES, 1, p.chained, s, hi, lo, g, base, out, p);
 }
-template <typename T, int RP, bool KROWS>
-int outer(const LoraParams& p, cudaStream_t s) {
+template <typename T, int RP>
+int outer(const LoraParams& p, OuterJobs j, cudaStream_t s) {
     using S = OuterTc<RP>;
-    auto* kernel = lora_outer_tc_kernel<T, RP, KROWS>;
+    auto* kernel = lora_outer_tc_kernel<T, RP>;
     NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
-    CUtensorMap x, hi, lo;
-    if (!(make_map<T>(&x, p.x, p.T, p.K, p.stride_x, KB) && make_map<T>(&hi, p.hi, p.T, p.R, p.R, KB) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, KB)))
-        return NB_ERR_UNSUPPORTED;
-    return launch(kernel, dim3(ceil_div(p.K, kTcCols), item_count(p.T, p.requests, p.rows_per_item)), S::THREADS, S::BYTES, 1, p.chained, s, x, hi, lo, p);
+    OuterMaps m;
+    int groups = 0;
+    for (int i = 0; i < 2; ++i) {
+        const OuterJob& o = j.job[j.job[i].K ? i : 1 - i];  // (a job that is not there has no CTAs; its maps are the other's)
+        if (!(make_map<T>(&m.x[i], o.x, p.T, o.K, o.stride_x, KB) && make_map<T>(&m.hi[i], o.hi, p.T, p.R, p.R, KB) &&
+              make_map<T>(&m.lo[i], o.lo, p.T, p.R, p.R, KB)))
+            return NB_ERR_UNSUPPORTED;
+        groups += ceil_div(j.job[i].K, kTcCols);
+    }
+    j.groups = ceil_div(j.job[0].K, kTcCols);
+    const int items = j.job[0].items > j.job[1].items ? j.job[0].items : j.job[1].items;
+    return launch(kernel, dim3(groups, items), S::THREADS, S::BYTES, 1, p.chained, s, m, p, j);
 }
 
 #define NB_LORA_RP(CALL)                         \
@@ -666,8 +680,8 @@ int expand_t(const LoraParams& p, bool ccontig, cudaStream_t s) {
 #undef NB_CALL
 }
 template <typename T>
-int outer_t(const LoraParams& p, bool krows, cudaStream_t s) {
-#define NB_CALL(RP) (krows ? outer<T, RP, true>(p, s) : outer<T, RP, false>(p, s))
+int outer_t(const LoraParams& p, const OuterJobs& j, cudaStream_t s) {
+#define NB_CALL(RP) (outer<T, RP>(p, j, s))
     NB_LORA_RP(NB_CALL);
 #undef NB_CALL
 }
@@ -680,8 +694,8 @@ int tc_shrink(LoraParams p, bool rcontig, int dtype, cudaStream_t s) {
 int tc_expand(LoraParams p, bool ccontig, int dtype, cudaStream_t s) {
     return dtype == NB_DTYPE_BF16 ? expand_t<__nv_bfloat16>(p, ccontig, s) : expand_t<__half>(p, ccontig, s);
 }
-int tc_outer(const LoraParams& p, bool krows, int dtype, cudaStream_t s) {
-    return dtype == NB_DTYPE_BF16 ? outer_t<__nv_bfloat16>(p, krows, s) : outer_t<__half>(p, krows, s);
+int tc_outer(const LoraParams& p, OuterJobs j, int dtype, cudaStream_t s) {
+    return dtype == NB_DTYPE_BF16 ? outer_t<__nv_bfloat16>(p, j, s) : outer_t<__half>(p, j, s);
 }
 
 }  // namespace lora
