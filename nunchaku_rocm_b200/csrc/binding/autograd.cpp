@@ -3,7 +3,7 @@
 // These operators run inside training steps, where a Python autograd function costs more than the kernels of a small call:
 // the engine's worker thread has to take the interpreter lock and interpret the backward pass on another core.  Measured on
 // a B200's host for a layer norm of 154 x 1152, forward and backward: 120 us a step with Python functions (23 forward, about
-// 45 the engine itself), 82 with these (torch's own layer norm: 72).  The arguments' checks are here for the same reason:
+// 45 the engine itself), 74 with these (torch's own layer norm: 76).  The arguments' checks are here for the same reason:
 // they took a third of a small call in Python.
 //
 // The library's functions are bound by address, so that this module calls the very library that ctypes loaded.

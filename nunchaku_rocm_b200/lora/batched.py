@@ -24,6 +24,7 @@ import threading
 import torch
 from torch import nn
 
+from .. import _lib as L
 from ..ops.lora import lora_batched
 from .runtime import RANK_GRANULARITY, _is_svdq
 
@@ -156,8 +157,8 @@ def attach_lora_batch(module: nn.Module, adapters, scale=None) -> None:
         down, up = stack_loras(adapters, ref.device, ref.dtype)
     if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2] or down.shape[1] % RANK_GRANULARITY:
         raise ValueError(f"stacked factors must be (A, R, in) and (A, out, R), R a multiple of {RANK_GRANULARITY}; got {tuple(down.shape)} and {tuple(up.shape)}")
-    if down.shape[1] > 128:
-        raise NotImplementedError(f"rank {down.shape[1]}: stacks take ranks up to 128")
+    if down.shape[1] > L.LORA_MAX_RANK:
+        raise NotImplementedError(f"rank {down.shape[1]}: stacks take ranks up to {L.LORA_MAX_RANK}")
     n_in, n_out = getattr(module, "in_features", None), getattr(module, "out_features", None)
     if (n_in, n_out) != (down.shape[2], up.shape[1]):
         raise ValueError(f"LoRA factors {tuple(down.shape)}, {tuple(up.shape)} do not fit a {n_in} -> {n_out} layer")
