@@ -255,7 +255,7 @@ typedef struct nb_lora_args {
     void* workspace; int64_t workspace_bytes;
     int64_t stride_x, stride_base, stride_out, stride_dy;
     int32_t T, K, N, R, A, requests, dtype;
-    int32_t impl;          /* NB_IMPL_AUTO: the tcgen05 kernels where the requests are long, else the mma.sync ones (NB_IMPL_GENERIC) */
+    int32_t impl;          /* NB_IMPL_AUTO: tcgen05 kernels where the requests are long, else the mma.sync ones (NB_IMPL_GENERIC) */
     void* status;          /* device int32 a kernel sets non-zero if a bounded wait expires; may be null */
 } nb_lora_args;
 int nb_lora_forward(const nb_lora_args* args, void* stream);
