@@ -4,7 +4,8 @@
 // base, out or dy), so what the tensor cores give here is not arithmetic but the absence of it elsewhere: no operand passes
 // through registers, and the bytes in flight are the size of the shared-memory ring.  Measured on a B200 (bf16, 9216 rows,
 // rank 64): shrink 3072 -> 64 17.5 us and 9216 -> 64 35 us (3.2 and 4.9 TB/s), expand 64 -> 9216 60 us (5.6 TB/s), outer 49
-// us for both factors (4.6 TB/s): about 8 us of each are its start and its end, the rest its bytes.
+// us for both factors (4.6 TB/s): about 8 us of each are its start and its end, the rest its bytes (outer's CTAs are of two
+// lengths, and end at different times).
 //
 // A tile is loaded whole even where its item has fewer rows: the rows behind belong to other requests (or are filled with
 // zeros behind the last row).  They are multiplied along and not stored; where rows are summed (outer) they are set to zero
