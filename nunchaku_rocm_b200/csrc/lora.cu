@@ -359,11 +359,14 @@ struct FewParams {
     int N, cols;  // columns of a CTA, a multiple of 32
 };
 constexpr int kFewRows = 16, kFewWarps = 8, kFewCluster = 8;
+// CTAs per SM that the registers leave room for
+constexpr int few_per_sm(int R) { return R <= 64 ? 2 : 1; }
 template <int R>
 struct FewTile {
     static constexpr int LDH = R + 8;
-    // ranks of a warp in the first product (its sums and its steps of D in registers, two CTAs per SM), warps along k
-    static constexpr int RW = R <= 32 ? R : R / 2, KW = kFewWarps * RW / R;
+    // groups of warps that share the ranks in the first product (a warp has its sums and its steps of D in registers), tiles of
+    // eight ranks of a group, groups along k
+    static constexpr int GROUPS = R <= 32 ? 1 : R <= 64 ? 2 : 4, NT = (R / 8 + GROUPS - 1) / GROUPS, KW = kFewWarps / GROUPS;
     static constexpr int RED = KW * 16 * R * 4, PART = 16 * R * 4, H = 2 * 16 * LDH * 2;
     static int bytes(int cols) { return cols * R * 2 + RED + PART + H; }
     // 16-byte piece of U's row: pieces that half a warp reads together are on different banks
@@ -376,7 +379,7 @@ struct FewTile {
     }
 };
 template <typename T, int R>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) lora_few_kernel(const FewParams f) {
+__global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel(const FewParams f) {
     using S = FewTile<R>;
     extern __shared__ __align__(16) unsigned char few_smem[];
     const LoraParams& p = f.l;
@@ -406,9 +409,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) lora_few_kernel(const FewPa
     const int slice = (p.K + 32 * kFewCluster - 1) / (32 * kFewCluster) * 32, k1 = min((rank + 1) * slice, p.K);
     const T* x0 = static_cast<const T*>(p.x) + (it.first + g) * p.stride_x;
     const T* x1 = x0 + 8 * p.stride_x;
-    const int kw = warp % S::KW, r0 = warp / S::KW * S::RW;
+    const int kw = warp % S::KW, r0 = warp / S::KW * (S::NT * 8);
     const T* d0 = static_cast<const T*>(p.factor) + ((long long)it.adapter * R + r0 + g) * p.K;
-    constexpr int DEPTH = R == 16 ? 3 : 2, STEP = S::KW * 32, NT = S::RW / 8;  // steps on their way; tiles of r
+    constexpr int DEPTH = R == 16 ? 3 : 2, STEP = S::KW * 32, NT = S::NT;  // steps on their way
     uint4 xa[DEPTH], xb[DEPTH], d[DEPTH][NT];
     auto load = [&](int i, int k0) {
         const int k = k0 + t * 8;
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) lora_few_kernel(const FewPa
         xa[i] = in && on0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
         xb[i] = in && on1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) d[i][n] = in ? __ldg(reinterpret_cast<const uint4*>(d0 + (long long)n * 8 * p.K + k)) : zero;
+        for (int n = 0; n < NT; ++n) d[i][n] = in && r0 + n * 8 < R ? __ldg(reinterpret_cast<const uint4*>(d0 + (long long)n * 8 * p.K + k)) : zero;
     };
     const int first = rank * slice + kw * 32;
 #pragma unroll
@@ -461,6 +464,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) lora_few_kernel(const FewPa
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+        if (r0 + n * 8 >= R) break;  // (the last group may have fewer)
         float* at = red + (kw * 16 + g) * R + r0 + n * 8 + t * 2;
         *reinterpret_cast<float2*>(at) = make_float2(acc[n][0], acc[n][1]);
         *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[n][2], acc[n][3]);
@@ -744,11 +748,15 @@ bool use_tc(const nb_lora_args* a) {
 int few_need(const nb_lora_args* a) {  // clusters of an item that keep a CTA's part of U within 80 KB
     return ceil_div((long long)a->N * a->R * 2, kFewCluster * 80 * 1024);
 }
+// CTAs that are resident together.  With one CTA per SM (above rank 64), clusters of eight do not fill the SMs: 16 clusters of
+// rank 128 took two turns (8 rows of 8 requests, 12288 -> 3072: 25.9 us for 24.4 with two kernels), 8 one (128 rows at rank 80:
+// 13.2 for 15.9).
+int few_slots(int R) { return R <= 64 ? 2 * sms() : 3 * sms() / 4; }
 bool use_few(const nb_lora_args* a) {
-    if (a->impl == NB_IMPL_TCGEN05 || a->R > 64) return false;
+    if (a->impl == NB_IMPL_TCGEN05) return false;
     const long long tiles = ceil_div(a->T, kFewRows), requests = a->requests < a->T ? a->requests : a->T;
     const int need = few_need(a);
-    return (tiles > requests ? tiles : requests) * need * kFewCluster <= 2ll * sms() * (need == 1 ? 2 : 1);
+    return (tiles > requests ? tiles : requests) * need * kFewCluster <= (long long)few_slots(a->R) * (need == 1 && a->R <= 64 ? 2 : 1);
 }
 // A tcgen05 launch, or the mma.sync one where there is no tensor map for the operands (rows a stride of zero apart) and the
 // caller did not insist.
@@ -811,7 +819,7 @@ int few(const nb_lora_args* a, const LoraParams& p, cudaStream_t s) {
     // clusters of an item: more than it needs where few items leave SMs idle, each of which computes h anew, as long as that
     // reads less than its columns
     const int live = live_items(f.l, kFewRows), need = few_need(a);
-    int splits = 2 * sms() / (kFewCluster * live);
+    int splits = few_slots(R) / (kFewCluster * live);
     if (splits > ceil_div(a->N, a->K)) splits = ceil_div(a->N, a->K);
     if (splits < need) splits = need;
     f.cols = ceil_div(ceil_div(a->N, kFewCluster * splits), 32) * 32;
@@ -868,7 +876,11 @@ int forward_t(const nb_lora_args* a, cudaStream_t s) {
             case 16: return few<T, 16>(a, p, s);
             case 32: return few<T, 32>(a, p, s);
             case 48: return few<T, 48>(a, p, s);
-            default: return few<T, 64>(a, p, s);
+            case 64: return few<T, 64>(a, p, s);
+            case 80: return few<T, 80>(a, p, s);
+            case 96: return few<T, 96>(a, p, s);
+            case 112: return few<T, 112>(a, p, s);
+            default: return few<T, 128>(a, p, s);
         }
     p.x = a->x; p.stride_x = a->stride_x; p.factor = a->down; p.K = a->K;
     if (int rc = NB_TC_OR(a, tc_shrink(p, false, a->dtype, s), (shrink<T, RM, false>(p, s)))) return rc;

@@ -365,7 +365,7 @@ def test_more_than_2_31_elements(cuda_dev, impl):
 
 
 @gpu
-@pytest.mark.parametrize("R", [16, 32, 48, 64])
+@pytest.mark.parametrize("R", [16, 32, 48, 64, 80, 96, 112, 128])
 @pytest.mark.parametrize("K,N", [(8, 8), (40, 264), (2048, 18432), (12288, 72)])
 @pytest.mark.parametrize("T,offsets,adapters", [
     (1, [0, 1], [0]),
