@@ -380,3 +380,12 @@ def test_few_rows(cuda_dev, R, K, N, T, offsets, adapters):
     out = p["base"].clone()
     lora_batched(p["x"], p["down"], p["up"], *index(cuda_dev, offsets, adapters), base=out, scale=p["scale"], out=out)
     assert torch.equal(out, lora_batched(p["x"], p["down"], p["up"], *index(cuda_dev, offsets, adapters), base=p["base"], scale=p["scale"]))
+
+
+@gpu
+@pytest.mark.parametrize("K,N", [(520, 328), (72, 136), (40, 1032)])
+@pytest.mark.parametrize("R", [16, 32, 48, 64, 96, 128])
+def test_more_than_a_few_rows(cuda_dev, R, K, N):
+    # too many for the one kernel: the shrink and the expand of their own, with odd sizes and short items among long ones
+    p = make(cuda_dev, 1301, K, N, R, 3, BF16 if R % 32 else FP16, seed=R + N)
+    check(cuda_dev, p, [3, 3, 20, 21, 149, 640, 640, 1290], [1, 0, 2, -1, 1, 5, 2])
