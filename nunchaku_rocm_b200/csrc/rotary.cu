@@ -148,20 +148,39 @@ __device__ __forceinline__ Item locate(const RotParams& p, uint32_t row0, uint32
     return it;
 }
 
-// VEC: an item is 16 bytes of a head (interleaved), two 16-byte pieces R/2 apart (HALF), or 16 bytes that pass through.
-// Otherwise an item is one channel pair or one channel that passes through: every size and alignment.
-template <typename T, bool HALF, bool VEC>
+// W neighbouring channels (4 or 8 bytes) in one access
+template <typename T, int W>
+struct alignas(sizeof(T) * W) Pack {
+    T v[W];
+};
+template <typename T, int W>
+__device__ __forceinline__ Pack<T, W> load_pack(const T* at) {
+    static_assert(sizeof(T) * W == 4 || sizeof(T) * W == 8, "others go by 16 bytes or one by one");
+    Pack<T, W> p;
+    if constexpr (sizeof(T) * W == 8) *reinterpret_cast<uint2*>(&p) = __ldg(reinterpret_cast<const uint2*>(at));
+    else *reinterpret_cast<uint32_t*>(&p) = __ldg(reinterpret_cast<const uint32_t*>(at));
+    return p;
+}
+
+// W channels per access.  16 bytes (VEC): an item is 16 bytes of a head (interleaved), two 16-byte pieces R/2 apart (HALF), or
+// 16 bytes that pass through; with SHARED, the last rotated pairs and the first channels that pass through are in one piece.
+// HALF with fewer: two pieces of W channels, or W that pass through.  One: a channel pair, or one channel that passes through,
+// for every size and alignment.  Measured, 9000 tokens of 24 + 24 heads, bf16: halves of 36 of 72 channels 67 us with single
+// channels, 36 with four; 63 interleaved pairs of 128 channels 116 us pair by pair, 51 with a shared piece (64 pairs, without the
+// tests that a shared piece needs: 43).
+template <typename T, bool HALF, int W, bool SHARED>
 __global__ void __launch_bounds__(kThreads, HALF ? 4 : 5) rotary_kernel(const __grid_constant__ RotParams p) {
-    extern __shared__ float2 cs[];  // [tok][pairs]
+    extern __shared__ float2 cs[];  // [tok][cols]
+    constexpr bool VEC = W * sizeof(T) == 16;
     const uint32_t row0 = blockIdx.x * (uint32_t)p.tok;
     const int ntok = (int)min((uint32_t)p.tok, p.rows - row0);
     const uint32_t items = (uint32_t)ntok * (p.H + p.Hk) * p.units;
 
     // The first items' loads are issued before the angles are computed, so that they travel meanwhile.
     constexpr int N = Vec<T>::N;
-    constexpr int PER = HALF ? N : N / 2;  // pairs of an item
+    constexpr int PER = HALF ? W : VEC ? N / 2 : 1;  // pairs of an item
     constexpr int AHEAD = HALF ? 4 : 3;
-    const int steps = p.pairs / PER;
+    const int steps = (p.pairs + PER - 1) / PER, cols = steps * PER;  // (a shared piece's places behind the last pair are not read)
     Item it[AHEAD];
     uint4 r0[AHEAD], r1[AHEAD];
     auto fetch = [&](uint32_t first) {
@@ -189,13 +208,13 @@ __global__ void __launch_bounds__(kThreads, HALF ? 4 : 5) rotary_kernel(const __
     if (threadIdx.x < per * p.pairs) {
         const double rate = p.ladder.turns[pair];
         const long long axis = axis_of(p.ladder, pair) * p.si_a;
-        // VEC: the PER pairs of an item lie pairs / PER apart, so that the lanes of a warp read neighbouring words
-        const int at = VEC ? (pair % PER) * steps + pair / PER : pair;
+        // the PER pairs of an item lie `steps` apart, so that the lanes of a warp read neighbouring words
+        const int at = (pair % PER) * steps + pair / PER;
         for (int tok = threadIdx.x / p.pairs; tok < ntok; tok += per) {
             const uint32_t row = row0 + tok, b = fastdiv(row, p.div_s), s = row - b * p.div_s.d;
             float2 v = cos_sin_turns(load_id(p.ids, p.ids_type, b * p.si_b + s * p.si_s + axis) * rate);
             v.y *= p.sign;
-            cs[tok * p.pairs + at] = v;
+            cs[tok * cols + at] = v;
         }
     }
     __syncthreads();
@@ -207,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, HALF ? 4 : 5) rotary_kernel(const __
             for (int a = 0; a < AHEAD; ++a) {
                 if (first + a * kThreads >= items) continue;
                 T* dst = static_cast<T*>(it[a].dst);
-                const float2* w = cs + it[a].tok * p.pairs;
+                const float2* w = cs + it[a].tok * cols;
                 if (it[a].unit >= p.rot_units) {
                     const int at = HALF ? 2 * p.pairs + (it[a].unit - p.rot_units) * N : it[a].unit * N;
                     *reinterpret_cast<uint4*>(dst + at) = r0[a];
@@ -226,8 +245,14 @@ __global__ void __launch_bounds__(kThreads, HALF ? 4 : 5) rotary_kernel(const __
                 } else {
                     float u[N], x[N];
                     Vec<T>::widen(r0[a], u);
+                    const int left = p.pairs - it[a].unit * PER;  // pairs of this piece that turn
 #pragma unroll
                     for (int j = 0; j < N / 2; ++j) {
+                        if (SHARED && j >= left) {
+                            x[2 * j] = u[2 * j];
+                            x[2 * j + 1] = u[2 * j + 1];
+                            continue;
+                        }
                         const float2 c = w[j * steps + it[a].unit];
                         x[2 * j] = u[2 * j] * c.x - u[2 * j + 1] * c.y;
                         x[2 * j + 1] = u[2 * j] * c.y + u[2 * j + 1] * c.x;
@@ -235,6 +260,32 @@ __global__ void __launch_bounds__(kThreads, HALF ? 4 : 5) rotary_kernel(const __
                     *reinterpret_cast<uint4*>(dst + it[a].unit * N) = Vec<T>::narrow(x);
                 }
             }
+        }
+    } else if constexpr (W > 1) {
+        static_assert(HALF, "interleaved pairs go by 16 bytes or one by one");
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
+            const Item m = locate<T>(p, row0, i);
+            const T* src = static_cast<const T*>(m.src);
+            T* dst = static_cast<T*>(m.dst);
+            if (m.unit >= p.rot_units) {
+                const int at = 2 * p.pairs + (m.unit - p.rot_units) * W;
+                *reinterpret_cast<Pack<T, W>*>(dst + at) = load_pack<T, W>(src + at);
+                continue;
+            }
+            const int at = m.unit * W;
+            const float2* w = cs + m.tok * cols + m.unit;
+            const Pack<T, W> u = load_pack<T, W>(src + at), v = load_pack<T, W>(src + p.pairs + at);
+            Pack<T, W> x, y;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float2 c = w[j * steps];
+                const float a = load1<T>(u.v + j), b = load1<T>(v.v + j);
+                store1<T>(x.v + j, a * c.x - b * c.y);
+                store1<T>(y.v + j, a * c.y + b * c.x);
+            }
+            *reinterpret_cast<Pack<T, W>*>(dst + at) = x;
+            *reinterpret_cast<Pack<T, W>*>(dst + p.pairs + at) = y;
         }
     } else {
         for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
@@ -246,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, HALF ? 4 : 5) rotary_kernel(const __
                 dst[at] = src[at];
             } else {
                 const int at = HALF ? m.unit : 2 * m.unit, to = HALF ? m.unit + p.pairs : at + 1;
-                const float2 c = cs[m.tok * p.pairs + m.unit];
+                const float2 c = cs[m.tok * cols + m.unit];
                 const float u = load1<T>(src + at), v = load1<T>(src + to);
                 store1<T>(dst + at, u * c.x - v * c.y);
                 store1<T>(dst + to, u * c.y + v * c.x);
@@ -269,18 +320,25 @@ __global__ void __launch_bounds__(kThreads) rotary_table_kernel(const __grid_con
     }
 }
 
-template <typename T, bool HALF>
-int launch_rot(const RotParams& p, bool vec, cudaStream_t s) {
+template <typename T, bool HALF, int W, bool SHARED = false>
+int launch_w(const RotParams& p, cudaStream_t s) {
     const uint32_t blocks = (p.rows + p.tok - 1) / p.tok;
-    const size_t smem = sizeof(float2) * (size_t)p.tok * p.pairs;  // at most 16 tokens x 128 pairs x 8 bytes = 16 KB
-    if (vec) rotary_kernel<T, HALF, true><<<blocks, kThreads, smem, s>>>(p);
-    else rotary_kernel<T, HALF, false><<<blocks, kThreads, smem, s>>>(p);
+    const size_t smem = sizeof(float2) * (size_t)p.tok * ((p.pairs + 7) / 8 * 8);  // at most 16 tokens x 128 pairs x 8 bytes = 16 KB
+    rotary_kernel<T, HALF, W, SHARED><<<blocks, kThreads, smem, s>>>(p);
     NB_CUDA_CHECK(cudaGetLastError());
     return NB_OK;
 }
 template <typename T>
-int launch_rot(const RotParams& p, bool half, bool vec, cudaStream_t s) {
-    return half ? launch_rot<T, true>(p, vec, s) : launch_rot<T, false>(p, vec, s);
+int launch_rot(const RotParams& p, bool half, int w, cudaStream_t s) {
+    constexpr int N = 16 / sizeof(T);
+    if (half) {
+        if (w == N) return launch_w<T, true, N>(p, s);
+        if (w == N / 2) return launch_w<T, true, N / 2>(p, s);
+        if constexpr (N > 4) if (w == 2) return launch_w<T, true, 2>(p, s);
+        return launch_w<T, true, 1>(p, s);
+    }
+    if (w < N) return launch_w<T, false, 1>(p, s);
+    return 2 * p.pairs % N ? launch_w<T, false, N, true>(p, s) : launch_w<T, false, N>(p, s);
 }
 
 bool good_ladder(const nb_rotary_ladder* l) {
@@ -333,17 +391,24 @@ extern "C" int nb_rotary_axes(const nb_rotary_args* a, const nb_rotary_ladder* l
     p.rows = (uint32_t)rows;
     p.sign = a->inverse ? -1.f : 1.f;
     p.ladder = *l;
-    // 16-byte items: whole pieces of both the rotary and the remaining channels (of each half when the pairs are split),
-    // every row of every tensor on a 16-byte boundary
-    bool vec = a->D % n == 0 && (a->half ? pairs : 2 * pairs) % n == 0 && aligned16(a->q) && aligned16(a->q_out) && a->stride_qb % n == 0 &&
-               a->stride_qs % n == 0 && a->stride_qh % n == 0;
-    if (a->Hk) vec = vec && aligned16(a->k) && aligned16(a->k_out) && a->stride_kb % n == 0 && a->stride_ks % n == 0 && a->stride_kh % n == 0;
-    if (vec) {
-        p.rot_units = a->half ? pairs / n : 2 * pairs / n;
-        p.units = p.rot_units + (a->D - 2 * pairs) / n;
+    // channels per access: the rows of all tensors start on its multiples, and it divides a head and, where the pairs are split,
+    // each half
+    const auto fits = [&](int w) {
+        const auto on = [&](const void* at, int64_t b, int64_t s, int64_t h) {
+            return reinterpret_cast<uintptr_t>(at) % (w * size) == 0 && b % w == 0 && s % w == 0 && h % w == 0;
+        };
+        return a->D % w == 0 && (!a->half || pairs % w == 0) && on(a->q, a->stride_qb, a->stride_qs, a->stride_qh) && on(a->q_out, 0, 0, 0) &&
+               (a->Hk == 0 || (on(a->k, a->stride_kb, a->stride_ks, a->stride_kh) && on(a->k_out, 0, 0, 0)));
+    };
+    int w = n;
+    while (w > 1 && !fits(w)) w /= 2;
+    if (!a->half && w < n) w = 1;
+    if (a->half || w < n) {
+        p.rot_units = a->half ? pairs / w : pairs;
+        p.units = p.rot_units + (a->D - 2 * pairs) / w;
     } else {
-        p.rot_units = pairs;
-        p.units = pairs + (a->D - 2 * pairs);
+        p.rot_units = (2 * pairs + n - 1) / n;
+        p.units = a->D / n;
     }
     // Tokens per CTA: about four items per thread, but never so many that the CTAs do not cover the SMs.
     int sms = nb_num_sms();
@@ -356,9 +421,9 @@ extern "C" int nb_rotary_axes(const nb_rotary_args* a, const nb_rotary_ladder* l
     p.div_heads = make_fastdiv((uint32_t)heads);
     p.div_s = make_fastdiv(a->S);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->dtype == NB_DTYPE_BF16) return launch_rot<__nv_bfloat16>(p, a->half, vec, s);
-    if (a->dtype == NB_DTYPE_FP16) return launch_rot<__half>(p, a->half, vec, s);
-    return launch_rot<float>(p, a->half, vec, s);
+    if (a->dtype == NB_DTYPE_BF16) return launch_rot<__nv_bfloat16>(p, a->half, w, s);
+    if (a->dtype == NB_DTYPE_FP16) return launch_rot<__half>(p, a->half, w, s);
+    return launch_rot<float>(p, a->half, w, s);
 }
 
 extern "C" int nb_rotary_table(const void* ids, int32_t ids_type, int32_t B, int32_t S, int64_t stride_ib, int64_t stride_is,

@@ -444,3 +444,30 @@ def test_more_than_2_31_elements(cuda_dev):
     ids = torch.randint(0, 500, (T, 1, 2), device=cuda_dev)
     got = rotary_axes(q, None, ids, (4, 4))
     assert torch.equal(got[-tail:], rotary_axes(q[-tail:], None, ids[-tail:], (4, 4)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("D,axes", [(128, (42, 42, 42)), (72, (24, 24, 24)), (72, (20, 24, 22)), (64, (2,)), (66, (22, 22, 22)), (68, (8, 26))])
+def test_rotary_splits_inside_a_piece(cuda_dev, dtype, interleaved, D, axes):
+    # channel counts that no 16-byte piece divides; what is behind the axes passes through, whatever it holds
+    q, k = torch.randn(2, 37, 3, D, device=cuda_dev).to(dtype), torch.randn(2, 37, 1, D, device=cuda_dev).to(dtype)
+    if sum(axes) < D:
+        q[0, 3, 1, sum(axes):] = float("inf")
+    ids = torch.randint(-50, 50, (37, len(axes)), device=cuda_dev)
+    got = rotary_axes(q, k, ids, axes, interleaved=interleaved)
+    for t, out in zip((q, k), got):
+        R = sum(axes)
+        rates = torch.cat([10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64, device=cuda_dev) / d) for d in axes])
+        angle = torch.cat([ids[:, i : i + 1].double().expand(-1, d // 2) for i, d in enumerate(axes)], 1) * rates
+        c, s = angle.cos()[None, :, None], angle.sin()[None, :, None]
+        x = t[..., :R].double()
+        u, v = (x[..., 0::2], x[..., 1::2]) if interleaved else (x[..., : R // 2], x[..., R // 2 :])
+        a, b = u * c - v * s, u * s + v * c
+        ref = torch.stack([a, b], -1).flatten(-2) if interleaved else torch.cat([a, b], -1)
+        # one rounding; cos and sin off by 2^-24 of a turn's part (4 of fp32's half steps), the rotation's own two roundings
+        big = torch.stack([u.abs() + v.abs()] * 2, -1).flatten(-2) if interleaved else torch.cat([u.abs() + v.abs()] * 2, -1)
+        tol = torch.finfo(dtype).eps / 2 * ref.abs() + 8 * 2.0**-24 * big + torch.finfo(dtype).smallest_normal
+        assert ((out[..., :R].double() - ref).abs() <= tol * (1 + 2.0**-10)).all()
+        assert torch.equal(out[..., R:], t[..., R:])
