@@ -727,9 +727,8 @@ int ctas_per_group(int resident, int groups) {
     const int sms = nb_num_sms(), per = resident * (sms > 0 ? sms : 148) / groups;
     return per < 1 ? 1 : per;
 }
-// `ring`: the rows are whole 16-byte pieces.  The ring has 8 slots while two CTAs of it (three in the
-// backward pass) fit an SM, else 4; rows too long for
-// that (over 27 KB a slot: 13 K channels of 16 bits in the backward pass) go to the kernel without one.
+// `ring`: the rows are whole 16-byte pieces.  The ring has 8 slots while two CTAs of it (three in the backward pass) fit an
+// SM, else 4; rows too long for that (over 27 KB a slot: 13 K channels of 16 bits in the backward pass) go to the kernel without one.
 Shape shape_of(int groups, int rows, int dim, int size, bool backward, bool ring) {
     Shape s;
     const int eights = (dim + 7) / 8;
