@@ -239,9 +239,10 @@ int nb_gated_residual(const void* x, const void* gate, const void* y, const void
  * none: out is base there (zero when base is null).  `offsets` (requests + 1) and `adapters` (requests) are DEVICE arrays,
  * read by the kernels only; offsets must not go down (no access is out of bounds if they do, but the result is undefined).
  * out may be base.  scale (A fp32) may be null (1).
- * forward:  writes h (2, T, R) of dtype: scale * x down^T as hi + lo, rows without an adapter left as they were
+ * forward:  writes h, nb_lora_h_bytes() bytes for the backward pass: scale * x down^T as planes (T, R) of dtype that add up to
+ *           it, with float16 divided by a power of two per row, T floats behind them; rows without an adapter stay as they were
  * backward: reads dy, x, h and the factors; writes dx (T, K), ddown (A, R, K), dup (A, N, R), contiguous; each may be null;
- *           g is scratch like h (needed for dx and ddown); workspace: nb_lora_workspace_bytes() for the same arguments,
+ *           g is scratch like h, as large (needed for dx and ddown); workspace: nb_lora_workspace_bytes() for the same arguments,
  *           256-byte aligned (needed for ddown and dup).  Sums over rows are taken in a fixed order.
  * R a multiple of 16 up to NB_LORA_MAX_RANK, K and N multiples of 8 (else NB_ERR_UNSUPPORTED); every row 16-byte aligned.
  */
@@ -261,6 +262,7 @@ typedef struct nb_lora_args {
 int nb_lora_forward(const nb_lora_args* args, void* stream);
 int nb_lora_backward(const nb_lora_args* args, void* stream);
 int64_t nb_lora_workspace_bytes(const nb_lora_args* args);
+int64_t nb_lora_h_bytes(const nb_lora_args* args);  /* of T, R and dtype */
 
 /*
  * Layer norm with a weight and a bias and its backward pass.  NO COUNTERPART IN THE REFERENCE as an operator (it runs

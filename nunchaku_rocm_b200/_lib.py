@@ -190,6 +190,8 @@ def lib() -> C.CDLL:
                 l.nb_lora_backward.argtypes = [C.POINTER(LoraArgs), C.c_void_p]
                 l.nb_lora_workspace_bytes.argtypes = [C.POINTER(LoraArgs)]
                 l.nb_lora_workspace_bytes.restype = C.c_int64
+                l.nb_lora_h_bytes.argtypes = [C.POINTER(LoraArgs)]
+                l.nb_lora_h_bytes.restype = C.c_int64
                 l.nb_layer_norm.argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
                 l.nb_layer_norm_backward.argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
                 l.nb_layer_norm_workspace_bytes.argtypes = [C.c_int32] * 4
@@ -228,7 +230,7 @@ def binding():
                         "`python -m nunchaku_rocm_b200.build`. There is no fallback path."
                     ) from e
                 names = ["layer_norm", "layer_norm_backward", "layer_norm_workspace_bytes", "rotary_ladder_init", "rotary_axes", "rotary_table",
-                         "lora_forward", "lora_backward", "lora_workspace_bytes", "strerror", "last_error_detail", "last_cuda_error",
+                         "lora_forward", "lora_backward", "lora_workspace_bytes", "lora_h_bytes", "strerror", "last_error_detail", "last_cuda_error",
                          "last_cuda_error_string"]
                 b.bind({f"nb_{n}": C.cast(getattr(l, f"nb_{n}"), C.c_void_p).value for n in names}, _first_use)
                 _binding = b

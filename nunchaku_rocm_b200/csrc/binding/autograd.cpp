@@ -32,6 +32,7 @@ struct Library {
     decltype(&nb_lora_forward) lora_forward;
     decltype(&nb_lora_backward) lora_backward;
     decltype(&nb_lora_workspace_bytes) lora_workspace_bytes;
+    decltype(&nb_lora_h_bytes) lora_h_bytes;
     decltype(&nb_strerror) strerror;
     decltype(&nb_last_error_detail) last_error_detail;
     decltype(&nb_last_cuda_error) last_cuda_error;
@@ -46,7 +47,7 @@ void bind(const std::map<std::string, uintptr_t>& at, py::function on_first_use)
 #define NB_BIND(name) lib.name = reinterpret_cast<decltype(lib.name)>(at.at("nb_" #name))
     NB_BIND(layer_norm); NB_BIND(layer_norm_backward); NB_BIND(layer_norm_workspace_bytes);
     NB_BIND(rotary_ladder_init); NB_BIND(rotary_axes); NB_BIND(rotary_table);
-    NB_BIND(lora_forward); NB_BIND(lora_backward); NB_BIND(lora_workspace_bytes);
+    NB_BIND(lora_forward); NB_BIND(lora_backward); NB_BIND(lora_workspace_bytes); NB_BIND(lora_h_bytes);
     NB_BIND(strerror); NB_BIND(last_error_detail); NB_BIND(last_cuda_error); NB_BIND(last_cuda_error_string);
 #undef NB_BIND
 }
@@ -412,14 +413,14 @@ nb_lora_args lora_args(int64_t rows, const Tensor& down, const Tensor& up, const
     a.status = reinterpret_cast<void*>(status);
     return a;
 }
-// out, and the two 16-bit parts of scale x down^T
+// out, and scale x down^T as the backward pass reads it
 Tensor run_lora(const Tensor& x, const Tensor& base, const Tensor& down, const Tensor& up, const Tensor& offsets, const Tensor& adapters, const Tensor& scale,
                 const Tensor& out, int64_t impl, int64_t status) {
     const int64_t rows = x.numel() / down.size(2);
-    const Tensor h = empty_of({2, rows, down.size(1)}, x);
-    if (rows == 0) return h;
+    if (rows == 0) return empty_of({0}, at::kByte, x);
     const c10::cuda::CUDAGuard guard(x.device());
     nb_lora_args a = lora_args(rows, down, up, offsets, adapters, scale, impl, status);
+    const Tensor h = empty_of({lib.lora_h_bytes(&a)}, at::kByte, x);
     const Tensor xr = strided_rows(x, &a.stride_x, true);
     a.x = xr.const_data_ptr();
     Tensor br;
@@ -486,7 +487,7 @@ struct Lora : torch::autograd::Function<Lora> {
             // the workspace and g in one allocation (each costs the worker thread some microseconds)
             a.workspace_bytes = need_down || need_up ? lib.lora_workspace_bytes(&a) : 0;
             const int64_t at_g = (a.workspace_bytes + 255) / 256 * 256;
-            ws = empty_of({at_g + (need_x || need_down ? 4 * rows * down.size(1) : 0)}, at::kByte, down);
+            ws = empty_of({at_g + (need_x || need_down ? lib.lora_h_bytes(&a) : 0)}, at::kByte, down);
             if (a.workspace_bytes) a.workspace = ws.data_ptr();
             if (need_x || need_down) a.g = ws.data_ptr<uint8_t>() + at_g;
             check(lib.lora_backward(&a, stream_of(down)), "lora_batched backward");

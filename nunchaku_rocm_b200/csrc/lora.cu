@@ -15,9 +15,10 @@
 // pass over the offsets: border j of the offsets has floor(offset / BM) + 1 tile borders before it.
 //
 // h and g are sums in fp32.  Where they are operands again they are held as TWO 16-bit numbers, v = hi + lo (hi = v rounded
-// to T, lo = v - hi rounded to T): 16 significant bits for bf16 and 22 for fp16, so the second product loses nothing that
-// the final rounding would show; one rounding alone would add an error as large as that of the output itself.  It doubles
-// the matrix instructions of the second products, which move more bytes than they compute.
+// to T, lo = v - hi rounded to T), in fp16 after a power of two per row (Split, lora.cuh): 16 significant bits for bf16 and 22
+// for fp16, so the second product loses nothing that the final rounding would show; one rounding alone would add an error as
+// large as that of the output itself.  It doubles the matrix instructions of the second products, which move more bytes than
+// they compute.
 //
 // Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out); for a few rows the latency of two
 // dependent kernels, 24 single rows of 24 requests, 3072 -> 18432, rank 16: 12.9 us back to back in a graph.  The forward
@@ -57,12 +58,15 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // ------------------------------------------------------------------------------------------------------------------ shrink
-// v[t, r] = s_a sum_k X[t, k] F_a[r, k], written as hi + lo.  A CTA has one item and one slice of K; the slices of an item
+// v[t, r] = s_a sum_k X[t, k] F_a[r, k], written in parts.  A CTA has one item and one slice of K; the slices of an item
 // are a cluster, whose sums meet in shared memory (in a fixed order), so a few rows of a long K still use many SMs and no
 // partial sums go through memory.  The tiles of X and F travel by cp.async, ST stages deep.  With fewer than 64 rows the
 // warps that have no rows take a share of K instead.
@@ -78,6 +82,7 @@ struct ShrinkTile {
 template <typename T, int RM, bool RCONTIG>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraParams p) {
     using S = ShrinkTile<RM, RCONTIG>;
+    constexpr int PARTS = Split<T>::PARTS;
     extern __shared__ __align__(128) unsigned char smem[];
     chain_next();
     const Item it = find_item<kThreads>(p, blockIdx.x, p.rows_per_item);
@@ -171,29 +176,48 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const LoraParams 
     cg::cluster_group cluster = cg::this_cluster();
     if (splits > 1) cluster.sync();
     const float scale = p.scale ? __ldg(p.scale + it.adapter) : 1.f;
-    const int half = p.R / 2;  // pairs of a row
-    for (int e = split * kThreads + t; e < it.rows * half; e += splits * kThreads) {
-        const int row = e / half, r = (e - row * half) * 2;
-        float2 v = make_float2(0.f, 0.f);
-        for (int q = 0; q < splits; ++q) {
-            const float* from = splits > 1 ? cluster.map_shared_rank(sums, q) : sums;
-            const float2 u = *reinterpret_cast<const float2*>(from + row * LD + r);
-            v.x += u.x; v.y += u.y;
+    // LANES neighbours have a row, each a pair of its ranks (two at RM 8)
+    constexpr int LANES = RM == 1 ? 8 : RM == 2 ? 16 : 32, EACH = RM * 8 / LANES, TEAMS = kThreads / LANES;
+    for (int r0 = split * TEAMS; r0 < it.rows; r0 += splits * TEAMS) {
+        const int row = r0 + t / LANES;
+        float2 v[EACH];
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int r = (t % LANES + i * LANES) * 2;
+            v[i] = make_float2(0.f, 0.f);
+            if (row < it.rows && r < p.R)
+                for (int q = 0; q < splits; ++q) {
+                    const float* from = splits > 1 ? cluster.map_shared_rank(sums, q) : sums;
+                    const float2 u = *reinterpret_cast<const float2*>(from + row * LD + r);
+                    v[i].x += u.x; v[i].y += u.y;
+                }
+            v[i].x *= scale; v[i].y *= scale;
+            big = fmaxf(big, fmaxf(finite_abs(v[i].x), finite_abs(v[i].y)));
         }
-        v.x *= scale; v.y *= scale;
-        const uint32_t hi = pack2<T>(v.x, v.y);
-        const float2 back = unpack2<T>(hi);
-        // a value beyond T's range is infinite in hi; its remainder is then left out (inf - inf)
-        const uint32_t lo = pack2<T>(isfinite(back.x) ? v.x - back.x : 0.f, isfinite(back.y) ? v.y - back.y : 0.f);
-        const long long at = ((long long)(it.first + row) * p.R + r) * 2;
-        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.hi) + at) = hi;
-        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.lo) + at) = lo;
+        float down = 1.f;
+        if constexpr (Split<T>::SCALED) {
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const int e = row_exponent(big);
+            down = exp2_of(-e);
+            if (t % LANES == 0 && row < it.rows) p.row_scale[it.first + row] = exp2_of(e);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int r = (t % LANES + i * LANES) * 2;
+            if (row >= it.rows || r >= p.R) continue;
+            uint32_t part[PARTS];
+            split_pair<T>(v[i].x * down, v[i].y * down, part);
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) *reinterpret_cast<uint32_t*>(static_cast<char*>(p.v) + k * plane_bytes(p.T, p.R) + ((long long)(it.first + row) * p.R + r) * 2) = part[k];
+        }
     }
     if (splits > 1) cluster.sync();  // nobody's shared memory goes while others read it
 }
 
 // ------------------------------------------------------------------------------------------------------------------ expand
-// out[t, c] = base[t, c] + sum_r v[t, r] G_a[c, r], v = hi + lo.  A CTA keeps its item's v as matrix operands in registers
+// out[t, c] = base[t, c] + sum_r v[t, r] G_a[c, r].  A CTA keeps its item's v as matrix operands in registers
 // and walks over its columns, BN at a time, two tiles of G in shared memory.  The columns of a matrix instruction are
 // permuted (its operand rows may come from anywhere) so that a thread's results are eight neighbours: base and out are then
 // read and written 16 bytes at a time straight from and to memory.  Warps without rows take a share of the columns.
@@ -209,7 +233,7 @@ struct ExpandTile {
 template <typename T, int RM, bool CCONTIG>
 __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams p) {
     using S = ExpandTile<RM, CCONTIG>;
-    constexpr int BN = S::BN;
+    constexpr int BN = S::BN, PARTS = Split<T>::PARTS;
     extern __shared__ __align__(128) unsigned char smem[];
     const Item it = find_item<kThreads>(p, blockIdx.y, p.rows_per_item);
     if (it.rows == 0) return;
@@ -285,20 +309,23 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
     };
     fetch(0);
     chain_wait();
-    uint32_t hi[RM][4], lo[RM][4];
-    {
-        const char* ph = static_cast<const char*>(p.hi);
-        const char* pl = static_cast<const char*>(p.lo);
+    uint32_t v[PARTS][RM][4];
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+        const char* plane = static_cast<const char*>(p.v) + part * plane_bytes(p.T, p.R);
 #pragma unroll
         for (int k = 0; k < RM; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = i & 1 ? row1 : row0, r = k * 16 + (i >> 1) * 8 + (lane & 3) * 2;
                 const bool real = row < it.rows && r < p.R;
-                const long long at = ((long long)(it.first + row) * p.R + r) * 2;
-                hi[k][i] = real ? *reinterpret_cast<const uint32_t*>(ph + at) : 0u;
-                lo[k][i] = real ? *reinterpret_cast<const uint32_t*>(pl + at) : 0u;
+                v[part][k][i] = real ? *reinterpret_cast<const uint32_t*>(plane + ((long long)(it.first + row) * p.R + r) * 2) : 0u;
             }
+    }
+    float f0 = 1.f, f1 = 1.f;  // the rows' powers of two
+    if constexpr (Split<T>::SCALED) {
+        if (row0 < it.rows) f0 = p.row_scale[at0];
+        if (row1 < it.rows) f1 = p.row_scale[at1];
     }
     for (int tile = 0; tile < tiles; ++tile) {
         const int c0 = col0 + tile * BN;
@@ -326,16 +353,23 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
                         const int n = q * 32 + (i >> 1) * 8 + j * 2 + (i & 1);
                         ldsm4(b[h], smem_u32(gs) + n * S::GROW + (n >> 3) * 32 + k * 32 + ((lane >> 3) & 1) * 16);
                     }
-                    mma16816<T>(acc[2 * h], hi[k], b[h][0], b[h][1]);
-                    mma16816<T>(acc[2 * h + 1], hi[k], b[h][2], b[h][3]);
-                    mma16816<T>(acc[2 * h], lo[k], b[h][0], b[h][1]);
-                    mma16816<T>(acc[2 * h + 1], lo[k], b[h][2], b[h][3]);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        mma16816<T>(acc[2 * h], v[part][k], b[h][0], b[h][1]);
+                        mma16816<T>(acc[2 * h + 1], v[part][k], b[h][2], b[h][3]);
+                    }
                 }
             }
             auto joined = [&](const uint4& b, int o) {
-                const float2 f0 = unpack2<T>(b.x), f1 = unpack2<T>(b.y), f2 = unpack2<T>(b.z), f3 = unpack2<T>(b.w);
-                return make_uint4(pack2<T>(f0.x + acc[0][o], f0.y + acc[0][o + 1]), pack2<T>(f1.x + acc[1][o], f1.y + acc[1][o + 1]),
-                                  pack2<T>(f2.x + acc[2][o], f2.y + acc[2][o + 1]), pack2<T>(f3.x + acc[3][o], f3.y + acc[3][o + 1]));
+                const uint32_t in[4] = {b.x, b.y, b.z, b.w};
+                const float f = o ? f1 : f0;
+                uint32_t r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 u = unpack2<T>(in[j]);
+                    r[j] = pack2<T>(fmaf(acc[j][o], f, u.x), fmaf(acc[j][o + 1], f, u.y));
+                }
+                return make_uint4(r[0], r[1], r[2], r[3]);
             };
             if (row0 < it.rows && c < col1) *reinterpret_cast<uint4*>(out + at0 * p.stride_out + c) = joined(b0[g32], 0);
             if (row1 < it.rows && c < col1) *reinterpret_cast<uint4*>(out + at1 * p.stride_out + c) = joined(b1[g32], 2);
@@ -367,8 +401,11 @@ struct FewTile {
     // groups of warps that share the ranks in the first product (a warp has its sums and its steps of D in registers), tiles of
     // eight ranks of a group, groups along k
     static constexpr int GROUPS = R <= 32 ? 1 : R <= 64 ? 2 : 4, NT = (R / 8 + GROUPS - 1) / GROUPS, KW = kFewWarps / GROUPS;
-    static constexpr int RED = KW * 16 * R * 4, PART = 16 * R * 4, H = 2 * 16 * LDH * 2;
-    static int bytes(int cols) { return cols * R * 2 + RED + PART + H; }
+    static constexpr int RED = KW * 16 * R * 4, PART = 16 * R * 4;
+    template <typename T>
+    static constexpr int H = Split<T>::PARTS * 16 * LDH * 2 + 16 * 4;  // the parts of h, the rows' powers of two
+    template <typename T>
+    static int bytes(int cols) { return cols * R * 2 + RED + PART + H<T>; }
     // 16-byte piece of U's row: pieces that half a warp reads together are on different banks
     static __device__ __forceinline__ int piece(int row, int ch) {
         const int far = (row >> 3) & 1;
@@ -381,6 +418,7 @@ struct FewTile {
 template <typename T, int R>
 __global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel(const FewParams f) {
     using S = FewTile<R>;
+    constexpr int PARTS = Split<T>::PARTS;
     extern __shared__ __align__(16) unsigned char few_smem[];
     const LoraParams& p = f.l;
     const Item it = find_item<kFewWarps * 32>(p, blockIdx.x, kFewRows);
@@ -401,7 +439,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel
     unsigned char* us = few_smem;
     float* red = reinterpret_cast<float*>(few_smem + (size_t)f.cols * R * 2);
     float* part = red + S::RED / 4;
-    T* hs = reinterpret_cast<T*>(part + S::PART / 4);
+    float* powers = part + S::PART / 4;
+    T* hs = reinterpret_cast<T*>(powers + 16);
     const bool on0 = g < it.rows, on1 = g + 8 < it.rows;
     // this CTA's part of h: 32 values of k per step
     cg::cluster_group cluster = cg::this_cluster();
@@ -478,38 +517,63 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel
     }
     const float scale = p.scale ? __ldg(p.scale + it.adapter) : 1.f;
     cluster.sync();
-    for (int e = threadIdx.x; e < 16 * R; e += kFewWarps * 32) {
-        float v[kFewCluster], h = 0.f;
+    // LANES neighbours have a row
+    constexpr int LANES = R == 16 ? 16 : 32, EACH = (R + LANES - 1) / LANES, TEAMS = kFewWarps * 32 / LANES;
 #pragma unroll
-        for (int q = 0; q < kFewCluster; ++q) v[q] = cluster.map_shared_rank(part, q)[e];
+    for (int r0 = 0; r0 < kFewRows; r0 += TEAMS) {
+        const int row = r0 + threadIdx.x / LANES, l = threadIdx.x % LANES;
+        float h[EACH], big = 0.f;
 #pragma unroll
-        for (int q = 0; q < kFewCluster; ++q) h += v[q];
-        h *= scale;
-        const int row = e / R, r = e % R;
-        const T hi = from_f32<T>(h);
-        const float back = to_f32(hi);
-        const T lo = from_f32<T>(isfinite(back) ? h - back : 0.f);  // (beyond T: infinite in hi alone)
-        hs[row * S::LDH + r] = hi;
-        hs[(16 + row) * S::LDH + r] = lo;
-        if (blockIdx.y == 0 && row < it.rows) {  // for the backward pass
-            const long long at = (long long)(it.first + row) * R + r;
-            static_cast<T*>(p.hi)[at] = hi;
-            static_cast<T*>(p.lo)[at] = lo;
+        for (int i = 0; i < EACH; ++i) {
+            const int r = l + i * LANES;
+            float v[kFewCluster];
+            h[i] = 0.f;
+            if (R % LANES && r >= R) continue;
+#pragma unroll
+            for (int q = 0; q < kFewCluster; ++q) v[q] = cluster.map_shared_rank(part, q)[row * R + r];
+#pragma unroll
+            for (int q = 0; q < kFewCluster; ++q) h[i] += v[q];
+            h[i] *= scale;
+            big = fmaxf(big, finite_abs(h[i]));
+        }
+        float down = 1.f;
+        if constexpr (Split<T>::SCALED) {
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const int e = row_exponent(big);
+            down = exp2_of(-e);
+            if (l == 0) powers[row] = exp2_of(e);
+            if (l == 0 && blockIdx.y == 0 && row < it.rows) p.row_scale[it.first + row] = exp2_of(e);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int r = l + i * LANES;
+            if (R % LANES && r >= R) continue;
+            uint32_t words[PARTS];
+            split_pair<T>(h[i] * down, 0.f, words);
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) {
+                const T one = from_f32<T>(unpack2<T>(words[k]).x);
+                hs[(k * 16 + row) * S::LDH + r] = one;
+                if (blockIdx.y == 0 && row < it.rows)  // for the backward pass
+                    reinterpret_cast<T*>(static_cast<char*>(p.v) + k * plane_bytes(p.T, p.R))[(long long)(it.first + row) * R + r] = one;
+            }
         }
     }
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // the others' sums have been read
     cp_wait<0>();
     __syncthreads();
 
-    uint32_t a[2][R / 16][4];
+    uint32_t a[PARTS][R / 16][4];
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
+    for (int v = 0; v < PARTS; ++v)
 #pragma unroll
         for (int s = 0; s < R / 16; ++s) {
             const uint2 lo8 = *reinterpret_cast<const uint2*>(hs + (v * 16 + g) * S::LDH + s * 16 + t * 4);
             const uint2 hi8 = *reinterpret_cast<const uint2*>(hs + (v * 16 + g + 8) * S::LDH + s * 16 + t * 4);
             a[v][s][0] = lo8.x; a[v][s][1] = hi8.x; a[v][s][2] = lo8.y; a[v][s][3] = hi8.y;
         }
+    const float f0 = Split<T>::SCALED ? powers[g] : 1.f, f1 = Split<T>::SCALED ? powers[g + 8] : 1.f;
     for (int blk0 = warp; blk0 < blocks; blk0 += AHEAD * kFewWarps) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
@@ -523,17 +587,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel
 #pragma unroll
                 for (int s = 0; s < R / 16; ++s) {
                     const uint2 b = *reinterpret_cast<const uint2*>(us + S::piece(row, s * 2 + (t >> 1)) * 16 + (t & 1) * 8);
-                    mma16816<T>(o[j], a[0][s], b.x, b.y);
-                    mma16816<T>(o[j], a[1][s], b.x, b.y);
+#pragma unroll
+                    for (int v = 0; v < PARTS; ++v) mma16816<T>(o[j], a[v][s], b.x, b.y);
                 }
             }
             auto joined = [&](const uint4& b, int at) {
                 const uint32_t in[4] = {b.x, b.y, b.z, b.w};
+                const float f = at ? f1 : f0;
                 uint32_t r[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float2 v = unpack2<T>(in[j]);
-                    r[j] = pack2<T>(v.x + o[j][at], v.y + o[j][at + 1]);
+                    r[j] = pack2<T>(fmaf(o[j][at], f, v.x), fmaf(o[j][at + 1], f, v.y));
                 }
                 return make_uint4(r[0], r[1], r[2], r[3]);
             };
@@ -550,20 +615,21 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel
 // ------------------------------------------------------------------------------------------------------------------- outer
 // part[item][r, k] = sum over the item's rows of v[t, r] X[t, k] ([k, r] with KROWS, job 0), fp32, for one item of up to
 // rows_per_item rows and 128 columns.  Both operands are transposed on the way from shared memory to registers.
-template <int RM>
+template <typename T, int RM>
 struct OuterTile {
-    static constexpr int ST = RM >= 8 ? 3 : 4, BT = 32;
+    static constexpr int ST = RM >= 8 ? 3 : 4, BT = 32, PARTS = Split<T>::PARTS;
     static constexpr int XROW = 128 * 2 + 16, VROW = RM * 32 + 16;
     static constexpr int XBYTES = BT * XROW, VBYTES = BT * VROW;
-    static constexpr int STAGE = XBYTES + 2 * VBYTES, BYTES = ST * STAGE;
+    static constexpr int POWERS = XBYTES + PARTS * VBYTES;  // the rows' powers of two
+    static constexpr int STAGE = POWERS + (Split<T>::SCALED ? BT * 4 : 0), BYTES = ST * STAGE;
 };
 template <typename T, int RM, bool KROWS>
 __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJob& job, const Item& it, int w, int c0, unsigned char* smem) {
-    using S = OuterTile<RM>;
+    using S = OuterTile<T, RM>;
+    constexpr int PARTS = S::PARTS;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const T* x = static_cast<const T*>(job.x) + (long long)it.first * job.stride_x;
-    const char* hi = static_cast<const char*>(job.hi) + (long long)it.first * p.R * 2;
-    const char* lo = static_cast<const char*>(job.lo) + (long long)it.first * p.R * 2;
+    const char* v0 = static_cast<const char*>(job.v) + (long long)it.first * p.R * 2;
     const uint32_t sm = smem_u32(smem);
     const int n = (it.rows + S::BT - 1) / S::BT;
 
@@ -581,9 +647,11 @@ __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJo
                 const int row = e / (RM * 2), r = e % (RM * 2) * 8;
                 const bool real = r0 + row < it.rows && r < p.R;
                 const long long at = real ? ((long long)(r0 + row) * p.R + r) * 2 : 0;
-                cp16(st + S::XBYTES + row * S::VROW + r * 2, hi + at, real);
-                cp16(st + S::XBYTES + S::VBYTES + row * S::VROW + r * 2, lo + at, real);
+#pragma unroll
+                for (int k = 0; k < PARTS; ++k) cp16(st + S::XBYTES + k * S::VBYTES + row * S::VROW + r * 2, v0 + k * plane_bytes(p.T, p.R) + at, real);
             }
+            if constexpr (Split<T>::SCALED)
+                if (t < S::BT) cp4(st + S::POWERS + t * 4, job.row_scale + it.first + (r0 + t < it.rows ? r0 + t : 0));
         }
         cp_commit();
     };
@@ -598,6 +666,17 @@ __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJo
         for (int j = 0; j < NI; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
 #pragma unroll
     for (int s = 0; s < S::ST - 1; ++s) load(s);
+    // the item's largest power of two, which its rows are brought to
+    int top = 0;
+    if constexpr (Split<T>::SCALED) {
+        __shared__ int tops[kThreads / 32];
+        top = -126;
+        for (int r = t; r < it.rows; r += kThreads) top = max(top, (int)(__float_as_uint(job.row_scale[it.first + r]) >> 23) - 127);
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+        for (int w2 = 0; w2 < kThreads / 32; ++w2) top = max(top, tops[w2]);
+    }
     for (int s = 0; s < n; ++s) {
         cp_wait<S::ST - 2>();
         __syncthreads();
@@ -608,6 +687,26 @@ __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJo
             // operand with rows = columns of shared memory: matrices (t 0-7, c 0-7), (t 0-7, c 8-15), (t 8-15, ...) transposed
             const int arow = tt + (lane & 7) + (lane >> 4) * 8, acol = ((lane >> 3) & 1) * 16;
             const int brow = tt + (lane & 15), bcol = (lane >> 4) * 16;
+            // ratios of this lane's rows tt + 2 (lane % 4) + {0, 1} and eight rows on to the item's power, in two factors each
+            __half2 ratio[2][2];
+            if constexpr (Split<T>::SCALED) {
+                const float* f = reinterpret_cast<const float*>(smem + (s % S::ST) * S::STAGE + S::POWERS) + tt + (lane & 3) * 2;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float2 a, b;
+                    row_ratio(f[i * 8], top, a.x, b.x);
+                    row_ratio(f[i * 8 + 1], top, a.y, b.y);
+                    ratio[i][0] = __float22half2_rn(a);
+                    ratio[i][1] = __float22half2_rn(b);
+                }
+            }
+            auto level = [&](uint32_t& w, int i) {
+                if constexpr (Split<T>::SCALED) {
+                    __half2 h = *reinterpret_cast<__half2*>(&w);
+                    h = __hmul2(__hmul2(h, ratio[i][0]), ratio[i][1]);
+                    w = *reinterpret_cast<uint32_t*>(&h);
+                }
+            };
             if constexpr (KROWS) {
                 uint32_t a[2][4];
 #pragma unroll
@@ -615,9 +714,10 @@ __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJo
 #pragma unroll
                 for (int r = 0; r < RM; ++r)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < PARTS; ++h) {
                         uint32_t b[4];
                         ldsm4t(b, vs + h * S::VBYTES + brow * S::VROW + r * 32 + bcol);
+                        level(b[0], 0); level(b[1], 1); level(b[2], 0); level(b[3], 1);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             mma16816<T>(acc[i][2 * r], a[i], b[0], b[1]);
@@ -631,9 +731,10 @@ __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJo
 #pragma unroll
                 for (int r = 0; r < RM; ++r)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < PARTS; ++h) {
                         uint32_t a[4];
                         ldsm4t(a, vs + h * S::VBYTES + arow * S::VROW + r * 32 + acol);
+                        level(a[0], 0); level(a[1], 0); level(a[2], 1); level(a[3], 1);
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             mma16816<T>(acc[r][2 * j], a, b[j][0], b[j][1]);
@@ -645,6 +746,7 @@ __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJo
     }
     cp_wait<0>();
     float* part = job.part + (long long)w * p.R * job.K;
+    const float up = Split<T>::SCALED ? exp2_of(top) : 1.f;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -652,7 +754,7 @@ __device__ __forceinline__ void outer_product(const LoraParams& p, const OuterJo
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
                 const int mrow = i * 16 + (lane >> 2) + o * 8, ncol = j * 8 + (lane & 3) * 2;
-                const float2 v = make_float2(acc[i][j][2 * o], acc[i][j][2 * o + 1]);
+                const float2 v = make_float2(acc[i][j][2 * o] * up, acc[i][j][2 * o + 1] * up);
                 if constexpr (KROWS) {
                     const int k = c0 + warp * 32 + mrow;
                     if (k < job.K && ncol < p.R) *reinterpret_cast<float2*>(part + (long long)k * p.R + ncol) = v;
@@ -824,13 +926,13 @@ int few(const nb_lora_args* a, const LoraParams& p, cudaStream_t s) {
     if (splits < need) splits = need;
     f.cols = ceil_div(ceil_div(a->N, kFewCluster * splits), 32) * 32;
     auto* kernel = lora_few_kernel<T, R>;
-    const int bytes = FewTile<R>::bytes(f.cols);
+    const int bytes = FewTile<R>::template bytes<T>(f.cols);
     if (int rc = allow_smem(kernel, bytes)) return rc;
     return launch(kernel, dim3(item_count(a->T, a->requests, kFewRows), kFewCluster * splits), kFewWarps * 32, bytes, kFewCluster, false, s, f);
 }
 template <typename T, int RM>
 int outer(const nb_lora_args* a, const LoraParams& p, OuterJobs j, cudaStream_t s) {
-    using S = OuterTile<RM>;
+    using S = OuterTile<T, RM>;
     auto small = [&]() -> int {
         auto* kernel = lora_outer_kernel<T, RM>;
         if (int rc = allow_smem(kernel, S::BYTES)) return rc;
@@ -865,13 +967,13 @@ LoraParams params_of(const nb_lora_args* a) {
     p.status = static_cast<int*>(a->status);
     return p;
 }
-char* plane(void* h, const nb_lora_args* a, int which) { return static_cast<char*>(h) + (long long)which * a->T * a->R * 2; }
+float* powers_of(void* h, const nb_lora_args* a) { return reinterpret_cast<float*>(static_cast<char*>(h) + parts_of(a->dtype) * plane_bytes(a->T, a->R)); }
 
 template <typename T, int RM>
 int forward_t(const nb_lora_args* a, cudaStream_t s) {
     LoraParams p = params_of(a);
-    p.hi = plane(a->h, a, 0);
-    p.lo = plane(a->h, a, 1);
+    p.v = a->h;
+    p.row_scale = powers_of(a->h, a);
     if (use_few(a)) switch (a->R) {
             case 16: return few<T, 16>(a, p, s);
             case 32: return few<T, 32>(a, p, s);
@@ -892,8 +994,8 @@ template <typename T, int RM>
 int backward_t(const nb_lora_args* a, cudaStream_t s) {
     LoraParams g = params_of(a);
     if (a->dx || a->ddown) {
-        g.hi = plane(a->g, a, 0);
-        g.lo = plane(a->g, a, 1);
+        g.v = a->g;
+        g.row_scale = powers_of(a->g, a);
         g.x = a->dy; g.stride_x = a->stride_dy; g.factor = a->up; g.K = a->N;
         if (int rc = NB_TC_OR(a, tc_shrink(g, true, a->dtype, s), (shrink<T, RM, true>(g, s)))) return rc;
     }
@@ -909,7 +1011,7 @@ int backward_t(const nb_lora_args* a, cudaStream_t s) {
             used = w.end;
             float* part = reinterpret_cast<float*>(ws + w.part);
             int* table = reinterpret_cast<int*>(ws + w.table);
-            j.job[i] = {x, plane(planes, a, 0), plane(planes, a, 1), part, table, stride, cols, w.rows, w.items};
+            j.job[i] = {x, planes, powers_of(planes, a), part, table, stride, cols, w.rows, w.items};
             const long long size = (long long)a->R * cols;
             joins[n++] = {part, table, static_cast<T*>(grad), size, w.items, ceil_div(size, 1024)};
         };
@@ -959,6 +1061,13 @@ extern "C" int64_t nb_lora_workspace_bytes(const nb_lora_args* a) {
     if (a->dup) bytes = piece_of(a, a->N, bytes).end;
     if (a->ddown) bytes = piece_of(a, a->K, bytes).end;
     return bytes;
+}
+
+extern "C" int64_t nb_lora_h_bytes(const nb_lora_args* a) {
+    using namespace nb;
+    using namespace nb::lora;
+    if (check(a) != NB_OK) return 0;
+    return (parts_of(a->dtype) * plane_bytes(a->T, a->R) + (scaled(a->dtype) ? 4ll * a->T : 0) + 15) / 16 * 16;
 }
 
 extern "C" int nb_lora_forward(const nb_lora_args* a, void* stream) {

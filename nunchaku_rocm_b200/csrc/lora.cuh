@@ -1,16 +1,58 @@
 // What the kernels of the batched adapters share: their parameters and how the work is cut into items.
 #pragma once
 
+#include <type_traits>
+
 #include "nb_common.cuh"
 
 namespace nb {
 namespace lora {
 
+// h and g (fp32 sums, T x R) as the second products' operands: PARTS planes of 16-bit values that add up to them.  fp16 has
+// neither their range (scale x x down reaches far beyond 65504) nor, below 2^-14, its own 11 bits (gradients of adapters that
+// have just begun to train are that small), so with SCALED a row is divided by a power of two that brings its largest finite
+// value to 2^14 .. 2^15, and the T powers stand behind the planes as floats.  A second product over the ranks multiplies its
+// sums by them; one over the rows first brings its item's rows to their largest power.  Two parts then hold 22 bits of every
+// value down to 2^-17 of its row's (item's) largest, and 2^-39 of the largest below.
+template <typename T>
+struct Split {
+    static constexpr int PARTS = 2;
+    static constexpr bool SCALED = std::is_same<T, __half>::value;
+};
+__host__ __device__ inline int parts_of(int) { return 2; }
+inline bool scaled(int dtype) { return dtype == NB_DTYPE_FP16; }
+__host__ __device__ inline long long plane_bytes(int T, int R) { return (long long)T * R * 2; }
+
+// The power of two that divides a row whose largest finite magnitude is `big`; rows of zeros have the smallest.
+__device__ __forceinline__ int row_exponent(float big) { return min(max((int)(__float_as_uint(big) >> 23) - 127 - 14, -126), 126); }
+__device__ __forceinline__ float exp2_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 .. 127
+// `f` / 2^e, f a row's power of two and 2^e its item's largest, as a product of two that fp16 holds (down to 2^-44: smaller
+// ones leave nothing of a finite value, and an infinite one infinite)
+__device__ __forceinline__ void row_ratio(float f, int e, float& a, float& b) {
+    const int d = (int)(__float_as_uint(f) >> 23) - 127 - e;
+    a = exp2_of(min(max(d, -20), 0));
+    b = exp2_of(min(max(d + 20, -24), 0));
+}
+__device__ __forceinline__ float finite_abs(float v) { return isfinite(v) ? fabsf(v) : 0.f; }
+
+// A pair of values as PARTS words.
+template <typename T>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[Split<T>::PARTS]) {
+#pragma unroll
+    for (int i = 0; i < Split<T>::PARTS; ++i) {
+        part[i] = pack2<T>(x, y);
+        const float2 back = unpack2<T>(part[i]);
+        // (a value that is not finite is so in the first part alone)
+        x = isfinite(back.x) ? x - back.x : 0.f;
+        y = isfinite(back.y) ? y - back.y : 0.f;
+    }
+}
+
 struct LoraParams {
     const void* x;        // shrink: (T, K) operand; expand: base (T, C) or null
     void* out;            // expand: (T, C)
     const void* factor;   // shrink: (A, R, K) or (A, K, R); expand: (A, C, R) or (A, R, C)
-    void* hi; void* lo;   // (T, R) each
+    void* v; float* row_scale;  // h or g: planes of (T, R), and the rows' powers of two behind them
     const int* offsets; const int* adapters; const float* scale;
     long long stride_x, stride_out;
     int T, K, R, A, requests;  // K: length of the contraction (shrink), columns (expand)
@@ -22,7 +64,7 @@ struct LoraParams {
 // The gradients of both factors are one launch: the first `groups` CTAs of a row of the grid are job 0's, U's, with partial
 // products (items, K, R); the others job 1's, D's, (items, R, K).
 struct OuterJob {
-    const void* x; const void* hi; const void* lo;  // (T, K) and (T, R) operands
+    const void* x; const void* v; const float* row_scale;  // (T, K) and (T, R) operands
     float* part;
     int* item_adapter;  // (items): -1 for an item without rows or adapter
     long long stride_x;

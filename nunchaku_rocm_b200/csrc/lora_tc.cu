@@ -74,6 +74,12 @@ __device__ __forceinline__ uint8_t* align1k(unsigned char* p) {
     return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
 }
 
+// the planes of h or g as tensor maps
+template <typename T>
+struct PartMaps {
+    CUtensorMap part[Split<T>::PARTS];
+};
+
 // ------------------------------------------------------------------------------------------------------------------ shrink
 // 128 rows x R over one slice of K; the slices of an item are a cluster whose sums meet in shared memory.
 // Warps: TMA producer, MMA issuer, four for the sums.
@@ -196,25 +202,35 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
     __syncthreads();
     cg::cluster_group cluster = cg::this_cluster();
     if (splits > 1) cluster.sync();
-    // four values of r at a time, the slices' sums in order; all the loads of a value are on their way together
-    const int quads = p.R / 4;
-    for (int e = split * S::THREADS + threadIdx.x; e < it.rows * quads; e += splits * S::THREADS) {
-        const int row = e / quads, r = (e - row * quads) * 4;
+    // LANES neighbours have a row, each four of its ranks; the slices' sums in order, all the loads of a value on their way together
+    constexpr int LANES = RP / 4, TEAMS = S::THREADS / LANES, PARTS = Split<T>::PARTS;
+    for (int r0 = split * TEAMS; r0 < it.rows; r0 += splits * TEAMS) {
+        const int row = r0 + (int)threadIdx.x / LANES, r = (int)threadIdx.x % LANES * 4;
+        const bool on = row < it.rows && r < p.R;
         float4 u[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            if (q < splits) u[q] = *reinterpret_cast<const float4*>((splits > 1 ? cluster.map_shared_rank(sums, q) : sums) + row * S::LD + r);
+            if (on && q < splits) u[q] = *reinterpret_cast<const float4*>((splits > 1 ? cluster.map_shared_rank(sums, q) : sums) + row * S::LD + r);
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            if (q < splits) { v.x += u[q].x; v.y += u[q].y; v.z += u[q].z; v.w += u[q].w; }
+            if (on && q < splits) { v.x += u[q].x; v.y += u[q].y; v.z += u[q].z; v.w += u[q].w; }
         v.x *= scale; v.y *= scale; v.z *= scale; v.w *= scale;
-        const uint2 hi = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
-        const float2 b0 = unpack2<T>(hi.x), b1 = unpack2<T>(hi.y);
-        auto rest = [](float value, float back) { return isfinite(back) ? value - back : 0.f; };  // (beyond T: infinite in hi alone)
-        const uint2 lo = make_uint2(pack2<T>(rest(v.x, b0.x), rest(v.y, b0.y)), pack2<T>(rest(v.z, b1.x), rest(v.w, b1.y)));
-        const long long at = ((long long)(it.first + row) * p.R + r) * 2;
-        *reinterpret_cast<uint2*>(static_cast<char*>(p.hi) + at) = hi;
-        *reinterpret_cast<uint2*>(static_cast<char*>(p.lo) + at) = lo;
+        if constexpr (Split<T>::SCALED) {
+            float big = fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)));
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const int e = row_exponent(big);
+            const float down = exp2_of(-e);
+            v.x *= down; v.y *= down; v.z *= down; v.w *= down;
+            if (r == 0 && on) p.row_scale[it.first + row] = exp2_of(e);
+        }
+        if (!on) continue;
+        uint32_t xy[PARTS], zw[PARTS];
+        split_pair<T>(v.x, v.y, xy);
+        split_pair<T>(v.z, v.w, zw);
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k)
+            *reinterpret_cast<uint2*>(static_cast<char*>(p.v) + k * plane_bytes(p.T, p.R) + ((long long)(it.first + row) * p.R + r) * 2) = make_uint2(xy[k], zw[k]);
     }
     if (splits > 1) cluster.sync();
     else __syncthreads();
@@ -227,28 +243,27 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------------------------ expand
-// out[128 rows, columns col0 .. col1) = base + (hi + lo) G^T, 64 columns at a time.  The item's hi and lo stay in shared
+// out[128 rows, columns col0 .. col1) = base + v G^T, 64 columns at a time.  The parts of the item's v stay in shared
 // memory; a ring of SLOTS 16 KB tiles carries base in and out back: TMA load, tensor-memory result added in place, TMA
 // store (straight from registers where the item has fewer than 128 rows).  Warps: TMA producer, MMA issuer, eight that add
 // (a lane has a row, a warp half of a tile's columns), one that stores.  All of them take every tile, in order: a barrier of
 // the ring is then never more than one phase ahead of anybody who waits on it.
-template <int RP>
+template <typename T, int RP>
 struct ExpandTc {
-    static constexpr int HALVES = RP <= 64 ? 1 : 2;
-    static constexpr int VB = HALVES * kTcRows * 128;   // hi or lo
+    static constexpr int HALVES = RP <= 64 ? 1 : 2, PARTS = Split<T>::PARTS;
+    static constexpr int VB = HALVES * kTcRows * 128;   // a part of v
     // up to rank 64 two CTAs share an SM, so that one starts and drains under the other's tiles
     static constexpr int PER_SM = RP <= 64 ? 2 : 1;
     static constexpr int GB = HALVES * 64 * 128, GST = RP <= 64 ? 2 : 3;
     static constexpr int SLOT = kTcRows * 128, SLOTS = RP <= 64 ? 3 : 5;
-    static constexpr int OFF_G = 2 * VB, OFF_S = OFF_G + GST * GB, OFF_BAR = OFF_S + SLOTS * SLOT;
+    static constexpr int OFF_G = PARTS * VB, OFF_S = OFF_G + GST * GB, OFF_BAR = OFF_S + SLOTS * SLOT;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
     static constexpr int THREADS = 352;
 };
 template <typename T, int RP, bool CCONTIG>
-__global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tm_hi, const __grid_constant__ CUtensorMap tm_lo,
-                                                              const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_base,
+__global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_constant__ PartMaps<T> tm_v, const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_base,
                                                               const __grid_constant__ CUtensorMap tm_out, const LoraParams p) {
-    using S = ExpandTc<RP>;
+    using S = ExpandTc<T, RP>;
     extern __shared__ unsigned char raw[];
     const Item it = find_item<S::THREADS>(p, blockIdx.y, p.rows_per_item);
     if (it.rows == 0) return;
@@ -315,11 +330,9 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
                 }
                 if (i == min(S::GST, tiles) - 1) {  // the ring is filled as far as it goes without the kernel before this one
                     chain_wait();
-                    mbar_expect_tx(bar(V), 2 * S::VB);
-                    for (int h = 0; h < S::HALVES; ++h) {
-                        tma_load_2d(sb + h * kTcRows * 128, &tm_hi, bar(V), h * 64, it.first);
-                        tma_load_2d(sb + S::VB + h * kTcRows * 128, &tm_lo, bar(V), h * 64, it.first);
-                    }
+                    mbar_expect_tx(bar(V), S::PARTS * S::VB);
+                    for (int h = 0; h < S::HALVES; ++h)
+                        for (int v = 0; v < S::PARTS; ++v) tma_load_2d(sb + v * S::VB + h * kTcRows * 128, &tm_v.part[v], bar(V), h * 64, it.first);
                 }
             }
             if (!ok) let_copies_land();
@@ -335,7 +348,7 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t g = sb + S::OFF_G + gs * S::GB;
-                for (int v = 0; v < 2; ++v)  // hi, lo
+                for (int v = 0; v < S::PARTS; ++v)
                     for (int k = 0; k < k16; ++k) {
                         const uint64_t a = desc_k(sb + v * S::VB + (k >> 2) * kTcRows * 128) + (k & 3) * 2;
                         const uint64_t b = CCONTIG ? desc_mn(g + k * 16 * 128, 64 * 128) : desc_k(g + (k >> 2) * 64 * 128) + (k & 3) * 2;
@@ -349,6 +362,11 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
     } else if (warp < 10) {
         const int q = warp & 3, half = (warp - 2) >> 2, row = q * 32 + lane;
         const bool whole = it.rows == kTcRows;
+        float power = 1.f;  // of this lane's row
+        if constexpr (Split<T>::SCALED) {
+            chain_wait();
+            if (row < it.rows) power = *const_cast<const volatile float*>(p.row_scale + it.first + row);
+        }
         for (int i = 0; i < tiles; ++i) {
             const int ls = i % S::SLOTS, d = i & 1, c = col0 + i * 64 + half * 32;
             const uint32_t line = sb + S::OFF_S + ls * S::SLOT + row * 128;
@@ -375,10 +393,11 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
                     uint4 b;
                     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "r"(at) : "memory");
                     const float2 b0 = unpack2<T>(b.x), b1 = unpack2<T>(b.y), b2 = unpack2<T>(b.z), b3 = unpack2<T>(b.w);
-                    o = make_uint4(pack2<T>(f[0] + b0.x, f[1] + b0.y), pack2<T>(f[2] + b1.x, f[3] + b1.y), pack2<T>(f[4] + b2.x, f[5] + b2.y),
-                                   pack2<T>(f[6] + b3.x, f[7] + b3.y));
+                    const auto add = [&](float v0, float v1, float2 u) { return pack2<T>(fmaf(v0, power, u.x), fmaf(v1, power, u.y)); };
+                    o = make_uint4(add(f[0], f[1], b0), add(f[2], f[3], b1), add(f[4], f[5], b2), add(f[6], f[7], b3));
                 } else {
-                    o = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+                    const auto one = [&](float v0, float v1) { return pack2<T>(v0 * power, v1 * power); };
+                    o = make_uint4(one(f[0], f[1]), one(f[2], f[3]), one(f[4], f[5]), one(f[6], f[7]));
                 }
                 if (whole)
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w) : "memory");
@@ -414,49 +433,56 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------------------------- outer
-// part[item][r, k] (job 1; [k, r] for job 0) = sum over the item's rows of (hi + lo)[t, r] X[t, k], 256 columns of X per CTA
-// (two accumulators of 128: hi and lo come from the L2 cache once for both, 16 KB beside 32 KB of X at rank 64; with 128
-// columns the cache delivered as much of them as HBM of X).  Both operands run along the rows (MN-major), so they are used
-// as they lie.
-template <int RP>
+// part[item][r, k] (job 1; [k, r] for job 0) = sum over the item's rows of v[t, r] X[t, k], 256 columns of X per CTA
+// (two accumulators of 128: v comes from the L2 cache once for both, 16 KB beside 32 KB of X at rank 64; with 128
+// columns the cache delivered as much of it as HBM of X).  Both operands run along the rows (MN-major), so they are used
+// as they lie; where the rows have powers of two, the four warps that read the sums later bring the rows of v to the item's
+// power in shared memory before they are multiplied.
+template <typename T, int RP>
 struct OuterTc {
-    static constexpr int HALVES = RP <= 64 ? 1 : 2;
+    static constexpr int HALVES = RP <= 64 ? 1 : 2, PARTS = Split<T>::PARTS;
     static constexpr int TILE = KB * 128;  // 64 rows of 64 values
-    static constexpr int STAGE = (4 + 2 * HALVES) * TILE, ST = RP <= 64 ? 4 : 3;
+    static constexpr int STAGE = (4 + PARTS * HALVES) * TILE, ST = RP <= 64 ? 4 : 3;
     static constexpr int OFF_BAR = ST * STAGE;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
     static constexpr int ACC = RP < 32 ? 32 : RP, COLS = 2 * ACC;  // tensor-memory columns: read 32 at a time
     static constexpr int THREADS = 192;
 };
+template <typename T>
 struct OuterMaps {
-    CUtensorMap x[2], hi[2], lo[2];  // of the two jobs
+    CUtensorMap x[2];  // of the two jobs
+    PartMaps<T> v[2];
 };
 template <typename T, int RP>
-__global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constant__ OuterMaps maps, const LoraParams p,
+__global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constant__ OuterMaps<T> maps, const LoraParams p,
                                                             const __grid_constant__ OuterJobs jobs) {
-    using S = OuterTc<RP>;
+    using S = OuterTc<T, RP>;
+    constexpr bool SCALED = Split<T>::SCALED;
     const bool krows = (int)blockIdx.x < jobs.groups;
     const int which = krows ? 0 : 1, K = jobs.job[which].K;
-    const CUtensorMap &tm_x = maps.x[which], &tm_hi = maps.hi[which], &tm_lo = maps.lo[which];
+    const CUtensorMap& tm_x = maps.x[which];
+    const PartMaps<T>& tm_v = maps.v[which];
     extern __shared__ unsigned char raw[];
     chain_next();
     uint8_t* smem = align1k(raw);
     const uint32_t sb = smem_u32(smem), bars = sb + S::OFF_BAR;
     auto full = [&](int i) { return bars + 8u * i; };
     auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
-    const uint32_t done = bars + 8u * (2 * S::ST);
-    static_assert(8 * (2 * S::ST + 1) <= 192, "barriers");
+    auto level = [&](int i) { return bars + 8u * (2 * S::ST + i); };  // a slot's rows of v have the item's power
+    const uint32_t done = bars + 8u * (3 * S::ST);
+    static_assert(8 * (3 * S::ST + 1) <= 192, "barriers");
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
     volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
+    int* tops = reinterpret_cast<int*>(smem + S::OFF_BAR + 208);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // (set up while the offsets are on their way)
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tm_x);
-        tma_prefetch_desc(&tm_hi);
-        tma_prefetch_desc(&tm_lo);
+        for (int k = 0; k < S::PARTS; ++k) tma_prefetch_desc(&tm_v.part[k]);
         for (int i = 0; i < S::ST; ++i) {
             mbar_init(full(i), 1);
             mbar_init(empty(i), 1);
+            mbar_init(level(i), 4);
         }
         mbar_init(done, 1);
         *abort_s = 0;
@@ -489,12 +515,10 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                 const int st = s % S::ST, t0 = it.first + s * KB;
                 if (s >= S::ST && !mbar_wait(empty(st), ((s / S::ST) & 1) ^ 1, abort_s, E_OUTER | 1, 50)) { ok = false; break; }
                 const uint32_t at = sb + st * S::STAGE;
-                mbar_expect_tx(full(st), (quarters + 2 * S::HALVES) * S::TILE);
+                mbar_expect_tx(full(st), (quarters + S::PARTS * S::HALVES) * S::TILE);
                 for (int q = 0; q < quarters; ++q) tma_load_2d(at + q * S::TILE, &tm_x, full(st), c0 + q * 64, t0);
-                for (int h = 0; h < S::HALVES; ++h) {
-                    tma_load_2d(at + (4 + h) * S::TILE, &tm_hi, full(st), h * 64, t0);
-                    tma_load_2d(at + (4 + S::HALVES + h) * S::TILE, &tm_lo, full(st), h * 64, t0);
-                }
+                for (int v = 0; v < S::PARTS; ++v)
+                    for (int h = 0; h < S::HALVES; ++h) tma_load_2d(at + (4 + v * S::HALVES + h) * S::TILE, &tm_v.part[v], full(st), h * 64, t0);
             }
             if (!ok) let_copies_land();
         }
@@ -506,23 +530,21 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
             const uint32_t at = sb + st * S::STAGE;
             if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_OUTER | 2)) { ok = false; break; }
             if (rows < k16 * 16) {  // rows behind the item's last one: zeros in every tile
-                for (int tile = 0; tile < 4 + 2 * S::HALVES; ++tile)
+                for (int tile = 0; tile < 4 + S::PARTS * S::HALVES; ++tile)
                     for (int e = rows * 8 + lane; e < k16 * 16 * 8; e += 32)
                         asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + tile * S::TILE + e * 16), "r"(0) : "memory");
                 fence_proxy_async_smem();
                 __syncwarp();
             }
+            if (SCALED && !mbar_wait_warp(level(st), (s / S::ST) & 1, abort_s, E_OUTER | 4)) { ok = false; break; }
             tc_fence_after();
             if (elect_one()) {
-                for (int k = 0; k < k16; ++k) {
-                    const uint64_t hi = desc_mn(at + 4 * S::TILE + k * 16 * 128, S::TILE);
-                    const uint64_t lo = desc_mn(at + (4 + S::HALVES) * S::TILE + k * 16 * 128, S::TILE);
+                for (int k = 0; k < k16; ++k)
                     for (int h = 0; 2 * h < quarters; ++h) {
                         const uint64_t a = desc_mn(at + 2 * h * S::TILE + k * 16 * 128, S::TILE);
-                        mma_f16(tmem + h * S::ACC, a, hi, idesc, (s || k) ? 1u : 0u);
-                        mma_f16(tmem + h * S::ACC, a, lo, idesc, 1u);
+                        for (int v = 0; v < S::PARTS; ++v)
+                            mma_f16(tmem + h * S::ACC, a, desc_mn(at + (4 + v * S::HALVES) * S::TILE + k * 16 * 128, S::TILE), idesc, (s || k || v) ? 1u : 0u);
                     }
-                }
                 tc_commit(empty(st));
                 if (s == n - 1) tc_commit(done);
             }
@@ -531,7 +553,51 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
     } else {
         const int q = warp & 3;
         float* part = jobs.job[which].part + (long long)w * p.R * K;
-        if (mbar_wait_warp(done, 0, abort_s, E_OUTER | 3)) {
+        float up = 1.f;
+        bool ok = true;
+        if constexpr (SCALED) {
+            // two threads have a row of a slot, each half of its 16-byte pieces
+            const int t = threadIdx.x - 64, row = t >> 1;
+            const float* powers = jobs.job[which].row_scale + it.first;
+            int top = -126;
+#pragma unroll 4
+            for (int r = t; r < it.rows; r += 128) top = max(top, (int)(__float_as_uint(powers[r]) >> 23) - 127);
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) tops[q] = top;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (int i = 0; i < 4; ++i) top = max(top, tops[i]);
+            up = exp2_of(top);
+            float next = row < it.rows ? powers[row] : up;
+            for (int s = 0; s < n && ok; ++s) {
+                const int st = s % S::ST;
+                float a, b;
+                row_ratio(next, top, a, b);
+                if ((s + 1) * KB + row < it.rows) next = powers[(s + 1) * KB + row];
+                if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_OUTER | 5)) { ok = false; break; }
+                if (s * KB + row < it.rows && a * b < 1.f) {
+                    const __half2 a2 = __float2half2_rn(a), b2 = __float2half2_rn(b);
+                    const uint32_t at = sb + st * S::STAGE + 4 * S::TILE + row * 128 + (t & 1) * 64;
+                    for (int tile = 0; tile < S::PARTS * S::HALVES; ++tile)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t v[4];
+                            const uint32_t to = at + tile * S::TILE + c * 16;
+                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(to) : "memory");
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                __half2 h = *reinterpret_cast<__half2*>(&v[j]);
+                                h = __hmul2(__hmul2(h, a2), b2);
+                                v[j] = *reinterpret_cast<uint32_t*>(&h);
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                        }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(level(st));
+            }
+        }
+        if (ok && mbar_wait_warp(done, 0, abort_s, E_OUTER | 3)) {
             tc_fence_after();
             for (int h = 0; 2 * h < quarters; ++h) {
                 const int k = c0 + h * 128 + q * 32 + lane;
@@ -539,6 +605,10 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                     float v[32];
                     tmem_ld32(tmem + (q * 32 << 16) + h * S::ACC + c, v);
                     tmem_wait_ld();
+                    if constexpr (SCALED) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] *= up;
+                    }
                     if (k < K) {
                         const int left = p.R - c;  // 16 or more
                         if (krows) {
@@ -595,6 +665,13 @@ bool make_map(CUtensorMap* m, const void* base, long long rows, long long cols, 
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename T>
+bool make_part_maps(PartMaps<T>* m, const void* v, const LoraParams& p, int box_rows) {
+    bool ok = true;
+    for (int k = 0; k < Split<T>::PARTS; ++k) ok = ok && make_map<T>(&m->part[k], static_cast<const char*>(v) + k * plane_bytes(p.T, p.R), p.T, p.R, p.R, box_rows);
+    return ok;
+}
+
 template <typename T, int RP, bool RCONTIG>
 int shrink(LoraParams p, cudaStream_t s) {
     using S = ShrinkTc<RP>;
@@ -617,20 +694,20 @@ int shrink(LoraParams p, cudaStream_t s) {
 }
 template <typename T, int RP, bool CCONTIG>
 int expand(LoraParams p, cudaStream_t s) {
-    using S = ExpandTc<RP>;
+    using S = ExpandTc<T, RP>;
     p.rows_per_item = kTcRows;
     auto* kernel = lora_expand_tc_kernel<T, RP, CCONTIG>;
     NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
-    CUtensorMap hi, lo, g, base, out;
-    bool ok = make_map<T>(&hi, p.hi, p.T, p.R, p.R, kTcRows) && make_map<T>(&lo, p.lo, p.T, p.R, p.R, kTcRows) &&
-              make_map<T>(&out, p.out, p.T, p.K, p.stride_out, kTcRows) &&
+    PartMaps<T> v;
+    CUtensorMap g, base, out;
+    bool ok = make_part_maps<T>(&v, p.v, p, kTcRows) && make_map<T>(&out, p.out, p.T, p.K, p.stride_out, kTcRows) &&
               (CCONTIG ? make_map<T>(&g, p.factor, p.R, p.K, p.K, p.R, p.A) : make_map<T>(&g, p.factor, p.K, p.R, p.R, 64, p.A));
     if (ok && p.x) ok = make_map<T>(&base, p.x, p.T, p.K, p.stride_x, kTcRows);
     else base = out;
     if (!ok) return NB_ERR_UNSUPPORTED;
     const int items = item_count(p.T, p.requests, kTcRows), live = live_items(p, kTcRows);
     // columns of a CTA: the cut of a row into `cuts` pieces that is done soonest, a CTA's cost being its tiles (0.7 us of an
-    // SM's share of HBM each) and about three microseconds to start and to load the item's hi and lo, waves of the CTAs that
+    // SM's share of HBM each) and about three microseconds to start and to load the item's v, waves of the CTAs that
     // are resident together taking turns
     const int tiles = ceil_div(p.K, 64), slots = S::PER_SM * sms();
     int per = tiles;
@@ -641,20 +718,18 @@ int expand(LoraParams p, cudaStream_t s) {
         if (cost < best) best = cost, per = t;
     }
     p.cols_per_cta = per * 64;
-    return launch(kernel, dim3(ceil_div(tiles, per), items), S::THREADS, S::BYTES, 1, p.chained, s, hi, lo, g, base, out, p);
+    return launch(kernel, dim3(ceil_div(tiles, per), items), S::THREADS, S::BYTES, 1, p.chained, s, v, g, base, out, p);
 }
 template <typename T, int RP>
 int outer(const LoraParams& p, OuterJobs j, cudaStream_t s) {
-    using S = OuterTc<RP>;
+    using S = OuterTc<T, RP>;
     auto* kernel = lora_outer_tc_kernel<T, RP>;
     NB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
-    OuterMaps m;
+    OuterMaps<T> m;
     int groups = 0;
     for (int i = 0; i < 2; ++i) {
         const OuterJob& o = j.job[j.job[i].K ? i : 1 - i];  // (a job that is not there has no CTAs; its maps are the other's)
-        if (!(make_map<T>(&m.x[i], o.x, p.T, o.K, o.stride_x, KB) && make_map<T>(&m.hi[i], o.hi, p.T, p.R, p.R, KB) &&
-              make_map<T>(&m.lo[i], o.lo, p.T, p.R, p.R, KB)))
-            return NB_ERR_UNSUPPORTED;
+        if (!(make_map<T>(&m.x[i], o.x, p.T, o.K, o.stride_x, KB) && make_part_maps<T>(&m.v[i], o.v, p, KB))) return NB_ERR_UNSUPPORTED;
         groups += ceil_div(j.job[i].K, kTcCols);
     }
     j.groups = ceil_div(j.job[0].K, kTcCols);

@@ -33,6 +33,9 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     with the inputs otherwise.  At most 65535 adapters, and ``rows / 64 + requests`` at most 65000.  A backward pass needs a
     workspace of ``R (K + N)`` floats for every request and every few hundred rows.
 
+    ``x @ down^T`` may be beyond float16, and so may its gradient: both stay in 22 bits of a value and its row's own power of
+    two until the result is rounded.
+
     Differentiable in ``x``, ``base``, ``down`` and ``up`` (not in ``scale``); gradients of adapters that several requests
     share are summed in a fixed order.
     """
