@@ -1066,7 +1066,7 @@ extern "C" int64_t nb_lora_workspace_bytes(const nb_lora_args* a) {
 extern "C" int64_t nb_lora_h_bytes(const nb_lora_args* a) {
     using namespace nb;
     using namespace nb::lora;
-    if (check(a) != NB_OK) return 0;
+    if (!a || a->T < 0 || a->T > (1 << 30) || a->R <= 0 || a->R % 16 || a->R > NB_LORA_MAX_RANK) return 0;
     return (parts_of(a->dtype) * plane_bytes(a->T, a->R) + (scaled(a->dtype) ? 4ll * a->T : 0) + 15) / 16 * 16;
 }
 
