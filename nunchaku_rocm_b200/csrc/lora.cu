@@ -14,11 +14,10 @@
 // grid is known without reading the offsets on the host), every row is in exactly one, and a CTA finds its item with one
 // pass over the offsets: border j of the offsets has floor(offset / BM) + 1 tile borders before it.
 //
-// h and g are sums in fp32.  Where they are operands again they are held as TWO 16-bit numbers, v = hi + lo (hi = v rounded
-// to T, lo = v - hi rounded to T), in fp16 after a power of two per row (Split, lora.cuh): 16 significant bits for bf16 and 22
-// for fp16, so the second product loses nothing that the final rounding would show; one rounding alone would add an error as
-// large as that of the output itself.  It doubles the matrix instructions of the second products, which move more bytes than
-// they compute.
+// h and g are sums in fp32.  Where they are operands again they are held as several 16-bit numbers that add up to them: three
+// in bf16 (all 24 bits), two in fp16 after a power of two per row (22 bits; Split, lora.cuh).  One rounding alone would add an
+// error as large as that of the output itself.  It multiplies the matrix instructions of the second products, which move more
+// bytes than they compute.
 //
 // Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out); for a few rows the latency of two
 // dependent kernels, 24 single rows of 24 requests, 3072 -> 18432, rank 16: 12.9 us back to back in a graph.  The forward
@@ -617,7 +616,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel
 // rows_per_item rows and 128 columns.  Both operands are transposed on the way from shared memory to registers.
 template <typename T, int RM>
 struct OuterTile {
-    static constexpr int ST = RM >= 8 ? 3 : 4, BT = 32, PARTS = Split<T>::PARTS;
+    static constexpr int PARTS = Split<T>::PARTS, ST = PARTS * RM >= 12 ? 3 : 4, BT = 32;
     static constexpr int XROW = 128 * 2 + 16, VROW = RM * 32 + 16;
     static constexpr int XBYTES = BT * XROW, VBYTES = BT * VROW;
     static constexpr int POWERS = XBYTES + PARTS * VBYTES;  // the rows' powers of two

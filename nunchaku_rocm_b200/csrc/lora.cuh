@@ -8,18 +8,20 @@
 namespace nb {
 namespace lora {
 
-// h and g (fp32 sums, T x R) as the second products' operands: PARTS planes of 16-bit values that add up to them.  fp16 has
-// neither their range (scale x x down reaches far beyond 65504) nor, below 2^-14, its own 11 bits (gradients of adapters that
-// have just begun to train are that small), so with SCALED a row is divided by a power of two that brings its largest finite
-// value to 2^14 .. 2^15, and the T powers stand behind the planes as floats.  A second product over the ranks multiplies its
-// sums by them; one over the rows first brings its item's rows to their largest power.  Two parts then hold 22 bits of every
-// value down to 2^-17 of its row's (item's) largest, and 2^-39 of the largest below.
+// h and g (fp32 sums, T x R) as the second products' operands: PARTS planes of 16-bit values that add up to them.
+// bf16: three parts of eight bits each are the 24 bits of an fp32 value, exactly (two would lose its last eight).
+// fp16: two parts of eleven bits and the second one's sign, so 2^-22 of a value is lost at most.  fp16 has neither the values'
+// range (scale x x down reaches far beyond 65504) nor, below 2^-14, its own eleven bits (gradients of adapters that have just
+// begun to train are that small), so with SCALED a row is divided by a power of two that brings its largest finite value to
+// 2^14 .. 2^15, and the T powers stand behind the planes as floats.  A second product over the ranks multiplies its sums by
+// them; one over the rows first brings its item's rows to their largest power.  The 22 bits are there down to 2^-17 of a row's
+// (an item's) largest value; what is smaller is off by 2^-39 of the largest.
 template <typename T>
 struct Split {
-    static constexpr int PARTS = 2;
     static constexpr bool SCALED = std::is_same<T, __half>::value;
+    static constexpr int PARTS = SCALED ? 2 : 3;
 };
-__host__ __device__ inline int parts_of(int) { return 2; }
+__host__ __device__ inline int parts_of(int dtype) { return dtype == NB_DTYPE_FP16 ? 2 : 3; }
 inline bool scaled(int dtype) { return dtype == NB_DTYPE_FP16; }
 __host__ __device__ inline long long plane_bytes(int T, int R) { return (long long)T * R * 2; }
 
@@ -40,7 +42,8 @@ template <typename T>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[Split<T>::PARTS]) {
 #pragma unroll
     for (int i = 0; i < Split<T>::PARTS; ++i) {
-        part[i] = pack2<T>(x, y);
+        // bf16 takes the upper halves as they are: rounded, the largest fp32 values would be infinite
+        part[i] = Split<T>::SCALED ? pack2<T>(x, y) : __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
         const float2 back = unpack2<T>(part[i]);
         // (a value that is not finite is so in the first part alone)
         x = isfinite(back.x) ? x - back.x : 0.f;

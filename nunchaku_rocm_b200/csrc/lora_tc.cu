@@ -257,14 +257,14 @@ struct ExpandTc {
     static constexpr int GB = HALVES * 64 * 128, GST = RP <= 64 ? 2 : 3;
     static constexpr int SLOT = kTcRows * 128, SLOTS = RP <= 64 ? 3 : 5;
     static constexpr int OFF_G = PARTS * VB, OFF_S = OFF_G + GST * GB, OFF_BAR = OFF_S + SLOTS * SLOT;
-    static constexpr int BYTES = OFF_BAR + 256 + 1024;
+    static constexpr int BYTES = OFF_BAR + 256;  // (no room to align it by hand: 114944 bytes at rank 64, 115712 fit twice)
     static constexpr int THREADS = 352;
 };
+extern __shared__ __align__(1024) unsigned char expand_smem[];
 template <typename T, int RP, bool CCONTIG>
 __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_constant__ PartMaps<T> tm_v, const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_base,
                                                               const __grid_constant__ CUtensorMap tm_out, const LoraParams p) {
     using S = ExpandTc<T, RP>;
-    extern __shared__ unsigned char raw[];
     const Item it = find_item<S::THREADS>(p, blockIdx.y, p.rows_per_item);
     if (it.rows == 0) return;
     const int col0 = blockIdx.x * p.cols_per_cta, col1 = min(col0 + p.cols_per_cta, p.K);
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
         }
         return;
     }
-    uint8_t* smem = align1k(raw);
+    unsigned char* smem = expand_smem;
     const uint32_t sb = smem_u32(smem), bars = sb + S::OFF_BAR;
     auto bar = [&](int i) { return bars + 8u * i; };
     enum { V = 0, GF = 1, GE = GF + S::GST, DF = GE + S::GST, DE = DF + 2, LF = DE + 2, LE = LF + S::SLOTS, WF = LE + S::SLOTS, COUNT = WF + S::SLOTS };
@@ -441,8 +441,10 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
 template <typename T, int RP>
 struct OuterTc {
     static constexpr int HALVES = RP <= 64 ? 1 : 2, PARTS = Split<T>::PARTS;
-    static constexpr int TILE = KB * 128;  // 64 rows of 64 values
-    static constexpr int STAGE = (4 + PARTS * HALVES) * TILE, ST = RP <= 64 ? 4 : 3;
+    // rows of a stage: 64, or 32 where a stage of 64 is so large (80 KB) that two alone would fit
+    static constexpr int ROWS = PARTS * HALVES > 4 ? 32 : 64;
+    static constexpr int TILE = ROWS * 128;  // of 64 values
+    static constexpr int STAGE = (4 + PARTS * HALVES) * TILE, ST = ROWS == 32 ? 5 : RP <= 64 ? 4 : 3;
     static constexpr int OFF_BAR = ST * STAGE;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
     static constexpr int ACC = RP < 32 ? 32 : RP, COLS = 2 * ACC;  // tensor-memory columns: read 32 at a time
@@ -505,14 +507,14 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         if (warp == 1) tmem_dealloc(tmem, S::COLS);
         return;
     }
-    const int c0 = (blockIdx.x - (krows ? 0 : jobs.groups)) * kTcCols, n = (it.rows + KB - 1) / KB;
+    const int c0 = (blockIdx.x - (krows ? 0 : jobs.groups)) * kTcCols, n = (it.rows + S::ROWS - 1) / S::ROWS;
     const int quarters = min(4, (K - c0 + 63) / 64);  // tiles of 64 columns that exist
 
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
             for (int s = 0; s < n; ++s) {
-                const int st = s % S::ST, t0 = it.first + s * KB;
+                const int st = s % S::ST, t0 = it.first + s * S::ROWS;
                 if (s >= S::ST && !mbar_wait(empty(st), ((s / S::ST) & 1) ^ 1, abort_s, E_OUTER | 1, 50)) { ok = false; break; }
                 const uint32_t at = sb + st * S::STAGE;
                 mbar_expect_tx(full(st), (quarters + S::PARTS * S::HALVES) * S::TILE);
@@ -526,7 +528,7 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         const uint32_t idesc = umma_idesc(1u, Fmt<T>::value, Fmt<T>::value, p.R) | A_MN | B_MN;
         bool ok = true;
         for (int s = 0; s < n && ok; ++s) {
-            const int st = s % S::ST, rows = min(KB, it.rows - s * KB), k16 = (rows + 15) / 16;
+            const int st = s % S::ST, rows = min(S::ROWS, it.rows - s * S::ROWS), k16 = (rows + 15) / 16;
             const uint32_t at = sb + st * S::STAGE;
             if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_OUTER | 2)) { ok = false; break; }
             if (rows < k16 * 16) {  // rows behind the item's last one: zeros in every tile
@@ -557,6 +559,7 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         bool ok = true;
         if constexpr (SCALED) {
             // two threads have a row of a slot, each half of its 16-byte pieces
+            static_assert(S::ROWS == 64, "64 rows, 128 threads");
             const int t = threadIdx.x - 64, row = t >> 1;
             const float* powers = jobs.job[which].row_scale + it.first;
             int top = -126;
@@ -572,9 +575,9 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                 const int st = s % S::ST;
                 float a, b;
                 row_ratio(next, top, a, b);
-                if ((s + 1) * KB + row < it.rows) next = powers[(s + 1) * KB + row];
+                if ((s + 1) * S::ROWS + row < it.rows) next = powers[(s + 1) * S::ROWS + row];
                 if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_OUTER | 5)) { ok = false; break; }
-                if (s * KB + row < it.rows && a * b < 1.f) {
+                if (s * S::ROWS + row < it.rows && a * b < 1.f) {
                     const __half2 a2 = __float2half2_rn(a), b2 = __float2half2_rn(b);
                     const uint32_t at = sb + st * S::STAGE + 4 * S::TILE + row * 128 + (t & 1) * 64;
                     for (int tile = 0; tile < S::PARTS * S::HALVES; ++tile)
@@ -729,7 +732,7 @@ int outer(const LoraParams& p, OuterJobs j, cudaStream_t s) {
     int groups = 0;
     for (int i = 0; i < 2; ++i) {
         const OuterJob& o = j.job[j.job[i].K ? i : 1 - i];  // (a job that is not there has no CTAs; its maps are the other's)
-        if (!(make_map<T>(&m.x[i], o.x, p.T, o.K, o.stride_x, KB) && make_part_maps<T>(&m.v[i], o.v, p, KB))) return NB_ERR_UNSUPPORTED;
+        if (!(make_map<T>(&m.x[i], o.x, p.T, o.K, o.stride_x, S::ROWS) && make_part_maps<T>(&m.v[i], o.v, p, S::ROWS))) return NB_ERR_UNSUPPORTED;
         groups += ceil_div(j.job[i].K, kTcCols);
     }
     j.groups = ceil_div(j.job[0].K, kTcCols);

@@ -1,8 +1,8 @@
 """
 Batched adapters where the 16-bit types are narrow: h = s x D^T and g = s dy U far beyond and far below float16's own values.
 
-h and g are fp32 sums that the second products read in 16-bit parts: in float16 each row in two, after a power of two that
-brings its largest value below 2^15.  What that costs, and the tolerances count:
+h and g are fp32 sums that the second products read in 16-bit parts: bfloat16's three hold all of their 24 bits, float16's two
+follow a power of two that brings a row's largest value below 2^15.  What float16's cost, and the tolerances count:
 
 * 2^-22 of each value (half a step of 2^-11, twice);
 * 2^-39 of the row's largest (of the adapter's largest, where rows are summed): half of float16's smallest step, 2^-25, beside
@@ -26,7 +26,7 @@ gpu = pytest.mark.gpu
 def part(v, dim, dtype):
     """What the parts of `v` lose: rows (dim=-1) or all of an adapter's rows (dim=(0, 1)) share a power of two in float16."""
     if dtype == BF16:
-        return 2.0**-16 * v.abs()
+        return torch.zeros_like(v)
     return 2.0**-22 * v.abs() + 2.0**-39 * v.abs().amax(dim, keepdim=True)
 
 
@@ -160,5 +160,56 @@ def test_h_has_room_for_the_rows_powers():
     lib, a = L.lib(), L.LoraArgs(T=5, K=64, N=32, R=16, A=1, requests=1, dtype=1)  # float16
     rows = 5 * 16 * 2  # bytes of a part
     assert lib.nb_lora_h_bytes(a) >= 2 * rows + 5 * 4
+    assert lib.nb_lora_h_bytes(L.LoraArgs(T=5, K=64, N=32, R=16, A=1, requests=1, dtype=0)) >= 3 * rows
     a.R = 24
     assert lib.nb_lora_h_bytes(a) == 0  # refused sizes
+
+
+@gpu
+@pytest.mark.parametrize("impl", IMPLS.values(), ids=IMPLS)
+@pytest.mark.parametrize("R", [16, 32, 64, 128])
+@pytest.mark.parametrize("T", [2, 70, 300])
+def test_bfloat16_keeps_all_bits_of_h(cuda_dev, T, R, impl):
+    # two ranks (rows) whose first sixteen bits cancel: what is left is the last eight of h (g), exact in every step
+    K, N = 64, 96
+    off, ad = torch.tensor([0, T], dtype=torch.int32, device=cuda_dev), torch.tensor([0], dtype=torch.int32, device=cuda_dev)
+    z = lambda *s: torch.zeros(*s, dtype=BF16, device=cuda_dev)  # noqa: E731
+    digits, powers = (torch.tensor(v, dtype=BF16, device=cuda_dev) for v in ([0xAB, 0xCD, 0xEF], [2.0**16, 2.0**8, 1.0]))
+    upper = powers * torch.tensor([-1.0, -1.0, 0.0], dtype=BF16, device=cuda_dev)
+    x, down, up = z(T, K), z(1, R, K), z(1, N, R)
+    x[:, 8:11] = digits
+    down[0, 3, 8:11], down[0, R - 2, 8:11] = powers, upper  # h = 0xABCDEF and -0xABCD00
+    up[0, :, 3], up[0, :, R - 2] = 1.0, 1.0
+    assert (lora_batched(x, down, up, off, ad, _impl=impl) == 0xEF).all()
+    # g likewise through dy and up, read back by dx; and the sums over two rows
+    dy, up = z(T, N), z(1, N, R)
+    dy[:, 40:43] = digits
+    up[0, 40:43, 3], up[0, 40:43, R - 2] = powers, upper
+    down = z(1, R, K)
+    down[0, 3], down[0, R - 2] = 1.0, 1.0
+    leaves = [t.requires_grad_(True) for t in (z(T, K), down, up)]
+    (dx,) = torch.autograd.grad(lora_batched(*leaves, off, ad, _impl=impl), leaves[:1], dy)
+    assert (dx == 0xEF).all()
+    x, dy, down, up = z(T, K), z(T, N), z(1, R, K), z(1, N, R)
+    x[0, 8:11], x[T - 1, 8:11] = digits, digits * torch.tensor([-1.0, -1.0, 0.0], dtype=BF16, device=cuda_dev)
+    down[0, 5, 8:11] = powers
+    dy[0, 7], dy[T - 1, 7] = 1.0, 1.0
+    leaves = [t.requires_grad_(True) for t in (x, down, up)]
+    (dup,) = torch.autograd.grad(lora_batched(*leaves, off, ad, _impl=impl), leaves[2:], dy)
+    assert dup[0, 7, 5] == 0xEF and dup.count_nonzero() == 1
+    x, dy, down, up = z(T, K), z(T, N), z(1, R, K), z(1, N, R)
+    dy[0, 40:43], dy[T - 1, 40:43] = digits, digits * torch.tensor([-1.0, -1.0, 0.0], dtype=BF16, device=cuda_dev)
+    up[0, 40:43, 5] = powers
+    x[0, 9], x[T - 1, 9] = 1.0, 1.0
+    leaves = [t.requires_grad_(True) for t in (x, down, up)]
+    (ddown,) = torch.autograd.grad(lora_batched(*leaves, off, ad, _impl=impl), leaves[1:2], dy)
+    assert ddown[0, 5, 9] == 0xEF and ddown.count_nonzero() == 1
+
+
+@gpu
+@pytest.mark.parametrize("impl", IMPLS.values(), ids=IMPLS)
+@pytest.mark.parametrize("R", [16, 48, 64, 80, 128])
+@pytest.mark.parametrize("T,offsets,adapters", [(21, [0, 9, 21], [1, 0]), (700, [0, 330, 690], [0, 1])])
+def test_bfloat16_differs_by_fp32_roundings_alone(cuda_dev, R, T, offsets, adapters, impl):
+    p = make(cuda_dev, T, 328, 264, R, 2, BF16, up=0.1, seed=R)
+    check(p, offsets, adapters, impl)
