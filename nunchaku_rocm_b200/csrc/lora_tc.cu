@@ -7,6 +7,11 @@
 // us for both factors (4.6 TB/s): about 8 us of each are its start and its end, the rest its bytes (outer's CTAs are of two
 // lengths, and end at different times).
 //
+// A tensor-memory accumulator is fp32, but each step into it TRUNCATES, the sum and (fp16, whose products have 22 bits) the
+// products that it takes: a long chain is biased towards zero (432 steps: 1.4e-5 of the sum; fp32 with rounding 1.7e-6).  The
+// long sums (shrink, outer) are therefore taken out of it every 32 to 48 steps and added up in registers, where additions
+// round, while the ring keeps the loads coming and a second accumulator takes the next steps.
+//
 // A tile is loaded whole even where its item has fewer rows: the rows behind belong to other requests (or are filled with
 // zeros behind the last row).  They are multiplied along and not stored; where rows are summed (outer) they are set to zero
 // in shared memory first.  Every mbarrier wait is bounded; on expiry the CTA records a code in the status word and unwinds.
@@ -92,8 +97,9 @@ struct ShrinkTc {
     static constexpr int PIPE = ST * STAGE, SUMS = kTcRows * LD * 4;
     static constexpr int OFF_BAR = PIPE > SUMS ? PIPE : SUMS;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
-    static constexpr int COLS = RP < 32 ? 32 : RP;
+    static constexpr int ACC = RP < 32 ? 32 : RP, COLS = 2 * ACC;  // two accumulators take turns
     static constexpr int THREADS = 192;
+    static constexpr int CHAIN = 8;  // steps of 64 of K into an accumulator before it is taken out
 };
 template <typename T, int RP, bool RCONTIG>
 __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_f,
@@ -105,8 +111,10 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
     const uint32_t base = smem_u32(smem), bars = base + S::OFF_BAR;
     auto full = [&](int i) { return bars + 8u * i; };
     auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
-    const uint32_t done = bars + 8u * (2 * S::ST);
-    static_assert(8 * (2 * S::ST + 1) <= 192, "barriers");
+    // an accumulator has a chain's sums / may be used again
+    auto done = [&](int b) { return bars + 8u * (2 * S::ST + b); };
+    auto taken = [&](int b) { return bars + 8u * (2 * S::ST + 2 + b); };
+    static_assert(8 * (2 * S::ST + 4) <= 192, "barriers");
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
     volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -118,7 +126,10 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
             mbar_init(full(i), 1);
             mbar_init(empty(i), 1);
         }
-        mbar_init(done, 1);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(done(b), 1);
+            mbar_init(taken(b), 4);
+        }
         *abort_s = 0;
         fence_barrier_init();
     }
@@ -165,39 +176,48 @@ __global__ void __launch_bounds__(192) lora_shrink_tc_kernel(const __grid_consta
         for (int s = 0; s < n && ok; ++s) {
             const int st = s % S::ST;
             if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_SHRINK | 2)) { ok = false; break; }
+            const int chain = s / S::CHAIN, b = chain & 1;
+            if (chain >= 2 && s % S::CHAIN == 0 && !mbar_wait_warp(taken(b), ((chain >> 1) - 1) & 1, abort_s, E_SHRINK | 4)) { ok = false; break; }
             tc_fence_after();
             if (elect_one()) {
                 const uint64_t a = desc_k(base + st * S::STAGE);
-                const uint64_t b = RCONTIG ? desc_mn(base + st * S::STAGE + S::XB, 64 * 128) : desc_k(base + st * S::STAGE + S::XB);
+                const uint64_t f = RCONTIG ? desc_mn(base + st * S::STAGE + S::XB, 64 * 128) : desc_k(base + st * S::STAGE + S::XB);
                 const int k16 = min(4, (p.K - (step0 + s) * KB + 15) / 16);
-                for (int k = 0; k < k16; ++k) mma_f16(tmem, a + k * 2, b + k * (RCONTIG ? 16 * 128 >> 4 : 2), idesc, (s || k) ? 1u : 0u);
+                for (int k = 0; k < k16; ++k) mma_f16(tmem + b * S::ACC, a + k * 2, f + k * (RCONTIG ? 16 * 128 >> 4 : 2), idesc, (s % S::CHAIN || k) ? 1u : 0u);
                 tc_commit(empty(st));
-                if (s == n - 1) tc_commit(done);
+                if (s == n - 1 || s % S::CHAIN == S::CHAIN - 1) tc_commit(done(b));
             }
             __syncwarp();
         }
     }
     const float scale = p.scale ? __ldg(p.scale + it.adapter) : 1.f;
     float* sums = reinterpret_cast<float*>(smem);
-    bool ok = true;
     if (warp >= 2) {
+        bool ok = true;
         const int row = (warp & 3) * 32 + lane;
-        if (n > 0) ok = mbar_wait_warp(done, 0, abort_s, E_SHRINK | 3);
-        tc_fence_after();
-        for (int c = 0; c < RP && ok; c += 32) {
-            float v[32];
-            if (n > 0) {
-                tmem_ld32(tmem + ((warp & 3) * 32 << 16) + c, v);
+        float total[RP] = {};
+        for (int s = 0, chain = 0; s < n && ok; s += S::CHAIN, ++chain) {
+            ok = mbar_wait_warp(done(chain & 1), (chain >> 1) & 1, abort_s, E_SHRINK | 3);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < RP; c += 32) {
+                float v[32];
+                tmem_ld32(tmem + ((warp & 3) * 32 << 16) + (chain & 1) * S::ACC + c, v);
                 tmem_wait_ld();
-            } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                for (int i = 0; i < (RP < 32 ? RP : 32); ++i) total[c + i] += v[i];
             }
-#pragma unroll
-            for (int i = 0; i < (RP < 32 ? RP : 32); i += 4)
-                *reinterpret_cast<float4*>(sums + row * S::LD + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(taken(chain & 1));
+            __syncwarp();
         }
-        tc_fence_before();
+        if (ok) {
+#pragma unroll
+            for (int i = 0; i < RP; i += 4)
+                *reinterpret_cast<float4*>(sums + row * S::LD + i) = make_float4(total[i], total[i + 1], total[i + 2], total[i + 3]);
+        }
     }
     __syncthreads();
     cg::cluster_group cluster = cg::this_cluster();
@@ -436,8 +456,8 @@ __global__ void __launch_bounds__(352) lora_expand_tc_kernel(const __grid_consta
 // part[item][r, k] (job 1; [k, r] for job 0) = sum over the item's rows of v[t, r] X[t, k], 256 columns of X per CTA
 // (two accumulators of 128: v comes from the L2 cache once for both, 16 KB beside 32 KB of X at rank 64; with 128
 // columns the cache delivered as much of it as HBM of X).  Both operands run along the rows (MN-major), so they are used
-// as they lie; where the rows have powers of two, the four warps that read the sums later bring the rows of v to the item's
-// power in shared memory before they are multiplied.
+// as they lie.  Warps: TMA producer, MMA issuer, eight for the sums (four for each accumulator); where the rows have powers of
+// two, these bring the rows of v to the item's power in shared memory before they are multiplied.
 template <typename T, int RP>
 struct OuterTc {
     static constexpr int HALVES = RP <= 64 ? 1 : 2, PARTS = Split<T>::PARTS;
@@ -447,8 +467,10 @@ struct OuterTc {
     static constexpr int STAGE = (4 + PARTS * HALVES) * TILE, ST = ROWS == 32 ? 5 : RP <= 64 ? 4 : 3;
     static constexpr int OFF_BAR = ST * STAGE;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
-    static constexpr int ACC = RP < 32 ? 32 : RP, COLS = 2 * ACC;  // tensor-memory columns: read 32 at a time
-    static constexpr int THREADS = 192;
+    // tensor-memory columns, read 32 at a time: two accumulators, and up to rank 64 two pairs that take turns
+    static constexpr int ACC = RP < 32 ? 32 : RP, BUF = RP <= 64 ? 2 : 1, COLS = 2 * ACC * BUF;
+    static constexpr int THREADS = 320;
+    static constexpr int CHAIN = 256 / ROWS;  // stages into the accumulators before they are taken out
 };
 template <typename T>
 struct OuterMaps {
@@ -456,7 +478,7 @@ struct OuterMaps {
     PartMaps<T> v[2];
 };
 template <typename T, int RP>
-__global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constant__ OuterMaps<T> maps, const LoraParams p,
+__global__ void __launch_bounds__(320) lora_outer_tc_kernel(const __grid_constant__ OuterMaps<T> maps, const LoraParams p,
                                                             const __grid_constant__ OuterJobs jobs) {
     using S = OuterTc<T, RP>;
     constexpr bool SCALED = Split<T>::SCALED;
@@ -471,8 +493,9 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
     auto full = [&](int i) { return bars + 8u * i; };
     auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
     auto level = [&](int i) { return bars + 8u * (2 * S::ST + i); };  // a slot's rows of v have the item's power
-    const uint32_t done = bars + 8u * (3 * S::ST);
-    static_assert(8 * (3 * S::ST + 1) <= 192, "barriers");
+    auto done = [&](int b) { return bars + 8u * (3 * S::ST + b); };  // (as in shrink)
+    auto taken = [&](int b) { return bars + 8u * (3 * S::ST + S::BUF + b); };
+    static_assert(8 * (3 * S::ST + 2 * S::BUF) <= 192, "barriers");
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
     volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
     int* tops = reinterpret_cast<int*>(smem + S::OFF_BAR + 208);
@@ -484,9 +507,12 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
         for (int i = 0; i < S::ST; ++i) {
             mbar_init(full(i), 1);
             mbar_init(empty(i), 1);
-            mbar_init(level(i), 4);
+            mbar_init(level(i), 8);
         }
-        mbar_init(done, 1);
+        for (int b = 0; b < S::BUF; ++b) {
+            mbar_init(done(b), 1);
+            mbar_init(taken(b), 8);
+        }
         *abort_s = 0;
         fence_barrier_init();
     }
@@ -538,6 +564,8 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                 fence_proxy_async_smem();
                 __syncwarp();
             }
+            const int chain = s / S::CHAIN, b = chain % S::BUF;
+            if (chain >= S::BUF && s % S::CHAIN == 0 && !mbar_wait_warp(taken(b), (chain / S::BUF - 1) & 1, abort_s, E_OUTER | 6)) { ok = false; break; }
             if (SCALED && !mbar_wait_warp(level(st), (s / S::ST) & 1, abort_s, E_OUTER | 4)) { ok = false; break; }
             tc_fence_after();
             if (elect_one()) {
@@ -545,33 +573,35 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                     for (int h = 0; 2 * h < quarters; ++h) {
                         const uint64_t a = desc_mn(at + 2 * h * S::TILE + k * 16 * 128, S::TILE);
                         for (int v = 0; v < S::PARTS; ++v)
-                            mma_f16(tmem + h * S::ACC, a, desc_mn(at + (4 + v * S::HALVES) * S::TILE + k * 16 * 128, S::TILE), idesc, (s || k || v) ? 1u : 0u);
+                            mma_f16(tmem + (2 * b + h) * S::ACC, a, desc_mn(at + (4 + v * S::HALVES) * S::TILE + k * 16 * 128, S::TILE), idesc, (s % S::CHAIN || k || v) ? 1u : 0u);
                     }
                 tc_commit(empty(st));
-                if (s == n - 1) tc_commit(done);
+                if (s == n - 1 || s % S::CHAIN == S::CHAIN - 1) tc_commit(done(b));
             }
             __syncwarp();
         }
     } else {
-        const int q = warp & 3;
+        const int q = warp & 3, h = (warp - 2) >> 2;
         float* part = jobs.job[which].part + (long long)w * p.R * K;
-        float up = 1.f;
+        const float* powers = jobs.job[which].row_scale + it.first;
+        // four threads have a row of a slot, each two of its eight 16-byte pieces
+        const int t = threadIdx.x - 64, row = t >> 2;
+        int top = 0;
+        float next = 1.f, total[RP] = {};
         bool ok = true;
         if constexpr (SCALED) {
-            // two threads have a row of a slot, each half of its 16-byte pieces
-            static_assert(S::ROWS == 64, "64 rows, 128 threads");
-            const int t = threadIdx.x - 64, row = t >> 1;
-            const float* powers = jobs.job[which].row_scale + it.first;
-            int top = -126;
+            static_assert(S::ROWS == 64, "64 rows, 256 threads");
+            top = -126;
 #pragma unroll 4
-            for (int r = t; r < it.rows; r += 128) top = max(top, (int)(__float_as_uint(powers[r]) >> 23) - 127);
+            for (int r = t; r < it.rows; r += 256) top = max(top, (int)(__float_as_uint(powers[r]) >> 23) - 127);
             top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) tops[q] = top;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            for (int i = 0; i < 4; ++i) top = max(top, tops[i]);
-            up = exp2_of(top);
-            float next = row < it.rows ? powers[row] : up;
-            for (int s = 0; s < n && ok; ++s) {
+            if (lane == 0) tops[warp - 2] = top;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
+            if (row < it.rows) next = powers[row];
+        }
+        for (int s = 0; s < n; ++s) {
+            if constexpr (SCALED) {
                 const int st = s % S::ST;
                 float a, b;
                 row_ratio(next, top, a, b);
@@ -579,18 +609,18 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                 if (!mbar_wait_warp(full(st), (s / S::ST) & 1, abort_s, E_OUTER | 5)) { ok = false; break; }
                 if (s * S::ROWS + row < it.rows && a * b < 1.f) {
                     const __half2 a2 = __float2half2_rn(a), b2 = __float2half2_rn(b);
-                    const uint32_t at = sb + st * S::STAGE + 4 * S::TILE + row * 128 + (t & 1) * 64;
+                    const uint32_t at = sb + st * S::STAGE + 4 * S::TILE + row * 128 + (t & 3) * 32;
                     for (int tile = 0; tile < S::PARTS * S::HALVES; ++tile)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
+                        for (int c = 0; c < 2; ++c) {
                             uint32_t v[4];
                             const uint32_t to = at + tile * S::TILE + c * 16;
                             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(to) : "memory");
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                __half2 h = *reinterpret_cast<__half2*>(&v[j]);
-                                h = __hmul2(__hmul2(h, a2), b2);
-                                v[j] = *reinterpret_cast<uint32_t*>(&h);
+                                __half2 x2 = *reinterpret_cast<__half2*>(&v[j]);
+                                x2 = __hmul2(__hmul2(x2, a2), b2);
+                                v[j] = *reinterpret_cast<uint32_t*>(&x2);
                             }
                             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
                         }
@@ -598,38 +628,46 @@ __global__ void __launch_bounds__(192) lora_outer_tc_kernel(const __grid_constan
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(level(st));
+                __syncwarp();
             }
-        }
-        if (ok && mbar_wait_warp(done, 0, abort_s, E_OUTER | 3)) {
+            if (s != n - 1 && s % S::CHAIN != S::CHAIN - 1) continue;
+            const int chain = s / S::CHAIN, b = chain % S::BUF;
+            if (!mbar_wait_warp(done(b), (chain / S::BUF) & 1, abort_s, E_OUTER | 3)) { ok = false; break; }
             tc_fence_after();
-            for (int h = 0; 2 * h < quarters; ++h) {
-                const int k = c0 + h * 128 + q * 32 + lane;
-                for (int c = 0; c < p.R; c += 32) {
+            if (2 * h < quarters) {
+#pragma unroll
+                for (int c = 0; c < RP; c += 32) {
                     float v[32];
-                    tmem_ld32(tmem + (q * 32 << 16) + h * S::ACC + c, v);
+                    tmem_ld32(tmem + (q * 32 << 16) + (2 * b + h) * S::ACC + c, v);
                     tmem_wait_ld();
-                    if constexpr (SCALED) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= up;
-                    }
-                    if (k < K) {
-                        const int left = p.R - c;  // 16 or more
-                        if (krows) {
-                            float* to = part + (long long)k * p.R + c;
-#pragma unroll
-                            for (int i = 0; i < 32; i += 8)
-                                if (i < left)
-                                    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + i), "f"(v[i]), "f"(v[i + 1]),
-                                                 "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7]) : "memory");
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i < left) part[(long long)(c + i) * K + k] = v[i];
-                        }
-                    }
+                    for (int i = 0; i < (RP < 32 ? RP : 32); ++i) total[c + i] += v[i];
                 }
             }
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(taken(b));
+            __syncwarp();
+        }
+        const int k = c0 + h * 128 + q * 32 + lane;
+        if (ok && 2 * h < quarters && k < K) {
+            if constexpr (SCALED) {
+                const float up = exp2_of(top);
+#pragma unroll
+                for (int i = 0; i < RP; ++i) total[i] *= up;
+            }
+            if (krows) {
+                float* to = part + (long long)k * p.R;
+#pragma unroll
+                for (int i = 0; i < RP; i += 8)
+                    if (i < p.R)
+                        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + i), "f"(total[i]), "f"(total[i + 1]),
+                                     "f"(total[i + 2]), "f"(total[i + 3]), "f"(total[i + 4]), "f"(total[i + 5]), "f"(total[i + 6]), "f"(total[i + 7]) : "memory");
+            } else {
+#pragma unroll
+                for (int i = 0; i < RP; ++i)
+                    if (i < p.R) part[(long long)i * K + k] = total[i];
+            }
         }
     }
     __syncthreads();

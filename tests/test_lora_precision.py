@@ -213,3 +213,49 @@ def test_bfloat16_keeps_all_bits_of_h(cuda_dev, T, R, impl):
 def test_bfloat16_differs_by_fp32_roundings_alone(cuda_dev, R, T, offsets, adapters, impl):
     p = make(cuda_dev, T, 328, 264, R, 2, BF16, up=0.1, seed=R)
     check(p, offsets, adapters, impl)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_long_contractions_do_not_drift(cuda_dev, dtype):
+    # the tensor cores' accumulators truncate: sums of one sign fall short by up to 2^-23 of what is there in each step.  A chain
+    # of 64 steps loses at most sum(i / 64) = 32.5 of those, a product of 16 terms is rounded once (2 more allowed), and the
+    # nine chains are added with rounding.  One chain of 576 steps loses some 1.5e-5.
+    T, K, N, R = 9600, 9216, 64, 64
+    g = torch.Generator(device=cuda_dev).manual_seed(0)
+    x, down = (torch.rand(s, generator=g, device=cuda_dev).add_(0.5).to(dtype) for s in ((T, K), (1, R, K)))
+    up, out = torch.zeros(1, N, R, dtype=dtype, device=cuda_dev), torch.empty(T, N, dtype=dtype, device=cuda_dev)
+    off, ad = torch.tensor([0, T], dtype=torch.int32, device=cuda_dev), torch.zeros(1, dtype=torch.int32, device=cuda_dev)
+    parts = 2 if dtype == FP16 else 3
+    a = L.LoraArgs(T=T, K=K, N=N, R=R, A=1, requests=1, dtype=1 if dtype == FP16 else 0, stride_x=K, stride_out=N,
+                   **{n: t.data_ptr() for n, t in (("x", x), ("down", down), ("up", up), ("offsets", off), ("adapters", ad), ("out", out))})
+    h = torch.empty(L.lib().nb_lora_h_bytes(a), dtype=torch.uint8, device=cuda_dev)
+    a.h = h.data_ptr()
+    assert L.lib().nb_lora_forward(a, L.stream_of(x)) == L.NB_OK
+    value = h[: parts * T * R * 2].view(dtype).view(parts, T, R).double().sum(0)
+    if dtype == FP16:
+        value = value * h[parts * T * R * 2 :].view(torch.float32)[:T].double()[:, None]
+    want = x.double() @ down[0].double().t()
+    assert ((value - want).abs() / want).max() <= 35 * 2.0**-23 + 16 * F32 + (0 if dtype == BF16 else 2.0**-22)
+
+
+@gpu
+@pytest.mark.parametrize("impl", [L.IMPL_TCGEN05, L.IMPL_AUTO])
+def test_long_sums_over_rows_do_not_drift(cuda_dev, impl):
+    # all rows but the last three add up with one sign, and these take the sum off again up to its last bit, so that the error of
+    # a sum of 9213 terms is what is left.  Chains of 16 steps of each of h's parts: sum(i / 48) = 24.5 truncations of 2^-23, nine
+    # more where the sum is taken off, and some twenty rounded additions; one chain of 432 steps loses some 1.3e-5.
+    T, K, N, R = 9216, 64, 9216, 64
+    off, ad = torch.tensor([0, T], dtype=torch.int32, device=cuda_dev), torch.zeros(1, dtype=torch.int32, device=cuda_dev)
+    x, down = torch.zeros(T, K, dtype=BF16, device=cuda_dev), torch.zeros(1, R, K, dtype=BF16, device=cuda_dev)
+    x[:, 8:11], down[0, 3, 8:11] = torch.tensor([0xAB, 0xCD, 0xEF]), torch.tensor([2.0**16, 2.0**8, 1.0])  # h = 0xABCDEF
+    up = torch.zeros(1, N, R, dtype=BF16, device=cuda_dev, requires_grad=True)
+    dy = torch.rand(T, N, generator=torch.Generator(device=cuda_dev).manual_seed(0), device=cuda_dev).add_(0.5).to(BF16)
+    total = dy[:-3].sum(0, dtype=torch.float64)
+    left = total.clone()
+    for t in (T - 3, T - 2, T - 1):
+        dy[t] = -left.to(BF16)
+        left += dy[t].double()
+    (dup,) = torch.autograd.grad(lora_batched(x, down, up, off, ad, _impl=impl), up, dy)
+    off_by = (dup[0, :, 3].double() - left * 0xABCDEF).abs() / (total * 0xABCDEF)
+    assert off_by.max() <= 34 * 2.0**-23 + 20 * F32
