@@ -352,12 +352,14 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const LoraParams 
                         const int n = q * 32 + (i >> 1) * 8 + j * 2 + (i & 1);
                         ldsm4(b[h], smem_u32(gs) + n * S::GROW + (n >> 3) * 32 + k * 32 + ((lane >> 3) & 1) * 16);
                     }
+                }
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part) {
+                for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
                         mma16816<T>(acc[2 * h], v[part][k], b[h][0], b[h][1]);
                         mma16816<T>(acc[2 * h + 1], v[part][k], b[h][2], b[h][3]);
                     }
-                }
             }
             auto joined = [&](const uint4& b, int o) {
                 const uint32_t in[4] = {b.x, b.y, b.z, b.w};
@@ -580,15 +582,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_per_sm(R)) lora_few_kernel
             if (blk >= blocks) break;
             float o[4][4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // column n of tile j; behind the last column: some other row of U, whose result is not stored
-                const int row = min(blk * 32 + (g >> 1) * 8 + j * 2 + (g & 1), ncols - 1);
+            for (int s = 0; s < R / 16; ++s) {
+                uint2 b[4];
 #pragma unroll
-                for (int s = 0; s < R / 16; ++s) {
-                    const uint2 b = *reinterpret_cast<const uint2*>(us + S::piece(row, s * 2 + (t >> 1)) * 16 + (t & 1) * 8);
-#pragma unroll
-                    for (int v = 0; v < PARTS; ++v) mma16816<T>(o[j], a[v][s], b.x, b.y);
+                for (int j = 0; j < 4; ++j) {
+                    // column n of tile j; behind the last column: some other row of U, whose result is not stored
+                    const int row = min(blk * 32 + (g >> 1) * 8 + j * 2 + (g & 1), ncols - 1);
+                    b[j] = *reinterpret_cast<const uint2*>(us + S::piece(row, s * 2 + (t >> 1)) * 16 + (t & 1) * 8);
                 }
+#pragma unroll
+                for (int v = 0; v < PARTS; ++v)  // (neighbouring instructions do not wait for one another)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma16816<T>(o[j], a[v][s], b[j].x, b[j].y);
             }
             auto joined = [&](const uint4& b, int at) {
                 const uint32_t in[4] = {b.x, b.y, b.z, b.w};

@@ -467,10 +467,12 @@ struct OuterTc {
     static constexpr int STAGE = (4 + PARTS * HALVES) * TILE, ST = ROWS == 32 ? 5 : RP <= 64 ? 4 : 3;
     static constexpr int OFF_BAR = ST * STAGE;
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
-    // tensor-memory columns, read 32 at a time: two accumulators, and up to rank 64 two pairs that take turns
-    static constexpr int ACC = RP < 32 ? 32 : RP, BUF = RP <= 64 ? 2 : 1, COLS = 2 * ACC * BUF;
+    // Up to rank 64 the parts of v are one operand, 64 columns each: X is read from shared memory once for all (one at a time,
+    // three parts of rank 64 read 144 KB for a stage of 56), and the small parts do not meet the truncation of the large.
+    static constexpr bool WIDE = RP <= 64;
+    static constexpr int ACC = WIDE ? PARTS * 64 : RP, COLS = 2 * ACC <= 256 ? 256 : 512;  // tensor-memory columns: two accumulators
     static constexpr int THREADS = 320;
-    static constexpr int CHAIN = 256 / ROWS;  // stages into the accumulators before they are taken out
+    static constexpr int CHAIN = (WIDE ? 512 : 256) / ROWS;  // stages into the accumulators before they are taken out
 };
 template <typename T>
 struct OuterMaps {
@@ -493,9 +495,8 @@ __global__ void __launch_bounds__(320) lora_outer_tc_kernel(const __grid_constan
     auto full = [&](int i) { return bars + 8u * i; };
     auto empty = [&](int i) { return bars + 8u * (S::ST + i); };
     auto level = [&](int i) { return bars + 8u * (2 * S::ST + i); };  // a slot's rows of v have the item's power
-    auto done = [&](int b) { return bars + 8u * (3 * S::ST + b); };  // (as in shrink)
-    auto taken = [&](int b) { return bars + 8u * (3 * S::ST + S::BUF + b); };
-    static_assert(8 * (3 * S::ST + 2 * S::BUF) <= 192, "barriers");
+    const uint32_t done = bars + 8u * (3 * S::ST), taken = done + 8;  // (as in shrink)
+    static_assert(8 * (3 * S::ST + 2) <= 192, "barriers");
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + S::OFF_BAR + 192);
     volatile int* abort_s = reinterpret_cast<volatile int*>(smem + S::OFF_BAR + 200);
     int* tops = reinterpret_cast<int*>(smem + S::OFF_BAR + 208);
@@ -509,10 +510,8 @@ __global__ void __launch_bounds__(320) lora_outer_tc_kernel(const __grid_constan
             mbar_init(empty(i), 1);
             mbar_init(level(i), 8);
         }
-        for (int b = 0; b < S::BUF; ++b) {
-            mbar_init(done(b), 1);
-            mbar_init(taken(b), 8);
-        }
+        mbar_init(done, 1);
+        mbar_init(taken, 8);
         *abort_s = 0;
         fence_barrier_init();
     }
@@ -551,7 +550,7 @@ __global__ void __launch_bounds__(320) lora_outer_tc_kernel(const __grid_constan
             if (!ok) let_copies_land();
         }
     } else if (warp == 1) {
-        const uint32_t idesc = umma_idesc(1u, Fmt<T>::value, Fmt<T>::value, p.R) | A_MN | B_MN;
+        const uint32_t idesc = umma_idesc(1u, Fmt<T>::value, Fmt<T>::value, S::WIDE ? S::ACC : p.R) | A_MN | B_MN;
         bool ok = true;
         for (int s = 0; s < n && ok; ++s) {
             const int st = s % S::ST, rows = min(S::ROWS, it.rows - s * S::ROWS), k16 = (rows + 15) / 16;
@@ -564,19 +563,18 @@ __global__ void __launch_bounds__(320) lora_outer_tc_kernel(const __grid_constan
                 fence_proxy_async_smem();
                 __syncwarp();
             }
-            const int chain = s / S::CHAIN, b = chain % S::BUF;
-            if (chain >= S::BUF && s % S::CHAIN == 0 && !mbar_wait_warp(taken(b), (chain / S::BUF - 1) & 1, abort_s, E_OUTER | 6)) { ok = false; break; }
+            if (s && s % S::CHAIN == 0 && !mbar_wait_warp(taken, (s / S::CHAIN - 1) & 1, abort_s, E_OUTER | 6)) { ok = false; break; }
             if (SCALED && !mbar_wait_warp(level(st), (s / S::ST) & 1, abort_s, E_OUTER | 4)) { ok = false; break; }
             tc_fence_after();
             if (elect_one()) {
                 for (int k = 0; k < k16; ++k)
                     for (int h = 0; 2 * h < quarters; ++h) {
                         const uint64_t a = desc_mn(at + 2 * h * S::TILE + k * 16 * 128, S::TILE);
-                        for (int v = 0; v < S::PARTS; ++v)
-                            mma_f16(tmem + (2 * b + h) * S::ACC, a, desc_mn(at + (4 + v * S::HALVES) * S::TILE + k * 16 * 128, S::TILE), idesc, (s % S::CHAIN || k || v) ? 1u : 0u);
+                        for (int v = 0; v < (S::WIDE ? 1 : S::PARTS); ++v)
+                            mma_f16(tmem + h * S::ACC, a, desc_mn(at + (4 + v * S::HALVES) * S::TILE + k * 16 * 128, S::TILE), idesc, (s % S::CHAIN || k || v) ? 1u : 0u);
                     }
                 tc_commit(empty(st));
-                if (s == n - 1 || s % S::CHAIN == S::CHAIN - 1) tc_commit(done(b));
+                if (s == n - 1 || s % S::CHAIN == S::CHAIN - 1) tc_commit(done);
             }
             __syncwarp();
         }
@@ -631,22 +629,23 @@ __global__ void __launch_bounds__(320) lora_outer_tc_kernel(const __grid_constan
                 __syncwarp();
             }
             if (s != n - 1 && s % S::CHAIN != S::CHAIN - 1) continue;
-            const int chain = s / S::CHAIN, b = chain % S::BUF;
-            if (!mbar_wait_warp(done(b), (chain / S::BUF) & 1, abort_s, E_OUTER | 3)) { ok = false; break; }
+            if (!mbar_wait_warp(done, (s / S::CHAIN) & 1, abort_s, E_OUTER | 3)) { ok = false; break; }
             tc_fence_after();
             if (2 * h < quarters) {
 #pragma unroll
-                for (int c = 0; c < RP; c += 32) {
-                    float v[32];
-                    tmem_ld32(tmem + (q * 32 << 16) + (2 * b + h) * S::ACC + c, v);
-                    tmem_wait_ld();
+                for (int part = S::WIDE ? S::PARTS - 1 : 0; part >= 0; --part)  // the smallest first
 #pragma unroll
-                    for (int i = 0; i < (RP < 32 ? RP : 32); ++i) total[c + i] += v[i];
-                }
+                    for (int c = 0; c < RP; c += 32) {
+                        float v[32];
+                        tmem_ld32(tmem + (q * 32 << 16) + h * S::ACC + part * 64 + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < (RP < 32 ? RP : 32); ++i) total[c + i] += v[i];
+                    }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(taken(b));
+            if (lane == 0) mbar_arrive(taken);
             __syncwarp();
         }
         const int k = c0 + h * 128 + q * 32 + lane;

@@ -243,8 +243,8 @@ def test_long_contractions_do_not_drift(cuda_dev, dtype):
 @pytest.mark.parametrize("impl", [L.IMPL_TCGEN05, L.IMPL_AUTO])
 def test_long_sums_over_rows_do_not_drift(cuda_dev, impl):
     # all rows but the last three add up with one sign, and these take the sum off again up to its last bit, so that the error of
-    # a sum of 9213 terms is what is left.  Chains of 16 steps of each of h's parts: sum(i / 48) = 24.5 truncations of 2^-23, nine
-    # more where the sum is taken off, and some twenty rounded additions; one chain of 432 steps loses some 1.3e-5.
+    # a sum of 9213 terms is what is left.  Chains of at most 48 steps: sum(i / 48) = 24.5 truncations of 2^-23, nine more where
+    # the sum is taken off, and some twenty rounded additions; one chain of 432 steps loses some 1.3e-5.
     T, K, N, R = 9216, 64, 9216, 64
     off, ad = torch.tensor([0, T], dtype=torch.int32, device=cuda_dev), torch.zeros(1, dtype=torch.int32, device=cuda_dev)
     x, down = torch.zeros(T, K, dtype=BF16, device=cuda_dev), torch.zeros(1, R, K, dtype=BF16, device=cuda_dev)
