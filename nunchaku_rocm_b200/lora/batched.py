@@ -99,17 +99,27 @@ def has_lora_batch(module: nn.Module) -> bool:
 
 
 def _stack_on(module: nn.Module, x: torch.Tensor):
-    """The module's stack and scale where ``x`` is and in its dtype (the module may have moved after the attachment)."""
+    """
+    The module's stack and scale where ``x`` is and in its dtype (the module may have moved after the attachment).  A stack
+    that was given as tensors is converted anew in every call: its owner may change it, by ways that leave no trace (a graph's
+    replay, ``.data``), and may train it.  One that was made at the attachment is nobody else's: its conversion takes its place,
+    and further ones start from what was attached.
+    """
     (down, up), scale = module._lora_stack, module._lora_stack_scale
-    if down.device == x.device and down.dtype == x.dtype:
+    if down.device == x.device and down.dtype == x.dtype and (scale is None or scale.device == x.device):
         return down, up, scale
+    made = getattr(module, "_lora_stack_made", None)
+    if made is not None and made[1] is module._lora_stack:
+        (down, up), scale = made[0], made[2]
     with torch.inference_mode(False):
-        down, up = down.to(x.device, x.dtype), up.to(x.device, x.dtype)
+        pair = tuple(t if t.device == x.device and t.dtype == x.dtype else t.to(x.device, x.dtype) for t in (down, up))
         scale = None if scale is None else scale.to(x.device)
-    trained = any(t.requires_grad for t in module._lora_stack)  # (each step converts the leaves anew)
-    if not trained and not (x.is_cuda and torch.cuda.is_current_stream_capturing()):
-        module._lora_stack, module._lora_stack_scale = (down, up), scale
-    return down, up, scale
+    keep = made is not None and made[1] is module._lora_stack and not any(t.requires_grad for t in made[0])
+    if keep and not (x.is_cuda and torch.cuda.is_current_stream_capturing()):
+        if x.is_cuda:  # later calls may come on other streams, which would not wait for this one
+            torch.cuda.current_stream(x.device).synchronize()
+        module._lora_stack, module._lora_stack_scale, module._lora_stack_made = pair, scale, (made[0], pair, made[2])
+    return *pair, scale
 
 
 def add_lora_batch(module: nn.Module, x: torch.Tensor, out: torch.Tensor, samples: int | None = None,
@@ -144,17 +154,16 @@ def _hook(module, args, kwargs, output):
 def attach_lora_batch(module: nn.Module, adapters, scale=None) -> None:
     """
     Give the layer a stack of adapters: ``adapters`` as in :func:`stack_loras`, or an already stacked ``(down, up)`` pair of
-    3-D tensors, which is used as it is (and may require gradients).  ``scale``: one float per adapter.  Replaces an earlier
-    stack; :func:`detach_lora_batch` removes it.  Ranks up to 128.
+    3-D tensors, which every call reads as they are then (an adapter may be replaced in place, and they may require
+    gradients); in the layer's 16-bit dtype and on its device, else every call converts them.  ``scale``: one float per adapter.
+    Replaces an earlier stack; :func:`detach_lora_batch` removes it.  Ranks up to 128.
     """
     svdq = _is_svdq(module)
     ref = module.proj_down if svdq else next((p for p in module.parameters() if p.is_floating_point()), None)
     if ref is None:
         raise ValueError(f"{type(module).__name__} has no floating-point parameter to take the LoRA dtype from")
-    if len(adapters) == 2 and all(isinstance(t, torch.Tensor) and t.dim() == 3 for t in adapters):
-        down, up = adapters
-    else:
-        down, up = stack_loras(adapters, ref.device, ref.dtype)
+    given = len(adapters) == 2 and all(isinstance(t, torch.Tensor) and t.dim() == 3 for t in adapters)
+    down, up = adapters if given else stack_loras(adapters, ref.device, ref.dtype)
     if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2] or down.shape[1] % RANK_GRANULARITY:
         raise ValueError(f"stacked factors must be (A, R, in) and (A, out, R), R a multiple of {RANK_GRANULARITY}; got {tuple(down.shape)} and {tuple(up.shape)}")
     if down.shape[1] > L.LORA_MAX_RANK:
@@ -168,6 +177,8 @@ def attach_lora_batch(module: nn.Module, adapters, scale=None) -> None:
             raise ValueError(f"scale must have one value for each of {down.shape[0]} adapters, got {tuple(scale.shape)}")
     detach_lora_batch(module)
     module._lora_stack, module._lora_stack_scale = (down, up), scale
+    if not given:  # (what was attached, what it was converted to)
+        module._lora_stack_made = (module._lora_stack, module._lora_stack, scale)
     if not svdq:  # (SVDQW4A4Linear and the fused operators look for the stack themselves)
         module._lora_stack_hook = module.register_forward_hook(_hook, with_kwargs=True)
 
@@ -177,6 +188,6 @@ def detach_lora_batch(module: nn.Module) -> None:
     if hasattr(module, "_lora_stack_hook"):
         module._lora_stack_hook.remove()
         del module._lora_stack_hook
-    for name in ("_lora_stack", "_lora_stack_scale"):
+    for name in ("_lora_stack", "_lora_stack_scale", "_lora_stack_made"):
         if hasattr(module, name):
             delattr(module, name)

@@ -1,0 +1,118 @@
+"""
+Stacks of adapters over time: what their owner changes is seen, conversions start from what was attached, and a layer that is
+recomputed in a backward pass uses the requests of its forward pass.
+"""
+
+import pytest
+import torch
+from torch import nn
+
+from nunchaku_rocm_b200.lora import attach_lora_batch, batched, detach_lora_batch, lora_requests, stack_loras
+
+gpu = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def factors(A, R, n_in, n_out, dtype, dev="cpu", seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(A, R, n_in, generator=g) * n_in**-0.5).to(dev, dtype), (torch.randn(A, n_out, R, generator=g) * 0.25).to(dev, dtype)
+
+
+# ------------------------------------------------------------------------------------------------------------ conversions
+@pytest.mark.parametrize("change", ["in place", "data", "trained later"])
+def test_a_given_stack_is_read_in_every_call(change):
+    lin = nn.Linear(32, 24)
+    down, up = factors(2, 16, 32, 24, torch.float32)
+    attach_lora_batch(lin, (down, up), scale=[1.0, 0.5])
+    x = torch.zeros(3, 32, dtype=BF16)
+    first = batched._stack_on(lin, x)  # converted: the stack is float32
+    assert first[0].dtype == BF16 and torch.equal(first[0], down.to(BF16))
+    if change == "in place":
+        down.mul_(5)
+        up[1].zero_()
+    elif change == "data":
+        down.data.mul_(5)
+        up.data[1].zero_()
+    else:
+        down.requires_grad_(True)
+        up.requires_grad_(True)
+    d, u, scale = batched._stack_on(lin, x)
+    assert torch.equal(d, down.to(BF16)) and torch.equal(u, up.to(BF16)) and scale.tolist() == [1.0, 0.5]
+    if change == "trained later":
+        (d.float().sum() + u.float().sum()).backward()
+        assert (down.grad == 1).all() and (up.grad == 1).all()
+    assert lin._lora_stack[0] is down and lin._lora_stack[1] is up
+    # in the input's own dtype it is that very tensor
+    assert batched._stack_on(lin, x.float())[0] is down
+
+
+def test_conversions_start_from_what_was_attached():
+    lin = nn.Linear(32, 24)
+    g = torch.Generator().manual_seed(1)
+    attach_lora_batch(lin, [(torch.randn(16, 32, generator=g), torch.randn(24, 16, generator=g)) for _ in range(2)])
+    down, up = lin._lora_stack
+    for dtype in (BF16, FP16, torch.float32, torch.float64, FP16):
+        d, u, _ = batched._stack_on(lin, torch.zeros(1, 32, dtype=dtype))
+        assert torch.equal(d, down.to(dtype)) and torch.equal(u, up.to(dtype))
+        assert batched._stack_on(lin, torch.zeros(1, 32, dtype=dtype))[0] is d  # kept while the dtype stays
+    leaf = torch.randn(16, 32, requires_grad=True)
+    attach_lora_batch(lin, [(leaf, torch.randn(24, 16))])
+    with torch.no_grad():
+        batched._stack_on(lin, torch.zeros(1, 32, dtype=BF16))  # not kept: the next call may train
+    batched._stack_on(lin, torch.zeros(1, 32, dtype=BF16))[0].float().sum().backward()
+    assert (leaf.grad == 1).all()
+    detach_lora_batch(lin)
+    assert not hasattr(lin, "_lora_stack_made")
+
+
+@gpu
+def test_a_replayed_graph_reads_a_given_stack(cuda_dev):
+    lin = nn.Linear(64, 48, dtype=BF16, device=cuda_dev).requires_grad_(False)
+    down, up = factors(2, 16, 64, 48, torch.float32, cuda_dev)
+    attach_lora_batch(lin, (down, up))
+    ids = torch.tensor([1, 0], dtype=torch.int32, device=cuda_dev)
+    x = torch.randn(2, 9, 64, device=cuda_dev).to(BF16)
+    with lora_requests(ids):
+        lin(x)
+        graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s), torch.cuda.graph(graph, stream=s):
+            out = lin(x)
+        torch.cuda.current_stream().wait_stream(s)
+        for factor in (3.0, -0.5):
+            down.mul_(factor)
+            graph.replay()
+            want = lin(x)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    base = lin(x)
+    down.zero_()
+    with lora_requests(ids):
+        assert torch.equal(lin(x), base)
+
+
+@gpu
+def test_a_converted_stack_on_several_streams(cuda_dev):
+    x = torch.randn(2, 30, 64, device=cuda_dev).to(FP16)
+    ids = torch.tensor([1, 0], dtype=torch.int32, device=cuda_dev)
+    g = torch.Generator().manual_seed(2)
+    pairs = [(torch.randn(16, 64, generator=g) / 8, torch.randn(48, 16, generator=g) / 8) for _ in range(2)]
+    results = []
+    for _ in range(4):
+        lin = nn.Linear(64, 48, device=cuda_dev).requires_grad_(False)
+        attach_lora_batch(lin, pairs)  # float32, from the layer
+        lin.half().weight.zero_()
+        lin.bias.zero_()
+        torch.cuda.synchronize()
+        with lora_requests(ids):
+            for _ in range(3):
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    results.append(lin(x))
+    torch.cuda.synchronize()
+    down, up = stack_loras(pairs, cuda_dev, FP16)
+    want = torch.stack([(x[b].double() @ down[a].double().t()) @ up[a].double().t() for b, a in enumerate((1, 0))])
+    # fp32 sums of 64 and 16 terms, 2^-22 of h for its parts, one rounding of the result
+    terms = torch.stack([(x[b].double().abs() @ down[a].double().abs().t()) @ up[a].double().abs().t() for b, a in enumerate((1, 0))])
+    tol = (2.0**-24 * 90 + 2.0**-22) * terms
+    tol = tol + torch.finfo(FP16).eps / 2 * (want.abs() + tol) + 2.0**-25
+    assert all(torch.equal(r, results[0]) for r in results) and ((results[0].double() - want).abs() <= tol).all()
