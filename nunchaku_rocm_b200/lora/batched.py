@@ -28,9 +28,21 @@ from .. import _lib as L
 from ..ops.lora import lora_batched
 from .runtime import RANK_GRANULARITY, _is_svdq
 
-__all__ = ["add_lora_batch", "attach_lora_batch", "detach_lora_batch", "has_lora_batch", "lora_requests", "stack_loras"]
+__all__ = ["add_lora_batch", "attach_lora_batch", "detach_lora_batch", "has_lora_batch", "keep_lora_requests", "lora_requests",
+           "stack_loras"]
 
-_active = threading.local()
+
+class _Active(threading.local):
+    adapters = None  # of the innermost lora_requests
+    task = -1        # the backward pass that it was entered in, -1: none
+
+
+_active = _Active()
+
+
+def _task() -> int:
+    """The backward pass that runs on this thread, -1: none."""
+    return torch._C._current_graph_task_id()
 
 
 def stack_loras(adapters, device=None, dtype=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -62,20 +74,54 @@ def stack_loras(adapters, device=None, dtype=None) -> tuple[torch.Tensor, torch.
 
 
 @contextlib.contextmanager
+def _entered(adapters):
+    before = _active.adapters, _active.task
+    _active.adapters, _active.task = adapters, _task()
+    try:
+        yield
+    finally:
+        _active.adapters, _active.task = before
+
+
 def lora_requests(adapters: torch.Tensor):
     """
     While active (in this thread), sample ``b`` of every layer's input uses adapter ``adapters[b]`` of the layer's stack;
     -1 (any value outside the stack): none.  ``adapters (B,)`` int32 on the model's device.  It may be changed in place
     between the replays of a graph that was captured while it was active.
+
+    A function that is recomputed in a backward pass (``torch.utils.checkpoint``) runs on autograd's threads, after or
+    beside other requests: give it through :func:`keep_lora_requests`.  Without, its layers refuse to be recomputed.
     """
     if adapters.dtype != torch.int32 or adapters.dim() != 1:
         raise ValueError(f"adapters must be a 1-D int32 tensor, got {tuple(adapters.shape)} {adapters.dtype}")
-    before = getattr(_active, "adapters", None)
-    _active.adapters = adapters
-    try:
-        yield
-    finally:
-        _active.adapters = before
+    return _entered(adapters)
+
+
+def keep_lora_requests(fn):
+    """
+    ``fn``, run under the requests that are active now (or none) wherever and whenever it is called::
+
+        with lora_requests(ids):
+            y = checkpoint(keep_lora_requests(block), x, use_reentrant=False)
+        y.sum().backward()  # recomputes block with the adapters of ids
+
+    The adapters must not be changed in place in between.
+    """
+    adapters = _requests()
+    version = None if adapters is None or adapters.is_inference() else adapters._version
+
+    def run(*args, **kwargs):
+        if version is not None and adapters._version != version:
+            raise RuntimeError("the adapters of lora_requests were changed in place after keep_lora_requests")
+        with _entered(adapters):
+            return fn(*args, **kwargs)
+
+    return run
+
+
+def _requests():
+    """The active requests' adapters, or ``None``; in a backward pass only those that were entered in it count."""
+    return _active.adapters if _active.task == _task() else None
 
 
 @functools.lru_cache(maxsize=256)
@@ -95,7 +141,12 @@ def _offsets(samples, rows, device):
 
 def has_lora_batch(module: nn.Module) -> bool:
     """Whether ``module`` has a stack of adapters and requests are active that may use it."""
-    return getattr(module, "_lora_stack", None) is not None and getattr(_active, "adapters", None) is not None
+    if getattr(module, "_lora_stack", None) is None:
+        return False
+    if _active.task != _task() and (_active.adapters is not None or getattr(module, "_lora_stack_used", False)):
+        raise RuntimeError("a layer with adapters of several requests is recomputed in a backward pass, which does not know its "
+                           "requests: give the recomputed function through keep_lora_requests()")
+    return _requests() is not None
 
 
 def _stack_on(module: nn.Module, x: torch.Tensor):
@@ -130,7 +181,8 @@ def add_lora_batch(module: nn.Module, x: torch.Tensor, out: torch.Tensor, sample
     A quantised layer has gradients of its adapters but none of its input (its weight has no backward pass), and a ``fused``
     path, whose next kernels have no backward pass either, has none at all: both refuse to be asked.
     """
-    adapters = _active.adapters
+    adapters = _requests()
+    module._lora_stack_used = True
     samples = x.shape[0] if samples is None else samples
     if adapters.shape[0] != samples:
         raise ValueError(f"lora_requests has {adapters.shape[0]} samples, the layer's input {samples}")
@@ -188,6 +240,6 @@ def detach_lora_batch(module: nn.Module) -> None:
     if hasattr(module, "_lora_stack_hook"):
         module._lora_stack_hook.remove()
         del module._lora_stack_hook
-    for name in ("_lora_stack", "_lora_stack_scale", "_lora_stack_made"):
+    for name in ("_lora_stack", "_lora_stack_scale", "_lora_stack_made", "_lora_stack_used"):
         if hasattr(module, name):
             delattr(module, name)

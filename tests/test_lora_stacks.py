@@ -116,3 +116,107 @@ def test_a_converted_stack_on_several_streams(cuda_dev):
     tol = (2.0**-24 * 90 + 2.0**-22) * terms
     tol = tol + torch.finfo(FP16).eps / 2 * (want.abs() + tol) + 2.0**-25
     assert all(torch.equal(r, results[0]) for r in results) and ((results[0].double() - want).abs() <= tol).all()
+
+
+# ---------------------------------------------------------------------------------------------------------- recomputation
+def plain_lora(x, down, up, offsets, adapters, base=None, scale=None, out=None):
+    rows, y = x.reshape(-1, x.shape[-1]), []
+    for i, a in enumerate(adapters.tolist()):
+        r = rows[offsets[i] : offsets[i + 1]]
+        y.append((r @ down[a].t()) @ up[a].t() if 0 <= a < len(down) else r @ torch.zeros_like(down[0]).t() @ up[0].t())
+    y = torch.cat(y).view(*x.shape[:-1], -1)
+    return y if base is None else base + y
+
+
+def block(dev, dtype, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    lin = nn.Linear(32, 32, dtype=dtype, device=dev)
+    with torch.no_grad():
+        lin.weight.copy_(torch.randn(32, 32, generator=g) / 6)
+        lin.bias.zero_()
+    stack = tuple(t.requires_grad_(True) for t in factors(2, 16, 32, 32, dtype, dev, seed))
+    attach_lora_batch(lin.requires_grad_(False), stack)
+    return (lambda x: torch.tanh(lin(torch.tanh(x)))), lin, stack
+
+
+def recomputed(dev, dtype, reentrant, after, wrap):
+    """The gradients of x, down and up with and without torch.utils.checkpoint."""
+    from torch.utils.checkpoint import checkpoint
+
+    fn, _, stack = block(dev, dtype)
+    ids = torch.tensor([1, 0, -1], dtype=torch.int32, device=dev)
+    x = torch.randn(3, 5, 32, generator=torch.Generator().manual_seed(4)).to(dev, dtype).requires_grad_(True)
+    dy = torch.randn(3, 5, 32, generator=torch.Generator().manual_seed(5)).to(dev, dtype)
+    grads = []
+    for run in (lambda: fn(x), lambda: checkpoint(wrap(fn), x, use_reentrant=reentrant)):
+        for t in (x, *stack):
+            t.grad = None
+        with lora_requests(ids):
+            y = run()
+            if not after:
+                y.backward(dy)
+        if after:
+            with lora_requests(ids.flip(0).contiguous()):  # another step's
+                y.backward(dy)
+        grads.append([t.grad for t in (x, *stack)])
+    return grads
+
+
+@pytest.mark.parametrize("after", [False, True])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_layers_use_their_requests_or_refuse(monkeypatch, reentrant, after):
+    from nunchaku_rocm_b200.lora import keep_lora_requests
+
+    monkeypatch.setattr(batched, "lora_batched", plain_lora)
+    want, got = recomputed("cpu", torch.float64, reentrant, after, keep_lora_requests)
+    assert all(g is not None and torch.equal(w, g) for w, g in zip(want, got)) and want[1].any()
+    with pytest.raises(RuntimeError, match="keep_lora_requests"):
+        recomputed("cpu", torch.float64, reentrant, after, lambda fn: fn)
+
+
+def test_kept_requests(monkeypatch):
+    from torch.utils.checkpoint import checkpoint
+
+    from nunchaku_rocm_b200.lora import keep_lora_requests
+
+    monkeypatch.setattr(batched, "lora_batched", plain_lora)
+    fn, lin, stack = block("cpu", torch.float64)
+    x = torch.randn(2, 4, 32, dtype=torch.float64, requires_grad=True)
+    ids = torch.tensor([0, 1], dtype=torch.int32)
+    # a layer that no requests have used yet may be recomputed as it is, and with none kept afterwards too
+    checkpoint(fn, x, use_reentrant=True).sum().backward()
+    want = x.grad.clone()
+    none = keep_lora_requests(fn)
+    with lora_requests(ids):
+        kept = keep_lora_requests(fn)
+        y = fn(x)
+        assert torch.equal(none(x), lin_only(lin, x))
+    assert torch.equal(kept(x), y) and torch.equal(fn(x), lin_only(lin, x))
+    x.grad = None
+    checkpoint(none, x, use_reentrant=True).sum().backward()
+    assert torch.equal(x.grad, want)
+    with pytest.raises(RuntimeError, match="keep_lora_requests"):
+        checkpoint(fn, x, use_reentrant=True).sum().backward()
+    ids.flip(0)
+    assert torch.equal(kept(x), y)
+    ids.copy_(ids.flip(0))
+    with pytest.raises(RuntimeError, match="in place"):
+        kept(x)
+    detach_lora_batch(lin)
+    checkpoint(fn, x, use_reentrant=True).sum().backward()  # without a stack there is nothing to know
+
+
+def lin_only(lin, x):
+    return torch.tanh(torch.nn.functional.linear(torch.tanh(x), lin.weight, lin.bias))
+
+
+@gpu
+@pytest.mark.parametrize("after", [False, True])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_on_the_gpu(cuda_dev, reentrant, after):
+    from nunchaku_rocm_b200.lora import keep_lora_requests
+
+    want, got = recomputed(cuda_dev, BF16, reentrant, after, keep_lora_requests)
+    assert all(g is not None and torch.equal(w, g) for w, g in zip(want, got)) and want[1].any()
+    with pytest.raises(RuntimeError, match="keep_lora_requests"):
+        recomputed(cuda_dev, BF16, reentrant, after, lambda fn: fn)
