@@ -97,6 +97,13 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_
 bool defined(const OptTensor& t) { return t.has_value() && t->defined(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && wants_grad(*t); }
+// A tensor with a tangent (forward-mode differentiation) would lose it here without a word.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename... Tensors>
+void refuse_tangents(const char* what, const Tensors&... tensors) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(tensors) || ...), what, " has no forward-mode derivative");
+}
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
@@ -264,6 +271,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, double add) {
     Tensor w = or_none(weight), b = or_none(bias);
     ln_prepare(x, w, b, add);
+    refuse_tangents("layer_norm", x, w, b);
     require_cuda(x, w, b);
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) return LayerNorm::apply(x, or_none(w), or_none(b), eps, add);
     const Tensor y = empty_of(x.sizes(), x);
@@ -373,6 +381,7 @@ py::object rotary_axes(const Tensor& q, const OptTensor& k, const Tensor& ids, c
     check_ids("rotary_axes", ids, ladder->l.n_axes, q.size(0), q.size(1));
     TORCH_CHECK_VALUE(2 * ladder->pairs() <= q.size(3), "the axes have ", 2 * ladder->pairs(), " channels, more than a head (", q.size(3), ")");
     TORCH_CHECK_VALUE(q.size(2) > 0 && (!defined(k) || k->size(2) > 0), "no heads");
+    refuse_tangents("rotary_axes", q, k, ids);
     require_cuda(q, or_none(k), ids);
     const bool graph = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k));
     const variable_list out = graph ? Rotary::apply(q, k, ids, ladder, half, inverse) : rotate(q, or_none(k), ids, *ladder, half, inverse);
@@ -381,6 +390,7 @@ py::object rotary_axes(const Tensor& q, const OptTensor& k, const Tensor& ids, c
 Tensor rotary_table(const Tensor& ids, const LadderPtr& ladder) {
     TORCH_CHECK_VALUE(ids.dim() == 2 || ids.dim() == 3, "ids must be (S, axes) or (B, S, axes), got ", ids.sizes());
     check_ids("rotary_table", ids, ladder->l.n_axes, ids.size(0), ids.size(-2));
+    refuse_tangents("rotary_table", ids);
     require_cuda(ids);
     const c10::cuda::CUDAGuard guard(ids.device());
     const bool batched = ids.dim() == 3;
@@ -528,6 +538,7 @@ Tensor lora_batched(const Tensor& x, const Tensor& down_, const Tensor& up_, con
     const bool grad = at::GradMode::is_enabled();
     TORCH_CHECK_VALUE(!grad || !wants_grad(scale_), "lora_batched has no gradient for scale");
     TORCH_CHECK_VALUE(!defined(out) || writable_rows(*out), "out must have evenly strided rows on 16-byte boundaries that do not overlap");
+    refuse_tangents("lora_batched", x, down_, up_, base, scale_, out);
     const int64_t status = require_cuda(x, down_, up_, offsets_, adapters_, or_none(base), or_none(scale_), or_none(out));
     const bool graph = grad && (wants_grad(x) || wants_grad(down_) || wants_grad(up_) || wants_grad(base));
     TORCH_CHECK_VALUE(!defined(out) || !(graph || (grad && wants_grad(out))), "out cannot be given where a gradient is asked for");
@@ -544,6 +555,7 @@ Tensor lora_batched(const Tensor& x, const Tensor& down_, const Tensor& up_, con
 
 PYBIND11_MODULE(_binding, m) {
     m.def("bind", &bind);
+    m.def("has_tangent", py::overload_cast<const Tensor&>(&has_tangent));
     m.def("layer_norm", &layer_norm);
     m.def("layer_norm_forward", &layer_norm_forward);
     m.def("layer_norm_backward", &layer_norm_backward);

@@ -44,6 +44,8 @@ def layernorm_modulate(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor
     B, T, D = x.shape
     if D % 1024 or D > 4096:
         return torch.nn.functional.layer_norm(x, (D,), eps=eps) * (scale + scale_add)[:, None] + shift[:, None]
+    if torch.autograd.forward_ad._current_level >= 0 and any(map(L.binding().has_tangent, (x, scale, shift))):
+        raise NotImplementedError("layernorm_modulate has no forward-mode derivative")
     if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or shift.requires_grad):
         return _LayerNormModulate.apply(x, scale, shift, scale_add, eps)
     return _layernorm_modulate(x, scale, shift, scale_add, eps)
