@@ -197,6 +197,8 @@ void ln_prepare(const Tensor& x, Tensor& weight, Tensor& bias, double add) {
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm needs at least one channel, got x ", x.sizes());
     TORCH_CHECK_NOT_IMPLEMENTED(x.size(-1) <= NB_LAYER_NORM_MAX_DIM, "layer_norm takes up to ", NB_LAYER_NORM_MAX_DIM, " channels, got ", x.size(-1));
     TORCH_CHECK_VALUE(known_type(x), "layer_norm takes bfloat16, float16 and float32, got ", x.scalar_type());
+    const bool grouped = (weight.defined() && weight.dim() == 2) || (bias.defined() && bias.dim() == 2);
+    TORCH_CHECK(!grouped || x.size(0) <= 65535 || x.numel() == 0, "layer_norm: more than 65535 samples with a row of weights each");
     TORCH_CHECK_VALUE(weight.defined() || add == 0, "weight_add without a weight");
     if (weight.defined()) weight = ln_weight("weight", weight, x);
     if (!bias.defined()) return;
@@ -300,6 +302,8 @@ struct Ladder : torch::CustomClassHolder {
 };
 using LadderPtr = c10::intrusive_ptr<Ladder>;
 
+constexpr int64_t kMaxRows = 0x7fffffff;
+
 int ids_type(const Tensor& ids) {
     switch (ids.scalar_type()) {
         case at::kFloat: return NB_IDS_F32;
@@ -379,6 +383,9 @@ py::object rotary_axes(const Tensor& q, const OptTensor& k, const Tensor& ids, c
         TORCH_CHECK_VALUE(k->dim() == 4 && k->scalar_type() == q.scalar_type() && k->size(0) == q.size(0) && k->size(1) == q.size(1) && k->size(3) == q.size(3),
                           "k must be (B, S, Hk, D) beside q, got ", k->sizes(), " ", k->scalar_type(), " for ", q.sizes(), " ", q.scalar_type());
     check_ids("rotary_axes", ids, ladder->l.n_axes, q.size(0), q.size(1));
+    // (as the C entry, whose sizes have 32 bits)
+    TORCH_CHECK(q.size(0) <= kMaxRows && q.size(1) <= kMaxRows && q.size(2) <= kMaxRows && q.size(3) <= kMaxRows && (!defined(k) || k->size(2) <= kMaxRows),
+                "rotary_axes: more than 2^31 rows or 2^26 channels per row");
     TORCH_CHECK_VALUE(2 * ladder->pairs() <= q.size(3), "the axes have ", 2 * ladder->pairs(), " channels, more than a head (", q.size(3), ")");
     TORCH_CHECK_VALUE(q.size(2) > 0 && (!defined(k) || k->size(2) > 0), "no heads");
     refuse_tangents("rotary_axes", q, k, ids);
@@ -390,6 +397,7 @@ py::object rotary_axes(const Tensor& q, const OptTensor& k, const Tensor& ids, c
 Tensor rotary_table(const Tensor& ids, const LadderPtr& ladder) {
     TORCH_CHECK_VALUE(ids.dim() == 2 || ids.dim() == 3, "ids must be (S, axes) or (B, S, axes), got ", ids.sizes());
     check_ids("rotary_table", ids, ladder->l.n_axes, ids.size(0), ids.size(-2));
+    TORCH_CHECK(ids.size(0) <= kMaxRows && ids.size(-2) <= kMaxRows, "rotary_table: more than 2^31 rows");
     refuse_tangents("rotary_table", ids);
     require_cuda(ids);
     const c10::cuda::CUDAGuard guard(ids.device());
@@ -535,6 +543,8 @@ Tensor lora_batched(const Tensor& x, const Tensor& down_, const Tensor& up_, con
                       offsets_.size(0));
     TORCH_CHECK_VALUE(!defined(scale_) || (scale_->scalar_type() == at::kFloat && scale_->dim() == 1 && scale_->size(0) == A), "scale must be (", A,
                       ",) float32");
+    // (as the C entry, whose sizes have 32 bits)
+    TORCH_CHECK(A <= 65535 && adapters_.size(0) <= 65535 && K <= (1 << 24) && N <= (1 << 24), "lora_batched: more than 65535 adapters or requests, or 2^24 columns");
     const bool grad = at::GradMode::is_enabled();
     TORCH_CHECK_VALUE(!grad || !wants_grad(scale_), "lora_batched has no gradient for scale");
     TORCH_CHECK_VALUE(!defined(out) || writable_rows(*out), "out must have evenly strided rows on 16-byte boundaries that do not overlap");
