@@ -5,7 +5,9 @@
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 //
 // A team of one or more warps has a row at a time; the mean is subtracted before the squares are summed (no cancellation)
-// and nothing is read from HBM twice.  A team walks over many rows and keeps its columns' weights in registers, and in the
+// and nothing is read from HBM twice.  The mean is a sum of two fp32 values, the second what the first one's rounding left (the
+// sum of the differences, which are exact where it matters): a row of one value has a variance of zero and gives the bias, and
+// a mean far above the deviation costs nothing.  Differences are taken before anything is multiplied by rstd.  A team walks over many rows and keeps its columns' weights in registers, and in the
 // backward pass the fp32 sums of its columns' weight gradients too: the rows of a sum are added in a fixed order, the teams
 // of a CTA and then the CTAs' sums (a second small kernel) likewise, with no atomics, so two calls give the same bits.
 //
@@ -145,6 +147,12 @@ __device__ __forceinline__ void team_sum(float (&s)[N], int warps, int t, float*
         for (int i = 0; i < N; ++i) s[i] += r[w * N + i];
 }
 
+// 1 / sqrt(var + eps) from the sums of the squares and of the values about a point that the mean is `rest` away from.
+__device__ __forceinline__ float rstd_of(float squares, float sum, float rest, const LnParams& p) {
+    const float var = fmaf(-sum, rest, squares) / (float)p.dim;
+    return 1.f / sqrtf((var < 0.f ? 0.f : var) + p.eps);
+}
+
 // blockDim = (team, teams of a CTA); more than one team only when a team is one warp.  grid = (CTAs of a group, groups).
 template <typename T, typename W, int U>
 __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const LnParams p) {
@@ -168,27 +176,29 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const LnParams 
     }
     const T* x = static_cast<const T*>(p.x);
     Held<T> next[U];
+    float next0 = ld1<T>(x + (first + row) * p.stride_x);  // a row's first value, which the others' differences are taken from
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (on[u]) next[u].load(x + (first + row) * p.stride_x, u, t, team, p.dim);
-    const float inv = 1.f / (float)p.dim;
     for (; row < p.rows; row += step) {
         float v[U][8], s[1] = {0.f};
+        const float x0 = next0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (!on[u]) continue;
             next[u].widen(v[u]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[0] += v[u][j];
+            for (int j = 0; j < 8; ++j) s[0] += col<false>(u, j, t, team) < p.dim ? v[u][j] - x0 : 0.f;
         }
         if (row + step < p.rows) {
+            next0 = ld1<T>(x + (first + row + step) * p.stride_x);
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (on[u]) next[u].load(x + (first + row + step) * p.stride_x, u, t, team, p.dim);
         }
         team_sum<1>(s, warps, t, red, flip);
-        const float mean = s[0] * inv;
-        s[0] = 0.f;
+        const float mean = x0 + s[0] / (float)p.dim;
+        float d2[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (!on[u]) continue;
@@ -196,12 +206,13 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const LnParams 
             for (int j = 0; j < 8; ++j) {
                 const float d = col<false>(u, j, t, team) < p.dim ? v[u][j] - mean : 0.f;
                 v[u][j] = d;
-                s[0] = fmaf(d, d, s[0]);
+                d2[0] += d;
+                d2[1] = fmaf(d, d, d2[1]);
             }
         }
-        team_sum<1>(s, warps, t, red, flip);
-        const float rstd = rsqrtf(s[0] * inv + p.eps);
-        if (t == 0 && p.mean) p.mean[first + row] = mean;
+        team_sum<2>(d2, warps, t, red, flip);
+        const float rest = d2[0] / (float)p.dim, rstd = rstd_of(d2[1], d2[0], rest, p);  // what the mean lacks
+        if (t == 0 && p.mean) p.mean[first + row] = mean + rest;
         if (t == 0 && p.rstd) p.rstd[first + row] = rstd;
         if (!p.y) continue;
         T* y = static_cast<T*>(p.y) + (first + row) * p.dim;
@@ -209,7 +220,7 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const LnParams 
         for (int u = 0; u < U; ++u) {
             if (!on[u]) continue;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[u][j] = fmaf(v[u][j] * rstd, w[u][j], b[u][j]);
+            for (int j = 0; j < 8; ++j) v[u][j] = fmaf((v[u][j] - rest) * rstd, w[u][j], b[u][j]);
             put<T, false>(y, v[u], u, t, team, p.dim);
         }
     }
@@ -291,7 +302,7 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_backward_kernel(const 
             ng[u].widen(g[u]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                xh[u][j] = (xh[u][j] - mean) * rstd;  // (columns behind dim: g is 0 there, and nothing is stored)
+                xh[u][j] = col<false>(u, j, t, team) < p.dim ? (xh[u][j] - mean) * rstd : 0.f;  // (g is 0 there too)
                 if constexpr (SUMS) {
                     dw[u][j] = fmaf(g[u][j], xh[u][j], dw[u][j]);
                     db[u][j] += g[u][j];
@@ -430,13 +441,14 @@ template <int N>
 __device__ __forceinline__ void wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // The forward pass with a ring.  The mean and the variance take ONE round over the team without cancellation: a thread takes
-// its own values' mean off before it squares, and such partial results (count, sum, squares about their own mean) are
-// joined by  squares += count (mean - joint mean)^2.  RB rows go through a round together; one warp joins the warps'
-// results of a row for the others.
+// its own values' mean off before it squares, and such partial results (count n, a point near their mean, the sums r of the
+// differences from it and q of their squares) are moved to a common point, `off` away, by  q += off (2 r + off n),  r += off n:
+// first to the warp's mean, then to the first warp's.  RB rows go through a round together; one warp joins the warps' results
+// of a row for the others.
 template <typename T, typename W, int U, int ST, int RB, int MT, int MB>
 __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams p) {
-    __shared__ float2 red[RB][MT / 32];
-    __shared__ float2 joint[RB];
+    __shared__ float4 red[RB][MT / 32];
+    __shared__ float4 joint[RB];
     extern __shared__ __align__(16) unsigned char smem[];
     const int t = threadIdx.x, team = blockDim.x, warps = team >> 5, lane = t & 31, warp = t >> 5;
     const int step = gridDim.x * blockDim.y, row0 = blockIdx.x * blockDim.y + threadIdx.y;
@@ -466,18 +478,17 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
     }
     const float own[1] = {count};
     const float in_warp = warp_sums<1>(own);
-    const float per_own = count > 0.f ? 1.f / count : 0.f, per_warp = in_warp > 0.f ? 1.f / in_warp : 0.f, per_row = 1.f / (float)p.dim;
+    const float per_own = count > 0.f ? 1.f / count : 0.f, per_warp = in_warp > 0.f ? 1.f / in_warp : 0.f;
     // (what the joining lane needs of warp `lane`: its columns are the same in every row)
     float their_count = 0.f;
     for (int u = 0; u < U; ++u) {
         const int c0 = (u * team + lane * 32) * 8, c1 = c0 + 256;
         if (lane < warps) their_count += (float)(min(max(p.dim - c0, 0), c1 - c0));
     }
-    const float per_their = their_count > 0.f ? 1.f / their_count : 0.f;
 
     for (int i = 0; i < mine; i += RB) {
         wait_but<ST - RB>();
-        float mean_own[RB], s[RB], q[RB];
+        float mean_own[RB], pivot[RB], s[RB], q[RB], left[RB];
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
             Eight d[U];
@@ -486,12 +497,27 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
             for (int u = 0; u < U; ++u) {
                 if (u == U - 1 && !last) continue;
                 d[u] = ring.read(i + r, 0, u, t, team);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) a = add_f32x2(a, d[u].v[k]);
+                a = add_f32x2(a, add_f32x2(add_f32x2(d[u].v[0], d[u].v[1]), add_f32x2(d[u].v[2], d[u].v[3])));
             }
-            s[r] = sum_pairs(a);
-            mean_own[r] = s[r] * per_own;
+            // exact for values that are all alike: sums by halves of a power of two of them, or differences from the first
+            mean_own[r] = sum_pairs(a) * per_own;
+            if constexpr (U > 2) {
+                const float x0 = unpack_f32x2(d[0].v[0]).x;
+                const uint64_t m0 = both(-x0);
+                a = 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (u == U - 1 && !last) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a = add_f32x2(a, add_f32x2(d[u].v[k], m0));
+                }
+                mean_own[r] = fmaf(sum_pairs(a), per_own, x0);
+            }
+            // (differences from the first lane's, for the warp's mean)
+            pivot[r] = __shfl_sync(0xffffffffu, mean_own[r], 0);
+            s[r] = count > 0.f ? (mean_own[r] - pivot[r]) * count : 0.f;
             const uint64_t m = both(-mean_own[r]);
+            uint64_t rest = 0;
             a = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -500,60 +526,65 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
                 for (int k = 0; k < 4; ++k) {
                     const uint64_t off = add_f32x2(d[u].v[k], m);
                     a = fma_f32x2(off, off, a);
+                    rest = add_f32x2(off, rest);
                 }
             }
             q[r] = sum_pairs(a);
+            left[r] = sum_pairs(rest);
         }
         const float ws = warp_sums<RB>(s);
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-            s[r] = __shfl_sync(0xffffffffu, ws, r * (32 / RB));  // the warp's sum
-            const float off = mean_own[r] - s[r] * per_warp;
-            q[r] = fmaf(off * off, count, q[r]);
+            s[r] = fmaf(__shfl_sync(0xffffffffu, ws, r * (32 / RB)), per_warp, pivot[r]);  // the warp's mean
+            const float off = count > 0.f ? mean_own[r] - s[r] : 0.f;
+            q[r] = fmaf(off, fmaf(off, count, 2.f * left[r]), q[r]);
+            left[r] = fmaf(off, count, left[r]);
         }
-        const float wq = warp_sums<RB>(q);
-        float mean[RB], rstd[RB];
+        const float wq = warp_sums<RB>(q), wl = warp_sums<RB>(left);
+        float mean[RB], rest[RB], rstd[RB];  // the mean is mean + rest
         if (warps == 1) {
+            const float mine_rest = wl / (float)p.dim, mine_rstd = rstd_of(wq, wl, mine_rest, p);  // of the row that this lane has
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
-                mean[r] = s[r] * per_row;
-                rstd[r] = rsqrtf(__shfl_sync(0xffffffffu, wq, r * (32 / RB)) * per_row + p.eps);
+                mean[r] = s[r];
+                rest[r] = __shfl_sync(0xffffffffu, mine_rest, r * (32 / RB));
+                rstd[r] = __shfl_sync(0xffffffffu, mine_rstd, r * (32 / RB));
             }
         } else {
 #pragma unroll
             for (int r = 0; r < RB; ++r)
-                if (lane == r * (32 / RB)) red[r][warp] = make_float2(s[r], wq);
+                if (lane == r * (32 / RB)) red[r][warp] = make_float4(s[r], wq, wl, 0.f);
             __syncthreads();
             for (int r = warp; r < RB; r += warps) {
-                const float2 v = lane < warps ? red[r][lane] : make_float2(0.f, 0.f);
-                const float total[1] = {v.x};
-                const float m = warp_sums<1>(total) * per_row;
-                const float off = v.x * per_their - m;
-                const float sq[1] = {fmaf(off * off, their_count, v.y)};
-                const float rs = rsqrtf(warp_sums<1>(sq) * per_row + p.eps);
-                if (lane == 0) joint[r] = make_float2(m, rs);
+                const float4 v = lane < warps ? red[r][lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float m = __shfl_sync(0xffffffffu, v.x, 0), off = lane < warps ? v.x - m : 0.f;
+                const float both_sums[2] = {fmaf(off, fmaf(off, their_count, 2.f * v.z), v.y), fmaf(off, their_count, v.z)};
+                const float sums = warp_sums<2>(both_sums);
+                const float sq = __shfl_sync(0xffffffffu, sums, 0), sl = __shfl_sync(0xffffffffu, sums, 16), c = sl / (float)p.dim;
+                if (lane == 0) joint[r] = make_float4(m, c, rstd_of(sq, sl, c, p), 0.f);
             }
             __syncthreads();
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
-                const float2 v = joint[r];
+                const float4 v = joint[r];
                 mean[r] = v.x;
-                rstd[r] = v.y;
+                rest[r] = v.y;
+                rstd[r] = v.z;
             }
         }
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
             if (i + r >= mine) continue;  // (its slot holds an older row)
-            if (t == 0 && p.mean) p.mean[first + row0 + (i + r) * step] = mean[r];
+            if (t == 0 && p.mean) p.mean[first + row0 + (i + r) * step] = mean[r] + rest[r];
             if (t == 0 && p.rstd) p.rstd[first + row0 + (i + r) * step] = rstd[r];
             if (!p.y) continue;
-            const uint64_t scale = both(rstd[r]), off = both(-mean[r] * rstd[r]);
+            const uint64_t scale = both(rstd[r]), off = both(-rest[r] * rstd[r]), m = both(-mean[r]);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (u == U - 1 && !last) continue;
                 Eight o = ring.read(i + r, 0, u, t, team);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o.v[k] = fma_f32x2(fma_f32x2(o.v[k], scale, off), w[u].v[k], b[u].v[k]);
+                for (int k = 0; k < 4; ++k) o.v[k] = fma_f32x2(fma_f32x2(add_f32x2(o.v[k], m), scale, off), w[u].v[k], b[u].v[k]);
                 put_pairs<T>(y + col<true>(u, 0, t, team), o);
             }
             y += along;
@@ -617,7 +648,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
             s[2 * r] = s[2 * r + 1] = 0.f;
             mean[r] = nm[r], rstd[r] = nr[r];
             if (i + r >= mine) continue;  // (its slot holds an older row)
-            const uint64_t scale = both(nr[r]), off = both(-nm[r] * nr[r]);
+            const uint64_t scale = both(nr[r]), m = both(-nm[r]);
             uint64_t a0 = 0, a1 = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -625,7 +656,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
                 const Eight xv = ring.read(i + r, 0, u, t, team), dv = ring.read(i + r, 1, u, t, team);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint64_t h = fma_f32x2(xv.v[k], scale, off), g = dv.v[k];
+                    const uint64_t h = mul_f32x2(add_f32x2(xv.v[k], m), scale), g = dv.v[k];
                     if constexpr (SUMS) {
                         dw[u].v[k] = fma_f32x2(g, h, dw[u].v[k]);
                         db[u].v[k] = add_f32x2(g, db[u].v[k]);
@@ -659,16 +690,15 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_backward_kernel(const 
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
             if (i + r >= mine || !p.dx) continue;
-            // v - mean(v) - xh mean(v xh) as a line in x beside v
-            const float slope = -rstd[r] * m[2 * r + 1];
-            const uint64_t scale = both(rstd[r]), c1 = both(slope), c0 = both(fmaf(-mean[r], slope, -m[2 * r]));
+            // v - mean(v) - xh mean(v xh) as a line in x - mean beside v
+            const uint64_t scale = both(rstd[r]), c1 = both(-rstd[r] * m[2 * r + 1]), c0 = both(-m[2 * r]), off = both(-mean[r]);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (u == U - 1 && !last) continue;
                 const Eight xv = ring.read(i + r, 0, u, t, team);
                 Eight o = ring.read(i + r, 1, u, t, team);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o.v[k] = mul_f32x2(fma_f32x2(o.v[k], w[u].v[k], fma_f32x2(xv.v[k], c1, c0)), scale);
+                for (int k = 0; k < 4; ++k) o.v[k] = mul_f32x2(fma_f32x2(o.v[k], w[u].v[k], fma_f32x2(add_f32x2(xv.v[k], off), c1, c0)), scale);
                 put_pairs<T>(dx + col<true>(u, 0, t, team), o);
             }
             dx += along;
