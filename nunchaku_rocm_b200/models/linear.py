@@ -67,12 +67,18 @@ class SVDQW4A4Linear(nn.Module):
     def forward(self, x: torch.Tensor, output: torch.Tensor | None = None) -> torch.Tensor:
         batch_size, seq_len, channels = x.shape
         x = x.reshape(batch_size * seq_len, channels)
-        if output is None:
+        given = output is not None
+        if not given:
             output = torch.empty(batch_size * seq_len, self.out_features, dtype=x.dtype, device=x.device)
         quantized_x, ascales, lora_act_out = self.quantize(x)
         output = self.forward_quant(quantized_x, ascales, lora_act_out, output)
         if has_lora_batch(self):
-            output = add_lora_batch(self, x, output, samples=batch_size)
+            rows = output.view(batch_size * seq_len, self.out_features)
+            added = add_lora_batch(self, x, rows, samples=batch_size)
+            if not given:
+                output = added
+            elif added is not rows:
+                rows.copy_(added)
         return output.reshape(batch_size, seq_len, -1)
 
     def quantize(self, x: torch.Tensor, pad_size: int = 256):

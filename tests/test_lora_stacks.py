@@ -220,3 +220,36 @@ def test_recomputed_on_the_gpu(cuda_dev, reentrant, after):
     assert all(g is not None and torch.equal(w, g) for w, g in zip(want, got)) and want[1].any()
     with pytest.raises(RuntimeError, match="keep_lora_requests"):
         recomputed(cuda_dev, BF16, reentrant, after, lambda fn: fn)
+
+
+# ------------------------------------------------------------------------------------------------------------- the outputs
+@gpu
+@pytest.mark.parametrize("precision", ["int4", "nvfp4"])
+def test_a_given_output_gets_the_adapters(cuda_dev, precision):
+    from nunchaku_rocm_b200.models.linear import SVDQW4A4Linear
+
+    B, S, n_in, n_out = 2, 21, 128, 256
+    g = torch.Generator().manual_seed(6)
+    lin = SVDQW4A4Linear(n_in, n_out, rank=16, precision=precision)
+    with torch.no_grad():
+        for name, t in lin.named_parameters():
+            t.copy_(torch.randint(-128, 128, t.shape, dtype=torch.int8, generator=g) if t.dtype == torch.int8 else (torch.rand(t.shape, generator=g) * 0.02 + 0.01).to(t.dtype))
+    lin.to(cuda_dev)
+    stack = factors(2, 16, n_in, n_out, BF16, cuda_dev)
+    attach_lora_batch(lin, stack)
+    x = torch.randn(B, S, n_in, generator=g).to(BF16).to(cuda_dev)
+    with lora_requests(torch.tensor([1, 0], dtype=torch.int32, device=cuda_dev)):
+        want = lin(x)
+        rows, samples = (torch.zeros(s, dtype=BF16, device=cuda_dev) for s in ((B * S, n_out), (B, S, n_out)))
+        for buf in (rows, samples):
+            got = lin(x, output=buf)
+            assert got.shape == want.shape and torch.equal(got, want) and torch.equal(buf.view_as(want), want)
+            assert got.data_ptr() == buf.data_ptr()
+        # where a gradient is asked for, the buffer holds the sum as well
+        for t in stack:
+            t.requires_grad_(True)
+        buf = torch.zeros(B * S, n_out, dtype=BF16, device=cuda_dev)
+        got = lin(x, output=buf)
+        assert torch.equal(buf.detach().view_as(want), want) and torch.equal(got.detach(), want)
+        ref = torch.autograd.grad(lin(x), stack, torch.ones_like(want))
+        assert all(torch.equal(a, b) and a.any() for a, b in zip(torch.autograd.grad(got, stack, torch.ones_like(want)), ref))
