@@ -16,10 +16,13 @@
 // keep several rows of every team on their way into shared memory (cp.async; a thread copies just the columns that it reads
 // itself, so no barrier guards a row) and reduce RB rows together.
 //
-// Measured on a B200: 32761 x 5120 fp16, forward 115 us (5.8 TB/s; a copy of the tensor takes 109), backward 207 (4.9 TB/s; a
-// sum of two such tensors takes 146); 9216 x 3072 bf16 with a scale and shift per sample, 27.5 and 42.5 us (a copy 24.3, a sum
-// 28.8).  The long backward pass runs at two CTAs per SM (registers of the column sums and the ring both allow no third) with
-// 53 % of the issue slots and 49 % of DRAM busy: what remains are the waits of a row's own reductions.
+// Measured on a B200, back to back: 32761 x 5120 fp16, forward 119 us (5.6 TB/s; a copy of the tensor takes 109), backward and
+// sums 223 (4.5 TB/s; a sum of two such tensors takes 146); 9216 x 3072 bf16 with a scale and shift per sample, 30.5 and 48.7 us
+// (a copy 24.3, a sum 28.8); 8192 x 1001 bf16, which no 16 bytes divide, 20.7 and 39.1 us (floors 5.0 and 7.5).  The long
+// backward pass runs at two CTAs per SM (registers of the column sums and the ring both allow no third): what remains are the
+// waits of a row's own reductions.  Above 8192 channels (four groups of columns a thread) the column sums do not fit the
+// registers: 270 to 480 bytes of a thread spill with a ring, 1530 to 1940 without one, and 4096 x 12288 bf16 takes 49.6 and 105
+// us (floors 30.7 and 46.1).
 #include "nb_common.cuh"
 
 namespace nb {
@@ -148,9 +151,15 @@ __device__ __forceinline__ void team_sum(float (&s)[N], int warps, int t, float*
 }
 
 // 1 / sqrt(var + eps) from the sums of the squares and of the values about a point that the mean is `rest` away from.
-__device__ __forceinline__ float rstd_of(float squares, float sum, float rest, const LnParams& p) {
-    const float var = fmaf(-sum, rest, squares) / (float)p.dim;
-    return 1.f / sqrtf((var < 0.f ? 0.f : var) + p.eps);
+__device__ __forceinline__ float rstd_of(float squares, float sum, float rest, float per_row, float eps) {
+    const float var = fmaf(-sum, rest, squares) * per_row, v = (var < 0.f ? 0.f : var) + eps;
+    const float r = rsqrtf(v), e = fmaf(-v * r, r, 1.f);  // one step of Newton's method: rsqrtf's last bits showed
+    return isfinite(e) ? fmaf(0.5f * e, r, r) : r;
+}
+// `sum` / n, exact where it is a value of fp32; `per` is 1 / n rounded.
+__device__ __forceinline__ float quotient(float sum, float n, float per) {
+    const float q = sum * per;
+    return fmaf(fmaf(-q, n, sum), per, q);
 }
 
 // blockDim = (team, teams of a CTA); more than one team only when a team is one warp.  grid = (CTAs of a group, groups).
@@ -176,6 +185,7 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const LnParams 
     }
     const T* x = static_cast<const T*>(p.x);
     Held<T> next[U];
+    const float inv = 1.f / (float)p.dim;
     float next0 = ld1<T>(x + (first + row) * p.stride_x);  // a row's first value, which the others' differences are taken from
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -197,7 +207,7 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const LnParams 
                 if (on[u]) next[u].load(x + (first + row + step) * p.stride_x, u, t, team, p.dim);
         }
         team_sum<1>(s, warps, t, red, flip);
-        const float mean = x0 + s[0] / (float)p.dim;
+        const float mean = fmaf(s[0], inv, x0);
         float d2[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -211,7 +221,7 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const LnParams 
             }
         }
         team_sum<2>(d2, warps, t, red, flip);
-        const float rest = d2[0] / (float)p.dim, rstd = rstd_of(d2[1], d2[0], rest, p);  // what the mean lacks
+        const float rest = d2[0] * inv, rstd = rstd_of(d2[1], d2[0], rest, inv, p.eps);  // what the mean lacks
         if (t == 0 && p.mean) p.mean[first + row] = mean + rest;
         if (t == 0 && p.rstd) p.rstd[first + row] = rstd;
         if (!p.y) continue;
@@ -444,9 +454,12 @@ __device__ __forceinline__ void wait_but() { asm volatile("cp.async.wait_group %
 // its own values' mean off before it squares, and such partial results (count n, a point near their mean, the sums r of the
 // differences from it and q of their squares) are moved to a common point, `off` away, by  q += off (2 r + off n),  r += off n:
 // first to the warp's mean, then to the first warp's.  RB rows go through a round together; one warp joins the warps' results
-// of a row for the others.
+// of a row for the others.  16-bit rows have no r of their own in a thread or a warp, and the mean is one fp32 value: it is at
+// most 2^11 deviations away unless all values are alike, so its rounding is 2^-14 of one (at 32761 x 5120 fp16 119 us; 129 with
+// both as in fp32).
 template <typename T, typename W, int U, int ST, int RB, int MT, int MB>
 __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams p) {
+    constexpr bool REST = sizeof(T) == 4;
     __shared__ float4 red[RB][MT / 32];
     __shared__ float4 joint[RB];
     extern __shared__ __align__(16) unsigned char smem[];
@@ -478,7 +491,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
     }
     const float own[1] = {count};
     const float in_warp = warp_sums<1>(own);
-    const float per_own = count > 0.f ? 1.f / count : 0.f, per_warp = in_warp > 0.f ? 1.f / in_warp : 0.f;
+    const float per_own = count > 0.f ? 1.f / count : 0.f, per_warp = in_warp > 0.f ? 1.f / in_warp : 0.f, per_row = 1.f / (float)p.dim;
     // (what the joining lane needs of warp `lane`: its columns are the same in every row)
     float their_count = 0.f;
     for (int u = 0; u < U; ++u) {
@@ -499,9 +512,10 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
                 d[u] = ring.read(i + r, 0, u, t, team);
                 a = add_f32x2(a, add_f32x2(add_f32x2(d[u].v[0], d[u].v[1]), add_f32x2(d[u].v[2], d[u].v[3])));
             }
-            // exact for values that are all alike: sums by halves of a power of two of them, or differences from the first
-            mean_own[r] = sum_pairs(a) * per_own;
-            if constexpr (U > 2) {
+            // exact for values that are all alike: 16 bits of them or a power of two have an exact sum, else differences have
+            s[r] = sum_pairs(a);
+            mean_own[r] = U > 2 && !REST ? quotient(s[r], count, per_own) : s[r] * per_own;
+            if constexpr (U > 2 && REST) {
                 const float x0 = unpack_f32x2(d[0].v[0]).x;
                 const uint64_t m0 = both(-x0);
                 a = 0;
@@ -513,9 +527,10 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
                 }
                 mean_own[r] = fmaf(sum_pairs(a), per_own, x0);
             }
-            // (differences from the first lane's, for the warp's mean)
-            pivot[r] = __shfl_sync(0xffffffffu, mean_own[r], 0);
-            s[r] = count > 0.f ? (mean_own[r] - pivot[r]) * count : 0.f;
+            if constexpr (REST) {  // (differences from the first lane's, for the warp's mean)
+                pivot[r] = __shfl_sync(0xffffffffu, mean_own[r], 0);
+                s[r] = count > 0.f ? (mean_own[r] - pivot[r]) * count : 0.f;
+            }
             const uint64_t m = both(-mean_own[r]);
             uint64_t rest = 0;
             a = 0;
@@ -526,7 +541,7 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
                 for (int k = 0; k < 4; ++k) {
                     const uint64_t off = add_f32x2(d[u].v[k], m);
                     a = fma_f32x2(off, off, a);
-                    rest = add_f32x2(off, rest);
+                    if constexpr (REST) rest = add_f32x2(off, rest);
                 }
             }
             q[r] = sum_pairs(a);
@@ -535,19 +550,20 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
         const float ws = warp_sums<RB>(s);
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-            s[r] = fmaf(__shfl_sync(0xffffffffu, ws, r * (32 / RB)), per_warp, pivot[r]);  // the warp's mean
+            s[r] = __shfl_sync(0xffffffffu, ws, r * (32 / RB));
+            s[r] = REST ? fmaf(s[r], per_warp, pivot[r]) : quotient(s[r], in_warp, per_warp);  // the warp's mean
             const float off = count > 0.f ? mean_own[r] - s[r] : 0.f;
-            q[r] = fmaf(off, fmaf(off, count, 2.f * left[r]), q[r]);
+            q[r] = REST ? fmaf(off, fmaf(off, count, 2.f * left[r]), q[r]) : fmaf(off * off, count, q[r]);
             left[r] = fmaf(off, count, left[r]);
         }
-        const float wq = warp_sums<RB>(q), wl = warp_sums<RB>(left);
+        const float wq = warp_sums<RB>(q), wl = REST ? warp_sums<RB>(left) : 0.f;
         float mean[RB], rest[RB], rstd[RB];  // the mean is mean + rest
         if (warps == 1) {
-            const float mine_rest = wl / (float)p.dim, mine_rstd = rstd_of(wq, wl, mine_rest, p);  // of the row that this lane has
+            const float mine_rest = wl * per_row, mine_rstd = rstd_of(wq, wl, mine_rest, per_row, p.eps);  // of the row that this lane has
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
                 mean[r] = s[r];
-                rest[r] = __shfl_sync(0xffffffffu, mine_rest, r * (32 / RB));
+                rest[r] = REST ? __shfl_sync(0xffffffffu, mine_rest, r * (32 / RB)) : 0.f;
                 rstd[r] = __shfl_sync(0xffffffffu, mine_rstd, r * (32 / RB));
             }
         } else {
@@ -559,16 +575,15 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
                 const float4 v = lane < warps ? red[r][lane] : make_float4(0.f, 0.f, 0.f, 0.f);
                 const float m = __shfl_sync(0xffffffffu, v.x, 0), off = lane < warps ? v.x - m : 0.f;
                 const float both_sums[2] = {fmaf(off, fmaf(off, their_count, 2.f * v.z), v.y), fmaf(off, their_count, v.z)};
-                const float sums = warp_sums<2>(both_sums);
-                const float sq = __shfl_sync(0xffffffffu, sums, 0), sl = __shfl_sync(0xffffffffu, sums, 16), c = sl / (float)p.dim;
-                if (lane == 0) joint[r] = make_float4(m, c, rstd_of(sq, sl, c, p), 0.f);
+                const float sq = warp_sums<2>(both_sums), sl = __shfl_down_sync(0xffffffffu, sq, 16), c = sl * per_row;  // (lane 0)
+                if (lane == 0) joint[r] = make_float4(REST ? m : m + c, c, rstd_of(sq, sl, c, per_row, p.eps), 0.f);
             }
             __syncthreads();
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
                 const float4 v = joint[r];
                 mean[r] = v.x;
-                rest[r] = v.y;
+                rest[r] = REST ? v.y : 0.f;
                 rstd[r] = v.z;
             }
         }
@@ -584,7 +599,10 @@ __global__ void __launch_bounds__(MT, MB) layer_norm_ring_kernel(const LnParams 
                 if (u == U - 1 && !last) continue;
                 Eight o = ring.read(i + r, 0, u, t, team);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o.v[k] = fma_f32x2(fma_f32x2(add_f32x2(o.v[k], m), scale, off), w[u].v[k], b[u].v[k]);
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t d = add_f32x2(o.v[k], m);
+                    o.v[k] = fma_f32x2(REST ? fma_f32x2(d, scale, off) : mul_f32x2(d, scale), w[u].v[k], b[u].v[k]);
+                }
                 put_pairs<T>(y + col<true>(u, 0, t, team), o);
             }
             y += along;

@@ -9,10 +9,11 @@ Adapters of many requests at once on the layers of a model.
     with lora_requests(torch.tensor([1, -1, 0], dtype=torch.int32, device="cuda")):   # sample 1 has none
         model(...)
 
-Outside of it, and for samples with -1, the layers compute what they did without the stack.  The quantised weight is read
-once for all samples; the adapters are added to its 16-bit output by :func:`nunchaku_rocm_b200.ops.lora.lora_batched`, so
-the fused paths that work on the output before it is rounded (Q/K normalisation and rotation, GELU and re-quantisation) run
-as their separate kernels on layers whose adapters are in use.
+Outside of it the layers compute what they did without the stack, and for samples with -1 a layer's own output is that too.
+The quantised weight is read once for all samples; the adapters are added to its 16-bit output by
+:func:`nunchaku_rocm_b200.ops.lora.lora_batched`, so the fused paths that work on the output before it is rounded (Q/K
+normalisation and rotation, GELU and re-quantisation) run as their separate kernels, for ALL samples, on layers that have a
+stack while requests are active: what they compute is then rounded to 16 bits once more, for samples with -1 as well.
 """
 
 from __future__ import annotations
@@ -182,7 +183,8 @@ def add_lora_batch(module: nn.Module, x: torch.Tensor, out: torch.Tensor, sample
     path, whose next kernels have no backward pass either, has none at all: both refuse to be asked.
     """
     adapters = _requests()
-    module._lora_stack_used = True
+    if "_lora_stack_used" not in module.__dict__:
+        module._lora_stack_used = True
     samples = x.shape[0] if samples is None else samples
     if adapters.shape[0] != samples:
         raise ValueError(f"lora_requests has {adapters.shape[0]} samples, the layer's input {samples}")
