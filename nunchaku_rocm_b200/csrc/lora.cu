@@ -20,8 +20,8 @@
 // bytes than they compute.
 //
 // Bound: HBM for ranks up to 64 or so (R multiply-adds per byte of x, base or out); for a few rows the latency of two
-// dependent kernels, 24 single rows of 24 requests, 3072 -> 18432, rank 16: 12.9 us back to back in a graph.  The forward
-// pass of so few rows is one kernel therefore (9.3 us; the floor by bytes is 2).
+// dependent kernels, 24 single rows of 24 requests, 3072 -> 18432, rank 16: 13.0 us back to back in a graph.  The forward
+// pass of so few rows is one kernel therefore (9.8 us; the floor by bytes is 2).
 #include <cooperative_groups.h>
 
 #include "lora.cuh"
@@ -834,10 +834,9 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const Join<T> first, con
 // Whether a call runs on the tcgen05 kernels.  Their tiles are 128 rows and a launch costs some 3 us more, so the requests
 // have to be long on the whole, and there has to be work: the mma.sync kernels fall behind with the rank (shared memory
 // feeds their instructions) and, having 64-row items in clusters of eight, with a long contraction over few rows.  Measured,
-// mma.sync / tcgen05, forward, K = 2048, N = 6144: rank 16: 512 rows 9.0 / 13.3 us, 8192 rows 50.9 / 48.8; rank 64: 512 rows
-// 15.6 / 12.2, 1024 rows 22.7 / 16.3; 64 requests of 32 rows 38.5 / 42.6, of 64 rows 57.0 / 54.6.  K = 12288, N = 3072: rank 32,
-// 128 rows 22.9 / 15.1 us; rank 64, 128 rows of 4 requests 26.6 / 16.6, 16 single rows 24.3 / 28.3.  Rank 128, K = 2048, N =
-// 6144: 2048 rows of 32 requests 46.4 / 38.5 us, 512 rows of 16 25.9 / 27.3.
+// mma.sync / tcgen05, forward, bf16, K = 2048, N = 6144: rank 16: 512 rows 8.6 / 13.3 us, 8192 rows 54.4 / 51.5; rank 64: 512
+// rows 17.8 / 13.4, 1024 rows 23.7 / 17.3; 64 requests of 32 rows 46.4 / 48.2, of 64 rows 67.7 / 59.8.  K = 12288, N = 3072, rank
+// 32: 1300 rows 28.3 / 21.2 us.  Rank 128, K = 2048, N = 6144: 2048 rows of 32 requests 56.7 / 44.1 us, 512 rows of 16 31.1 / 31.2.
 bool use_tc(const nb_lora_args* a) {
     if (a->impl != NB_IMPL_AUTO) return a->impl == NB_IMPL_TCGEN05;
     const int contraction = a->dy ? a->N : a->K;
@@ -846,17 +845,18 @@ bool use_tc(const nb_lora_args* a) {
     return a->T >= 96ll * a->requests && (double)a->T * a->R * a->R * ((double)a->K + a->N) >= 1e10;
 }
 // Whether the forward pass is the one kernel for few rows: where its clusters are resident together, or in two turns when
-// one cluster per item is enough (it then reads D once and still saves a kernel).  Two kernels / one, measured: rank 16, K =
-// 3072, N = 18432: 1 row 7.2 / 5.6 us, 24 rows of 24 requests 12.9 / 9.3, 64 of 64 (two turns) 25.3 / 17.2; rank 32, K =
-// 12288, N = 3072: 128 rows 22.9 / 7.6 (15.1 on tcgen05), 1024 rows of 64 requests (two turns) 26.6 / 22.5; K = 2048, N = 6144,
-// 1024 rows of 64 requests: rank 16 15.5 / 16.5, rank 32 20.4 / 19.9.  Not taken: rank 64, K = 3072, N = 18432 (four clusters
-// per item), 256 rows 19.1 / 22.6; rank 32, 24 rows of 24 requests (two clusters per item) 16.1 / 16.9.
+// one cluster per item is enough (it then reads D once and still saves a kernel).  Two kernels / one, measured in bf16: rank 16,
+// K = 3072, N = 18432: 1 row 6.9 / 5.2 us, 24 rows of 24 requests 13.0 / 9.8, 64 of 64 (two turns) 27.3 / 20.0; rank 32, K =
+// 12288, N = 3072: 128 rows 15.9 (tcgen05) / 9.1, 1024 rows of 64 requests (two turns) 50.6 (tcgen05) / 24.5; rank 64, 128 rows of 4
+// requests 16.3 (tcgen05) / 13.8; K = 2048, N = 6144, 1024 rows of 64 requests: rank 16 16.5 / 17.0, rank 32 22.8 / 20.2.  Not
+// taken, before h had its present parts: rank 64, K = 3072, N = 18432 (four clusters per item), 256 rows 19.1 / 22.6; rank 32, 24
+// rows of 24 requests (two clusters per item) 16.1 / 16.9.
 int few_need(const nb_lora_args* a) {  // clusters of an item that keep a CTA's part of U within 80 KB
     return ceil_div((long long)a->N * a->R * 2, kFewCluster * 80 * 1024);
 }
 // CTAs that are resident together.  With one CTA per SM (above rank 64), clusters of eight do not fill the SMs: 16 clusters of
-// rank 128 took two turns (8 rows of 8 requests, 12288 -> 3072: 25.9 us for 24.4 with two kernels), 8 one (128 rows at rank 80:
-// 13.2 for 15.9).
+// rank 128 took two turns (8 rows of 8 requests, 12288 -> 3072, before h had its present parts: 25.9 us for 24.4), 8 one (128 rows at rank 80:
+// 17.0 for 17.5 on tcgen05).
 int few_slots(int R) { return R <= 64 ? 2 * sms() : 3 * sms() / 4; }
 bool use_few(const nb_lora_args* a) {
     if (a->impl == NB_IMPL_TCGEN05) return false;

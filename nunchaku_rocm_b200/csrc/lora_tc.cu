@@ -3,9 +3,9 @@
 // that overlaps the next tiles.  The products move many bytes per multiplication (rank 64: 32 multiply-adds per byte of x,
 // base, out or dy), so what the tensor cores give here is not arithmetic but the absence of it elsewhere: no operand passes
 // through registers, and the bytes in flight are the size of the shared-memory ring.  Measured on a B200 (bf16, 9216 rows,
-// rank 64): shrink 3072 -> 64 17.5 us and 9216 -> 64 35 us (3.2 and 4.9 TB/s), expand 64 -> 9216 60 us (5.6 TB/s), outer 49
-// us for both factors (4.6 TB/s): about 8 us of each are its start and its end, the rest its bytes (outer's CTAs are of two
-// lengths, and end at different times).
+// rank 64, profiled): shrink 3072 -> 64 20.5 us and 9216 -> 64 37 us (2.8 and 4.6 TB/s), expand 64 -> 9216 62 us (5.5 TB/s),
+// outer 60 us for both factors (3.9 TB/s): about 8 us of each are its start and its end, the rest its bytes (outer's CTAs are
+// of two lengths, and end at different times).
 //
 // A tensor-memory accumulator is fp32, but each step into it TRUNCATES, the sum and (fp16, whose products have 22 bits) the
 // products that it takes: a long chain is biased towards zero (432 steps: 1.4e-5 of the sum; fp32 with rounding 1.7e-6).  The

@@ -14,8 +14,8 @@
 // and K) of the pairs.
 //
 // Bound: HBM.  Q and K are read once and written once (16-byte accesses when the layout allows), the ids are 4 to 12 bytes
-// per token.  Measured on a B200: Q and K of 4608 tokens and 24 + 24 heads of 128 as views of a packed QKV, bf16, 24.7 us (4.6
-// TB/s; a copy of as many bytes takes 24.3); 32986 tokens, 24 + 8 heads, halves paired, fp16, 84 us (6.4 TB/s).
+// per token.  Measured on a B200: Q and K of 4608 tokens and 24 + 24 heads of 128 as views of a packed QKV, bf16, 25.2 us (4.5
+// TB/s; a copy of as many bytes takes 24.3); 32986 tokens, 24 + 8 heads, halves paired, fp16, 85 us (6.4 TB/s).
 #include <math.h>
 
 #include "nb_common.cuh"

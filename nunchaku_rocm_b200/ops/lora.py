@@ -33,8 +33,9 @@ def lora_batched(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, offsets:
     with the inputs otherwise.  At most 65535 adapters, and ``rows / 64 + requests`` at most 65000.  A backward pass needs a
     workspace of ``R (K + N)`` floats for every request and every few hundred rows.
 
-    ``x @ down^T`` may be beyond float16, and so may its gradient: both stay in 22 bits of a value and its row's own power of
-    two until the result is rounded.
+    Between the products ``scale * x @ down^T`` and its gradient keep 24 bits in bfloat16; in float16 22 bits and a power of two
+    per row, so they may be far beyond float16 (what is below 2^-39 of the largest in a row, or of the rows that a gradient
+    sums, is lost).
 
     Differentiable in ``x``, ``base``, ``down`` and ``up`` (not in ``scale``); gradients of adapters that several requests
     share are summed in a fixed order.

@@ -3,7 +3,7 @@ Rotary positions with several axes (time, height, width), straight from position
 
 The fused QKV projection takes its rotation from a table (:func:`nunchaku_rocm_b200.models.embeddings.flux_pos_embed`);
 :func:`rotary_table` makes that table in one launch, and :func:`rotary_axes` rotates Q and K that come from elsewhere (a
-projection with per-request adapters, a 16-bit attention layer, a training step) without one.  The reference builds tables
+16-bit attention layer, a training step) without one.  The reference builds tables
 with torch operators (``rope`` / ``NunchakuFluxPosEmbed``, nunchaku/models/embeddings.py:11-50, 74-97).
 """
 
