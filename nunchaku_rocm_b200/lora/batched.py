@@ -209,8 +209,9 @@ def attach_lora_batch(module: nn.Module, adapters, scale=None) -> None:
     """
     Give the layer a stack of adapters: ``adapters`` as in :func:`stack_loras`, or an already stacked ``(down, up)`` pair of
     3-D tensors, which every call reads as they are then (an adapter may be replaced in place, and they may require
-    gradients); in the layer's 16-bit dtype and on its device, else every call converts them.  ``scale``: one float per adapter.
-    Replaces an earlier stack; :func:`detach_lora_batch` removes it.  Ranks up to 128.
+    gradients); in the layer's 16-bit dtype and on its device, else every call converts them.  ``scale``: one float per adapter; a
+    float32 tensor on the stack's device is read in every call too, anything else at the attachment.  Replaces an earlier
+    stack; :func:`detach_lora_batch` removes it.  Ranks up to 128.
     """
     svdq = _is_svdq(module)
     ref = module.proj_down if svdq else next((p for p in module.parameters() if p.is_floating_point()), None)
