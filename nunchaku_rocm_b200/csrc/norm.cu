@@ -7,7 +7,8 @@
 // A team of one or more warps has a row at a time; the mean is subtracted before the squares are summed (no cancellation)
 // and nothing is read from HBM twice.  The mean is a sum of two fp32 values, the second what the first one's rounding left (the
 // sum of the differences, which are exact where it matters): a row of one value has a variance of zero and gives the bias, and
-// a mean far above the deviation costs nothing.  Differences are taken before anything is multiplied by rstd.  A team walks over many rows and keeps its columns' weights in registers, and in the
+// a mean far above the deviation costs y nothing.  The backward pass reads the mean as one fp32 value (xh is off by its half
+// step times rstd, as in the plain form).  Differences are taken before anything is multiplied by rstd.  A team walks over many rows and keeps its columns' weights in registers, and in the
 // backward pass the fp32 sums of its columns' weight gradients too: the rows of a sum are added in a fixed order, the teams
 // of a CTA and then the CTAs' sums (a second small kernel) likewise, with no atomics, so two calls give the same bits.
 //
