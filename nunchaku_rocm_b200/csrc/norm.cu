@@ -8,9 +8,11 @@
 // and nothing is read from HBM twice.  The mean is a sum of two fp32 values, the second what the first one's rounding left (the
 // sum of the differences, which are exact where it matters): a row of one value has a variance of zero and gives the bias, and
 // a mean far above the deviation costs y nothing.  The backward pass reads the mean as one fp32 value (xh is off by its half
-// step times rstd, as in the plain form).  Differences are taken before anything is multiplied by rstd.  A team walks over many rows and keeps its columns' weights in registers, and in the
-// backward pass the fp32 sums of its columns' weight gradients too: the rows of a sum are added in a fixed order, the teams
-// of a CTA and then the CTAs' sums (a second small kernel) likewise, with no atomics, so two calls give the same bits.
+// step times rstd, as in the plain form).  Differences are taken before anything is multiplied by rstd.
+//
+// A team walks over many rows and keeps its columns' weights in registers, and in the backward pass the fp32 sums of its
+// columns' weight gradients too: the rows of a sum are added in a fixed order, the teams of a CTA and then the CTAs' sums (a
+// second small kernel) likewise, with no atomics, so two calls give the same bits.
 //
 // Bound: HBM.  Forward reads x and writes y, backward reads x and dy and writes dx; the partial sums are 8 dim bytes per
 // CTA.  What has to be covered is the latency of a row's load and of its reductions (shuffles, a barrier): the RING kernels
